@@ -23,6 +23,19 @@ class ChunkShape(C.Structure):
                 ("lane", C.c_int32), ("l2norm", C.c_int32), ("scale", C.c_float), ("forward_only", C.c_int32)]
 
 
+class RotaryShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tokens", "seq_len", "q_heads", "kv_heads", "head_dim", "rotary_dim", "table_len", "io_dtype", "interleaved",
+                                         "positions_64")] + [("eps", C.c_float)] + [
+        (n, C.c_int64) for n in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")]
+
+
+class PagedShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("tokens", "n_seq", "max_q_len", "q_heads", "kv_heads", "head_dim", "io_dtype", "n_pages", "page_size",
+                                         "table_width", "window")] + [("scale", C.c_float)] + [
+        (n, C.c_int64) for n in ("table_stride", "q_token_stride", "q_head_stride", "k_page_stride", "k_row_stride", "k_head_stride", "v_page_stride",
+                                 "v_row_stride", "v_head_stride")]
+
+
 _P = C.c_void_p
 _SIGNATURES = {
     "kda_error_string": (C.c_char_p, [C.c_int]),
@@ -67,6 +80,12 @@ _SIGNATURES = {
     "kda_rmsnorm_gate_bwd_scratch_bytes": (C.c_size_t, [C.c_int64, C.c_int32]),
     "kda_rmsnorm_gate_bwd": (C.c_int, [C.c_int64, C.c_int32, C.c_int32] + [_P] * 9 + [C.c_size_t, _P]),
     "kda_rmsnorm_gate_bwd_static": (C.c_int, [C.c_int64, C.c_int32, C.c_int32] + [_P] * 9),
+    "kda_norm_rope_fwd": (C.c_int, [C.POINTER(RotaryShape)] + [_P] * 10),
+    "kda_norm_rope_bwd_scratch_bytes": (C.c_size_t, [C.POINTER(RotaryShape)]),
+    "kda_norm_rope_bwd": (C.c_int, [C.POINTER(RotaryShape)] + [_P] * 14 + [C.c_size_t, _P]),
+    "kda_norm_rope_append": (C.c_int, [C.POINTER(RotaryShape), C.POINTER(PagedShape)] + [_P] * 14),
+    "kda_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedShape)]),
+    "kda_paged_attention": (C.c_int, [C.POINTER(PagedShape)] + [_P] * 9 + [C.c_size_t, _P]),
     "kda_launch_count": (C.c_ulonglong, []),
     "kda_profile_enable": (None, [C.c_int]),
     "kda_profile_report": (C.c_int, [C.c_char_p, C.c_size_t]),

@@ -1,0 +1,176 @@
+"""Softmax-attention layers beside the KDA layers: per-head norm and rotation of queries and keys, a paged cache, attention
+of new tokens over it.
+
+The reference's models mix KDA layers with full and sliding-window attention (nanochat/gpt.py:116-157: rotary embedding,
+norm of q and k, flash attention or its fallback).  There these layers are composed from library calls; here they are
+kernels of this package:
+
+    qk_norm_rope         training and prefill: norm + rotation, differentiable
+    qk_norm_rope_append  serving: the same, keys and values written to the pages of a cache
+    paged_attention      serving: a chunk of new tokens, or one token, of every sequence of a batch over that cache
+
+A batch of new tokens is packed, [tokens, heads, D], with `cu_seqlens` [N+1] as in `chunk_kda`, or without it when every
+sequence has as many.  `kv_lens` [N] counts a sequence's tokens, the new ones among them; `block_table` [N, P] names their
+pages.  These three are read on the device: a decode loop captures the calls in a CUDA graph and updates the arrays in place.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _native, ops
+
+Tensor = torch.Tensor
+
+_MAX_DIM = 256
+
+
+def _same_device(first: Tensor, *others: Optional[Tensor]) -> None:
+    for t in (first, *others):
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("attention operators cannot run on CPU tensors (there is no CPU fallback)")
+        if t.device != first.device:
+            raise RuntimeError("all attention tensors must be on the same CUDA device")
+
+
+def _same_dtype(first: Tensor, *others: Tensor) -> None:
+    ops._dt(first)
+    if any(t.dtype != first.dtype for t in others):
+        raise RuntimeError("q, k, v and the cache must share one dtype")
+
+
+def _check_rotation(q: Tensor, cos: Tensor, sin: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor]) -> None:
+    dim = q.shape[-1]
+    if not 1 <= dim <= _MAX_DIM:
+        raise ValueError(f"head_dim must be between 1 and {_MAX_DIM}")
+    if cos.ndim != 2 or cos.shape != sin.shape or cos.shape[0] == 0:
+        raise ValueError("cos and sin must share shape [positions, rotary_dim / 2]")
+    if 2 * cos.shape[1] > dim:
+        raise ValueError("cos and sin rotate more values than a head has")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError("cos and sin must be float32")
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError("cos and sin have no gradient")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (dim,) or not w.is_floating_point()):
+            raise ValueError(f"{name} must have shape {(dim,)}")
+
+
+def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, *, positions: Optional[Tensor] = None, q_weight: Optional[Tensor] = None,
+                 k_weight: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tuple[Tensor, Tensor]:
+    """RMS norm of every head of q [B,T,Hq,D] and k [B,T,Hk,D], then the rotation by position; returns dense (q', k').
+
+    `cos`, `sin` [P, R/2] float32 rotate the first R <= D values of a head in pairs (i, i + R/2), or (2i, 2i+1) when
+    `interleaved`: (a, b) -> (a cos - b sin, b cos + a sin).  `positions` [B,T] int32 or int64, or None: 0 .. T-1.  `q_weight`,
+    `k_weight` [D] or None.  q and k may be slices of one projection's output.  Differentiable in q, k and the weights."""
+    out = None
+    if q.is_cuda:
+        call = lambda q, k, cos, sin, pos, qw, kw: _native.load().norm_rope(q, k, cos, sin, pos, qw, kw, eps, bool(interleaved))
+        tensors = (q, k, cos, sin, positions, q_weight, k_weight)
+        out = call(*tensors)
+        if out is None:
+            out = ops.traced(call, tensors)
+    if out is not None:
+        return out
+    if q.ndim != 4 or k.ndim != 4 or q.shape[:2] != k.shape[:2] or q.shape[-1] != k.shape[-1] or 0 in q.shape[2:] or 0 in k.shape[2:]:
+        raise ValueError("q and k must have shapes [B, T, Hq, D] and [B, T, Hk, D]")
+    _check_rotation(q, cos, sin, q_weight, k_weight)
+    if positions is not None:
+        if positions.shape != q.shape[:2] or positions.dtype not in (torch.int32, torch.int64):
+            raise ValueError("positions must be int32 or int64 with shape [B, T]")
+    elif q.shape[1] > cos.shape[0]:
+        raise ValueError(f"{q.shape[1]} tokens, but cos and sin have {cos.shape[0]} positions")
+    _same_device(q, k, cos, sin, positions, q_weight, k_weight)
+    _same_dtype(q, k)
+    raise RuntimeError("qk_norm_rope: too many rows for one call")
+
+
+def _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens):
+    if q.ndim != 3 or 0 in q.shape[1:]:
+        raise ValueError("q must have shape [tokens, Hq, D]")
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] == 0:
+        raise ValueError("k_cache and v_cache must share shape [pages, page_size, Hk, D]")
+    heads, dim = q.shape[1:]
+    if k_cache.shape[3] != dim or not dim <= _MAX_DIM:
+        raise ValueError(f"q and the cache must share a head_dim of at most {_MAX_DIM}")
+    if k_cache.shape[2] == 0 or heads % k_cache.shape[2] != 0:
+        raise ValueError("the cache's heads must divide the query heads")
+    if block_table.ndim != 2 or block_table.dtype != torch.int32 or block_table.shape[0] == 0:
+        raise ValueError("block_table must be int32 with shape [N, pages of a sequence]")
+    n = block_table.shape[0]
+    if tuple(kv_lens.shape) != (n,) or kv_lens.dtype != torch.int32:
+        raise ValueError(f"kv_lens must be int32 with shape {(n,)}")
+    if cu_seqlens is None:
+        if q.shape[0] % n != 0:
+            raise ValueError("without cu_seqlens every sequence has the same number of new tokens")
+    elif tuple(cu_seqlens.shape) != (n + 1,) or cu_seqlens.dtype != torch.int32:
+        raise ValueError(f"cu_seqlens must be int32 with shape {(n + 1,)}")
+    _same_device(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
+    _same_dtype(q, k_cache, v_cache)
+    for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache), ("block_table", block_table)):
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} must have adjacent values along its last dimension")
+    if not kv_lens.is_contiguous() or (cu_seqlens is not None and not cu_seqlens.is_contiguous()):
+        raise ValueError("kv_lens and cu_seqlens must be contiguous")
+
+
+def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is inference-only")
+
+
+def qk_norm_rope_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                        kv_lens: Tensor, cu_seqlens: Optional[Tensor] = None, *, q_weight: Optional[Tensor] = None,
+                        k_weight: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tensor:
+    """`qk_norm_rope` of a serving batch with its keys and values going to their pages: returns q' [tokens,Hq,D], dense, and
+    writes k' and v IN PLACE into k_cache, v_cache [pages, page_size, Hk, D].
+
+    The i-th of a sequence's n new tokens has position kv_len - n + i; a token whose position is negative is padding (q' = 0,
+    nothing is written).  Inference only."""
+    out = None
+    if q.is_cuda:
+        out = _native.load().append(q, k, v, cos, sin, k_cache, v_cache, block_table, kv_lens, cu_seqlens, q_weight, k_weight, eps, bool(interleaved))
+    if out is not None:
+        return out
+    _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
+    expected = (q.shape[0], k_cache.shape[2], q.shape[2])
+    if tuple(k.shape) != expected or tuple(v.shape) != expected:
+        raise ValueError(f"k and v must have shape {expected}")
+    _check_rotation(q, cos, sin, q_weight, k_weight)
+    _same_device(q, k, v, cos, sin, q_weight, k_weight)
+    _same_dtype(q, k, v)
+    for name, t in (("k", k), ("v", v)):
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise ValueError(f"{name} must have adjacent values along its last dimension")
+    _no_grad("qk_norm_rope_append", q, k, v, k_cache, v_cache, q_weight, k_weight)
+    raise RuntimeError("qk_norm_rope_append: the batch or the block table is too large for one call, or a trace is being recorded")
+
+
+def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kv_lens: Tensor, cu_seqlens: Optional[Tensor] = None, *,
+                    max_q_len: int = 0, window: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+    """Causal attention of new tokens q [tokens,Hq,D] over a paged cache that holds their own keys and values already.
+
+    The token at position p sees positions p - window + 1 .. p (window 0: all up to p); Hq / Hk query heads share a kv head.
+    `max_q_len` bounds the new tokens of any sequence (0: unknown); a batch that says so is cut into blocks accordingly.
+    Returns o [tokens,Hq,D], or (o, lse [tokens,Hq]) with the natural log of each row's sum of exponentials.  A padding token
+    (negative position) gets o = 0 and lse = -inf.  Pages that no new token reaches are not touched, and their entries in
+    the table may be anything.  Inference only."""
+    out = None
+    if q.is_cuda:
+        out = _native.load().attention(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, max_q_len, window, scale, bool(return_lse))
+    if out is not None:
+        return out if return_lse else out[0]
+    _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
+    if window < 0 or max_q_len < 0:
+        raise ValueError("window and max_q_len must not be negative")
+    if scale is not None and not (0 < scale < float("inf")):
+        raise ValueError("scale must be positive and finite")
+    _no_grad("paged_attention", q, k_cache, v_cache)
+    raise RuntimeError("paged_attention: the batch or the block table is too large for one call, or a trace is being recorded")
+
+
+__all__ = ["paged_attention", "qk_norm_rope", "qk_norm_rope_append"]

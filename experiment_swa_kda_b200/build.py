@@ -95,7 +95,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
 # torch.utils.cpp_extension.load(is_python_module=False) in the reference loader)
 # ----------------------------------------------------------------------------------------------
 SHIM_DIR = os.path.join(PKG, "torch_shim")
-SHIM_SRCS = [os.path.join(SHIM_DIR, f) for f in ("nanochat_kda_ops.cpp", "kda_host.cpp", "kda_layer.cpp")]
+SHIM_SRCS = [os.path.join(SHIM_DIR, f) for f in ("nanochat_kda_ops.cpp", "kda_host.cpp", "kda_layer.cpp", "attention_host.cpp")]
 SHIM_LIB = os.path.join(LIBDIR, "libkda_b200_torch.so")
 
 

@@ -1,0 +1,270 @@
+// Attention over a paged cache for any head width up to 256, any page size and both types: float32 arithmetic on the CUDA
+// cores.  o_i = sum_j 2^(s_ij - m_i) v_j / sum_j 2^(s_ij - m_i), s in units of log 2, in one pass over the keys with the
+// running maximum m and sum.
+//
+// A block holds 64 rows (token-major, the query heads of one kv head side by side, so that a key tile serves them all) and
+// goes through its keys in tiles of 64.  Both products are 4 x 4 outputs a thread from 16-byte shared-memory reads.
+
+#include "attn.cuh"
+
+namespace kda {
+namespace attn {
+namespace {
+
+constexpr int kRows = 64, kKeys = 64, kThreads = 256;
+
+template <int DP>
+struct Smem {
+    float q[kRows][DP + 4];
+    float k[kKeys][DP + 4];
+    float v[kKeys][DP + 4];
+    float p[kRows][kKeys + 4];
+    int bad;      // a value in the tile is not finite
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles tiles, int splits, float* part_o, float2* part_ml) {
+    extern __shared__ float4 raw[];
+    Smem<DP>& sm = *reinterpret_cast<Smem<DP>*>(raw);
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int hk = blockIdx.y, z = blockIdx.z, g = c.heads.group, D = c.heads.dim;
+    const Batch& b = c.batch;
+    Unit u;
+    if (!make_unit(b, tiles, blockIdx.x, c.window, u)) {
+        int n, tile;
+        if (hk == 0 && z == 0 && tid == 0 && tiles.find(b, blockIdx.x, n, tile)) check_batch(b, tiles, n, tile);
+        return;
+    }
+    if (hk == 0 && z == 0 && tid == 0) check_batch(b, tiles, u.n, u.row0 / kRows);
+    const int t0 = u.lo / kKeys, nt = max((u.hi + kKeys - 1) / kKeys - t0, 0);
+    const int t_begin = t0 + (int)((long long)nt * z / splits), t_end = t0 + (int)((long long)nt * (z + 1) / splits);
+
+    auto token_of = [&](int r) { return u.first + (u.row0 + r) / g; };
+    auto head_of = [&](int r) { return hk * g + (u.row0 + r) % g; };
+    for (int e = tid; e < kRows * DP; e += kThreads) {
+        const int r = e / DP, d = e - r * DP;
+        float x = 0.f;
+        if (r < u.rows && d < D) x = ld_io(c.q, (size_t)(token_of(r) * c.strides.q_token + head_of(r) * c.strides.q_head + d), c.bf16);
+        sm.q[r][d] = x;
+    }
+    // the keys each of this thread's rows sees
+    int last[4], first[4];
+    float m[4], l[4], acc[4][DP / 64][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        last[i] = r < u.rows ? u.base + (u.row0 + r) / g : -1;
+        first[i] = c.window > 0 ? last[i] - c.window + 1 : 0;
+        m[i] = -INFINITY;
+        l[i] = 0.f;
+#pragma unroll
+        for (int x = 0; x < DP / 64; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][x][j] = 0.f;
+    }
+    const float scale = c.scale * 1.4426950408889634f;
+
+    for (int t = t_begin; t < t_end; ++t) {
+        __syncthreads();
+        if (tid == 0) sm.bad = 0;
+        __syncthreads();
+        bool bad = false;
+        for (int e = tid; e < kKeys * DP; e += kThreads) {
+            const int r = e / DP, d = e - r * DP, key = t * kKeys + r;
+            float x = 0.f, y = 0.f;
+            if (d < D && key >= u.lo && key < u.hi) {
+                const int page = b.page(u.n, key / b.page_size), row = key % b.page_size;
+                if (page >= 0) {
+                    x = ld_io(c.k, (size_t)(page * c.strides.k_page + row * c.strides.k_row + hk * c.strides.k_head + d), c.bf16);
+                    y = ld_io(c.v, (size_t)(page * c.strides.v_page + row * c.strides.v_row + hk * c.strides.v_head + d), c.bf16);
+                } else if (d == 0) {
+                    b.tell(KDA_ERR_BLOCK_TABLE);
+                }
+            }
+            sm.k[r][d] = x;
+            sm.v[r][d] = y;
+            bad |= !isfinite(y);
+        }
+        if (bad) sm.bad = 1;
+        __syncthreads();
+
+        float s[4][4] = {};
+#pragma unroll 4
+        for (int d = 0; d < DP; d += 4) {
+            float4 a[4], k[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(&sm.q[ty + 16 * i][d]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(&sm.k[tx + 16 * j][d]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[i][j] = fmaf(a[i].x, k[j].x, s[i][j]);
+                    s[i][j] = fmaf(a[i].y, k[j].y, s[i][j]);
+                    s[i][j] = fmaf(a[i].z, k[j].z, s[i][j]);
+                    s[i][j] = fmaf(a[i].w, k[j].w, s[i][j]);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float top = -INFINITY;
+            bool seen[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = t * kKeys + tx + 16 * j;
+                seen[j] = key <= last[i] && key >= first[i];
+                s[i][j] *= scale;
+                if (seen[j]) top = fmaxf(top, fmaxf(s[i][j], kLowest));
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const float next = fmaxf(m[i], top);
+            const float keep = m[i] == -INFINITY ? 0.f : exp2f(m[i] - next);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = seen[j] ? exp2f(s[i][j] - next) : 0.f;
+                sum += p;
+                sm.p[ty + 16 * i][tx + 16 * j] = p;
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            l[i] = l[i] * keep + sum;
+            m[i] = next;
+#pragma unroll
+            for (int x = 0; x < DP / 64; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][x][j] *= keep;
+        }
+        __syncthreads();
+        if (!sm.bad) {
+#pragma unroll 2
+            for (int j = 0; j < kKeys; j += 4) {
+                float4 p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(&sm.p[ty + 16 * i][j]);
+#pragma unroll
+                for (int x = 0; x < DP / 64; ++x)
+#pragma unroll
+                    for (int jj = 0; jj < 4; ++jj) {
+                        const float4 v = *reinterpret_cast<const float4*>(&sm.v[j + jj][4 * tx + 64 * x]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float w = jj == 0 ? p[i].x : jj == 1 ? p[i].y : jj == 2 ? p[i].z : p[i].w;
+                            acc[i][x][0] = fmaf(w, v.x, acc[i][x][0]);
+                            acc[i][x][1] = fmaf(w, v.y, acc[i][x][1]);
+                            acc[i][x][2] = fmaf(w, v.z, acc[i][x][2]);
+                            acc[i][x][3] = fmaf(w, v.w, acc[i][x][3]);
+                        }
+                    }
+            }
+        } else {
+            // 0 times a value that is not finite is NaN: keys that a row does not see are left out of its sum
+            for (int j = 0; j < kKeys; ++j) {
+                const int key = t * kKeys + j;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (key <= last[i] && key >= first[i]) {
+                        const float w = sm.p[ty + 16 * i][j];
+#pragma unroll
+                        for (int x = 0; x < DP / 64; ++x)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) acc[i][x][q] = fmaf(w, sm.v[j][4 * tx + 64 * x + q], acc[i][x][q]);
+                    }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = ty + 16 * i;
+        if (r >= u.rows) continue;
+        const size_t row = (size_t)token_of(r) * c.heads.q_heads + head_of(r);
+        if (splits > 1) {
+            const size_t at = (size_t)z * b.tokens * c.heads.q_heads + row;
+            if (tx == 0) part_ml[at] = make_float2(m[i], l[i]);
+#pragma unroll
+            for (int x = 0; x < DP / 64; ++x)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int d = 4 * tx + 64 * x + j;
+                    if (d < D) part_o[at * D + d] = acc[i][x][j];
+                }
+            continue;
+        }
+        const float inv = m[i] == -INFINITY ? 0.f : 1.f / l[i];
+        if (tx == 0 && c.lse != nullptr) c.lse[row] = m[i] == -INFINITY ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+#pragma unroll
+        for (int x = 0; x < DP / 64; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int d = 4 * tx + 64 * x + j;
+                if (d < D) st_io(c.o, row * D + d, c.bf16, acc[i][x][j] * inv);
+            }
+    }
+}
+
+// Joins the parts of a row: a warp a row.
+__global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
+    const long long rows = (long long)c.tokens * c.q_heads;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    float m = -INFINITY;
+    for (int z = lane; z < c.splits; z += 32) m = fmaxf(m, c.part_ml[z * rows + row].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float acc[8] = {}, l = 0.f;
+    for (int z = 0; z < c.splits; ++z) {
+        const float2 ml = c.part_ml[z * rows + row];
+        if (ml.x == -INFINITY) continue;
+        const float w = exp2f(ml.x - m);
+        l += ml.y * w;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const int d = lane + 32 * x;
+            if (d < c.dim) acc[x] = fmaf(w, c.part_o[(z * rows + row) * c.dim + d], acc[x]);
+        }
+    }
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    if (lane == 0 && c.lse != nullptr) c.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        const int d = lane + 32 * x;
+        if (d < c.dim) st_io(c.o, row * c.dim + d, c.bf16, acc[x] * inv);
+    }
+}
+
+template <int DP>
+int launch(const Call& c, const Tiles& t, dim3 grid, int splits, float* part_o, float2* part_ml, cudaStream_t st) {
+    const size_t smem = sizeof(Smem<DP>);
+    if (int rc = set_smem_limit(attn_general_kernel<DP>, smem)) return rc;
+    KDA_LAUNCH("attn_general_kernel", st, attn_general_kernel<DP><<<grid, kThreads, smem, st>>>(c, t, splits, part_o, part_ml));
+    return launch_status();
+}
+
+}  // namespace
+
+int combine(const Combine& c, cudaStream_t st) {
+    const long long rows = (long long)c.tokens * c.q_heads;
+    KDA_LAUNCH("attn_combine_kernel", st, attn_combine_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(c));
+    return launch_status();
+}
+
+int general(const Call& c, int splits, cudaStream_t st) {
+    Tiles t{kRows, c.heads.group, 0};
+    const long long slots = tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, t.group, kRows, c.batch.cu != nullptr, t.per_seq);
+    const dim3 grid((unsigned)slots, (unsigned)c.heads.kv_heads, (unsigned)splits);
+    const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
+    float2* part_ml = static_cast<float2*>(c.workspace);
+    float* part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * splits * sizeof(float2), 256));
+    int rc;
+    if (c.heads.dim <= 64) rc = launch<64>(c, t, grid, splits, part_o, part_ml, st);
+    else if (c.heads.dim <= 128) rc = launch<128>(c, t, grid, splits, part_o, part_ml, st);
+    else rc = launch<256>(c, t, grid, splits, part_o, part_ml, st);
+    if (rc || splits == 1) return rc;
+    return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, splits, part_o, part_ml, c.o, c.lse, c.bf16}, st);
+}
+
+}  // namespace attn
+}  // namespace kda

@@ -65,6 +65,8 @@ extern "C" const char* kda_error_string(int code) {
         case KDA_ERR_NULL: return "required pointer is null";
         case KDA_ERR_DEVICE_STATUS: return "kernel reported a device-side status (bounded wait expired)";
         case KDA_ERR_CU_SEQLENS: return "cu_seqlens is inconsistent: not starting at 0, not ending at the token count, decreasing, or describing more chunks than the workspace holds";
+        case KDA_ERR_BLOCK_TABLE: return "block table names no page for a cached token in reach, or a cached length exceeds the table";
+        case KDA_ERR_POSITION: return "a position lies outside the rotation tables";
         default: return "unknown error";
     }
 }

@@ -1506,8 +1506,9 @@ int simt_chunk_fwd(const KdaChunkShape* sh, const void* q, const void* k, const 
 }
 
 // Device status word of a forward / backward pair that used `workspace`: 0, kStatusBadCuSeqlens, or the code of the
-// bounded wait that expired in the tensor-core lane.
+// bounded wait that expired in the tensor-core lane.  The attention kernels report their KDA_ERR_* codes as they are.
 static int status_code(int v) {
+    if (v == KDA_ERR_BLOCK_TABLE || v == KDA_ERR_POSITION || v == KDA_ERR_CU_SEQLENS) return v;
     return v == 0 ? KDA_OK : (v == simt::kStatusBadCuSeqlens ? KDA_ERR_CU_SEQLENS : KDA_ERR_DEVICE_STATUS);
 }
 

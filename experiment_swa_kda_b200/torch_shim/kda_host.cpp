@@ -631,6 +631,7 @@ OptTensor rmsnorm(const Tensor& x_, const Tensor& gate_, const Tensor& w_, doubl
 
 namespace kda_host {
 void bind_layer(pybind11::module_& m);      // kda_layer.cpp
+void bind_attention(pybind11::module_& m);  // attention_host.cpp
 }
 
 PYBIND11_MODULE(libkda_b200_torch, m) {
@@ -647,4 +648,5 @@ PYBIND11_MODULE(libkda_b200_torch, m) {
     m.def("conv_multi", &conv_multi, nogil());
     m.def("rmsnorm", &rmsnorm, nogil());
     bind_layer(m);
+    bind_attention(m);
 }

@@ -33,6 +33,8 @@ extern "C" {
 #define KDA_ERR_NULL (-5)          /* a required pointer is null */
 #define KDA_ERR_DEVICE_STATUS (-6) /* a kernel raised its device-side status word (bounded wait expired) */
 #define KDA_ERR_CU_SEQLENS (-7)    /* cu_seqlens (read on the device) is inconsistent with tokens / the workspace */
+#define KDA_ERR_BLOCK_TABLE (-8)   /* a block table (read on the device) names no page for a token in reach, or a length exceeds it */
+#define KDA_ERR_POSITION (-9)      /* a position (read on the device) lies outside the rotation's tables */
 
 #define KDA_DTYPE_F32 0
 #define KDA_DTYPE_BF16 1
@@ -357,6 +359,66 @@ int kda_rmsnorm_gate_bwd_static(int64_t rows, int32_t dim, int32_t io_dtype, con
 unsigned long long kda_launch_count(void);
 void kda_profile_enable(int on);
 int kda_profile_report(char* out, size_t cap);
+
+/* ---- attention layers beside the KDA layers ------------------------------------
+ * What a softmax-attention layer of a model that mixes both needs (in the reference these layers are composed from
+ * library calls: nanochat/gpt.py:116-157, nanochat/flash_attention.py): per-head RMS norm of queries and keys with the
+ * rotation by position, the same with keys and values going to a paged cache, and attention of new tokens over that cache.
+ *
+ * Norm and rotation.  Per row x of head_dim values: u = x * rsqrt(mean(x^2) + eps) * weight (weight NULL: ones), and for
+ * each of the rotary_dim/2 pairs (a, b) of the first rotary_dim values - (i, i + rotary_dim/2), or (2i, 2i+1) when
+ * interleaved -: y_a = u_a cos_i - u_b sin_i, y_b = u_b cos_i + u_a sin_i.  cos, sin [table_len, rotary_dim/2] float32.
+ * q rows are q_token_stride / q_head_stride elements apart (k, v alike), their values adjacent; outputs are dense
+ * [tokens, heads, head_dim].  positions [tokens]: int32, int64 (positions_64), or NULL: token t is at t % seq_len.
+ * A position outside the tables is clamped and the status word reports KDA_ERR_POSITION.
+ */
+typedef struct KdaRotaryShape {
+    int32_t tokens, seq_len;
+    int32_t q_heads, kv_heads, head_dim, rotary_dim;
+    int32_t table_len;
+    int32_t io_dtype;
+    int32_t interleaved;
+    int32_t positions_64;
+    float eps;
+    int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} KdaRotaryShape;
+int kda_norm_rope_fwd(const KdaRotaryShape* shape, const void* q, const void* k, const float* cos, const float* sin, const void* positions,
+                      const float* q_weight, const float* k_weight, void* q_out, void* k_out, void* stream);
+/* d_q_out, d_k_out, dq, dk dense; dq_weight, dk_weight [head_dim] float32, or NULL where the weight is. */
+size_t kda_norm_rope_bwd_scratch_bytes(const KdaRotaryShape* shape);
+int kda_norm_rope_bwd(const KdaRotaryShape* shape, const void* q, const void* k, const float* cos, const float* sin, const void* positions,
+                      const float* q_weight, const float* k_weight, const void* d_q_out, const void* d_k_out, void* dq, void* dk,
+                      float* dq_weight, float* dk_weight, void* scratch, size_t scratch_bytes, void* stream);
+
+/* Paged cache.  k_cache, v_cache [n_pages, page_size, kv_heads, head_dim] at the strides given (in elements, values of a
+ * head adjacent).  block_table [n_seq, table_width] int32, rows table_stride apart: position p of sequence n lies in page
+ * block_table[n][p / page_size], row p % page_size.  kv_lens [n_seq] int32: tokens of the sequence, the new ones among
+ * them.  cu_seqlens [n_seq+1] int32: new tokens of the packed batch, or NULL: tokens / n_seq each.  The i-th of a
+ * sequence's n new tokens is at position kv_len - n + i; a negative one is padding.  max_q_len: a bound on the new tokens of
+ * any sequence, or 0.  All three are read on the device, and pages that no new token reaches are never touched.
+ */
+typedef struct KdaPagedShape {
+    int32_t tokens, n_seq, max_q_len;
+    int32_t q_heads, kv_heads, head_dim;
+    int32_t io_dtype;
+    int32_t n_pages, page_size, table_width;
+    int32_t window;                 /* a token sees itself and window - 1 before it; 0: all */
+    float scale;                    /* > 0 */
+    int64_t table_stride;
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_page_stride, k_row_stride, k_head_stride, v_page_stride, v_row_stride, v_head_stride;
+} KdaPagedShape;
+/* Norm and rotation of the new tokens' q and k (rotary: dims, strides, tables; tokens, positions and seq_len are the paged
+ * batch's): q_out dense, k and the unchanged v to their places in the cache.  Padding tokens: q_out = 0, nothing else. */
+int kda_norm_rope_append(const KdaRotaryShape* rotary, const KdaPagedShape* paged, const void* q, const void* k, const void* v,
+                         const float* cos, const float* sin, const float* q_weight, const float* k_weight, const int32_t* block_table,
+                         const int32_t* kv_lens, const int32_t* cu_seqlens, void* q_out, void* k_cache, void* v_cache, void* stream);
+/* o [tokens, q_heads, head_dim] dense, lse [tokens, q_heads] float32 (log of the sum of exponentials) or NULL.  Query
+ * heads h*g .. h*g + g - 1 share kv head h.  Padding tokens: o = 0, lse = -inf. */
+size_t kda_paged_attention_workspace_bytes(const KdaPagedShape* shape);
+int kda_paged_attention(const KdaPagedShape* shape, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                        const int32_t* kv_lens, const int32_t* cu_seqlens, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }

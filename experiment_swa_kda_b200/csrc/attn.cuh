@@ -167,6 +167,8 @@ struct Call {
     void* workspace;
 };
 int general(const Call& c, int splits, cudaStream_t st);
+bool tc_takes(const Call& c);      // bf16, head width, page size and strides that the tensor-core kernel can load
+int tc(const Call& c, int splits, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace kda

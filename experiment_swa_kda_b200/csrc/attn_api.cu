@@ -20,20 +20,22 @@ int check(const KdaPagedShape* s, bool packed) {
     return KDA_OK;
 }
 
-// Parts a row's keys are cut into.  A part is worth its own block while the machine has room; what a row sees is known on the
-// device alone, so the bound is the table's.
-int split_count(const KdaPagedShape& s, bool packed) {
+// Parts a row's keys are cut into where its blocks alone leave SMs idle.  What a row sees is known on the device alone, so the
+// bound is the table's; a part has two key tiles at least.
+int split_count(const KdaPagedShape& s, bool packed, int rows, int keys, int resident) {
     int per_seq;
     const int group = s.q_heads / s.kv_heads;
     const int max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
-    const long long blocks = tile_slots(s.tokens, s.n_seq, max_q, group, 64, packed, per_seq) * s.kv_heads;
+    const long long blocks = tile_slots(s.tokens, s.n_seq, max_q, group, rows, packed, per_seq) * s.kv_heads;
     long long reach = (long long)s.table_width * s.page_size;
-    if (s.window > 0 && max_q > 0 && reach > s.window + max_q) reach = s.window + max_q;
-    const long long tiles = (reach + 63) / 64;
-    long long n = 2 * 148 / (blocks > 0 ? blocks : 1);
+    if (s.window > 0 && max_q > 0 && reach > (long long)s.window + max_q) reach = (long long)s.window + max_q;
+    const long long tiles = (reach + keys - 1) / keys;
+    long long n = resident / (blocks > 0 ? blocks : 1);
     if (n > tiles / 2) n = tiles / 2;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
+int general_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 64, 64, 2 * 148); }
+int tc_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 256, 128, 148); }
 
 }  // namespace
 
@@ -41,8 +43,10 @@ extern "C" size_t kda_paged_attention_workspace_bytes(const KdaPagedShape* s) {
     if (check(s, true)) return 0;
     const size_t rows = (size_t)s->tokens * s->q_heads;
     size_t most = 0;
-    for (int packed = 0; packed < 2; ++packed) {
-        const size_t n = (size_t)split_count(*s, packed);
+    for (int way = 0; way < 4; ++way) {
+        const bool packed = way & 1;
+        if (!packed && s->tokens % s->n_seq != 0) continue;
+        const size_t n = (size_t)(way & 2 ? tc_splits(*s, packed) : general_splits(*s, packed));
         const size_t need = n > 1 ? align_up(rows * n * sizeof(float2), 256) + rows * n * s->head_dim * sizeof(float) : 0;
         if (need > most) most = need;
     }
@@ -71,5 +75,5 @@ extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const 
     c.bf16 = s->io_dtype == KDA_DTYPE_BF16;
     c.max_q_len = packed ? s->max_q_len : q_len;
     c.workspace = workspace;
-    return general(c, split_count(*s, packed), (cudaStream_t)stream);
+    return tc_takes(c) ? tc(c, tc_splits(*s, packed), (cudaStream_t)stream) : general(c, general_splits(*s, packed), (cudaStream_t)stream);
 }

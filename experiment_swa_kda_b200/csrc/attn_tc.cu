@@ -1,0 +1,531 @@
+// Attention over a paged cache on the tensor cores (bf16, heads up to 128 wide).
+//
+//   S = Q K^T,  p_ij = 2^(c s_ij - c m_i),  o_i = sum_j p_ij v_j / sum_j p_ij,   c = scale / ln 2
+//
+// in one pass over the keys.  A block has 256 rows - token-major, the query heads of one kv head side by side, so that every
+// key tile serves all of them and a chunk of few tokens still fills the tile - as two tiles of 128, and walks through the keys
+// 128 at a time.  Per key tile and row tile the tensor pipe does S (M128 N128 K = head) and O += P V (M128 N = head K128); the
+// two row tiles take turns: while one's scores are turned into weights by its four warps, the other's products run.  S and O
+// live in tensor memory, P (bf16) takes S's place there and is the A operand of its product, so nothing but K and V goes through
+// shared memory.  A thread owns a row: maximum and sum need no exchange.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^kLazy since the last time (the weights are then at most
+// 2^kLazy, which costs bf16 nothing: its rounding is relative); after a few tiles that no longer happens.
+// P is rounded to bf16 because the product takes one type and V is bf16; sums and statistics are float32.
+//
+// K and V come page by page by TMA into one ring (K 0, V 0, K 1, V 1, ...).  A tile that some row sees only in part is masked
+// in registers; in its V tile the keys that no row sees are blanked, since 0 times what lies in an unused slot may be NaN, and
+// so are values that are not finite at keys only some rows see: these are added by the rows that see them at the end.
+
+#include "attn.cuh"
+#include "tc_common.cuh"
+
+namespace kda {
+namespace tc {
+int make_map_paged(CUtensorMap* m, const void* ptr, uint64_t dim, uint64_t rows, uint64_t heads, uint64_t pages, int64_t row_ld, int64_t head_ld, int64_t page_ld,
+                   uint32_t box_rows);
+}
+namespace attn {
+namespace {
+
+using namespace tc;
+
+constexpr int kKeys = 128, kRows = 256;
+constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kFixWarp = 10, kThreads = 384;
+constexpr float kLazy = 8.f;
+constexpr int kStatusWait = 120;      // device status of an expired wait
+
+template <int DP>
+struct Layout {
+    static constexpr int kTile = DP / 64 * 16384;             // 128 rows of Q, K or V: one or two blocks of 64 columns
+    static constexpr int kStages = DP == 128 ? 5 : 10;
+    static constexpr int kRing = 2 * kTile;
+    static constexpr int kBars = kRing + kStages * kTile;
+    static constexpr int kBytes = kBars + 512 + 1024;         // barriers; slack to align the tiles
+};
+
+struct Args {
+    Call c;
+    Tiles tiles;
+    int slots, splits, box_rows, q16;
+    float* part_o;
+    float2* part_ml;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// a maximum that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ bool finite_bf16x2(uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; }
+
+// The key tiles a row tile goes through, of those of its block.
+struct Range {
+    int begin, end;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
+                                                              const __grid_constant__ Args a) {
+    using L = Layout<DP>;
+    extern __shared__ uint8_t raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::kBars);
+    uint64_t *bar_q = bar, *bar_s = bar + 1, *bar_p = bar + 3, *bar_o = bar + 5, *bar_end = bar + 7, *bar_full = bar + 8, *bar_free = bar_full + L::kStages,
+             *bar_part = bar_free + L::kStages;
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bar + 60);
+    volatile int& abort_flag = *reinterpret_cast<volatile int*>(bar + 61);
+    volatile int& odd_values = *reinterpret_cast<volatile int*>(bar + 62);
+
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const Batch& b = a.c.batch;
+    const int g = a.c.heads.group, D = a.c.heads.dim, hk = blockIdx.y, z = blockIdx.z, window = a.c.window;
+    // a sequence's last rows see the most keys: they start first
+    const int slot = a.slots - 1 - (int)blockIdx.x;
+    Unit u;
+    const bool some = make_unit(b, a.tiles, slot, window, u);
+    if (hk == 0 && z == 0 && tid == 0) {
+        int n, tile;
+        if (a.tiles.find(b, slot, n, tile)) check_batch(b, a.tiles, n, tile);
+    }
+    if (!some) return;
+
+    // keys any row of the block sees: [u.lo, u.hi); keys all of them see: [all_lo, all_hi)
+    const int first_pos = u.base + u.row0 / g, last_pos = u.base + (u.row0 + u.rows - 1) / g;
+    const int all_lo = window > 0 ? max(last_pos - window + 1, 0) : 0, all_hi = first_pos + 1;
+    const int t0 = u.lo / kKeys, nt = max((u.hi + kKeys - 1) / kKeys - t0, 0);
+    const int t_begin = t0 + (int)((long long)nt * z / a.splits), t_end = t0 + (int)((long long)nt * (z + 1) / a.splits);
+    auto range_of = [&](int t) {      // key tiles of row tile t
+        const int r0 = u.row0 + 128 * t, r1 = min(r0 + 128, u.row0 + u.rows) - 1;
+        if (r0 > r1) return Range{0, 0};
+        const int hi = u.base + r1 / g + 1, lo = window > 0 ? max(u.base + r0 / g - window + 1, 0) : 0;
+        Range r{max(t_begin, lo / kKeys), min(t_end, (max(hi, 0) + kKeys - 1) / kKeys)};
+        if (r.end < r.begin) r.end = r.begin;
+        return r;
+    };
+    const Range range[2] = {range_of(0), range_of(1)};
+    // the tiles some row sees only in part
+    auto partial = [&](int j) { return j * kKeys < all_lo || (j + 1) * kKeys > all_hi; };
+
+    if (warp == 0 && elect_one()) {
+        mbar_init(bar_q, kSoftmaxWarps);
+        mbar_init(bar_end, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(bar_s + t, 1);
+            mbar_init(bar_p + t, 4);
+            mbar_init(bar_o + t, 1);
+        }
+        for (int s = 0; s < L::kStages; ++s) {
+            mbar_init(bar_full + s, 1);
+            mbar_init(bar_free + s, 1);
+            mbar_init(bar_part + s, 1);
+        }
+        mbar_fence_init();
+        abort_flag = 0;
+        odd_values = 0;
+    }
+    if (warp == kMmaWarp) tmem_alloc(&tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    constexpr uint32_t cS = 0, cO = 256;      // S (then P) of the two row tiles: 128 columns each; O: DP each
+    auto wait = [&](uint64_t* w, uint32_t parity) {
+        if (mbar_poll(w, parity, kSpinLimit)) return true;
+        abort_flag = 1;
+        b.tell(kStatusWait);
+        return false;
+    };
+    // stage and phase of the ring's i-th tile
+    auto stage = [](int i) { return i % L::kStages; };
+    auto turn = [](int i) { return (uint32_t)(i / L::kStages) & 1u; };
+
+    if (warp < kSoftmaxWarps) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int t = warp >> 2;
+        // ------------------------------------------------------------------ Q into shared memory
+        {
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.c.q);
+            uint8_t* tile = sm + t * L::kTile;
+            constexpr int kChunks = DP / 8;
+            for (int e = tid & 127; e < 128 * kChunks; e += 128) {
+                const int r = e / kChunks, c = e - r * kChunks, row = 128 * t + r;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (row < u.rows && 8 * c < D) {
+                    const int pr = u.row0 + row, tok = pr / g;
+                    const __nv_bfloat16* src = q + (u.first + tok) * a.c.strides.q_token + (hk * g + pr - tok * g) * a.c.strides.q_head + 8 * c;
+                    if (a.q16) {
+                        x = __ldg(reinterpret_cast<const uint4*>(src));
+                    } else {
+                        const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
+                        x = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16, s[6] | (uint32_t)s[7] << 16);
+                    }
+                }
+                *reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + sw128_off(r, c & 7)) = x;
+            }
+            fence_async_smem();
+            warp_arrive(bar_q, lane);
+        }
+        // ------------------------------------------------------------------ softmax of row tile t, a row a thread
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + lanes + cS + 128 * t, tO = tmem + lanes + cO + DP * t;
+        const int row = 128 * t + (tid & 127), prow = u.row0 + row;
+        const int last = row < u.rows ? u.base + prow / g : last_pos;      // rows behind the last one compute along, unseen
+        const int first = window > 0 ? last - window + 1 : 0;
+        // keys all rows of the warp see
+        const int w_lo = __reduce_max_sync(0xffffffffu, first), w_hi = __reduce_min_sync(0xffffffffu, last) + 1;
+        const float c = a.c.scale * 1.4426950408889634f, lazy = kLazy / c;
+        const Range r = t ? range[1] : range[0];
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int j = r.begin; j < r.end; ++j) {
+            const int i = j - r.begin;
+            ok = wait(bar_s + t, i & 1);
+            __syncwarp();
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, s[q]);
+            tmem_ld_wait();
+            float top = -INFINITY;
+            if (j * kKeys < w_lo || (j + 1) * kKeys > w_hi) {
+                const int k0 = j * kKeys;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int key = k0 + 32 * q + e;
+                        if (key < first || key > last) s[q][e] = 0xff800000u;
+                    }
+                if (last >= k0 && first < k0 + kKeys) top = kLowest;
+            } else {
+                top = kLowest;
+            }
+            {
+                float x[4] = {top, top, top, top};
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) x[q] = max_nan(x[q], __uint_as_float(s[q][e]));
+                top = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+            }
+            const bool grow = !(top <= m + lazy) && !(top == -INFINITY);      // a NaN too
+            if (__any_sync(0xffffffffu, grow)) {
+                const float next = max_nan(m, top);
+                const float f = grow ? (m == -INFINITY ? 0.f : ex2((m - next) * c)) : 1.f;
+                if (grow) m = next;
+                l *= f;
+                if (i > 0) {      // the sums so far are complete once the product before has ended
+                    ok = wait(bar_o + t, (i - 1) & 1);
+                    __syncwarp();
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int q = 0; q < DP / 32; ++q) {
+                        uint32_t o[32];
+                        tmem_ld32(tO + 32 * q, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st32(tO + 32 * q, o);
+                    }
+                }
+            }
+            const float mc = m == -INFINITY ? 0.f : max_nan(m * c, kLowest);
+            const f2 c2 = f2_all(c), n2 = f2_all(-mc);
+            f2 sum[2] = {f2_all(0.f), f2_all(0.f)};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t p[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const int q = 2 * h + (e >> 4), at = 2 * (e & 15);
+                    const float2 x = f2_get(f2_fma(f2_make(__uint_as_float(s[q][at]), __uint_as_float(s[q][at + 1])), c2, n2));
+                    const f2 y = f2_make(ex2(x.x), ex2(x.y));
+                    sum[e & 1] = f2_add(sum[e & 1], y);
+                    p[e] = f2_to_bf16(y);
+                }
+                tmem_st32(tS + 32 * h, p);
+            }
+            const float2 both = f2_get(f2_add(sum[0], sum[1]));
+            l += both.x + both.y;
+            tmem_st_wait();
+            tc_fence_before();
+            warp_arrive(bar_p + t, lane);
+        }
+        // ------------------------------------------------------------------ O / l
+        const int n = r.end - r.begin;
+        if (ok && n > 0) {
+            ok = wait(bar_o + t, (n - 1) & 1);
+            __syncwarp();
+        }
+        if (ok && 128 * t + 32 * (warp & 3) < u.rows) {
+            tc_fence_after();
+            const bool mine = row < u.rows;
+            if (m == kLowest) l = 0.f;      // nothing but -inf: 0 / 0
+            const int tok = u.first + prow / g, head = hk * g + prow % g;
+            const size_t out = (size_t)tok * a.c.heads.q_heads + head;
+            const bool split = a.splits > 1;
+            const size_t at = (size_t)z * b.tokens * a.c.heads.q_heads + out;
+            const float inv = split ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
+            if (mine && split) a.part_ml[at] = make_float2(m * c, l);
+            if (mine && !split && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m * c + log2f(l)) * kLn2;
+            uint8_t* stage_out = sm + t * L::kTile + (warp & 3) * 32 * (DP * 2);      // Q has been read
+#pragma unroll
+            for (int q = 0; q < DP / 32; ++q) {
+                uint32_t o[32];
+                if (n > 0) {
+                    tmem_ld32(tO + 32 * q, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (odd_values && n > 0) {
+                    // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
+#pragma unroll 1
+                    for (int key = max(first, r.begin * kKeys); key <= min(last, r.end * kKeys - 1); ++key) {
+                        if (key >= all_lo && key < all_hi) {
+                            key = all_hi - 1;
+                            continue;
+                        }
+                        const int page = b.page(u.n, key / b.page_size);
+                        if (page < 0) continue;
+                        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v) + page * a.c.strides.v_page + (key % b.page_size) * a.c.strides.v_row +
+                                                 hk * a.c.strides.v_head + 32 * q;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (32 * q + e < D) {
+                                const float x = __bfloat162float(v[e]);
+                                if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                            }
+                    }
+                }
+                if (split) {
+                    float* dst = a.part_o + at * D + 32 * q;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        if (mine && 32 * q + e < D)
+                            *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(o[8 * x + 2 * e]) * inv, __uint_as_float(o[8 * x + 2 * e + 1]) * inv);
+                        const int chunk = 4 * q + x;
+                        *reinterpret_cast<uint4*>(stage_out + lane * (DP * 2) + ((chunk ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            if (!split) {
+                __syncwarp();
+                constexpr int kLanes = DP / 8;      // lanes that hold a row
+                __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.c.o);
+#pragma unroll 4
+                for (int x = lane / kLanes; x < 32; x += 32 / kLanes) {
+                    const int chunk = lane % kLanes, wr = 128 * t + 32 * (warp & 3) + x;
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage_out + x * (DP * 2) + ((chunk ^ (x & 7)) << 4));
+                    if (wr < u.rows && 8 * chunk < D) {
+                        const int pr = u.row0 + wr, tk = pr / g;
+                        *reinterpret_cast<uint4*>(o + ((size_t)(u.first + tk) * a.c.heads.q_heads + hk * g + pr - tk * g) * D + 8 * chunk) = v;
+                    }
+                }
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        if (warp == kMmaWarp) {
+            // -------------------------------------------------------------- products
+            if (t_begin < t_end && elect_one()) {
+                const uint32_t s0 = smem_u32(sm);
+                constexpr uint32_t idS = umma_idesc_bf16(128, 128, kMajorK, kMajorK), idO = umma_idesc_bf16(128, DP, kMajorK, kMajorMN);
+                bool ok = wait(bar_q, 0);
+                auto in = [&](int t, int j) { return j >= range[t].begin && j < range[t].end; };
+                auto scores = [&](int t, int j, int i) {      // S_t = Q_t K_j^T
+                    const UmmaDesc q = umma_smem_desc_sw128(s0 + t * L::kTile, 16, 1024), k = umma_smem_desc_sw128(s0 + L::kRing + stage(i) * L::kTile, 16, 1024);
+#pragma unroll
+                    for (int x = 0; x < DP / 16; ++x) {
+                        const uint32_t off = (x >> 2) * 16384 + (x & 3) * 32;
+                        umma_bf16_ss(tmem + cS + 128 * t, q + off, k + off, idS, x > 0);
+                    }
+                    umma_commit(bar_s + t);
+                };
+                if (ok) ok = wait(bar_full + stage(0), turn(0));
+                if (ok) {
+                    tc_fence_after();
+                    for (int t = 0; t < 2; ++t)
+                        if (in(t, t_begin)) scores(t, t_begin, 0);
+                    umma_commit(bar_free + stage(0));
+                }
+                for (int j = t_begin; j < t_end && ok; ++j) {
+                    const int iv = 2 * (j - t_begin) + 1, ik = iv + 1;      // places of V_j and K_j+1 in the ring
+                    ok = wait(bar_full + stage(iv), turn(iv));
+                    if (ok && j + 1 < t_end) ok = wait(bar_full + stage(ik), turn(ik));
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        if (in(t, j)) {
+                            const int i = j - range[t].begin;
+                            ok = wait(bar_p + t, i & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const UmmaDesc v = umma_smem_desc_sw128(s0 + L::kRing + stage(iv) * L::kTile, 16384, 1024);
+#pragma unroll
+                            for (int x = 0; x < 8; ++x)      // O_t += P_t V_j
+                                umma_bf16_ts(tmem + cO + DP * t, tmem + cS + 128 * t + 8 * x, v + (x * 2048), idO, i > 0 || x > 0);
+                            umma_commit(bar_o + t);
+                        }
+                        if (j + 1 < t_end && in(t, j + 1)) scores(t, j + 1, ik);
+                    }
+                    if (ok) {
+                        umma_commit(bar_free + stage(iv));
+                        if (j + 1 < t_end) umma_commit(bar_free + stage(ik));
+                    }
+                }
+                // no product may be in flight when the block ends
+                umma_commit(bar_end);
+                wait(bar_end, 0);
+            }
+        } else if (warp == kLoadWarp) {
+            // -------------------------------------------------------------- K and V, a box a lane
+            constexpr int kHalves = DP / 64;
+            const int boxes = kKeys / a.box_rows, box = lane / kHalves, half = lane - box * kHalves;
+            const uint32_t box_bytes = (uint32_t)a.box_rows * 128;
+            bool ok = true;
+            const int total = 2 * (t_end - t_begin);
+            auto look = [&](int j, int& row) {      // page of this lane's box, -1: nothing to load
+                const int key = j * kKeys + box * a.box_rows;
+                if (box >= boxes || j >= t_end || key >= u.hi || key + a.box_rows <= u.lo) return -1;
+                const int col = key / b.page_size;
+                row = key - col * b.page_size;
+                const int page = b.page(u.n, col);
+                if (page < 0) b.tell(KDA_ERR_BLOCK_TABLE);
+                return page;
+            };
+            int row = 0, next_row = 0, page = look(t_begin, row), next_page = -1, i = 0;
+            for (; i < total; ++i) {
+                const int j = t_begin + (i >> 1), s = stage(i);
+                const bool isv = i & 1;
+                if (i >= L::kStages) ok = wait(bar_free + s, turn(i - L::kStages));
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                if (!isv) next_page = look(j + 1, next_row);
+                uint64_t* f = isv && partial(j) ? bar_part + s : bar_full + s;
+                const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
+                if (lane == 0) mbar_expect_tx(f, loads * box_bytes);
+                __syncwarp();
+                if (page >= 0) {
+                    const CUtensorMap* map = isv ? &mV : &mK;
+                    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+                                     smem_u32(sm + L::kRing + s * L::kTile + half * 16384 + box * box_bytes)),
+                                 "l"(map), "r"(smem_u32(f)), "r"(half * 64), "r"(row), "r"(hk), "r"(page)
+                                 : "memory");
+                }
+                if (isv) {
+                    page = next_page;
+                    row = next_row;
+                }
+            }
+            // no copy may be in flight when the block ends
+            if (!ok && lane == 0)
+                for (int x = i > L::kStages ? i - L::kStages : 0; x < i; ++x)
+                    mbar_poll((x & 1) && partial(t_begin + (x >> 1)) ? bar_part + stage(x) : bar_full + stage(x), turn(x), kSpinLimit / 8);
+        } else {
+            // -------------------------------------------------------------- V tiles that some row sees only in part
+            uint32_t phase = 0;      // of each stage's barrier
+            bool odd = false;
+            for (int j = t_begin; j < t_end; ++j) {
+                if (!partial(j)) continue;
+                const int i = 2 * (j - t_begin) + 1, s = stage(i);
+                bool ok = wait(bar_part + s, (phase >> s) & 1u);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                phase ^= 1u << s;
+                uint8_t* v = sm + L::kRing + s * L::kTile;
+                for (int e = tid - kFixWarp * 32; e < kKeys * DP / 8; e += 64) {
+                    const int r = e & 127, ch = e >> 7, key = j * kKeys + r;
+                    if (key >= all_lo && key < all_hi) continue;
+                    uint4* at = reinterpret_cast<uint4*>(v + (ch >> 3) * 16384 + sw128_off(r, ch & 7));
+                    if (key < u.lo || key >= u.hi) {
+                        *at = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    uint4 x = *at;
+                    if (!(finite_bf16x2(x.x) && finite_bf16x2(x.y) && finite_bf16x2(x.z) && finite_bf16x2(x.w))) {
+                        odd = true;
+                        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u;
+                            if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu;
+                        }
+                        *at = x;
+                    }
+                }
+                if (odd) odd_values = 1;
+                __threadfence_block();
+                fence_async_smem();
+                asm volatile("bar.sync 1, 64;" ::: "memory");
+                if (tid == kFixWarp * 32) mbar_arrive(bar_full + s);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+}
+
+template <int DP>
+int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, Args& a, cudaStream_t st) {
+    if (int rc = set_smem_limit(attn_tc_kernel<DP>, Layout<DP>::kBytes)) return rc;
+    const dim3 grid((unsigned)a.slots, (unsigned)c.heads.kv_heads, (unsigned)a.splits);
+    KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, a));
+    return launch_status();
+}
+
+}  // namespace
+
+
+
+bool tc_takes(const Call& c) {
+    const Strides& s = c.strides;
+    const int page = c.batch.page_size;
+    if (!c.bf16 || c.heads.dim > 128 || c.heads.dim % 8 != 0 || !(page % kKeys == 0 || (kKeys % page == 0 && page >= 8))) return false;
+    if (c.batch.n_pages == 0 || c.batch.table_width == 0) return false;
+    const long long all = s.k_page | s.k_row | s.k_head | s.v_page | s.v_row | s.v_head;
+    if (all % 8 != 0 || reinterpret_cast<uintptr_t>(c.k) % 16 != 0 || reinterpret_cast<uintptr_t>(c.v) % 16 != 0 || reinterpret_cast<uintptr_t>(c.o) % 16 != 0)
+        return false;
+    for (long long x : {s.k_page, s.k_row, s.k_head, s.v_page, s.v_row, s.v_head})
+        if (x <= 0 || x >= 1ll << 39) return false;
+    return true;
+}
+
+int tc(const Call& c, int splits, cudaStream_t st) {
+    Args a;
+    a.c = c;
+    a.tiles = Tiles{kRows, c.heads.group, 0};
+    a.slots = (int)tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq);
+    a.splits = splits;
+    a.box_rows = c.batch.page_size < kKeys ? c.batch.page_size : kKeys;
+    a.q16 = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.strides.q_token % 8 == 0 && c.strides.q_head % 8 == 0;
+    const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
+    a.part_ml = static_cast<float2*>(c.workspace);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * splits * sizeof(float2), 256));
+    CUtensorMap mK, mV;
+    const Strides& s = c.strides;
+    int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
+    if (!rc) rc = make_map_paged(&mV, c.v, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.v_row, s.v_head, s.v_page, a.box_rows);
+    if (!rc) rc = c.heads.dim <= 64 ? launch<64>(c, mK, mV, a, st) : launch<128>(c, mK, mV, a, st);
+    if (rc || splits == 1) return rc;
+    return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, splits, a.part_o, a.part_ml, c.o, c.lse, c.bf16}, st);
+}
+
+}  // namespace attn
+}  // namespace kda

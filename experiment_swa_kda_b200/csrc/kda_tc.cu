@@ -29,6 +29,22 @@ static EncodeFn encode_fn() {
     return fn;
 }
 
+static CUresult encode(EncodeFn enc, CUtensorMap* m, uint32_t rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                       const cuuint32_t* es) {
+    auto call = [&]() {
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = call();
+    if (r == CUDA_ERROR_INVALID_CONTEXT) {
+        // a host thread that has made no runtime call yet (e.g. an autograd worker) has no context bound:
+        // bind the current device's primary context and try once more
+        int dev = 0;
+        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && cudaFree(nullptr) == cudaSuccess) r = call();
+    }
+    return r;
+}
+
 // 2-D bf16 row-major tensor [rows][cols]; box = box_cols x box_rows; 128-byte swizzle (box_cols must be 64).
 // Rows are `ld` elements apart (a multiple of 8).
 int make_map_bf16_ld(CUtensorMap* m, const void* ptr, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows) {
@@ -38,18 +54,7 @@ int make_map_bf16_ld(CUtensorMap* m, const void* ptr, uint64_t rows, uint64_t co
     cuuint64_t strides[1] = {ld * 2};
     cuuint32_t box[2] = {box_cols, box_rows};
     cuuint32_t es[2] = {1, 1};
-    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r == CUDA_ERROR_INVALID_CONTEXT) {
-        // a host thread that has made no runtime call yet (e.g. an autograd worker) has no context bound:
-        // bind the current device's primary context and try once more
-        int dev = 0;
-        if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && cudaFree(nullptr) == cudaSuccess)
-            r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, es,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    }
+    const CUresult r = encode(enc, m, 2, ptr, dims, strides, box, es);
     if (r != CUDA_SUCCESS && getenv("KDA_B200_VERBOSE"))
         fprintf(stderr, "libkda_b200: cuTensorMapEncodeTiled failed (%d): ptr %p rows %llu cols %llu box %u x %u\n", (int)r, ptr,
                 (unsigned long long)rows, (unsigned long long)cols, box_cols, box_rows);
@@ -58,6 +63,20 @@ int make_map_bf16_ld(CUtensorMap* m, const void* ptr, uint64_t rows, uint64_t co
 
 int make_map_bf16(CUtensorMap* m, const void* ptr, uint64_t rows, uint64_t cols, uint32_t box_cols, uint32_t box_rows) {
     return make_map_bf16_ld(m, ptr, rows, cols, cols, box_cols, box_rows);
+}
+
+// Paged cache [pages][heads][rows][dim] at the strides given (in elements); a box is 64 values of box_rows rows of one head and
+// page, so that a value past the head's width reads as 0.
+int make_map_paged(CUtensorMap* m, const void* ptr, uint64_t dim, uint64_t rows, uint64_t heads, uint64_t pages, int64_t row_ld, int64_t head_ld, int64_t page_ld,
+                   uint32_t box_rows) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return KDA_ERR_CUDA;
+    const cuuint64_t dims[4] = {dim, rows, heads, pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)row_ld * 2, (cuuint64_t)head_ld * 2, (cuuint64_t)page_ld * 2};
+    const cuuint32_t box[4] = {64, box_rows, 1, 1}, es[4] = {1, 1, 1, 1};
+    const CUresult r = encode(enc, m, 4, ptr, dims, strides, box, es);
+    if (r != CUDA_SUCCESS && getenv("KDA_B200_VERBOSE")) fprintf(stderr, "libkda_b200: cuTensorMapEncodeTiled failed (%d) for a paged cache\n", (int)r);
+    return r == CUDA_SUCCESS ? KDA_OK : KDA_ERR_CUDA;
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -62,6 +62,22 @@ struct Batch {
         }
         return lo;
     }
+    // The same by LANES converged lanes (lane l of them, `mask` in the warp): the place where t would lie in a batch of equal
+    // lengths is looked at first, then LANES places at a time.
+    template <int LANES>
+    __device__ __forceinline__ int seq_of(int t, int l, unsigned mask) const {
+        if (cu == nullptr) return t / q_len;
+        const int guess = (int)((long long)t * n_seq / tokens);
+        if (__ldg(cu + guess) <= t && t < __ldg(cu + guess + 1)) return guess;
+        int lo = 0, hi = n_seq;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + LANES - 1) / LANES, at = lo + step * l;
+            const unsigned below = __ballot_sync(mask, at < hi && __ldg(cu + at) <= t) & mask;
+            lo += step * max(__popc(below) - 1, 0);
+            hi = min(hi, lo + step);
+        }
+        return lo;
+    }
 };
 
 // Tiles of `rows` packed rows (token-major, the query heads of one kv head beside each other) of all sequences.  With a bound

@@ -7,6 +7,11 @@
 //
 // Everything is float32 between the load and the one rounding of the store.  r is formed again in the backward: it costs a sum
 // over values that are in registers anyway, a saved one would be read.
+//
+// Bound by memory.  Two forms each way: norm_rope_rows_* for widths, strides and addresses that allow 16-byte accesses, and
+// norm_rope_kernel / norm_rope_bwd_kernel for all others.
+
+#include <initializer_list>
 
 #include "attn.cuh"
 
@@ -15,6 +20,7 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kBwdBlocks = 4;      // blocks an SM of the backward: each leaves one part of the weights' gradients
 
 struct Rope {
     KdaRotaryShape s;
@@ -28,6 +34,7 @@ struct Rope {
     Batch batch;                    // append
     Strides cache;
     int* mirror;
+    int slice, slices;              // norm_rope_rows_*: heads of a token a group of lanes takes, and groups a token has
 };
 
 // Where a token goes: its position, and the cache rows of its key and value (append).
@@ -36,12 +43,12 @@ struct Place {
     long long k_at, v_at;           // element offsets of the page's row, or -1: no page
 };
 
-template <bool APPEND>
-__device__ __forceinline__ Place place_of(const Rope& p, int t) {
+template <bool APPEND, int LANES = 1>
+__device__ __forceinline__ Place place_of(const Rope& p, int t, int l = 0, unsigned mask = 0) {
     Place r;
     if (APPEND) {
         const Batch& b = p.batch;
-        const int n = b.seq_of(t);
+        const int n = LANES > 1 ? b.seq_of<LANES>(t, l, mask) : b.seq_of(t);
         int first, count;
         b.span(n, first, count);
         r.pos = b.kv_len(n) - count + (t - first);
@@ -210,15 +217,329 @@ __global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(Rope p) {
     }
 }
 
-// Sums of the blocks' parts, in their order: a warp a column.
-__global__ void __launch_bounds__(kThreads) norm_rope_dw_kernel(int blocks, int D, const float* part, float* dq_weight, float* dk_weight) {
-    const int e = blockIdx.x * kWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (e >= 2 * D) return;
+// ---------------------------------------------------------------------------------------------- 16-byte accesses
+// Eight adjacent values a lane, LANES lanes a row.  A group of lanes takes a token's heads one after the other - all of them, or a
+// slice where there are too few tokens to fill the machine -, so that the token's place, its cosines and sines and the
+// weights are read once for all of them.  In the split order a pair's members lie in two lanes and change places by shuffle, as
+// they were loaded: bf16 pairs in one word.
+
+template <bool BF16>
+struct Vec8 {
+    uint4 a, b;      // b: float32 only
+};
+template <bool BF16>
+__device__ __forceinline__ Vec8<BF16> ld8(const void* p, long long at) {
+    Vec8<BF16> r;
+    if (BF16) {
+        r.a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at));
+    } else {
+        const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at);
+        r.a = __ldg(s);
+        r.b = __ldg(s + 1);
+    }
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack(const Vec8<BF16>& v, f2 (&x)[4]) {
+    if (BF16) {
+        x[0] = f2_from_bf16(v.a.x); x[1] = f2_from_bf16(v.a.y); x[2] = f2_from_bf16(v.a.z); x[3] = f2_from_bf16(v.a.w);
+    } else {
+        x[0] = f2_make(__uint_as_float(v.a.x), __uint_as_float(v.a.y));
+        x[1] = f2_make(__uint_as_float(v.a.z), __uint_as_float(v.a.w));
+        x[2] = f2_make(__uint_as_float(v.b.x), __uint_as_float(v.b.y));
+        x[3] = f2_make(__uint_as_float(v.b.z), __uint_as_float(v.b.w));
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ void st8(void* p, long long at, const f2 (&x)[4]) {
+    if (BF16) {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) = make_uint4(f2_to_bf16(x[0]), f2_to_bf16(x[1]), f2_to_bf16(x[2]), f2_to_bf16(x[3]));
+    } else {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+        const float2 a = f2_get(x[0]), b = f2_get(x[1]), c = f2_get(x[2]), e = f2_get(x[3]);
+        d[0] = make_float4(a.x, a.y, b.x, b.y);
+        d[1] = make_float4(c.x, c.y, e.x, e.y);
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ Vec8<BF16> shuffle(const Vec8<BF16>& v, int src, int lanes, unsigned mask) {
+    Vec8<BF16> r;
+    r.a = make_uint4(__shfl_sync(mask, v.a.x, src, lanes), __shfl_sync(mask, v.a.y, src, lanes), __shfl_sync(mask, v.a.z, src, lanes),
+                     __shfl_sync(mask, v.a.w, src, lanes));
+    if (!BF16)
+        r.b = make_uint4(__shfl_sync(mask, v.b.x, src, lanes), __shfl_sync(mask, v.b.y, src, lanes), __shfl_sync(mask, v.b.z, src, lanes),
+                         __shfl_sync(mask, v.b.w, src, lanes));
+    return r;
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float x, unsigned mask) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
+    return x;
+}
+
+// A lane's share of a row: its values, where their partners are, their weights and the partners'.
+template <int LANES, bool INTER>
+struct Lane {
+    int l, d, src;                  // lane of the group, its first value, lane that holds the partners
+    bool on, turned;                // the row has these values; they are rotated
+    unsigned mask;
+    int at;                         // first of its cosines
+    float sign;                     // of the sine in y (split order)
+
+    __device__ __forceinline__ Lane(const KdaRotaryShape& s) {
+        const int lane = threadIdx.x & 31;
+        l = lane & (LANES - 1);
+        mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (lane & ~(LANES - 1));
+        d = 8 * l;
+        on = d < s.head_dim;
+        turned = d < s.rotary_dim;
+        src = l;
+        at = INTER ? d / 2 : 0;
+        sign = 0.f;
+        if (!INTER && turned) {
+            const int half = s.rotary_dim / 2;
+            src = d < half ? l + half / 8 : l - half / 8;
+            at = d < half ? d : d - half;
+            sign = d < half ? -1.f : 1.f;
+        }
+    }
+    // y_e = u_e c_e + u_other s_e for the lane's values
+    __device__ __forceinline__ void angles(const Rope& p, int pos, f2 (&c)[4], f2 (&s)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            c[i] = f2_all(1.f);
+            s[i] = f2_all(0.f);
+        }
+        if (!turned) return;
+        const float* pc = p.cos + (size_t)pos * (p.s.rotary_dim / 2) + at;
+        const float* ps = p.sin + (size_t)pos * (p.s.rotary_dim / 2) + at;
+        const float4 c0 = __ldg(reinterpret_cast<const float4*>(pc)), s0 = __ldg(reinterpret_cast<const float4*>(ps));
+        if (INTER) {
+            c[0] = f2_all(c0.x); c[1] = f2_all(c0.y); c[2] = f2_all(c0.z); c[3] = f2_all(c0.w);
+            s[0] = f2_make(-s0.x, s0.x); s[1] = f2_make(-s0.y, s0.y); s[2] = f2_make(-s0.z, s0.z); s[3] = f2_make(-s0.w, s0.w);
+        } else {
+            const float4 c1 = __ldg(reinterpret_cast<const float4*>(pc) + 1), s1 = __ldg(reinterpret_cast<const float4*>(ps) + 1);
+            c[0] = f2_make(c0.x, c0.y); c[1] = f2_make(c0.z, c0.w); c[2] = f2_make(c1.x, c1.y); c[3] = f2_make(c1.z, c1.w);
+            s[0] = f2_make(sign * s0.x, sign * s0.y); s[1] = f2_make(sign * s0.z, sign * s0.w);
+            s[2] = f2_make(sign * s1.x, sign * s1.y); s[3] = f2_make(sign * s1.z, sign * s1.w);
+        }
+    }
+    // the weights of values d .. d + 7, 1 without weights
+    __device__ __forceinline__ void weights(const float* w, int d0, f2 (&x)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = f2_all(1.f);
+        if (w == nullptr || !on) return;
+        const float4 a = __ldg(reinterpret_cast<const float4*>(w + d0)), b = __ldg(reinterpret_cast<const float4*>(w + d0) + 1);
+        x[0] = f2_make(a.x, a.y); x[1] = f2_make(a.z, a.w); x[2] = f2_make(b.x, b.y); x[3] = f2_make(b.z, b.w);
+    }
+    // the partners of a lane's values
+    template <bool BF16>
+    __device__ __forceinline__ void other(const Vec8<BF16>& v, const f2 (&x)[4], f2 (&o)[4]) const {
+        if (INTER) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 t = f2_get(x[i]);
+                o[i] = f2_make(t.y, t.x);
+            }
+        } else {
+            unpack<BF16>(shuffle<BF16>(v, src, LANES, mask), o);
+        }
+    }
+};
+
+__device__ __forceinline__ float f2_sum(const f2 (&x)[4], const f2 (&y)[4]) {
+    const float2 t = f2_get(f2_fma(x[0], y[0], f2_fma(x[1], y[1], f2_fma(x[2], y[2], f2_mul(x[3], y[3])))));
+    return t.x + t.y;
+}
+
+constexpr int kAhead = 4;      // rows whose loads are in flight together
+
+// `heads` rows of one token from `from` on, head_stride apart, to `to`, to_stride apart
+template <int LANES, bool BF16, bool INTER>
+__device__ __forceinline__ void turn_rows(const Lane<LANES, INTER>& ln, const KdaRotaryShape& sh, const void* src, long long from, long long from_stride, void* dst,
+                                          long long to, long long to_stride, int heads, const f2 (&a)[4], const f2 (&b)[4]) {
+    for (int h = 0; h < heads; h += kAhead) {
+        Vec8<BF16> v[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            v[i].a = v[i].b = make_uint4(0, 0, 0, 0);
+            if (ln.on && h + i < heads) v[i] = ld8<BF16>(src, from + (h + i) * from_stride + ln.d);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (h + i >= heads) break;      // the same for all lanes of the group
+            f2 x[4], o[4];
+            unpack<BF16>(v[i], x);
+            ln.template other<BF16>(v[i], x, o);
+            const float r = rsqrtf(group_sum<LANES>(f2_sum(x, x), ln.mask) / sh.head_dim + sh.eps);
+            const f2 r2 = f2_all(r);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = f2_mul(f2_fma(x[k], a[k], f2_mul(o[k], b[k])), r2);
+            if (ln.on) st8<BF16>(dst, to + (h + i) * to_stride + ln.d, x);
+        }
+    }
+}
+
+template <int LANES, bool BF16, bool INTER, bool APPEND>
+__global__ void __launch_bounds__(kThreads) norm_rope_rows_kernel(Rope p) {
+    constexpr int kGroups = kThreads / LANES;
+    const Lane<LANES, INTER> ln(p.s);
+    const int Hq = p.s.q_heads, Hk = p.s.kv_heads, all = Hq + Hk + (APPEND ? Hk : 0), D = p.s.head_dim;
+    const long long units = (long long)p.s.tokens * p.slices;
+    for (long long unit = (long long)blockIdx.x * kGroups + threadIdx.x / LANES; unit < units; unit += (long long)gridDim.x * kGroups) {
+        const int t = (int)(unit / p.slices), h0 = (int)(unit - (long long)t * p.slices) * p.slice, h1 = min(h0 + p.slice, all);
+        const Place at = place_of<APPEND, LANES>(p, t, ln.l, ln.mask);
+        f2 c[4], s[4];
+        ln.angles(p, max(at.pos, 0), c, s);
+        // y = r (x (w c) + x_other (w_other s))
+        auto coefficients = [&](const float* w, f2 (&a)[4], f2 (&b)[4]) {
+            f2 own[4], other[4];
+            ln.weights(w, ln.d, own);
+            if (INTER) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 x = f2_get(own[i]);
+                    other[i] = f2_make(x.y, x.x);
+                }
+            } else {
+                ln.weights(w, 8 * ln.src, other);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] = f2_mul(own[i], c[i]);
+                b[i] = f2_mul(other[i], s[i]);
+            }
+        };
+        f2 a[4], b[4];
+        if (h0 < Hq) {
+            const int n = min(h1, Hq) - h0;
+            const long long to = ((long long)t * Hq + h0) * D;
+            if (APPEND && at.pos < 0) {
+                const f2 none[4] = {f2_all(0.f), f2_all(0.f), f2_all(0.f), f2_all(0.f)};
+                for (int h = 0; h < n; ++h)
+                    if (ln.on) st8<BF16>(p.q_out, to + (long long)h * D + ln.d, none);
+            } else {
+                coefficients(p.q_weight, a, b);
+                turn_rows<LANES, BF16>(ln, p.s, p.q, t * p.s.q_token_stride + h0 * p.s.q_head_stride, p.s.q_head_stride, p.q_out, to, D, n, a, b);
+            }
+        }
+        if (APPEND && (at.pos < 0 || at.k_at < 0)) continue;
+        const int k0 = max(h0 - Hq, 0), k1 = min(h1 - Hq, Hk);
+        if (k0 < k1) {
+            coefficients(p.k_weight, a, b);
+            turn_rows<LANES, BF16>(ln, p.s, p.k, t * p.s.k_token_stride + k0 * p.s.k_head_stride, p.s.k_head_stride, p.k_out,
+                                   APPEND ? at.k_at + k0 * p.cache.k_head : ((long long)t * Hk + k0) * D, APPEND ? p.cache.k_head : D, k1 - k0, a, b);
+        }
+        if (APPEND && ln.on) {      // values go as they are
+            for (int v = max(h0 - Hq - Hk, 0); v < h1 - Hq - Hk; ++v) {
+                f2 x[4];
+                unpack<BF16>(ld8<BF16>(p.v, t * p.s.v_token_stride + v * p.s.v_head_stride + ln.d), x);
+                st8<BF16>(p.v_out, at.v_at + v * p.cache.v_head + ln.d, x);
+            }
+        }
+    }
+}
+
+// The same rows backward; each lane sums its weights' gradients over all rows it meets, a block over its lanes, and
+// norm_rope_dw_kernel over the blocks, all in a fixed order.
+template <int LANES, bool BF16, bool INTER>
+__global__ void __launch_bounds__(kThreads) norm_rope_rows_bwd_kernel(Rope p) {
+    constexpr int kGroups = kThreads / LANES, kRowsAhead = BF16 ? 2 : 1;
+    dependents_go();
+    const Lane<LANES, INTER> ln(p.s);
+    const int Hq = p.s.q_heads, Hk = p.s.kv_heads, all = Hq + Hk, D = p.s.head_dim;
+    const long long units = (long long)p.s.tokens * p.slices;
+    f2 dw[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dw[0][i] = dw[1][i] = f2_all(0.f);
+    for (long long unit = (long long)blockIdx.x * kGroups + threadIdx.x / LANES; unit < units; unit += (long long)gridDim.x * kGroups) {
+        const int t = (int)(unit / p.slices), h0 = (int)(unit - (long long)t * p.slices) * p.slice, h1 = min(h0 + p.slice, all);
+        const Place at = place_of<false>(p, t);
+        f2 c[4], s[4];
+        ln.angles(p, at.pos, c, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = f2_mul(s[i], f2_all(-1.f));      // the transposed rotation
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const int H = which ? Hk : Hq, a0 = which ? max(h0 - Hq, 0) : h0, a1 = which ? h1 - Hq : min(h1, Hq);
+            if (a0 >= a1) continue;
+            const long long ts = which ? p.s.k_token_stride : p.s.q_token_stride, hs = which ? p.s.k_head_stride : p.s.q_head_stride;
+            const void *src = which ? p.k : p.q, *grad = which ? p.d_k : p.d_q;
+            void* dst = which ? p.k_out : p.q_out;
+            const float* w = which ? p.k_weight : p.q_weight;
+            f2 own[4];
+            ln.weights(w, ln.d, own);
+            for (int h = a0; h < a1; h += kRowsAhead) {
+                Vec8<BF16> xv[kRowsAhead], gv[kRowsAhead];
+#pragma unroll
+                for (int i = 0; i < kRowsAhead; ++i) {
+                    xv[i].a = xv[i].b = gv[i].a = gv[i].b = make_uint4(0, 0, 0, 0);
+                    if (ln.on && h + i < a1) {
+                        xv[i] = ld8<BF16>(src, t * ts + (h + i) * hs + ln.d);
+                        gv[i] = ld8<BF16>(grad, ((long long)t * H + h + i) * D + ln.d);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kRowsAhead; ++i) {
+                    if (h + i >= a1) break;
+                    f2 x[4], du[4], o[4];
+                    unpack<BF16>(xv[i], x);
+                    unpack<BF16>(gv[i], du);
+                    ln.template other<BF16>(gv[i], du, o);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) du[k] = f2_fma(du[k], c[k], f2_mul(o[k], s[k]));
+                    const float ss = group_sum<LANES>(f2_sum(x, x), ln.mask);
+                    const float r = rsqrtf(ss / D + p.s.eps);
+                    const f2 r2 = f2_all(r);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        dw[which][k] = f2_fma(f2_mul(du[k], x[k]), r2, dw[which][k]);
+                        du[k] = f2_mul(du[k], own[k]);
+                    }
+                    const f2 f = f2_all(-r * r * group_sum<LANES>(f2_sum(du, x), ln.mask) / D);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) du[k] = f2_mul(f2_fma(x[k], f, du[k]), r2);
+                    if (ln.on) st8<BF16>(dst, ((long long)t * H + h + i) * D + ln.d, du);
+                }
+            }
+        }
+    }
+    if (p.part == nullptr) return;
+    __shared__ float sum[kGroups][8 * LANES];
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sum[threadIdx.x / LANES][ln.d + 2 * k]) = f2_get(dw[which][k]);
+        __syncthreads();
+        for (int d = threadIdx.x; d < D; d += kThreads) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < kGroups; ++k) v += sum[k][d];
+            p.part[((size_t)blockIdx.x * 2 + which) * D + d] = v;
+        }
+    }
+}
+
+// Sums of the blocks' parts: 32 columns a block, each warp a share of the parts in their order, then the warps in theirs.
+__global__ void __launch_bounds__(1024) norm_rope_dw_kernel(int blocks, int D, const float* part, float* dq_weight, float* dk_weight) {
+    __shared__ float sum[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+    dependency_wait();
     float s = 0.f;
-    for (int i = lane; i < blocks; i += 32) s += part[(size_t)i * 2 * D + e];
-    s = warp_sum(s);
-    float* out = e < D ? dq_weight : dk_weight;
-    if (lane == 0 && out != nullptr) out[e < D ? e : e - D] = s;
+    if (e < 2 * D)
+#pragma unroll 8
+        for (int i = warp; i < blocks; i += 32) s += ld_after_f32(part + (size_t)i * 2 * D + e);
+    sum[warp][lane] = s;
+    __syncthreads();
+    if (warp == 0 && e < 2 * D) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += sum[i][lane];
+        float* out = e < D ? dq_weight : dk_weight;
+        if (out != nullptr) out[e < D ? e : e - D] = s;
+    }
 }
 
 int check(const KdaRotaryShape* s) {
@@ -230,10 +551,60 @@ int check(const KdaRotaryShape* s) {
     return KDA_OK;
 }
 
-int blocks_for(long long rows) {
-    const long long most = 148 * 8, want = (rows + kWarps - 1) / kWarps;
+int blocks_for(long long units, int per_block, int per_sm) {
+    const long long most = 148ll * per_sm, want = (units + per_block - 1) / per_block;
     return (int)(want < 1 ? 1 : want < most ? want : most);
 }
+
+bool on16(std::initializer_list<const void*> ps) {
+    uintptr_t a = 0;
+    for (const void* p : ps) a |= reinterpret_cast<uintptr_t>(p);
+    return a % 16 == 0;
+}
+// Whether rows can be taken in pieces of eight values: the width, what is rotated, and every address and stride.
+bool rows8(const Rope& p, std::initializer_list<long long> strides) {
+    const KdaRotaryShape& s = p.s;
+    const int unit = s.io_dtype == KDA_DTYPE_BF16 ? 8 : 4;      // elements in 16 bytes
+    long long all = 0;
+    for (long long x : strides) all |= x;
+    return s.head_dim % 8 == 0 && s.rotary_dim % (s.interleaved ? 8 : 16) == 0 && all % unit == 0 &&
+           on16({p.q, p.k, p.v, p.cos, p.sin, p.q_weight, p.k_weight, p.q_out, p.k_out, p.v_out, p.d_q, p.d_k});
+}
+int lanes_for(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+// Heads of a token a group takes: all of them while that still gives every SM its threads, a part otherwise.
+void slice_heads(Rope& p, int heads, int lanes) {
+    const long long groups = 148ll * 2048 / lanes;
+    long long n = groups / (p.s.tokens > 0 ? p.s.tokens : 1);
+    if (n < 1) n = 1;
+    if (n > heads) n = heads;
+    p.slice = (int)((heads + n - 1) / n);
+    p.slices = (heads + p.slice - 1) / p.slice;
+}
+template <template <int, bool, bool> class K>
+void by_shape(const Rope& p, int blocks, cudaStream_t st) {
+    const bool bf = p.s.io_dtype == KDA_DTYPE_BF16, in = p.s.interleaved != 0;
+    const int lanes = lanes_for(p.s.head_dim);
+#define KDA_ROPE_CASE(L)                                                                                             \
+    if (lanes == L) {                                                                                                \
+        if (bf) in ? K<L, true, true>::run(p, blocks, st) : K<L, true, false>::run(p, blocks, st);                   \
+        else in ? K<L, false, true>::run(p, blocks, st) : K<L, false, false>::run(p, blocks, st);                    \
+    }
+    KDA_ROPE_CASE(8) KDA_ROPE_CASE(16) KDA_ROPE_CASE(32)
+#undef KDA_ROPE_CASE
+
+}
+template <int L, bool B, bool I>
+struct RunForward {
+    static void run(const Rope& p, int blocks, cudaStream_t st) { norm_rope_rows_kernel<L, B, I, false><<<blocks, kThreads, 0, st>>>(p); }
+};
+template <int L, bool B, bool I>
+struct RunAppend {
+    static void run(const Rope& p, int blocks, cudaStream_t st) { norm_rope_rows_kernel<L, B, I, true><<<blocks, kThreads, 0, st>>>(p); }
+};
+template <int L, bool B, bool I>
+struct RunBackward {
+    static void run(const Rope& p, int blocks, cudaStream_t st) { norm_rope_rows_bwd_kernel<L, B, I><<<blocks, kThreads, 0, st>>>(p); }
+};
 
 Rope fill(const KdaRotaryShape& s, const void* q, const void* k, const float* cos, const float* sin, const void* positions, const float* qw, const float* kw) {
     Rope p = {};
@@ -259,14 +630,21 @@ extern "C" int kda_norm_rope_fwd(const KdaRotaryShape* s, const void* q, const v
     Rope p = fill(*s, q, k, cos, sin, positions, q_weight, k_weight);
     p.q_out = q_out; p.k_out = k_out;
     cudaStream_t st = (cudaStream_t)stream;
-    const int blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads));
+    if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride})) {
+        const int lanes = lanes_for(s->head_dim);
+        slice_heads(p, s->q_heads + s->kv_heads, lanes);
+        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, 16);
+        KDA_LAUNCH("norm_rope_rows_kernel", st, by_shape<RunForward>(p, blocks, st));
+        return launch_status();
+    }
+    const int blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), kWarps, 8);
     KDA_LAUNCH("norm_rope_kernel", st, norm_rope_kernel<false><<<blocks, kThreads, 0, st>>>(p));
     return launch_status();
 }
 
 extern "C" size_t kda_norm_rope_bwd_scratch_bytes(const KdaRotaryShape* s) {
     if (check(s)) return 0;
-    return align_up((size_t)blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads)) * 2 * s->head_dim * sizeof(float), 256);
+    return align_up((size_t)blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), 1, kBwdBlocks) * 2 * s->head_dim * sizeof(float), 256);
 }
 
 extern "C" int kda_norm_rope_bwd(const KdaRotaryShape* s, const void* q, const void* k, const float* cos, const float* sin, const void* positions,
@@ -283,13 +661,22 @@ extern "C" int kda_norm_rope_bwd(const KdaRotaryShape* s, const void* q, const v
     Rope p = fill(*s, q, k, cos, sin, positions, q_weight, k_weight);
     p.q_out = dq; p.k_out = dk; p.d_q = d_q_out; p.d_k = d_k_out;
     p.part = sums ? static_cast<float*>(scratch) : nullptr;
-    const int blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads));
-    KDA_LAUNCH("norm_rope_bwd_kernel", st, norm_rope_bwd_kernel<<<blocks, kThreads, 0, st>>>(p));
+    int blocks;
+    if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride})) {
+        const int lanes = lanes_for(s->head_dim);
+        slice_heads(p, s->q_heads + s->kv_heads, lanes);
+        blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, kBwdBlocks);
+        KDA_LAUNCH("norm_rope_rows_bwd_kernel", st, by_shape<RunBackward>(p, blocks, st));
+    } else {
+        blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), kWarps, kBwdBlocks);
+        KDA_LAUNCH("norm_rope_bwd_kernel", st, norm_rope_bwd_kernel<<<blocks, kThreads, 0, st>>>(p));
+    }
     if (int rc = launch_status()) return rc;
     if (!sums) return KDA_OK;
+    cudaError_t e = cudaSuccess;
     KDA_LAUNCH("norm_rope_dw_kernel", st,
-               norm_rope_dw_kernel<<<(2 * s->head_dim + kWarps - 1) / kWarps, kThreads, 0, st>>>(blocks, s->head_dim, p.part, dq_weight, dk_weight));
-    return launch_status();
+               e = launch_early(norm_rope_dw_kernel, dim3((2 * s->head_dim + 31) / 32), 1024, 0, st, true, 1, blocks, s->head_dim, p.part, dq_weight, dk_weight));
+    return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 extern "C" int kda_norm_rope_append(const KdaRotaryShape* s, const KdaPagedShape* g, const void* q, const void* k, const void* v, const float* cos,
@@ -310,7 +697,15 @@ extern "C" int kda_norm_rope_append(const KdaRotaryShape* s, const KdaPagedShape
                     g->n_pages, g->page_size, g->table_width};
     p.cache = Strides{0, 0, g->k_page_stride, g->k_row_stride, g->k_head_stride, g->v_page_stride, g->v_row_stride, g->v_head_stride};
     cudaStream_t st = (cudaStream_t)stream;
-    const int blocks = blocks_for((long long)s->tokens * (s->q_heads + 2 * s->kv_heads));
+    if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride, s->v_token_stride, s->v_head_stride, g->k_page_stride, g->k_row_stride,
+                  g->k_head_stride, g->v_page_stride, g->v_row_stride, g->v_head_stride})) {
+        const int lanes = lanes_for(s->head_dim);
+        slice_heads(p, s->q_heads + 2 * s->kv_heads, lanes);
+        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, 16);
+        KDA_LAUNCH("norm_rope_append_rows_kernel", st, by_shape<RunAppend>(p, blocks, st));
+        return launch_status();
+    }
+    const int blocks = blocks_for((long long)s->tokens * (s->q_heads + 2 * s->kv_heads), kWarps, 8);
     KDA_LAUNCH("norm_rope_append_kernel", st, norm_rope_kernel<true><<<blocks, kThreads, 0, st>>>(p));
     return launch_status();
 }

@@ -50,7 +50,9 @@ extern "C" size_t kda_paged_attention_workspace_bytes(const KdaPagedShape* s) {
         const size_t need = n > 1 ? align_up(rows * n * sizeof(float2), 256) + rows * n * s->head_dim * sizeof(float) : 0;
         if (need > most) most = need;
     }
-    return align_up(most, 256);
+    const int each = s->tokens / s->n_seq, max_q = s->max_q_len > each ? s->max_q_len : each;
+    const size_t few = decode_workspace(s->n_seq, s->kv_heads, s->table_width, s->page_size, s->window, max_q, s->head_dim);
+    return align_up(most > few ? most : few, 256);
 }
 
 extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -75,5 +77,6 @@ extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const 
     c.bf16 = s->io_dtype == KDA_DTYPE_BF16;
     c.max_q_len = packed ? s->max_q_len : q_len;
     c.workspace = workspace;
+    if (decode_takes(c)) return decode(c, (cudaStream_t)stream);
     return tc_takes(c) ? tc(c, tc_splits(*s, packed), (cudaStream_t)stream) : general(c, general_splits(*s, packed), (cudaStream_t)stream);
 }

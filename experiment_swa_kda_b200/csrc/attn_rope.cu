@@ -8,7 +8,7 @@
 // Everything is float32 between the load and the one rounding of the store.  r is formed again in the backward: it costs a sum
 // over values that are in registers anyway, a saved one would be read.
 //
-// Bound by memory.  Two forms each way: norm_rope_rows_* for widths, strides and addresses that allow 16-byte accesses, and
+// Bound by memory.  Two forms each way: norm_rope_rows_* for widths, strides and addresses that allow wide accesses, and
 // norm_rope_kernel / norm_rope_bwd_kernel for all others.
 
 #include <initializer_list>
@@ -20,7 +20,12 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kBwdBlocks = 4;      // blocks an SM of the backward: each leaves one part of the weights' gradients
+#ifndef V_BG
+#define V_BG 2
+#define V_FG 3
+#endif
+constexpr int kFwdBlocks = V_FG;
+constexpr int kBwdBlocks = V_BG;      // blocks an SM of the backward: each leaves one part of the weights' gradients
 
 struct Rope {
     KdaRotaryShape s;
@@ -217,94 +222,98 @@ __global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(Rope p) {
     }
 }
 
-// ---------------------------------------------------------------------------------------------- 16-byte accesses
-// Eight adjacent values a lane, LANES lanes a row.  A group of lanes takes a token's heads one after the other - all of them, or a
-// slice where there are too few tokens to fill the machine -, so that the token's place, its cosines and sines and the
-// weights are read once for all of them.  In the split order a pair's members lie in two lanes and change places by shuffle, as
-// they were loaded: bf16 pairs in one word.
+#ifndef V_FB
+#define V_FB 3
+#define V_BB 2
+#endif
+// ---------------------------------------------------------------------------------------------- eight values a lane
+// LANES lanes a row, and both members of a pair in one lane: two pieces of four adjacent values, half the rotated width apart in the
+// split order.  A group of lanes takes a token's heads one after the other - all of them, or a slice where there are too few
+// tokens to fill the machine -, so that the token's place, its cosines and sines and the weights are read once for all of them.
+// What bounds such a loop after memory is issue and the shuffles of the rows' sums, so rows go four at a time (backward two, with
+// two sums each) and their four sums are reduced together: 5 shuffles, not 16, and 4 that hand them out.
 
+// values [0..3], [4..7] of a lane
 template <bool BF16>
-struct Vec8 {
-    uint4 a, b;      // b: float32 only
+struct Vec8;
+template <>
+struct Vec8<true> {
+    uint2 a, b;
+    __device__ __forceinline__ void load(const void* p, long long at0, long long at1) {
+        a = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + at0));
+        b = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + at1));
+    }
+    __device__ __forceinline__ void zero() { a = b = make_uint2(0, 0); }
+    __device__ __forceinline__ void get(f2 (&x)[4]) const {
+        x[0] = f2_from_bf16(a.x); x[1] = f2_from_bf16(a.y); x[2] = f2_from_bf16(b.x); x[3] = f2_from_bf16(b.y);
+    }
+    static __device__ __forceinline__ void store(void* p, long long at0, long long at1, const f2 (&x)[4]) {
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + at0) = make_uint2(f2_to_bf16(x[0]), f2_to_bf16(x[1]));
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + at1) = make_uint2(f2_to_bf16(x[2]), f2_to_bf16(x[3]));
+    }
 };
-template <bool BF16>
-__device__ __forceinline__ Vec8<BF16> ld8(const void* p, long long at) {
-    Vec8<BF16> r;
-    if (BF16) {
-        r.a = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at));
-    } else {
-        const uint4* s = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + at);
-        r.a = __ldg(s);
-        r.b = __ldg(s + 1);
+template <>
+struct Vec8<false> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const void* p, long long at0, long long at1) {
+        a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at0));
+        b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at1));
     }
-    return r;
-}
-template <bool BF16>
-__device__ __forceinline__ void unpack(const Vec8<BF16>& v, f2 (&x)[4]) {
-    if (BF16) {
-        x[0] = f2_from_bf16(v.a.x); x[1] = f2_from_bf16(v.a.y); x[2] = f2_from_bf16(v.a.z); x[3] = f2_from_bf16(v.a.w);
-    } else {
-        x[0] = f2_make(__uint_as_float(v.a.x), __uint_as_float(v.a.y));
-        x[1] = f2_make(__uint_as_float(v.a.z), __uint_as_float(v.a.w));
-        x[2] = f2_make(__uint_as_float(v.b.x), __uint_as_float(v.b.y));
-        x[3] = f2_make(__uint_as_float(v.b.z), __uint_as_float(v.b.w));
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void get(f2 (&x)[4]) const {
+        x[0] = f2_make(a.x, a.y); x[1] = f2_make(a.z, a.w); x[2] = f2_make(b.x, b.y); x[3] = f2_make(b.z, b.w);
     }
-}
-template <bool BF16>
-__device__ __forceinline__ void st8(void* p, long long at, const f2 (&x)[4]) {
-    if (BF16) {
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) = make_uint4(f2_to_bf16(x[0]), f2_to_bf16(x[1]), f2_to_bf16(x[2]), f2_to_bf16(x[3]));
-    } else {
-        float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+    static __device__ __forceinline__ void store(void* p, long long at0, long long at1, const f2 (&x)[4]) {
         const float2 a = f2_get(x[0]), b = f2_get(x[1]), c = f2_get(x[2]), e = f2_get(x[3]);
-        d[0] = make_float4(a.x, a.y, b.x, b.y);
-        d[1] = make_float4(c.x, c.y, e.x, e.y);
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + at0) = make_float4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<float4*>(static_cast<float*>(p) + at1) = make_float4(c.x, c.y, e.x, e.y);
     }
-}
-template <bool BF16>
-__device__ __forceinline__ Vec8<BF16> shuffle(const Vec8<BF16>& v, int src, int lanes, unsigned mask) {
-    Vec8<BF16> r;
-    r.a = make_uint4(__shfl_sync(mask, v.a.x, src, lanes), __shfl_sync(mask, v.a.y, src, lanes), __shfl_sync(mask, v.a.z, src, lanes),
-                     __shfl_sync(mask, v.a.w, src, lanes));
-    if (!BF16)
-        r.b = make_uint4(__shfl_sync(mask, v.b.x, src, lanes), __shfl_sync(mask, v.b.y, src, lanes), __shfl_sync(mask, v.b.z, src, lanes),
-                         __shfl_sync(mask, v.b.w, src, lanes));
-    return r;
-}
+};
+
+// The sums of four values over the lanes of a group; lane l ends with that of value l & 3.
 template <int LANES>
-__device__ __forceinline__ float group_sum(float x, unsigned mask) {
+__device__ __forceinline__ float sum4(float a0, float a1, float a2, float a3, int l, unsigned mask) {
+    const bool b0 = l & 1, b1 = l & 2;
+    float x = b0 ? a1 : a0, y = b0 ? a3 : a2;
+    x += __shfl_xor_sync(mask, b0 ? a0 : a1, 1);
+    y += __shfl_xor_sync(mask, b0 ? a2 : a3, 1);
+    float z = b1 ? y : x;
+    z += __shfl_xor_sync(mask, b1 ? x : y, 2);
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) x += __shfl_xor_sync(mask, x, o);
-    return x;
+    for (int o = 4; o < LANES; o <<= 1) z += __shfl_xor_sync(mask, z, o);
+    return z;
 }
 
-// A lane's share of a row: its values, where their partners are, their weights and the partners'.
+__device__ __forceinline__ f2 swapped(f2 a) {
+    const float2 x = f2_get(a);
+    return f2_make(x.y, x.x);
+}
+__device__ __forceinline__ float f2_dot(const f2 (&x)[4], const f2 (&y)[4]) {
+    const float2 t = f2_get(f2_fma(x[0], y[0], f2_fma(x[1], y[1], f2_fma(x[2], y[2], f2_mul(x[3], y[3])))));
+    return t.x + t.y;
+}
+
+// A lane's share of a row.
 template <int LANES, bool INTER>
 struct Lane {
-    int l, d, src;                  // lane of the group, its first value, lane that holds the partners
+    int l, d0, d1;                  // lane of the group, its first value of each piece
     bool on, turned;                // the row has these values; they are rotated
     unsigned mask;
-    int at;                         // first of its cosines
-    float sign;                     // of the sine in y (split order)
 
     __device__ __forceinline__ Lane(const KdaRotaryShape& s) {
         const int lane = threadIdx.x & 31;
         l = lane & (LANES - 1);
         mask = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (lane & ~(LANES - 1));
-        d = 8 * l;
-        on = d < s.head_dim;
-        turned = d < s.rotary_dim;
-        src = l;
-        at = INTER ? d / 2 : 0;
-        sign = 0.f;
+        on = 8 * l < s.head_dim;
+        turned = 8 * l < s.rotary_dim;
+        d0 = 8 * l;
+        d1 = d0 + 4;
         if (!INTER && turned) {
-            const int half = s.rotary_dim / 2;
-            src = d < half ? l + half / 8 : l - half / 8;
-            at = d < half ? d : d - half;
-            sign = d < half ? -1.f : 1.f;
+            d0 = 4 * l;
+            d1 = s.rotary_dim / 2 + 4 * l;
         }
     }
-    // y_e = u_e c_e + u_other s_e for the lane's values
+    // y_e = x_e c_e + x_other s_e for the lane's values; 1 and 0 where they are not rotated
     __device__ __forceinline__ void angles(const Rope& p, int pos, f2 (&c)[4], f2 (&s)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -312,77 +321,73 @@ struct Lane {
             s[i] = f2_all(0.f);
         }
         if (!turned) return;
-        const float* pc = p.cos + (size_t)pos * (p.s.rotary_dim / 2) + at;
-        const float* ps = p.sin + (size_t)pos * (p.s.rotary_dim / 2) + at;
-        const float4 c0 = __ldg(reinterpret_cast<const float4*>(pc)), s0 = __ldg(reinterpret_cast<const float4*>(ps));
+        const size_t at = (size_t)pos * (p.s.rotary_dim / 2) + 4 * l;
+        const float4 cc = __ldg(reinterpret_cast<const float4*>(p.cos + at)), ss = __ldg(reinterpret_cast<const float4*>(p.sin + at));
         if (INTER) {
-            c[0] = f2_all(c0.x); c[1] = f2_all(c0.y); c[2] = f2_all(c0.z); c[3] = f2_all(c0.w);
-            s[0] = f2_make(-s0.x, s0.x); s[1] = f2_make(-s0.y, s0.y); s[2] = f2_make(-s0.z, s0.z); s[3] = f2_make(-s0.w, s0.w);
+            c[0] = f2_all(cc.x); c[1] = f2_all(cc.y); c[2] = f2_all(cc.z); c[3] = f2_all(cc.w);
+            s[0] = f2_make(-ss.x, ss.x); s[1] = f2_make(-ss.y, ss.y); s[2] = f2_make(-ss.z, ss.z); s[3] = f2_make(-ss.w, ss.w);
         } else {
-            const float4 c1 = __ldg(reinterpret_cast<const float4*>(pc) + 1), s1 = __ldg(reinterpret_cast<const float4*>(ps) + 1);
-            c[0] = f2_make(c0.x, c0.y); c[1] = f2_make(c0.z, c0.w); c[2] = f2_make(c1.x, c1.y); c[3] = f2_make(c1.z, c1.w);
-            s[0] = f2_make(sign * s0.x, sign * s0.y); s[1] = f2_make(sign * s0.z, sign * s0.w);
-            s[2] = f2_make(sign * s1.x, sign * s1.y); s[3] = f2_make(sign * s1.z, sign * s1.w);
+            c[0] = c[2] = f2_make(cc.x, cc.y);
+            c[1] = c[3] = f2_make(cc.z, cc.w);
+            s[0] = f2_make(-ss.x, -ss.y);
+            s[1] = f2_make(-ss.z, -ss.w);
+            s[2] = f2_make(ss.x, ss.y);
+            s[3] = f2_make(ss.z, ss.w);
         }
     }
-    // the weights of values d .. d + 7, 1 without weights
-    __device__ __forceinline__ void weights(const float* w, int d0, f2 (&x)[4]) const {
+    __device__ __forceinline__ void weights(const float* w, f2 (&x)[4]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = f2_all(1.f);
         if (w == nullptr || !on) return;
-        const float4 a = __ldg(reinterpret_cast<const float4*>(w + d0)), b = __ldg(reinterpret_cast<const float4*>(w + d0) + 1);
+        const float4 a = __ldg(reinterpret_cast<const float4*>(w + d0)), b = __ldg(reinterpret_cast<const float4*>(w + d1));
         x[0] = f2_make(a.x, a.y); x[1] = f2_make(a.z, a.w); x[2] = f2_make(b.x, b.y); x[3] = f2_make(b.z, b.w);
     }
-    // the partners of a lane's values
-    template <bool BF16>
-    __device__ __forceinline__ void other(const Vec8<BF16>& v, const f2 (&x)[4], f2 (&o)[4]) const {
+    // the partners of a lane's values.  A lane that is not rotated has none: 0, since 0 times an infinite value would be NaN.
+    __device__ __forceinline__ void other(const f2 (&x)[4], f2 (&o)[4], bool all_turned) const {
         if (INTER) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 t = f2_get(x[i]);
-                o[i] = f2_make(t.y, t.x);
-            }
+            for (int i = 0; i < 4; ++i) o[i] = swapped(x[i]);
         } else {
-            unpack<BF16>(shuffle<BF16>(v, src, LANES, mask), o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = x[i ^ 2];
         }
+        if (!all_turned && !turned)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = f2_all(0.f);
     }
 };
 
-__device__ __forceinline__ float f2_sum(const f2 (&x)[4], const f2 (&y)[4]) {
-    const float2 t = f2_get(f2_fma(x[0], y[0], f2_fma(x[1], y[1], f2_fma(x[2], y[2], f2_mul(x[3], y[3])))));
-    return t.x + t.y;
-}
-
-constexpr int kAhead = 4;      // rows whose loads are in flight together
-
-// `heads` rows of one token from `from` on, head_stride apart, to `to`, to_stride apart
+// `heads` rows of one token from `from` on, from_stride apart, to `to`, to_stride apart: y = r (x a + x_other b)
 template <int LANES, bool BF16, bool INTER>
 __device__ __forceinline__ void turn_rows(const Lane<LANES, INTER>& ln, const KdaRotaryShape& sh, const void* src, long long from, long long from_stride, void* dst,
                                           long long to, long long to_stride, int heads, const f2 (&a)[4], const f2 (&b)[4]) {
-    for (int h = 0; h < heads; h += kAhead) {
-        Vec8<BF16> v[kAhead];
+    const bool all_turned = sh.rotary_dim == sh.head_dim;
+    const float inv = 1.f / sh.head_dim;
+    for (int h = 0; h < heads; h += 4) {
+        Vec8<BF16> v[4];
+        f2 x[4][4];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            v[i].a = v[i].b = make_uint4(0, 0, 0, 0);
-            if (ln.on && h + i < heads) v[i] = ld8<BF16>(src, from + (h + i) * from_stride + ln.d);
+        for (int i = 0; i < 4; ++i) {
+            v[i].zero();
+            if (ln.on && h + i < heads) v[i].load(src, from + (h + i) * from_stride + ln.d0, from + (h + i) * from_stride + ln.d1);
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            if (h + i >= heads) break;      // the same for all lanes of the group
-            f2 x[4], o[4];
-            unpack<BF16>(v[i], x);
-            ln.template other<BF16>(v[i], x, o);
-            const float r = rsqrtf(group_sum<LANES>(f2_sum(x, x), ln.mask) / sh.head_dim + sh.eps);
-            const f2 r2 = f2_all(r);
+        for (int i = 0; i < 4; ++i) v[i].get(x[i]);
+        const float r = rsqrtf(fmaf(sum4<LANES>(f2_dot(x[0], x[0]), f2_dot(x[1], x[1]), f2_dot(x[2], x[2]), f2_dot(x[3], x[3]), ln.l, ln.mask), inv, sh.eps));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] = f2_mul(f2_fma(x[k], a[k], f2_mul(o[k], b[k])), r2);
-            if (ln.on) st8<BF16>(dst, to + (h + i) * to_stride + ln.d, x);
+        for (int i = 0; i < 4; ++i) {
+            const f2 r2 = f2_all(__shfl_sync(ln.mask, r, i, LANES));
+            f2 o[4], y[4];
+            ln.other(x[i], o, all_turned);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = f2_mul(f2_fma(x[i][k], a[k], f2_mul(o[k], b[k])), r2);
+            if (ln.on && h + i < heads) Vec8<BF16>::store(dst, to + (h + i) * to_stride + ln.d0, to + (h + i) * to_stride + ln.d1, y);
         }
     }
 }
 
 template <int LANES, bool BF16, bool INTER, bool APPEND>
-__global__ void __launch_bounds__(kThreads) norm_rope_rows_kernel(Rope p) {
+__global__ void __launch_bounds__(kThreads, V_FB) norm_rope_rows_kernel(Rope p) {
     constexpr int kGroups = kThreads / LANES;
     const Lane<LANES, INTER> ln(p.s);
     const int Hq = p.s.q_heads, Hk = p.s.kv_heads, all = Hq + Hk + (APPEND ? Hk : 0), D = p.s.head_dim;
@@ -392,23 +397,14 @@ __global__ void __launch_bounds__(kThreads) norm_rope_rows_kernel(Rope p) {
         const Place at = place_of<APPEND, LANES>(p, t, ln.l, ln.mask);
         f2 c[4], s[4];
         ln.angles(p, max(at.pos, 0), c, s);
-        // y = r (x (w c) + x_other (w_other s))
+        // u_e c + u_other s with u = x r w: a = w_e c, b = w_other s
         auto coefficients = [&](const float* w, f2 (&a)[4], f2 (&b)[4]) {
-            f2 own[4], other[4];
-            ln.weights(w, ln.d, own);
-            if (INTER) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 x = f2_get(own[i]);
-                    other[i] = f2_make(x.y, x.x);
-                }
-            } else {
-                ln.weights(w, 8 * ln.src, other);
-            }
+            f2 own[4];
+            ln.weights(w, own);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 a[i] = f2_mul(own[i], c[i]);
-                b[i] = f2_mul(other[i], s[i]);
+                b[i] = f2_mul(INTER ? swapped(own[i]) : own[i ^ 2], s[i]);
             }
         };
         f2 a[4], b[4];
@@ -418,7 +414,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_rows_kernel(Rope p) {
             if (APPEND && at.pos < 0) {
                 const f2 none[4] = {f2_all(0.f), f2_all(0.f), f2_all(0.f), f2_all(0.f)};
                 for (int h = 0; h < n; ++h)
-                    if (ln.on) st8<BF16>(p.q_out, to + (long long)h * D + ln.d, none);
+                    if (ln.on) Vec8<BF16>::store(p.q_out, to + (long long)h * D + ln.d0, to + (long long)h * D + ln.d1, none);
             } else {
                 coefficients(p.q_weight, a, b);
                 turn_rows<LANES, BF16>(ln, p.s, p.q, t * p.s.q_token_stride + h0 * p.s.q_head_stride, p.s.q_head_stride, p.q_out, to, D, n, a, b);
@@ -433,9 +429,11 @@ __global__ void __launch_bounds__(kThreads) norm_rope_rows_kernel(Rope p) {
         }
         if (APPEND && ln.on) {      // values go as they are
             for (int v = max(h0 - Hq - Hk, 0); v < h1 - Hq - Hk; ++v) {
-                f2 x[4];
-                unpack<BF16>(ld8<BF16>(p.v, t * p.s.v_token_stride + v * p.s.v_head_stride + ln.d), x);
-                st8<BF16>(p.v_out, at.v_at + v * p.cache.v_head + ln.d, x);
+                Vec8<BF16> x;
+                f2 y[4];
+                x.load(p.v, t * p.s.v_token_stride + v * p.s.v_head_stride + ln.d0, t * p.s.v_token_stride + v * p.s.v_head_stride + ln.d1);
+                x.get(y);
+                Vec8<BF16>::store(p.v_out, at.v_at + v * p.cache.v_head + ln.d0, at.v_at + v * p.cache.v_head + ln.d1, y);
             }
         }
     }
@@ -444,11 +442,13 @@ __global__ void __launch_bounds__(kThreads) norm_rope_rows_kernel(Rope p) {
 // The same rows backward; each lane sums its weights' gradients over all rows it meets, a block over its lanes, and
 // norm_rope_dw_kernel over the blocks, all in a fixed order.
 template <int LANES, bool BF16, bool INTER>
-__global__ void __launch_bounds__(kThreads) norm_rope_rows_bwd_kernel(Rope p) {
-    constexpr int kGroups = kThreads / LANES, kRowsAhead = BF16 ? 2 : 1;
+__global__ void __launch_bounds__(kThreads, V_BB) norm_rope_rows_bwd_kernel(Rope p) {
+    constexpr int kGroups = kThreads / LANES;
     dependents_go();
     const Lane<LANES, INTER> ln(p.s);
     const int Hq = p.s.q_heads, Hk = p.s.kv_heads, all = Hq + Hk, D = p.s.head_dim;
+    const bool all_turned = p.s.rotary_dim == D;
+    const float inv = 1.f / D;
     const long long units = (long long)p.s.tokens * p.slices;
     f2 dw[2][4];
 #pragma unroll
@@ -464,43 +464,54 @@ __global__ void __launch_bounds__(kThreads) norm_rope_rows_bwd_kernel(Rope p) {
         for (int which = 0; which < 2; ++which) {
             const int H = which ? Hk : Hq, a0 = which ? max(h0 - Hq, 0) : h0, a1 = which ? h1 - Hq : min(h1, Hq);
             if (a0 >= a1) continue;
-            const long long ts = which ? p.s.k_token_stride : p.s.q_token_stride, hs = which ? p.s.k_head_stride : p.s.q_head_stride;
+            const long long hs = which ? p.s.k_head_stride : p.s.q_head_stride;
+            const long long from = t * (which ? p.s.k_token_stride : p.s.q_token_stride), to = (long long)t * H * D;
             const void *src = which ? p.k : p.q, *grad = which ? p.d_k : p.d_q;
             void* dst = which ? p.k_out : p.q_out;
-            const float* w = which ? p.k_weight : p.q_weight;
             f2 own[4];
-            ln.weights(w, ln.d, own);
-            for (int h = a0; h < a1; h += kRowsAhead) {
-                Vec8<BF16> xv[kRowsAhead], gv[kRowsAhead];
+            ln.weights(which ? p.k_weight : p.q_weight, own);
+            for (int h = a0; h < a1; h += 2) {
+                Vec8<BF16> xv[2], gv[2];
+                f2 x[2][4], du[2][4];
+                float ss[2], dot[2];
 #pragma unroll
-                for (int i = 0; i < kRowsAhead; ++i) {
-                    xv[i].a = xv[i].b = gv[i].a = gv[i].b = make_uint4(0, 0, 0, 0);
+                for (int i = 0; i < 2; ++i) {
+                    xv[i].zero();
+                    gv[i].zero();
                     if (ln.on && h + i < a1) {
-                        xv[i] = ld8<BF16>(src, t * ts + (h + i) * hs + ln.d);
-                        gv[i] = ld8<BF16>(grad, ((long long)t * H + h + i) * D + ln.d);
+                        xv[i].load(src, from + (h + i) * hs + ln.d0, from + (h + i) * hs + ln.d1);
+                        gv[i].load(grad, to + (long long)(h + i) * D + ln.d0, to + (long long)(h + i) * D + ln.d1);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < kRowsAhead; ++i) {
-                    if (h + i >= a1) break;
-                    f2 x[4], du[4], o[4];
-                    unpack<BF16>(xv[i], x);
-                    unpack<BF16>(gv[i], du);
-                    ln.template other<BF16>(gv[i], du, o);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) du[k] = f2_fma(du[k], c[k], f2_mul(o[k], s[k]));
-                    const float ss = group_sum<LANES>(f2_sum(x, x), ln.mask);
-                    const float r = rsqrtf(ss / D + p.s.eps);
-                    const f2 r2 = f2_all(r);
+                for (int i = 0; i < 2; ++i) {
+                    f2 o[4];
+                    xv[i].get(x[i]);
+                    gv[i].get(du[i]);
+                    ln.other(du[i], o, all_turned);
+                    ss[i] = f2_dot(x[i], x[i]);
+                    f2 sum = f2_all(0.f);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        dw[which][k] = f2_fma(f2_mul(du[k], x[k]), r2, dw[which][k]);
-                        du[k] = f2_mul(du[k], own[k]);
+                        const f2 d = f2_fma(o[k], s[k], f2_mul(du[i][k], c[k]));
+                        sum = f2_fma(f2_mul(d, own[k]), x[i][k], sum);
+                        du[i][k] = d;
                     }
-                    const f2 f = f2_all(-r * r * group_sum<LANES>(f2_sum(du, x), ln.mask) / D);
+                    const float2 t2 = f2_get(sum);
+                    dot[i] = t2.x + t2.y;
+                }
+                const float mean = sum4<LANES>(ss[0], ss[1], dot[0], dot[1], ln.l, ln.mask) * inv;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) du[k] = f2_mul(f2_fma(x[k], f, du[k]), r2);
-                    if (ln.on) st8<BF16>(dst, ((long long)t * H + h + i) * D + ln.d, du);
+                for (int i = 0; i < 2; ++i) {
+                    const float r = rsqrtf(__shfl_sync(ln.mask, mean, i, LANES) + p.s.eps), f = -r * r * __shfl_sync(ln.mask, mean, 2 + i, LANES);
+                    const f2 r2 = f2_all(r), g2 = f2_all(f);
+                    f2 y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        dw[which][k] = f2_fma(f2_mul(du[i][k], x[i][k]), r2, dw[which][k]);
+                        y[k] = f2_mul(f2_fma(x[i][k], g2, f2_mul(du[i][k], own[k])), r2);
+                    }
+                    if (ln.on && h + i < a1) Vec8<BF16>::store(dst, to + (long long)(h + i) * D + ln.d0, to + (long long)(h + i) * D + ln.d1, y);
                 }
             }
         }
@@ -511,7 +522,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_rows_bwd_kernel(Rope p) {
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sum[threadIdx.x / LANES][ln.d + 2 * k]) = f2_get(dw[which][k]);
+        for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sum[threadIdx.x / LANES][(k < 2 ? ln.d0 : ln.d1 - 4) + 2 * k]) = f2_get(dw[which][k]);
         __syncthreads();
         for (int d = threadIdx.x; d < D; d += kThreads) {
             float v = 0.f;
@@ -567,7 +578,7 @@ bool rows8(const Rope& p, std::initializer_list<long long> strides) {
     const int unit = s.io_dtype == KDA_DTYPE_BF16 ? 8 : 4;      // elements in 16 bytes
     long long all = 0;
     for (long long x : strides) all |= x;
-    return s.head_dim % 8 == 0 && s.rotary_dim % (s.interleaved ? 8 : 16) == 0 && all % unit == 0 &&
+    return s.head_dim % 8 == 0 && s.rotary_dim % 8 == 0 && all % unit == 0 &&
            on16({p.q, p.k, p.v, p.cos, p.sin, p.q_weight, p.k_weight, p.q_out, p.k_out, p.v_out, p.d_q, p.d_k});
 }
 int lanes_for(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
@@ -633,7 +644,7 @@ extern "C" int kda_norm_rope_fwd(const KdaRotaryShape* s, const void* q, const v
     if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride})) {
         const int lanes = lanes_for(s->head_dim);
         slice_heads(p, s->q_heads + s->kv_heads, lanes);
-        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, 16);
+        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, kFwdBlocks);
         KDA_LAUNCH("norm_rope_rows_kernel", st, by_shape<RunForward>(p, blocks, st));
         return launch_status();
     }
@@ -701,7 +712,7 @@ extern "C" int kda_norm_rope_append(const KdaRotaryShape* s, const KdaPagedShape
                   g->k_head_stride, g->v_page_stride, g->v_row_stride, g->v_head_stride})) {
         const int lanes = lanes_for(s->head_dim);
         slice_heads(p, s->q_heads + 2 * s->kv_heads, lanes);
-        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, 16);
+        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, kFwdBlocks);
         KDA_LAUNCH("norm_rope_append_rows_kernel", st, by_shape<RunAppend>(p, blocks, st));
         return launch_status();
     }

@@ -12,8 +12,11 @@
 //   attn_decode_join_kernel puts the parts together.
 // - A warp takes 16 keys of a tile through a ring of its own (K and V by TMA, 128-byte swizzle), so that warps meet only where a
 //   sequence or the stretch ends.  The ring runs ahead across those places.
-// - Products are mma.sync m16n8k16: 16 rows are its height, and at 23 bytes a cycle and SM its rate is not felt.  The weights go as
-//   two bf16 terms, p = hi + lo, which costs products that nothing waits for and leaves the output with the error of its own rounding.
+// - Products are mma.sync m16n8k16 with the keys as their 16 rows and the query rows as their 8 columns: S^T = K Q^T and O^T = V^T P^T
+//   (P^T comes from S^T's registers by movmatrix).  Up to 8 rows take half the products that rows of queries would.  The weights
+//   go as two bf16 terms, p = hi + lo, which leaves the output with the error of its own rounding.
+// - What runs once a sequence (its queries, the join of the warps' sums) is kept short in code: unrolled it was fetched anew every time
+//   and took 5 us.
 
 #include "attn.cuh"
 #include "tc_common.cuh"
@@ -28,35 +31,50 @@ namespace {
 
 using namespace tc;
 
-constexpr int kRows = 16, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
+constexpr int kMaxRows = 16, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
 constexpr int kPerSm = 2;             // blocks an SM: 98 KB each
-constexpr int kMinTiles = 2;          // a stretch has at least these many tiles
+#ifndef V_MT
+#define V_MT 2
+#endif
+constexpr int kMinTiles = V_MT;          // a stretch has at least these many tiles
 constexpr float kLazy = 8.f;          // as in the kernel for long chunks: sums are rescaled when a maximum grew by 2^8
 constexpr int kStatusWait = 121;
 
-template <int DP>
+template <int DP, int NR>
 struct Layout {
     static constexpr int kHalf = 16 * 128;                            // 16 keys of 64 values
     static constexpr int kStage = 2 * (DP / 64) * kHalf;              // K and V of 16 keys
-    static constexpr int kBars = kWarps * kStages * kStage;
+    static constexpr int kRowsOf = 8 * NR;
+    static constexpr int kQ = kWarps * kStages * kStage;              // two sequences' queries
+    static constexpr int kBars = kQ + 2 * kRowsOf * DP * 2;
     static constexpr int kBytes = kBars + 1024 + 1024;
 };
 
 struct Args {
     Call c;
-    int blocks, box_rows, q4;
-    float* part_o;        // [blocks][2][16][D]
-    float2* part_ml;      // [blocks][2][16]
+    int blocks, box_rows, q16;
+    float* part_o;        // [blocks][2][rows][D]
+    float2* part_ml;      // [blocks][2][rows]
 };
 
 // One sequence's tiles and rows.
 struct Seq {
     int first, count, base, lo, hi, t0, t1;
 };
-__device__ __forceinline__ Seq seq_at(const Batch& b, int n, int window) {
+// what a sequence is read from: the ends of its new tokens and its length, as they stand in memory
+struct Raw {
+    int a, b, len;
+};
+__device__ __forceinline__ Raw raw_at(const Batch& b, int n) {
+    if (n >= b.n_seq) return Raw{0, 0, 0};
+    return b.cu != nullptr ? Raw{__ldg(b.cu + n), __ldg(b.cu + n + 1), __ldg(b.kv_lens + n)} : Raw{n * b.q_len, (n + 1) * b.q_len, __ldg(b.kv_lens + n)};
+}
+__device__ __forceinline__ Seq seq_of_raw(const Batch& b, const Raw& r, int window) {
     Seq s;
-    b.span(n, s.first, s.count);
-    const int len = b.kv_len(n);
+    s.first = min(max(r.a, 0), b.tokens);
+    s.count = min(max(r.b, s.first), b.tokens) - s.first;
+    const long long room = (long long)b.table_width * b.page_size;
+    const int len = max(r.len, 0) > room ? (int)room : max(r.len, 0);
     s.base = len - s.count;
     s.hi = s.count > 0 ? len : 0;
     s.lo = window > 0 ? min(max(s.base - window + 1, 0), s.hi) : 0;
@@ -64,16 +82,18 @@ __device__ __forceinline__ Seq seq_at(const Batch& b, int n, int window) {
     s.t1 = (s.hi + kTile - 1) / kTile;
     return s;
 }
+__device__ __forceinline__ Seq seq_at(const Batch& b, int n, int window) { return seq_of_raw(b, raw_at(b, n), window); }
 
 struct Start {
     long long total, begin, end;      // tiles of the batch; this stretch
     int blocks;                       // stretches in use
     int n, hk, tile;                  // where it begins
 };
-// The stretch of block `id`; called by all threads of a block of kThreads.
+// The stretch of block `id`; called by all THREADS of a block, `sums` has a place for each warp.
+template <int THREADS>
 __device__ __forceinline__ void find_start(const Batch& b, int kv_heads, int window, int blocks, int id, Start* shared, long long* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int each = (b.n_seq + kThreads - 1) / kThreads, n0 = min(tid * each, b.n_seq), n1 = min(n0 + each, b.n_seq);
+    const int each = (b.n_seq + THREADS - 1) / THREADS, n0 = min(tid * each, b.n_seq), n1 = min(n0 + each, b.n_seq);
     long long mine = 0;
     for (int n = n0; n < n1; ++n) {
         const Seq s = seq_at(b, n, window);
@@ -88,7 +108,8 @@ __device__ __forceinline__ void find_start(const Batch& b, int kv_heads, int win
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
     long long total = 0;
-    for (int w = 0; w < kWarps; ++w) {
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) upto += sums[w];
         total += sums[w];
     }
@@ -121,12 +142,14 @@ __device__ __forceinline__ void find_start(const Batch& b, int kv_heads, int win
 // A place in the list.
 struct Walk {
     Seq s;
+    Raw after;      // of the next sequence, read when this one is entered: nothing waits for it
     int n, hk, tile;
     __device__ __forceinline__ void set(const Batch& b, const Start& at, int window) {
         n = at.n;
         hk = at.hk;
         tile = at.tile;
         s = seq_at(b, n, window);
+        after = raw_at(b, n + 1);
     }
     __device__ __forceinline__ void next(const Batch& b, int kv_heads, int window) {
         if (++tile < s.t1) return;
@@ -134,7 +157,8 @@ struct Walk {
             hk = 0;
             do {
                 if (++n >= b.n_seq) return;      // behind the end of the list: not used
-                s = seq_at(b, n, window);
+                s = seq_of_raw(b, after, window);
+                after = raw_at(b, n + 1);
             } while (s.t1 <= s.t0);
         }
         tile = s.t0;
@@ -162,19 +186,24 @@ __device__ __forceinline__ void ldm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldm4t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+__device__ __forceinline__ uint32_t turned(uint32_t x) {      // an 8 x 8 tile of 16-bit values, transposed
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
-template <int DP>
+template <int DP, int NR>
 __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                                        const __grid_constant__ Args a) {
-    using L = Layout<DP>;
-    constexpr int kHalves = DP / 64, kNt = DP / 8;
+    using L = Layout<DP, NR>;
+    constexpr int kHalves = DP / 64, kSteps = DP / 16, kRows = 8 * NR;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
     Start& start = *reinterpret_cast<Start*>(bars + kWarps * kStages);
     long long* sums = reinterpret_cast<long long*>(&start + 1);
-    volatile int* flags = reinterpret_cast<volatile int*>(sums + kWarps);      // [0] an expired wait, [1] values that are not finite
-    float2* row_ml = reinterpret_cast<float2*>(sums + kWarps + 2);             // [warps][16]
+    volatile int* flags = reinterpret_cast<volatile int*>(sums + kWarps);      // [0] an expired wait, [1], [2] values that are not finite (of sequences in turn)
+    float2* row_ml = reinterpret_cast<float2*>(sums + kWarps + 2);             // [warps][rows]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, c4 = lane & 3, r8 = lane >> 2;
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window;
@@ -185,29 +214,12 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         for (int s = 0; s < kStages; ++s) mbar_init(bar + s, 1);
         mbar_fence_init();
     }
-    if (tid == 0) flags[0] = flags[1] = 0;
-    find_start(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
-
-    // sequences without a key in reach have no tile: their rows are nothing
-    for (int n = blockIdx.x; n < b.n_seq; n += gridDim.x) {
-        const Seq s = seq_at(b, n, window);
-        if (tid == 0) {
-            if (!b.span_ok(n) || s.count * g > kRows) b.tell(KDA_ERR_CU_SEQLENS);
-            if (!b.kv_len_ok(n)) b.tell(KDA_ERR_BLOCK_TABLE);
-        }
-        if (s.t1 > s.t0) continue;
-        const size_t r0 = (size_t)s.first * Hq;
-        for (long long e = tid; e < (long long)s.count * Hq * D; e += kThreads) static_cast<__nv_bfloat16*>(a.c.o)[r0 * D + e] = __float2bfloat16(0.f);
-        if (a.c.lse != nullptr)
-            for (int e = tid; e < s.count * Hq; e += kThreads) a.c.lse[r0 + e] = -INFINITY;
-    }
+    if (tid == 0) flags[0] = flags[1] = flags[2] = 0;
+    find_start<kThreads>(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
     const long long tiles = start.end - start.begin;
-    if (tiles <= 0) return;
 
     uint8_t* ring = sm + warp * kStages * L::kStage;
-    Walk ahead, w;
-    ahead.set(b, start, window);
-    w.set(b, start, window);
+    Walk ahead = {}, w = {};
     auto in_reach = [&](const Walk& x) {
         const int k0 = x.tile * kTile + 16 * warp;
         return k0 < x.s.hi && k0 + 16 > x.s.lo;
@@ -240,14 +252,63 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         ahead.next(b, Hk, window);
         look();
     };
-    look();
+    // queries of one sequence and kv head: a piece of eight values a thread and 8 rows, first to registers, then to shared memory
+    uint4 piece[NR];
+    auto fetch_q = [&](const Walk& x) {
+        const int rows = min(x.s.count * g, kRows);
+#pragma unroll
+        for (int y = 0; y < NR; ++y) {
+            const int e = tid + y * kThreads, r = e / (DP / 8), d = 8 * (e % (DP / 8));
+            piece[y] = make_uint4(0, 0, 0, 0);
+            if (r < rows && d < D) {
+                const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.c.q) + (x.s.first + r / g) * a.c.strides.q_token + (x.hk * g + r % g) * a.c.strides.q_head + d;
+                if (a.q16) {
+                    piece[y] = __ldg(reinterpret_cast<const uint4*>(src));
+                } else {
+                    const unsigned short* p = reinterpret_cast<const unsigned short*>(src);
+                    piece[y] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+                }
+            }
+        }
+    };
+    auto q_at = [&](int buffer, int r, int chunk) { return sm + L::kQ + buffer * kRows * DP * 2 + r * DP * 2 + ((chunk ^ (r & 7)) << 4); };
+    auto put_q = [&](int buffer) {
+#pragma unroll
+        for (int y = 0; y < NR; ++y) {
+            const int e = tid + y * kThreads;
+            if (e < kRows * DP / 8) *reinterpret_cast<uint4*>(q_at(buffer, e / (DP / 8), e % (DP / 8))) = piece[y];
+        }
+    };
+
     long long issued = 0;
-    for (; issued < kStages - 1 && issued < tiles; ++issued) load(issued);
+    if (tiles > 0) {
+        ahead.set(b, start, window);
+        w = ahead;
+        look();
+        fetch_q(w);
+        for (; issued < kStages - 1 && issued < tiles; ++issued) load(issued);
+    }
+    // sequences without a key in reach have no tile: their rows are nothing
+    for (int n = blockIdx.x; n < b.n_seq; n += gridDim.x) {
+        const Seq s = seq_at(b, n, window);
+        if (tid == 0) {
+            if (!b.span_ok(n) || s.count * g > kRows) b.tell(KDA_ERR_CU_SEQLENS);
+            if (!b.kv_len_ok(n)) b.tell(KDA_ERR_BLOCK_TABLE);
+        }
+        if (s.t1 > s.t0) continue;
+        const size_t r0 = (size_t)s.first * Hq;
+        for (long long e = tid; e < (long long)s.count * Hq * D; e += kThreads) static_cast<__nv_bfloat16*>(a.c.o)[r0 * D + e] = __float2bfloat16(0.f);
+        if (a.c.lse != nullptr)
+            for (int e = tid; e < s.count * Hq; e += kThreads) a.c.lse[r0 + e] = -INFINITY;
+    }
+    if (tiles <= 0) return;
+    put_q(0);
+    __syncthreads();
 
     const float c = a.c.scale * 1.4426950408889634f, lazy = kLazy / c;
-    uint32_t q[kHalves * 4][4];
-    float acc[kNt][4], m[2], l[2];
-    int last[2], first[2], all_lo = 0, all_hi = 0, unit_begin = 0;
+    uint32_t q[NR][kSteps][2];
+    float acc[NR][kSteps][4], m[NR][2], l[NR][2];      // O^T: values r8, r8 + 8 of each 16, rows 2 c4, 2 c4 + 1 of each 8
+    int last[NR][2], first[NR][2], rows = 0, all_lo = 0, all_hi = 0, unit_begin = 0, q_buffer = 0;
     bool fresh = true;
     uint32_t phases = 0;      // of the ring's barriers: a tile out of this warp's reach leaves its place as it is
     const int mi = lane >> 3, mr = lane & 7;
@@ -257,45 +318,37 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             __syncwarp();
             load(issued++);
         }
-        const int rows = w.s.count * g < kRows ? w.s.count * g : kRows;
-        auto global_row = [&](int r) { return (size_t)(w.s.first + r / g) * Hq + w.hk * g + r % g; };
         if (fresh) {
             fresh = false;
+            Walk then = w;      // the queries that come next, on their way while these work
+            then.tile = w.s.t1 - 1;
+            then.next(b, Hk, window);
+            if (tiles - i > w.s.t1 - w.tile) fetch_q(then);
+            rows = min(w.s.count * g, kRows);
             unit_begin = w.tile;
             all_lo = window > 0 ? max(w.s.base + (rows - 1) / g - window + 1, 0) : 0;
             all_hi = w.s.base + 1;
-            const __nv_bfloat16* src[2];
-            bool is[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int r = r8 + 8 * x;
-                is[x] = r < rows;
-                last[x] = is[x] ? w.s.base + r / g : -1;
-                first[x] = window > 0 ? last[x] - window + 1 : 0;
-                src[x] = static_cast<const __nv_bfloat16*>(a.c.q) + (w.s.first + r / g) * a.c.strides.q_token + (w.hk * g + r % g) * a.c.strides.q_head;
-                m[x] = -INFINITY;
-                l[x] = 0.f;
-            }
+            for (int y = 0; y < NR; ++y) {
 #pragma unroll
-            for (int k = 0; k < kHalves * 4; ++k)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {      // rows r8, r8 + 8; values 2 c4, 2 c4 + 8 of step k
-                    const int d = 16 * k + 2 * c4 + 8 * (x >> 1);
-                    uint32_t v = 0;
-                    if (is[x & 1] && d < D) {
-                        if (a.q4) {
-                            v = __ldg(reinterpret_cast<const uint32_t*>(src[x & 1] + d));
-                        } else {
-                            const unsigned short* s = reinterpret_cast<const unsigned short*>(src[x & 1] + d);
-                            v = s[0] | (uint32_t)s[1] << 16;
-                        }
-                    }
-                    q[k][x] = v;
+                for (int x = 0; x < 2; ++x) {
+                    const int r = 8 * y + 2 * c4 + x;
+                    last[y][x] = r < rows ? w.s.base + r / g : -1;
+                    first[y][x] = window > 0 ? last[y][x] - window + 1 : 0;
+                    m[y][x] = -INFINITY;
+                    l[y][x] = 0.f;
                 }
 #pragma unroll
-            for (int t = 0; t < kNt; ++t)
+                for (int t = 0; t < kSteps; ++t)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) acc[t][x] = 0.f;
+                    for (int x = 0; x < 4; ++x) acc[y][t][x] = 0.f;
+#pragma unroll
+                for (int k = 0; k < kSteps; k += 2) {
+                    uint32_t f[4];
+                    ldm4(f, smem_u32(q_at(q_buffer, 8 * y + mr, 2 * k + mi)));
+                    q[y][k][0] = f[0]; q[y][k][1] = f[1]; q[y][k + 1][0] = f[2]; q[y][k + 1][1] = f[3];
+                }
+            }
         }
         if (in_reach(w)) {
             const int s = (int)(i % kStages), k0 = w.tile * kTile + 16 * warp;
@@ -311,6 +364,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             if (partial) {
                 // keys that no row sees hold anything: their values are blanked, and so are values that are not finite at keys
                 // only some rows see (added at the end by those that do)
+#pragma unroll 1
                 for (int e = lane; e < 16 * kHalves * 8; e += 32) {
                     const int r = e & 15, ch = e >> 4, key = k0 + r;
                     if (key >= all_lo && key < all_hi) continue;
@@ -329,247 +383,271 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                     }
                     if (odd) {
                         *at = x;
-                        flags[1] = 1;
+                        flags[1 + q_buffer] = 1;
                     }
                 }
                 fence_async_smem();
                 __syncwarp();
             }
-            float s2[2][2][4] = {};      // scores of keys 0 .. 7, 8 .. 15; two chains each
+            float s2[2][NR][4] = {};      // S^T: keys r8, r8 + 8, rows 2 c4, 2 c4 + 1; two chains
 #pragma unroll
-            for (int k = 0; k < kHalves * 4; ++k) {
+            for (int k = 0; k < kSteps; ++k) {
                 uint32_t kf[4];
-                ldm4(kf, sk + (k >> 2) * L::kHalf + sw128_off((mi >> 1) * 8 + mr, 2 * (k & 3) + (mi & 1)));
-                mma(s2[k & 1][0], q[k], kf[0], kf[1]);
-                mma(s2[k & 1][1], q[k], kf[2], kf[3]);
+                ldm4(kf, sk + (k >> 2) * L::kHalf + sw128_off((mi & 1) * 8 + mr, 2 * (k & 3) + (mi >> 1)));
+#pragma unroll
+                for (int y = 0; y < NR; ++y) mma(s2[k & 1][y], kf, q[y][k][0], q[y][k][1]);
             }
-            float sc[2][4];
+            float sc[NR][4];
+            bool grow = false;
+            float top[NR][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int y = 0; y < NR; ++y) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) sc[t][x] = s2[0][t][x] + s2[1][t][x];
-            float top[2] = {kLowest, kLowest};
-            if (partial) {
+                for (int x = 0; x < 4; ++x) sc[y][x] = s2[0][y][x] + s2[1][y][x];
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int x = 0; x < 2; ++x) top[y][x] = kLowest;
+                if (partial) {
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        const int key = k0 + 8 * t + 2 * c4 + (x & 1);
-                        if (key < first[x >> 1] || key > last[x >> 1]) sc[t][x] = -INFINITY;
+                        const int key = k0 + r8 + 8 * (x >> 1);
+                        if (key < first[y][x & 1] || key > last[y][x & 1]) sc[y][x] = -INFINITY;
                     }
 #pragma unroll
-                for (int x = 0; x < 2; ++x)
-                    if (last[x] < k0 || first[x] >= k0 + 16) top[x] = -INFINITY;
-            }
-            bool grow = false;
+                    for (int x = 0; x < 2; ++x)
+                        if (last[y][x] < k0 || first[y][x] >= k0 + 16) top[y][x] = -INFINITY;
+                }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                top[x] = max_nan(top[x], max_nan(max_nan(sc[0][2 * x], sc[0][2 * x + 1]), max_nan(sc[1][2 * x], sc[1][2 * x + 1])));
-                top[x] = max_nan(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
-                top[x] = max_nan(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
-                grow |= !(top[x] <= m[x] + lazy) && !(top[x] == -INFINITY);
+                for (int x = 0; x < 2; ++x) {
+                    top[y][x] = max_nan(top[y][x], max_nan(sc[y][x], sc[y][x + 2]));
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) top[y][x] = max_nan(top[y][x], __shfl_xor_sync(0xffffffffu, top[y][x], o));
+                    grow |= !(top[y][x] <= m[y][x] + lazy) && !(top[y][x] == -INFINITY);
+                }
             }
             if (__any_sync(0xffffffffu, grow)) {
-                float f[2];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const float next = max_nan(m[x], top[x]);
-                    f[x] = m[x] == -INFINITY ? 0.f : ex2((m[x] - next) * c);
-                    m[x] = next;
-                    l[x] *= f[x];
+                for (int y = 0; y < NR; ++y) {
+                    float f[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const float next = max_nan(m[y][x], top[y][x]);
+                        f[x] = m[y][x] == -INFINITY ? 0.f : ex2((m[y][x] - next) * c);
+                        m[y][x] = next;
+                        l[y][x] *= f[x];
+                    }
+#pragma unroll
+                    for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) acc[y][t][x] *= f[x & 1];
                 }
-#pragma unroll
-                for (int t = 0; t < kNt; ++t)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) acc[t][x] *= f[x >> 1];
             }
-            uint32_t hi[4], lo[4];
+            uint32_t hi[NR][2], lo[NR][2];      // P^T: keys 0 .. 7, 8 .. 15
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int y = 0; y < NR; ++y) {
+                float mc[2];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const float mc = m[x] == -INFINITY ? 0.f : max_nan(m[x] * c, kLowest);
-                    const float p0 = ex2(fmaf(sc[t][2 * x], c, -mc)), p1 = ex2(fmaf(sc[t][2 * x + 1], c, -mc));
-                    l[x] += p0 + p1;
+                for (int x = 0; x < 2; ++x) mc[x] = m[y][x] == -INFINITY ? 0.f : max_nan(m[y][x] * c, kLowest);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const float p0 = ex2(fmaf(sc[y][2 * t], c, -mc[0])), p1 = ex2(fmaf(sc[y][2 * t + 1], c, -mc[1]));
+                    l[y][0] += p0;
+                    l[y][1] += p1;
                     const uint32_t h = pack_bf16(p0, p1);
-                    hi[2 * t + x] = h;
-                    lo[2 * t + x] = pack_bf16(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u));
+                    hi[y][t] = turned(h);
+                    lo[y][t] = turned(pack_bf16(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u)));
                 }
+            }
 #pragma unroll
-            for (int t = 0; t < kNt / 2; ++t) {
+            for (int t = 0; t < kSteps; ++t) {
                 uint32_t vf[4];
-                ldm4t(vf, sv + (t >> 2) * L::kHalf + sw128_off((mi & 1) * 8 + mr, 2 * (t & 3) + (mi >> 1)));
-                mma(acc[2 * t], hi, vf[0], vf[1]);
-                mma(acc[2 * t + 1], hi, vf[2], vf[3]);
-                mma(acc[2 * t], lo, vf[0], vf[1]);
-                mma(acc[2 * t + 1], lo, vf[2], vf[3]);
+                ldm4t(vf, sv + (t >> 2) * L::kHalf + sw128_off((mi >> 1) * 8 + mr, 2 * (t & 3) + (mi & 1)));
+#pragma unroll
+                for (int y = 0; y < NR; ++y) {
+                    mma(acc[y][t], vf, hi[y][0], hi[y][1]);
+                    mma(acc[y][t], vf, lo[y][0], lo[y][1]);
+                }
             }
         }
         const bool ends = w.tile + 1 == w.s.t1;
+        Walk then = w;
+        then.next(b, Hk, window);
         if (ends || i + 1 == tiles) {
             // ------------------------------------------------------------------ the warps' sums become one
             fresh = true;
+            // through the ring's places of this tile, which are free until the next but one; [row][value], pieces of eight values
+            // exchanged so that the lanes' rows lie in different banks
+            static_assert(L::kStage >= kRows * DP * 4, "a warp's sums fit a place of the ring");
+            const int place = (int)(i % kStages) * L::kStage;
+            float* mine = reinterpret_cast<float*>(ring + place);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-                l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-                if (c4 == 0) row_ml[warp * kRows + r8 + 8 * x] = make_float2(m[x], l[x]);
-            }
-            __syncthreads();
-            float M[2], Lsum[2];
+            for (int y = 0; y < NR; ++y)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float2 o[kWarps];
-                M[x] = -INFINITY;
+                for (int x = 0; x < 2; ++x) {
+                    const int r = 8 * y + 2 * c4 + x;
 #pragma unroll
-                for (int k = 0; k < kWarps; ++k) {
-                    o[k] = row_ml[k * kRows + r8 + 8 * x];
-                    M[x] = max_nan(M[x], o[k].x);
-                }
-                Lsum[x] = 0.f;
+                    for (int o = 4; o < 32; o <<= 1) l[y][x] += __shfl_xor_sync(0xffffffffu, l[y][x], o);
+                    if (r8 == 0) row_ml[warp * kRows + r] = make_float2(m[y][x], l[y][x]);
 #pragma unroll
-                for (int k = 0; k < kWarps; ++k) Lsum[x] += o[k].x == -INFINITY ? 0.f : o[k].y * ex2((o[k].x - M[x]) * c);
-                const float f = m[x] == -INFINITY ? 0.f : ex2((m[x] - M[x]) * c);
-#pragma unroll
-                for (int t = 0; t < kNt; ++t) {
-                    acc[t][2 * x] *= f;
-                    acc[t][2 * x + 1] *= f;
-                }
-            }
-            // through the ring's places of this tile, which are free until the next but one
-            static_assert(L::kStage == kRows * DP * 4, "a warp's sums fill a place of the ring");
-#pragma unroll
-            for (int half = kWarps / 2; half > 0; half >>= 1) {
-                if (warp >= half && warp < 2 * half) {
-                    float4* join = reinterpret_cast<float4*>(ring + (int)(i % kStages) * L::kStage);
-#pragma unroll
-                    for (int t = 0; t < kNt; ++t) join[t * 32 + lane] = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
-                }
-                __syncthreads();
-                if (warp < half) {
-                    const float4* join = reinterpret_cast<const float4*>(sm + ((warp + half) * kStages + (int)(i % kStages)) * L::kStage);
-#pragma unroll
-                    for (int t = 0; t < kNt; ++t) {
-                        const float4 o = join[t * 32 + lane];
-                        acc[t][0] += o.x; acc[t][1] += o.y; acc[t][2] += o.z; acc[t][3] += o.w;
+                    for (int t = 0; t < kSteps; ++t) {
+                        mine[r * DP + ((16 * t + r8) ^ (c4 << 3))] = acc[y][t][x];
+                        mine[r * DP + ((16 * t + r8 + 8) ^ (c4 << 3))] = acc[y][t][x + 2];
                     }
                 }
-            }
-            fence_async_smem();
-            if (warp == 0) {
-                const bool begins = unit_begin == w.s.t0, whole = begins && ends;
-                if (flags[1]) {
-                    for (int key = max(w.s.lo, unit_begin * kTile); key < min(w.s.hi, (w.tile + 1) * kTile); ++key) {
+            __syncthreads();
+            const bool begins = unit_begin == w.s.t0, whole = begins && ends;
+            // a stretch's part: place 0 goes on from the block before, place 1 begins here
+            const size_t part = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRows;
+#pragma unroll 1
+            for (int e = tid; e < rows * (D / 4); e += kThreads) {
+                const int r = e / (D / 4), d = 4 * (e - r * (D / 4));
+                float2 ml[kWarps];
+                float M = -INFINITY, sum = 0.f;
+                f2 o0 = f2_all(0.f), o1 = f2_all(0.f);
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) {
+                    ml[k] = row_ml[k * kRows + r];
+                    M = max_nan(M, ml[k].x);
+                }
+#pragma unroll
+                for (int k = 0; k < kWarps; ++k) {
+                    if (ml[k].x == -INFINITY) continue;      // its sums are 0
+                    const float f = ex2((ml[k].x - M) * c);
+                    sum = fmaf(ml[k].y, f, sum);
+                    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm + k * kStages * L::kStage + place) + r * DP + (d ^ (((r >> 1) & 3) << 3)));
+                    o0 = f2_fma(f2_make(x.x, x.y), f2_all(f), o0);
+                    o1 = f2_fma(f2_make(x.z, x.w), f2_all(f), o1);
+                }
+                float2 oa = f2_get(o0), ob = f2_get(o1);
+                float o[4] = {oa.x, oa.y, ob.x, ob.y};
+                if (M == kLowest) sum = 0.f;      // nothing but -inf: 0 / 0
+                if (flags[1 + q_buffer]) {
+                    const int to = w.s.base + r / g, from = window > 0 ? to - window + 1 : 0;
+#pragma unroll 1
+                    for (int key = max(max(from, 0), unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
                         if (key >= all_lo && key < all_hi) continue;
                         const int pg = b.page(w.n, key / b.page_size);
                         if (pg < 0) continue;
                         const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v) + pg * a.c.strides.v_page + (key % b.page_size) * a.c.strides.v_row +
-                                                 w.hk * a.c.strides.v_head;
+                                                 w.hk * a.c.strides.v_head + d;
 #pragma unroll
-                        for (int t = 0; t < kNt; ++t)
-#pragma unroll
-                            for (int x = 0; x < 4; ++x) {
-                                const int d = 8 * t + 2 * c4 + (x & 1);
-                                if (d >= D || key < first[x >> 1] || key > last[x >> 1]) continue;
-                                const float val = __bfloat162float(v[d]);
-                                if (!isfinite(val)) acc[t][x] += val;
-                            }
+                        for (int x = 0; x < 4; ++x) {
+                            const float val = __bfloat162float(v[x]);
+                            if (!isfinite(val)) o[x] += val;
+                        }
                     }
-                    __syncwarp();
-                    if (lane == 0) flags[1] = 0;
                 }
-                // a stretch's part: place 0 goes on from the block before, place 1 begins here
-                const size_t part = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRows;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int r = r8 + 8 * x;
-                    if (r >= rows) continue;
-                    if (M[x] == kLowest) Lsum[x] = 0.f;      // nothing but -inf: 0 / 0
-                    if (!whole) {
-                        if (c4 == 0) a.part_ml[part + r] = make_float2(M[x] * c, Lsum[x]);
-#pragma unroll
-                        for (int t = 0; t < kNt; ++t)
-                            if (8 * t < D) *reinterpret_cast<float2*>(a.part_o + (part + r) * D + 8 * t + 2 * c4) = make_float2(acc[t][2 * x], acc[t][2 * x + 1]);
-                        continue;
-                    }
-                    const size_t out = global_row(r);
-                    const float inv = M[x] == -INFINITY ? 0.f : 1.f / Lsum[x];
-                    if (c4 == 0 && a.c.lse != nullptr) a.c.lse[out] = M[x] == -INFINITY ? -INFINITY : (M[x] * c + log2f(Lsum[x])) * kLn2;
-#pragma unroll
-                    for (int t = 0; t < kNt; ++t)
-                        if (8 * t < D)
-                            *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + 8 * t + 2 * c4) =
-                                pack_bf16(acc[t][2 * x] * inv, acc[t][2 * x + 1] * inv);
+                if (!whole) {
+                    if (d == 0) a.part_ml[part + r] = make_float2(M * c, sum);
+                    *reinterpret_cast<float4*>(a.part_o + (part + r) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                    continue;
                 }
+                const size_t out = (size_t)(w.s.first + r / g) * Hq + w.hk * g + r % g;
+                const float inv = M == -INFINITY ? 0.f : 1.f / sum;
+                if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = M == -INFINITY ? -INFINITY : (M * c + log2f(sum)) * kLn2;
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
             }
+            q_buffer ^= 1;
+            if (tid == 0) flags[1 + q_buffer] = 0;
+            if (i + 1 < tiles) put_q(q_buffer);
+            fence_async_smem();
             __syncthreads();
         }
-        w.next(b, Hk, window);
+        w = then;
     }
     if (flags[0])      // no copy may be in flight when the block ends
         for (int s = 0; s < kStages; ++s) mbar_poll(bar + s, (phases >> s) & 1u, kSpinLimit / 8);
 }
 
 // Joins the parts of a sequence's kv head that more than one stretch has worked on.  Block i looks at the place where stretch i + 1
-// begins; the first such place inside a sequence takes all its parts.
-__global__ void __launch_bounds__(kThreads) attn_decode_join_kernel(const __grid_constant__ Args a) {
+// begins; the first such place inside a sequence takes all its parts.  Four values a thread; with few rows several threads share the
+// parts of one place and add up through shared memory.
+constexpr int kJoinThreads = 512, kMaxBlocks = 148 * kPerSm;
+template <int NR>
+__global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __grid_constant__ Args a) {
+    constexpr int kRows = 8 * NR;
     __shared__ Start start;
-    __shared__ long long sums[kWarps];
+    __shared__ long long sums[kJoinThreads / 32];
+    __shared__ float weight[kMaxBlocks * kRows], row_l[kRows], row_m[kRows];
+    __shared__ float4 acc[kJoinThreads];
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
-    find_start(b, Hk, window, a.blocks, id, &start, sums);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    find_start<kJoinThreads>(b, Hk, window, a.blocks, id, &start, sums);
     if (start.begin >= start.end) return;
     const Seq s = seq_at(b, start.n, window);
     const long long unit = start.begin - (start.tile - s.t0), unit_end = unit + (s.t1 - s.t0);      // of the list
     if (unit == start.begin || start.total * (id - 1) / start.blocks > unit) return;
     int parts = 1;      // stretches id - 1 .. id - 1 + parts
     while (id + parts < start.blocks && start.total * (id + parts) / start.blocks < unit_end) ++parts;
-    dependency_wait();
     const int rows = min(s.count * g, kRows);
-    for (int e = threadIdx.x; e < rows * (D / 4); e += kThreads) {
-        const int r = e / (D / 4), d = 4 * (e - r * (D / 4));
-        auto place = [&](int k) { return ((size_t)(id - 1 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
-        auto ml = [&](int k) {
-            const uint2 x = ld_after8(a.part_ml + place(k));
-            return make_float2(__uint_as_float(x.x), __uint_as_float(x.y));
-        };
-        float m = -INFINITY, l = 0.f, o[4] = {};
-#pragma unroll 4
-        for (int k = 0; k <= parts; ++k) m = max_nan(m, ml(k).x);
-#pragma unroll 4
-        for (int k = 0; k <= parts; ++k) {
-            const float2 x = ml(k);
-            const uint4 v = ld_after16(a.part_o + place(k) * D + d);
-            const float f = x.x == -INFINITY ? 0.f : ex2(x.x - m);
-            l = fmaf(x.y, f, l);
-            if (x.x == -INFINITY) continue;      // its sums are 0
+    auto place = [&](int k, int r) { return ((size_t)(id - 1 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
+    dependency_wait();
+    for (int r = warp; r < rows; r += kJoinThreads / 32) {      // a warp a row: 2^(m_k - m) of each part
+        float m = -INFINITY, l = 0.f;
+        for (int k = lane; k <= parts; k += 32) m = max_nan(m, ld_after_f32(&a.part_ml[place(k, r)].x));
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int k = lane; k <= parts; k += 32) {
+            const uint2 x = ld_after8(a.part_ml + place(k, r));
+            const float f = __uint_as_float(x.x) == -INFINITY ? 0.f : ex2(__uint_as_float(x.x) - m);
+            l = fmaf(__uint_as_float(x.y), f, l);
+            weight[k * kRows + r] = f;
+        }
+        l = warp_sum(l);
+        if (lane == 0) {
+            row_m[r] = m;
+            row_l[r] = l;
+        }
+    }
+    __syncthreads();
+    const int items = rows * (D / 4), share = max(kJoinThreads / items, 1), at = tid % min(items, kJoinThreads), of = tid / min(items, kJoinThreads);
+    if (of < share) {
+        const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
+        float o[4] = {};
+#pragma unroll 8
+        for (int k = of; k <= parts; k += share) {
+            const uint4 v = ld_after16(a.part_o + place(k, r) * D + d);
+            const float f = weight[k * kRows + r];
+            if (f == 0.f) continue;
             o[0] = fmaf(__uint_as_float(v.x), f, o[0]);
             o[1] = fmaf(__uint_as_float(v.y), f, o[1]);
             o[2] = fmaf(__uint_as_float(v.z), f, o[2]);
             o[3] = fmaf(__uint_as_float(v.w), f, o[3]);
         }
+        acc[tid] = make_float4(o[0], o[1], o[2], o[3]);
+    }
+    __syncthreads();
+    if (of != 0) return;
+    {
+        const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
+        float4 o = acc[at];
+        for (int k = 1; k < share; ++k) {
+            const float4 x = acc[k * items + at];
+            o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        }
         const size_t out = (size_t)(s.first + r / g) * Hq + start.hk * g + r % g;
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;
+        const float m = row_m[r], l = row_l[r], inv = m == -INFINITY ? 0.f : 1.f / l;
         if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
 }
 
-template <int DP>
+template <int DP, int NR>
 int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStream_t st) {
-    if (int rc = set_smem_limit(attn_decode_kernel<DP>, Layout<DP>::kBytes)) return rc;
-    KDA_LAUNCH("attn_decode_kernel", st, attn_decode_kernel<DP><<<a.blocks, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, a));
+    constexpr int kBytes = Layout<DP, NR>::kBytes;
+    if (int rc = set_smem_limit(attn_decode_kernel<DP, NR>, kBytes)) return rc;
+    KDA_LAUNCH("attn_decode_kernel", st, attn_decode_kernel<DP, NR><<<a.blocks, kThreads, kBytes, st>>>(mK, mV, a));
     if (int rc = launch_status()) return rc;
     if (a.blocks == 1) return KDA_OK;
     cudaError_t e = cudaSuccess;
-    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel, dim3(a.blocks - 1), kThreads, 0, st, true, 1, a));
+    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 // Stretches: as many as the machine holds, or as the longest batch that fits the table could use.
 int stretches(int n_seq, int kv_heads, long long reach) {
     const long long tiles = ((reach + kTile - 1) / kTile + 1) * n_seq * kv_heads, n = tiles / kMinTiles;
-    return (int)(n < 1 ? 1 : n < 148 * kPerSm ? n : 148 * kPerSm);
+    return (int)(n < 1 ? 1 : n < kMaxBlocks ? n : kMaxBlocks);
 }
 long long reach_of(int table_width, int page_size, int window, int max_q) {
     long long reach = (long long)table_width * page_size;
@@ -579,10 +657,10 @@ long long reach_of(int table_width, int page_size, int window, int max_q) {
 
 }  // namespace
 
-bool decode_takes(const Call& c) { return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= kRows && tc_takes(c); }
+bool decode_takes(const Call& c) { return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= kMaxRows && tc_takes(c); }
 
 size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim) {
-    const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q)) * 2 * kRows;
+    const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q)) * 2 * kMaxRows;
     return align_up(rows * sizeof(float2), 256) + rows * dim * sizeof(float);
 }
 
@@ -591,15 +669,17 @@ int decode(const Call& c, cudaStream_t st) {
     a.c = c;
     a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
     a.box_rows = c.batch.page_size < 16 ? c.batch.page_size : 16;
-    a.q4 = reinterpret_cast<uintptr_t>(c.q) % 4 == 0 && c.strides.q_token % 2 == 0 && c.strides.q_head % 2 == 0;
+    a.q16 = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.strides.q_token % 8 == 0 && c.strides.q_head % 8 == 0;
     a.part_ml = static_cast<float2*>(c.workspace);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up((size_t)a.blocks * 2 * kRows * sizeof(float2), 256));
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up((size_t)a.blocks * 2 * kMaxRows * sizeof(float2), 256));
     CUtensorMap mK, mV;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
     if (!rc) rc = make_map_paged(&mV, c.v, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.v_row, s.v_head, s.v_page, a.box_rows);
     if (rc) return rc;
-    return c.heads.dim <= 64 ? launch<64>(mK, mV, a, st) : launch<128>(mK, mV, a, st);
+    const bool few = c.max_q_len * c.heads.group <= 8;
+    if (c.heads.dim <= 64) return few ? launch<64, 1>(mK, mV, a, st) : launch<64, 2>(mK, mV, a, st);
+    return few ? launch<128, 1>(mK, mV, a, st) : launch<128, 2>(mK, mV, a, st);
 }
 
 }  // namespace attn

@@ -11,7 +11,8 @@
 //   lengths itself.  Where a stretch ends inside a sequence its part of the softmax goes to the workspace, and
 //   attn_decode_join_kernel puts the parts together.
 // - A warp takes 16 keys of a tile through a ring of its own (K and V by TMA, 128-byte swizzle), so that warps meet only where a
-//   sequence or the stretch ends.  The ring runs ahead across those places.
+//   sequence or the stretch ends.  The ring runs ahead across those places.  (Warps with stretches of their own, which never meet, left
+//   four times the parts to join and took longer: 32 x 16 heads 118 us, one conversation 22.)
 // - Products are mma.sync m16n8k16 with the keys as their 16 rows and the query rows as their 8 columns: S^T = K Q^T and O^T = V^T P^T
 //   (P^T comes from S^T's registers by movmatrix).  Up to 8 rows take half the products that rows of queries would.  The weights
 //   go as two bf16 terms, p = hi + lo, which leaves the output with the error of its own rounding.
@@ -33,10 +34,7 @@ using namespace tc;
 
 constexpr int kMaxRows = 16, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
 constexpr int kPerSm = 2;             // blocks an SM: 98 KB each
-#ifndef V_MT
-#define V_MT 2
-#endif
-constexpr int kMinTiles = V_MT;          // a stretch has at least these many tiles
+constexpr int kMinTiles = 2;          // a stretch has at least these many tiles
 constexpr float kLazy = 8.f;          // as in the kernel for long chunks: sums are rescaled when a maximum grew by 2^8
 constexpr int kStatusWait = 121;
 
@@ -47,12 +45,12 @@ struct Layout {
     static constexpr int kRowsOf = 8 * NR;
     static constexpr int kQ = kWarps * kStages * kStage;              // two sequences' queries
     static constexpr int kBars = kQ + 2 * kRowsOf * DP * 2;
-    static constexpr int kBytes = kBars + 1024 + 1024;
+    static constexpr int kBytes = kBars + 1024 + 1024;      // barriers and what the warps tell each other; slack to align the tiles
 };
 
 struct Args {
     Call c;
-    int blocks, box_rows, q16;
+    int blocks, box_rows;
     float* part_o;        // [blocks][2][rows][D]
     float2* part_ml;      // [blocks][2][rows]
 };
@@ -84,59 +82,61 @@ __device__ __forceinline__ Seq seq_of_raw(const Batch& b, const Raw& r, int wind
 }
 __device__ __forceinline__ Seq seq_at(const Batch& b, int n, int window) { return seq_of_raw(b, raw_at(b, n), window); }
 
-struct Start {
-    long long total, begin, end;      // tiles of the batch; this stretch
-    int blocks;                       // stretches in use
-    int n, hk, tile;                  // where it begins
+// How the list is cut: the first `longer` stretches have `each` + 1 tiles, the others `each`.
+struct Cut {
+    int total, each, longer, used;
+    __device__ __forceinline__ int begin(int id) const { return id >= used ? total : id * each + min(id, longer); }
 };
-// The stretch of block `id`; called by all THREADS of a block, `sums` has a place for each warp.
+struct Start {
+    Seq s;                // where a stretch begins
+    Raw after;
+    int n, hk, tile;
+};
+// The cut, and where stretch `id` begins.  Called by all THREADS of a block; `sums` has a place for each warp.  The host takes
+// care that the list has less than 2^31 tiles.
 template <int THREADS>
-__device__ __forceinline__ void find_start(const Batch& b, int kv_heads, int window, int blocks, int id, Start* shared, long long* sums) {
+__device__ __forceinline__ Cut find_start(const Batch& b, int kv_heads, int window, int blocks, int id, Start* start, int* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = (b.n_seq + THREADS - 1) / THREADS, n0 = min(tid * each, b.n_seq), n1 = min(n0 + each, b.n_seq);
-    long long mine = 0;
+    int mine = 0;
     for (int n = n0; n < n1; ++n) {
         const Seq s = seq_at(b, n, window);
-        mine += (long long)(s.t1 - s.t0) * kv_heads;
+        mine += (s.t1 - s.t0) * kv_heads;
     }
-    long long upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += x;
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    long long total = 0;
+    Cut cut;
+    cut.total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) upto += sums[w];
-        total += sums[w];
+        cut.total += sums[w];
     }
-    const long long used = min((long long)blocks, max(total / kMinTiles, 1ll));
-    const long long begin = id < used ? total * id / used : total, end = id < used ? total * (id + 1) / used : total;
-    long long at = upto - mine;
-    if (begin < end && begin >= at && begin < upto) {
+    cut.used = min(blocks, max(cut.total / kMinTiles, 1));
+    cut.each = cut.total / cut.used;
+    cut.longer = cut.total - cut.each * cut.used;
+    const int begin = cut.begin(id);
+    int at = upto - mine;
+    if (begin >= at && begin < upto) {
         for (int n = n0; n < n1; ++n) {
             const Seq s = seq_at(b, n, window);
-            const long long here = (long long)(s.t1 - s.t0) * kv_heads;
+            const int nt = s.t1 - s.t0, here = nt * kv_heads;
             if (begin < at + here) {
-                const int rest = (int)(begin - at), nt = s.t1 - s.t0;
-                shared->n = n;
-                shared->hk = rest / nt;
-                shared->tile = s.t0 + rest % nt;
+                const int rest = begin - at, hk = rest / nt;
+                *start = Start{s, raw_at(b, n + 1), n, hk, s.t0 + rest - hk * nt};
                 break;
             }
             at += here;
         }
     }
-    if (tid == 0) {
-        shared->total = total;
-        shared->begin = begin;
-        shared->end = end;
-        shared->blocks = (int)used;
-    }
     __syncthreads();
+    return cut;
 }
 
 // A place in the list.
@@ -144,12 +144,12 @@ struct Walk {
     Seq s;
     Raw after;      // of the next sequence, read when this one is entered: nothing waits for it
     int n, hk, tile;
-    __device__ __forceinline__ void set(const Batch& b, const Start& at, int window) {
+    __device__ __forceinline__ void set(const Start& at) {
+        s = at.s;
+        after = at.after;
         n = at.n;
         hk = at.hk;
         tile = at.tile;
-        s = seq_at(b, n, window);
-        after = raw_at(b, n + 1);
     }
     __device__ __forceinline__ void next(const Batch& b, int kv_heads, int window) {
         if (++tile < s.t1) return;
@@ -201,9 +201,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
     Start& start = *reinterpret_cast<Start*>(bars + kWarps * kStages);
-    long long* sums = reinterpret_cast<long long*>(&start + 1);
+    int* sums = reinterpret_cast<int*>(&start + 1);
     volatile int* flags = reinterpret_cast<volatile int*>(sums + kWarps);      // [0] an expired wait, [1], [2] values that are not finite (of sequences in turn)
-    float2* row_ml = reinterpret_cast<float2*>(sums + kWarps + 2);             // [warps][rows]
+    float2* row_ml = reinterpret_cast<float2*>(bars + 64);                     // [warps][rows]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, c4 = lane & 3, r8 = lane >> 2;
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window;
@@ -215,8 +215,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         mbar_fence_init();
     }
     if (tid == 0) flags[0] = flags[1] = flags[2] = 0;
-    find_start<kThreads>(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
-    const long long tiles = start.end - start.begin;
+    const Cut cut = find_start<kThreads>(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
+    const int tiles = cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
 
     uint8_t* ring = sm + warp * kStages * L::kStage;
     Walk ahead = {}, w = {};
@@ -237,8 +237,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             if (page < 0) b.tell(KDA_ERR_BLOCK_TABLE);
         }
     };
-    auto load = [&](long long i) {      // the tile `ahead` is at, into the ring's place i; then on to the next one
-        const int s = (int)(i % kStages);
+    auto load = [&](int i) {      // the tile `ahead` is at, into the ring's place i; then on to the next one
+        const int s = i % kStages;
         if (in_reach(ahead)) {
             const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
             if (lane == 0) mbar_expect_tx(bar + s, loads * a.box_rows * 128);
@@ -262,12 +262,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             piece[y] = make_uint4(0, 0, 0, 0);
             if (r < rows && d < D) {
                 const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.c.q) + (x.s.first + r / g) * a.c.strides.q_token + (x.hk * g + r % g) * a.c.strides.q_head + d;
-                if (a.q16) {
-                    piece[y] = __ldg(reinterpret_cast<const uint4*>(src));
-                } else {
-                    const unsigned short* p = reinterpret_cast<const unsigned short*>(src);
-                    piece[y] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
-                }
+                piece[y] = __ldg(reinterpret_cast<const uint4*>(src));
             }
         }
     };
@@ -280,9 +275,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         }
     };
 
-    long long issued = 0;
+    int issued = 0;
     if (tiles > 0) {
-        ahead.set(b, start, window);
+        ahead.set(start);
         w = ahead;
         look();
         fetch_q(w);
@@ -313,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
     uint32_t phases = 0;      // of the ring's barriers: a tile out of this warp's reach leaves its place as it is
     const int mi = lane >> 3, mr = lane & 7;
 
-    for (long long i = 0; i < tiles; ++i) {
+    for (int i = 0; i < tiles; ++i) {
         if (issued < tiles) {
             __syncwarp();
             load(issued++);
@@ -351,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             }
         }
         if (in_reach(w)) {
-            const int s = (int)(i % kStages), k0 = w.tile * kTile + 16 * warp;
+            const int s = i % kStages, k0 = w.tile * kTile + 16 * warp;
             if (!flags[0] && !mbar_poll(bar + s, (phases >> s) & 1u, kSpinLimit)) {      // carries on: the warps meet further down
                 flags[0] = 1;
                 b.tell(kStatusWait);
@@ -477,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             // through the ring's places of this tile, which are free until the next but one; [row][value], pieces of eight values
             // exchanged so that the lanes' rows lie in different banks
             static_assert(L::kStage >= kRows * DP * 4, "a warp's sums fit a place of the ring");
-            const int place = (int)(i % kStages) * L::kStage;
+            const int place = i % kStages * L::kStage;
             float* mine = reinterpret_cast<float*>(ring + place);
 #pragma unroll
             for (int y = 0; y < NR; ++y)
@@ -537,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                     }
                 }
                 if (!whole) {
-                    if (d == 0) a.part_ml[part + r] = make_float2(M * c, sum);
+                    if (d == 0) a.part_ml[part + r] = make_float2(M == -INFINITY ? M : max_nan(M * c, kLowest), sum);
                     *reinterpret_cast<float4*>(a.part_o + (part + r) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
                     continue;
                 }
@@ -566,19 +561,19 @@ template <int NR>
 __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __grid_constant__ Args a) {
     constexpr int kRows = 8 * NR;
     __shared__ Start start;
-    __shared__ long long sums[kJoinThreads / 32];
+    __shared__ int sums[kJoinThreads / 32];
     __shared__ float weight[kMaxBlocks * kRows], row_l[kRows], row_m[kRows];
     __shared__ float4 acc[kJoinThreads];
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    find_start<kJoinThreads>(b, Hk, window, a.blocks, id, &start, sums);
-    if (start.begin >= start.end) return;
-    const Seq s = seq_at(b, start.n, window);
-    const long long unit = start.begin - (start.tile - s.t0), unit_end = unit + (s.t1 - s.t0);      // of the list
-    if (unit == start.begin || start.total * (id - 1) / start.blocks > unit) return;
+    const Cut cut = find_start<kJoinThreads>(b, Hk, window, a.blocks, id, &start, sums);
+    if (id >= cut.used) return;
+    const Seq s = start.s;
+    const int unit = cut.begin(id) - (start.tile - s.t0), unit_end = unit + (s.t1 - s.t0);      // of the list
+    if (unit == cut.begin(id) || cut.begin(id - 1) > unit) return;
     int parts = 1;      // stretches id - 1 .. id - 1 + parts
-    while (id + parts < start.blocks && start.total * (id + parts) / start.blocks < unit_end) ++parts;
+    while (id + parts < cut.used && cut.begin(id + parts) < unit_end) ++parts;
     const int rows = min(s.count * g, kRows);
     auto place = [&](int k, int r) { return ((size_t)(id - 1 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + r; };
     dependency_wait();
@@ -657,7 +652,10 @@ long long reach_of(int table_width, int page_size, int window, int max_q) {
 
 }  // namespace
 
-bool decode_takes(const Call& c) { return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= kMaxRows && tc_takes(c); }
+bool decode_takes(const Call& c) {
+    const long long tiles = (long long)c.batch.n_seq * c.heads.kv_heads * ((long long)c.batch.table_width * c.batch.page_size / kTile + 2);
+    return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= kMaxRows && tiles < 1ll << 31 && tc_takes(c);
+}
 
 size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim) {
     const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q)) * 2 * kMaxRows;
@@ -669,7 +667,6 @@ int decode(const Call& c, cudaStream_t st) {
     a.c = c;
     a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
     a.box_rows = c.batch.page_size < 16 ? c.batch.page_size : 16;
-    a.q16 = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.strides.q_token % 8 == 0 && c.strides.q_head % 8 == 0;
     a.part_ml = static_cast<float2*>(c.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up((size_t)a.blocks * 2 * kMaxRows * sizeof(float2), 256));
     CUtensorMap mK, mV;

@@ -47,7 +47,7 @@ struct Layout {
 struct Args {
     Call c;
     Tiles tiles;
-    int slots, splits, box_rows, q16;
+    int slots, splits, box_rows;
     float* part_o;
     float2* part_ml;
 };
@@ -160,12 +160,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (row < u.rows && 8 * c < D) {
                     const int pr = u.row0 + row, tok = pr / g;
                     const __nv_bfloat16* src = q + (u.first + tok) * a.c.strides.q_token + (hk * g + pr - tok * g) * a.c.strides.q_head + 8 * c;
-                    if (a.q16) {
-                        x = __ldg(reinterpret_cast<const uint4*>(src));
-                    } else {
-                        const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
-                        x = make_uint4(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16, s[4] | (uint32_t)s[5] << 16, s[6] | (uint32_t)s[7] << 16);
-                    }
+                    x = __ldg(reinterpret_cast<const uint4*>(src));
                 }
                 *reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + sw128_off(r, c & 7)) = x;
             }
@@ -275,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const bool split = a.splits > 1;
             const size_t at = (size_t)z * b.tokens * a.c.heads.q_heads + out;
             const float inv = split ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
-            if (mine && split) a.part_ml[at] = make_float2(m * c, l);
+            if (mine && split) a.part_ml[at] = make_float2(m == -INFINITY ? m : max_nan(m * c, kLowest), l);
             if (mine && !split && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m * c + log2f(l)) * kLn2;
             uint8_t* stage_out = sm + t * L::kTile + (warp & 3) * 32 * (DP * 2);      // Q has been read
 #pragma unroll
@@ -499,8 +494,8 @@ bool tc_takes(const Call& c) {
     const int page = c.batch.page_size;
     if (!c.bf16 || c.heads.dim > 128 || c.heads.dim % 8 != 0 || !(page % kKeys == 0 || (kKeys % page == 0 && page >= 8))) return false;
     if (c.batch.n_pages == 0 || c.batch.table_width == 0) return false;
-    const long long all = s.k_page | s.k_row | s.k_head | s.v_page | s.v_row | s.v_head;
-    if (all % 8 != 0 || reinterpret_cast<uintptr_t>(c.k) % 16 != 0 || reinterpret_cast<uintptr_t>(c.v) % 16 != 0 || reinterpret_cast<uintptr_t>(c.o) % 16 != 0)
+    const long long all = s.q_token | s.q_head | s.k_page | s.k_row | s.k_head | s.v_page | s.v_row | s.v_head;
+    if (all % 8 != 0 || reinterpret_cast<uintptr_t>(c.q) % 16 != 0 || reinterpret_cast<uintptr_t>(c.k) % 16 != 0 || reinterpret_cast<uintptr_t>(c.v) % 16 != 0 || reinterpret_cast<uintptr_t>(c.o) % 16 != 0)
         return false;
     for (long long x : {s.k_page, s.k_row, s.k_head, s.v_page, s.v_row, s.v_head})
         if (x <= 0 || x >= 1ll << 39) return false;
@@ -514,7 +509,6 @@ int tc(const Call& c, int splits, cudaStream_t st) {
     a.slots = (int)tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq);
     a.splits = splits;
     a.box_rows = c.batch.page_size < kKeys ? c.batch.page_size : kKeys;
-    a.q16 = reinterpret_cast<uintptr_t>(c.q) % 16 == 0 && c.strides.q_token % 8 == 0 && c.strides.q_head % 8 == 0;
     const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
     a.part_ml = static_cast<float2*>(c.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * splits * sizeof(float2), 256));

@@ -205,17 +205,25 @@ OptTensor append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
 
 using AttentionOut = c10::optional<std::tuple<Tensor, OptTensor>>;
 
-AttentionOut attention(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const OptTensor& cu, int64_t max_q,
+// q itself, or a copy where its address or strides would keep it from the kernels for wide accesses
+Tensor wide(const Tensor& q) {
+    const int64_t unit = q.scalar_type() == at::kBFloat16 ? 8 : 4;
+    return reinterpret_cast<uintptr_t>(q.const_data_ptr()) % 16 == 0 && q.stride(0) % unit == 0 && q.stride(1) % unit == 0 ? q : q.clone(at::MemoryFormat::Contiguous);
+}
+
+AttentionOut attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const OptTensor& cu, int64_t max_q,
                        int64_t window, c10::optional<double> scale, bool want_lse) {
     KdaPagedShape pg;
-    if (tracing() || !paged_shape(q, kc, vc, table, lens, cu, max_q, window, pg)) return c10::nullopt;
-    if (at::GradMode::is_enabled() && (q.requires_grad() || kc.requires_grad() || vc.requires_grad())) return c10::nullopt;
+    if (tracing() || !paged_shape(q_, kc, vc, table, lens, cu, max_q, window, pg)) return c10::nullopt;
+    if (at::GradMode::is_enabled() && (q_.requires_grad() || kc.requires_grad() || vc.requires_grad())) return c10::nullopt;
     pg.scale = scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)pg.head_dim));
     if (!(pg.scale > 0.f) || !std::isfinite(pg.scale)) return c10::nullopt;
-    refuse_tangents(q, kc, vc);
-    c10::cuda::CUDAGuard guard(q.device());
-    watch_status(q.device().index());
+    refuse_tangents(q_, kc, vc);
+    c10::cuda::CUDAGuard guard(q_.device());
+    watch_status(q_.device().index());
     at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor q = wide(q_);
+    pg.q_token_stride = q.stride(0), pg.q_head_stride = q.stride(1);
     Tensor o = empty(q.sizes(), q.scalar_type(), q), ws;
     OptTensor lse;
     if (want_lse) lse = empty({q.size(0), q.size(1)}, at::kFloat, q);

@@ -32,7 +32,15 @@ using namespace tc;
 
 constexpr int kKeys = 128, kRows = 256;
 constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kFixWarp = 10, kThreads = 384;
+// Registers a thread: a row of scores is 128, and the loop over them needs room to overlap its steps.  384 x 168 in all.
+#define KDA_SOFTMAX_REGS "216"
+#define KDA_OTHER_REGS "72"
 constexpr float kLazy = 8.f;
+#ifndef V_POLY
+#define V_POLY 1
+#define V_POLYOF 4
+#endif
+constexpr int kPoly = V_POLY, kPolyOf = V_POLYOF;      // pairs of weights made by ex2_pair, of so many
 constexpr int kStatusWait = 120;      // device status of an expired wait
 
 template <int DP>
@@ -62,6 +70,26 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     float y;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// 2^x of a pair on the multiply-add pipes: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest relative
+// error is least there (2.6e-6; degree 3 leaves 7.5e-5, which the sums of few weights show), n added to the exponent.  The special function unit gives 16 values a cycle and SM, the tensor
+// pipe wants 128 x 128 of them every 1,024 cycles, so part of them is made here.
+__device__ __forceinline__ f2 ex2_pair(f2 x) {
+    const float2 v = f2_get(x);
+    x = f2_make(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
+    const f2 magic = f2_all(12582912.f);      // 1.5 x 2^23: the sum's low bits are n
+    const f2 t = f2_add(x, magic), f = f2_add(x, f2_fma(t, f2_all(-1.f), magic));
+    f2 p = f2_fma(f2_all(0.0095701022f), f, f2_all(0.0559178591f));
+    p = f2_fma(p, f, f2_all(0.2402474433f));
+    p = f2_fma(p, f, f2_all(0.6931217909f));
+    p = f2_fma(p, f, f2_all(0.9999992847f));
+    const float2 r = f2_get(p), n = f2_get(t);
+    return f2_make(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
 }
 __device__ __forceinline__ bool finite_bf16x2(uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; }
 
@@ -147,23 +175,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     auto turn = [](int i) { return (uint32_t)(i / L::kStages) & 1u; };
 
     if (warp < kSoftmaxWarps) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 " KDA_SOFTMAX_REGS ";");
         const int t = warp >> 2;
         // ------------------------------------------------------------------ Q into shared memory
         {
-            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.c.q);
-            uint8_t* tile = sm + t * L::kTile;
-            constexpr int kChunks = DP / 8;
-            for (int e = tid & 127; e < 128 * kChunks; e += 128) {
-                const int r = e / kChunks, c = e - r * kChunks, row = 128 * t + r;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (row < u.rows && 8 * c < D) {
-                    const int pr = u.row0 + row, tok = pr / g;
-                    const __nv_bfloat16* src = q + (u.first + tok) * a.c.strides.q_token + (hk * g + pr - tok * g) * a.c.strides.q_head + 8 * c;
-                    x = __ldg(reinterpret_cast<const uint4*>(src));
-                }
-                *reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + sw128_off(r, c & 7)) = x;
+            // DP / 8 lanes a row; all of a thread's copies are in flight together
+            constexpr int kChunks = DP / 8, kStep = 128 / kChunks;      // rows a pass
+            const int x = tid & 127, c = x % kChunks;
+            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.c.q) + 8 * c;
+            int r = x / kChunks, pr = u.row0 + 128 * t + r, tok = pr / g, head = pr - tok * g;
+#pragma unroll 1
+            for (; r < 128; r += kStep) {
+                const bool is = 128 * t + r < u.rows && 8 * c < D;
+                const __nv_bfloat16* src = is ? q + (u.first + tok) * a.c.strides.q_token + (hk * g + head) * a.c.strides.q_head : q;
+                const uint32_t dst = smem_u32(sm + t * L::kTile + (c >> 3) * 16384 + sw128_off(r, c & 7));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(is ? 16 : 0) : "memory");
+                for (head += kStep; head >= g; head -= g) ++tok;
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             fence_async_smem();
             warp_arrive(bar_q, lane);
         }
@@ -189,27 +218,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
             for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, s[q]);
             tmem_ld_wait();
-            float top = -INFINITY;
+            float top = kLowest;
             if (j * kKeys < w_lo || (j + 1) * kKeys > w_hi) {
-                const int k0 = j * kKeys;
+                const int from = first - j * kKeys, to = last - j * kKeys;      // of the tile's keys the row sees [from, to]
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
+                for (int q = 0; q < 4; ++q) {
+                    const int lo = min(max(from - 32 * q, 0), 32), hi = min(max(to - 32 * q + 1, 0), 32);
+                    const uint32_t seen = (uint32_t)((1ull << hi) - 1) & ~(uint32_t)((1ull << lo) - 1);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int key = k0 + 32 * q + e;
-                        if (key < first || key > last) s[q][e] = 0xff800000u;
-                    }
-                if (last >= k0 && first < k0 + kKeys) top = kLowest;
-            } else {
-                top = kLowest;
+                    for (int e = 0; e < 32; ++e)
+                        if (!(seen & 1u << e)) s[q][e] = 0xff800000u;
+                }
+                if (to < 0 || from >= kKeys) top = -INFINITY;
             }
             {
                 float x[4] = {top, top, top, top};
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
+                for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) x[q] = max_nan(x[q], __uint_as_float(s[q][e]));
-                top = max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+                    for (int q = 0; q < 4; ++q) x[q] = max_nan(x[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
+                top = max_nan(max_nan(x[0], x[1], x[2]), x[3]);
             }
             const bool grow = !(top <= m + lazy) && !(top == -INFINITY);      // a NaN too
             if (__any_sync(0xffffffffu, grow)) {
@@ -222,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     __syncwarp();
                     if (!ok) break;
                     tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                     for (int q = 0; q < DP / 32; ++q) {
                         uint32_t o[32];
                         tmem_ld32(tO + 32 * q, o);
@@ -242,8 +270,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
                     const int q = 2 * h + (e >> 4), at = 2 * (e & 15);
-                    const float2 x = f2_get(f2_fma(f2_make(__uint_as_float(s[q][at]), __uint_as_float(s[q][at + 1])), c2, n2));
-                    const f2 y = f2_make(ex2(x.x), ex2(x.y));
+                    const f2 x = f2_fma(f2_make(__uint_as_float(s[q][at]), __uint_as_float(s[q][at + 1])), c2, n2);
+                    f2 y;
+                    if (e % kPolyOf < kPoly) {
+                        y = ex2_pair(x);
+                    } else {
+                        const float2 z = f2_get(x);
+                        y = f2_make(ex2(z.x), ex2(z.y));
+                    }
                     sum[e & 1] = f2_add(sum[e & 1], y);
                     p[e] = f2_to_bf16(y);
                 }
@@ -264,7 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (ok && 128 * t + 32 * (warp & 3) < u.rows) {
             tc_fence_after();
             const bool mine = row < u.rows;
-            if (m == kLowest) l = 0.f;      // nothing but -inf: 0 / 0
+            if (m == kLowest) l = 0.f;                  // nothing but -inf: 0 / 0
+            if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);      // a NaN or +inf among the scores, which ex2_pair does not pass on
             const int tok = u.first + prow / g, head = hk * g + prow % g;
             const size_t out = (size_t)tok * a.c.heads.q_heads + head;
             const bool split = a.splits > 1;
@@ -273,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (mine && split) a.part_ml[at] = make_float2(m == -INFINITY ? m : max_nan(m * c, kLowest), l);
             if (mine && !split && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m * c + log2f(l)) * kLn2;
             uint8_t* stage_out = sm + t * L::kTile + (warp & 3) * 32 * (DP * 2);      // Q has been read
-#pragma unroll
+#pragma unroll 1
             for (int q = 0; q < DP / 32; ++q) {
                 uint32_t o[32];
                 if (n > 0) {
@@ -324,19 +359,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 __syncwarp();
                 constexpr int kLanes = DP / 8;      // lanes that hold a row
                 __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.c.o);
-#pragma unroll 4
-                for (int x = lane / kLanes; x < 32; x += 32 / kLanes) {
-                    const int chunk = lane % kLanes, wr = 128 * t + 32 * (warp & 3) + x;
+                const int chunk = lane % kLanes, wr = 128 * t + 32 * (warp & 3);
+                int x = lane / kLanes, pr = u.row0 + wr + x, tk = pr / g, hd = pr - tk * g;
+#pragma unroll 2
+                for (; x < 32; x += 32 / kLanes) {
                     const uint4 v = *reinterpret_cast<const uint4*>(stage_out + x * (DP * 2) + ((chunk ^ (x & 7)) << 4));
-                    if (wr < u.rows && 8 * chunk < D) {
-                        const int pr = u.row0 + wr, tk = pr / g;
-                        *reinterpret_cast<uint4*>(o + ((size_t)(u.first + tk) * a.c.heads.q_heads + hk * g + pr - tk * g) * D + 8 * chunk) = v;
-                    }
+                    if (wr + x < u.rows && 8 * chunk < D)
+                        *reinterpret_cast<uint4*>(o + ((size_t)(u.first + tk) * a.c.heads.q_heads + hk * g + hd) * D + 8 * chunk) = v;
+                    for (hd += 32 / kLanes; hd >= g; hd -= g) ++tk;
                 }
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 " KDA_OTHER_REGS ";");
         if (warp == kMmaWarp) {
             // -------------------------------------------------------------- products
             if (t_begin < t_end && elect_one()) {

@@ -7,7 +7,8 @@
 // 128 at a time.  Per key tile and row tile the tensor pipe does S (M128 N128 K = head) and O += P V (M128 N = head K128); the
 // two row tiles take turns: while one's scores are turned into weights by its four warps, the other's products run.  S and O
 // live in tensor memory, P (bf16) takes S's place there and is the A operand of its product, so nothing but K and V goes through
-// shared memory.  A thread owns a row: maximum and sum need no exchange.
+// shared memory.  A thread owns a row: maximum and sum need no exchange.  (Two threads a row, with twice the warps to cover each other's
+// waits, took as long: what the exchange of "a maximum has grown" costs is what they gain.  8,191 tokens 265 us.)
 //
 // O is rescaled only when a row's maximum has grown by more than 2^kLazy since the last time (the weights are then at most
 // 2^kLazy, which costs bf16 nothing: its rounding is relative); after a few tiles that no longer happens.
@@ -24,6 +25,8 @@ namespace kda {
 namespace tc {
 int make_map_paged(CUtensorMap* m, const void* ptr, uint64_t dim, uint64_t rows, uint64_t heads, uint64_t pages, int64_t row_ld, int64_t head_ld, int64_t page_ld,
                    uint32_t box_rows);
+int make_map_packed(CUtensorMap* m, const void* ptr, uint64_t dim, uint64_t heads, uint64_t tokens, int64_t head_ld, int64_t token_ld, uint32_t box_heads,
+                    uint32_t box_tokens);
 }
 namespace attn {
 namespace {
@@ -35,12 +38,8 @@ constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kFixWarp = 10, kTh
 // Registers a thread: a row of scores is 128, and the loop over them needs room to overlap its steps.  384 x 168 in all.
 #define KDA_SOFTMAX_REGS "216"
 #define KDA_OTHER_REGS "72"
+constexpr int kPolyOf = 4;            // one pair of weights of so many is made by ex2_pair (8,191 tokens: none 252 us, 1/4 246, 1/2 263; 64-wide heads 229, 206, 231)
 constexpr float kLazy = 8.f;
-#ifndef V_POLY
-#define V_POLY 1
-#define V_POLYOF 4
-#endif
-constexpr int kPoly = V_POLY, kPolyOf = V_POLYOF;      // pairs of weights made by ex2_pair, of so many
 constexpr int kStatusWait = 120;      // device status of an expired wait
 
 template <int DP>
@@ -55,7 +54,7 @@ struct Layout {
 struct Args {
     Call c;
     Tiles tiles;
-    int slots, splits, box_rows;
+    int slots, splits, box_rows, q_boxes;
     float* part_o;
     float2* part_ml;
 };
@@ -91,8 +90,6 @@ __device__ __forceinline__ f2 ex2_pair(f2 x) {
     const float2 r = f2_get(p), n = f2_get(t);
     return f2_make(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
 }
-__device__ __forceinline__ bool finite_bf16x2(uint32_t w) { return (w & 0x7f80u) != 0x7f80u && (w & 0x7f800000u) != 0x7f800000u; }
-
 // The key tiles a row tile goes through, of those of its block.
 struct Range {
     int begin, end;
@@ -100,6 +97,7 @@ struct Range {
 
 template <int DP>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
+                                                              const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mO,
                                                               const __grid_constant__ Args a) {
     using L = Layout<DP>;
     extern __shared__ uint8_t raw[];
@@ -128,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int first_pos = u.base + u.row0 / g, last_pos = u.base + (u.row0 + u.rows - 1) / g;
     const int all_lo = window > 0 ? max(last_pos - window + 1, 0) : 0, all_hi = first_pos + 1;
     const int t0 = u.lo / kKeys, nt = max((u.hi + kKeys - 1) / kKeys - t0, 0);
-    const int t_begin = t0 + (int)((long long)nt * z / a.splits), t_end = t0 + (int)((long long)nt * (z + 1) / a.splits);
+    const int t_begin = a.splits > 1 ? t0 + nt * z / a.splits : t0, t_end = a.splits > 1 ? t0 + nt * (z + 1) / a.splits : t0 + nt;
     auto range_of = [&](int t) {      // key tiles of row tile t
         const int r0 = u.row0 + 128 * t, r1 = min(r0 + 128, u.row0 + u.rows) - 1;
         if (r0 > r1) return Range{0, 0};
@@ -142,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     auto partial = [&](int j) { return j * kKeys < all_lo || (j + 1) * kKeys > all_hi; };
 
     if (warp == 0 && elect_one()) {
-        mbar_init(bar_q, kSoftmaxWarps);
+        mbar_init(bar_q, a.q_boxes ? 1 : kSoftmaxWarps);
         mbar_init(bar_end, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(bar_s + t, 1);
@@ -177,8 +175,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 " KDA_SOFTMAX_REGS ";");
         const int t = warp >> 2;
-        // ------------------------------------------------------------------ Q into shared memory
-        {
+        // ------------------------------------------------------------------ Q into shared memory, where it does not come by TMA
+        if (!a.q_boxes) {
             // DP / 8 lanes a row; all of a thread's copies are in flight together
             constexpr int kChunks = DP / 8, kStep = 128 / kChunks;      // rows a pass
             const int x = tid & 127, c = x % kChunks;
@@ -272,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     const int q = 2 * h + (e >> 4), at = 2 * (e & 15);
                     const f2 x = f2_fma(f2_make(__uint_as_float(s[q][at]), __uint_as_float(s[q][at + 1])), c2, n2);
                     f2 y;
-                    if (e % kPolyOf < kPoly) {
+                    if (e % kPolyOf == 0) {
                         y = ex2_pair(x);
                     } else {
                         const float2 z = f2_get(x);
@@ -307,17 +305,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const float inv = split ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
             if (mine && split) a.part_ml[at] = make_float2(m == -INFINITY ? m : max_nan(m * c, kLowest), l);
             if (mine && !split && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m * c + log2f(l)) * kLn2;
-            uint8_t* stage_out = sm + t * L::kTile + (warp & 3) * 32 * (DP * 2);      // Q has been read
+            uint8_t* stage_out = sm + t * L::kTile;      // Q has been read; rows as TMA lays them out
+            const int x0 = 32 * (warp & 3);
 #pragma unroll 1
-            for (int q = 0; q < DP / 32; ++q) {
-                uint32_t o[32];
-                if (n > 0) {
-                    tmem_ld32(tO + 32 * q, o);
-                    tmem_ld_wait();
-                } else {
+            for (int q = 0; q < DP / 64; ++q) {
+                uint32_t o[2][32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                for (int y = 0; y < 2; ++y) {
+                    if (n > 0) tmem_ld32(tO + 64 * q + 32 * y, o[y]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[y][e] = 0;
                 }
+                tmem_ld_wait();
                 if (odd_values && n > 0) {
                     // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
 #pragma unroll 1
@@ -329,42 +329,55 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         const int page = b.page(u.n, key / b.page_size);
                         if (page < 0) continue;
                         const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v) + page * a.c.strides.v_page + (key % b.page_size) * a.c.strides.v_row +
-                                                 hk * a.c.strides.v_head + 32 * q;
+                                                 hk * a.c.strides.v_head + 64 * q;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (32 * q + e < D) {
+                        for (int e = 0; e < 64; ++e)
+                            if (64 * q + e < D) {
                                 const float x = __bfloat162float(v[e]);
-                                if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                                if (!isfinite(x)) o[e >> 5][e & 31] = __float_as_uint(__uint_as_float(o[e >> 5][e & 31]) + x);
                             }
                     }
                 }
                 if (split) {
-                    float* dst = a.part_o + at * D + 32 * q;
+                    float* dst = a.part_o + at * D + 64 * q;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        if (mine && 32 * q + e < D)
-                            *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
+                    for (int e = 0; e < 64; e += 4)
+                        if (mine && 64 * q + e < D)
+                            *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(o[e >> 5][e & 31]), __uint_as_float(o[e >> 5][(e & 31) + 1]),
+                                                                              __uint_as_float(o[e >> 5][(e & 31) + 2]), __uint_as_float(o[e >> 5][(e & 31) + 3]));
                 } else {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
+                    for (int x = 0; x < 8; ++x) {
                         uint32_t w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(o[8 * x + 2 * e]) * inv, __uint_as_float(o[8 * x + 2 * e + 1]) * inv);
-                        const int chunk = 4 * q + x;
-                        *reinterpret_cast<uint4*>(stage_out + lane * (DP * 2) + ((chunk ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = pack_bf16(__uint_as_float(o[x >> 2][8 * (x & 3) + 2 * e]) * inv, __uint_as_float(o[x >> 2][8 * (x & 3) + 2 * e + 1]) * inv);
+                        *reinterpret_cast<uint4*>(stage_out + q * 16384 + sw128_off(x0 + lane, x)) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
-            if (!split) {
+            if (!split && a.q_boxes && 128 * (t + 1) <= u.rows) {
+                // a full tile leaves by TMA, as Q came
+                fence_async_smem();
+                asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory");
+                if ((warp & 3) == 0 && elect_one()) {
+                    for (int h = 0; h < DP / 64; ++h)
+                        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(&mO), "r"(smem_u32(stage_out + h * 16384)),
+                                     "r"(h * 64), "r"(hk * g), "r"(u.first + (u.row0 + 128 * t) / g)
+                                     : "memory");
+                    tma_store_commit();
+                    tma_store_wait_read();
+                }
+            } else if (!split) {
                 __syncwarp();
                 constexpr int kLanes = DP / 8;      // lanes that hold a row
                 __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.c.o);
-                const int chunk = lane % kLanes, wr = 128 * t + 32 * (warp & 3);
-                int x = lane / kLanes, pr = u.row0 + wr + x, tk = pr / g, hd = pr - tk * g;
+                const int chunk = lane % kLanes;
+                int x = lane / kLanes, pr = u.row0 + 128 * t + x0 + x, tk = pr / g, hd = pr - tk * g;
 #pragma unroll 2
                 for (; x < 32; x += 32 / kLanes) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage_out + x * (DP * 2) + ((chunk ^ (x & 7)) << 4));
-                    if (wr + x < u.rows && 8 * chunk < D)
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage_out + (chunk >> 3) * 16384 + sw128_off(x0 + x, chunk & 7));
+                    if (128 * t + x0 + x < u.rows && 8 * chunk < D)
                         *reinterpret_cast<uint4*>(o + ((size_t)(u.first + tk) * a.c.heads.q_heads + hk * g + hd) * D + 8 * chunk) = v;
                     for (hd += 32 / kLanes; hd >= g; hd -= g) ++tk;
                 }
@@ -439,6 +452,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 return page;
             };
             int row = 0, next_row = 0, page = look(t_begin, row), next_page = -1, i = 0;
+            if (a.q_boxes && t_begin < t_end) {
+                // 128 rows are whole tokens of g heads.  Rows behind the sequence's last one come along, and stay by themselves.
+                const int tiles = u.rows > 128 ? 2 : 1;
+                if (lane == 0) mbar_expect_tx(bar_q, tiles * L::kTile);
+                __syncwarp();
+                const int t = lane / kHalves, h = lane - t * kHalves;
+                if (t < tiles)
+                    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                                     smem_u32(sm + t * L::kTile + h * 16384)),
+                                 "l"(&mQ), "r"(smem_u32(bar_q)), "r"(h * 64), "r"(hk * g), "r"(u.first + (u.row0 + 128 * t) / g)
+                                 : "memory");
+            }
             for (; i < total; ++i) {
                 const int j = t_begin + (i >> 1), s = stage(i);
                 const bool isv = i & 1;
@@ -463,6 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
             }
             // no copy may be in flight when the block ends
+            if (!ok && a.q_boxes && lane == 0) mbar_poll(bar_q, 0, kSpinLimit / 8);
             if (!ok && lane == 0)
                 for (int x = i > L::kStages ? i - L::kStages : 0; x < i; ++x)
                     mbar_poll((x & 1) && partial(t_begin + (x >> 1)) ? bar_part + stage(x) : bar_full + stage(x), turn(x), kSpinLimit / 8);
@@ -478,25 +504,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (!ok) break;
                 phase ^= 1u << s;
                 uint8_t* v = sm + L::kRing + s * L::kTile;
-                for (int e = tid - kFixWarp * 32; e < kKeys * DP / 8; e += 64) {
-                    const int r = e & 127, ch = e >> 7, key = j * kKeys + r;
-                    if (key >= all_lo && key < all_hi) continue;
+                // keys [0, head) and [tail, 128) of the tile; a piece of eight values a thread, DP / 8 threads a row
+                constexpr int kChunks = DP / 8, kStep = 64 / kChunks;
+                const int k0 = j * kKeys, head = min(max(all_lo - k0, 0), kKeys), tail = max(min(max(all_hi - k0, 0), kKeys), head);
+                const int x = tid - kFixWarp * 32, ch = x % kChunks;
+#pragma unroll 4
+                for (int y = x / kChunks; y < head + kKeys - tail; y += kStep) {
+                    const int r = y < head ? y : y - head + tail, key = k0 + r;
                     uint4* at = reinterpret_cast<uint4*>(v + (ch >> 3) * 16384 + sw128_off(r, ch & 7));
-                    if (key < u.lo || key >= u.hi) {
-                        *at = make_uint4(0, 0, 0, 0);
-                        continue;
-                    }
-                    uint4 x = *at;
-                    if (!(finite_bf16x2(x.x) && finite_bf16x2(x.y) && finite_bf16x2(x.z) && finite_bf16x2(x.w))) {
-                        odd = true;
-                        uint32_t* w = reinterpret_cast<uint32_t*>(&x);
+                    uint4 w = *at;
+                    uint32_t* p = reinterpret_cast<uint32_t*>(&w);
+                    const bool out = key < u.lo || key >= u.hi;
+                    bool here = out;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u;
-                            if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu;
-                        }
-                        *at = x;
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t keep = 0xffffffffu;
+                        if ((p[k] & 0x7f80u) == 0x7f80u) keep = 0xffff0000u;
+                        if ((p[k] & 0x7f800000u) == 0x7f800000u) keep &= 0xffffu;
+                        if (keep != 0xffffffffu && !out) here = odd = true;
+                        p[k] = out ? 0u : p[k] & keep;
                     }
+                    if (here) *at = w;
                 }
                 if (odd) odd_values = 1;
                 __threadfence_block();
@@ -513,10 +541,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 }
 
 template <int DP>
-int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, Args& a, cudaStream_t st) {
+int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CUtensorMap& mQ, const CUtensorMap& mO, const Args& a, cudaStream_t st) {
     if (int rc = set_smem_limit(attn_tc_kernel<DP>, Layout<DP>::kBytes)) return rc;
     const dim3 grid((unsigned)a.slots, (unsigned)c.heads.kv_heads, (unsigned)a.splits);
-    KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, a));
+    KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
     return launch_status();
 }
 
@@ -547,11 +575,16 @@ int tc(const Call& c, int splits, cudaStream_t st) {
     const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
     a.part_ml = static_cast<float2*>(c.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * splits * sizeof(float2), 256));
-    CUtensorMap mK, mV;
+    CUtensorMap mK, mV, mQ, mO;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
     if (!rc) rc = make_map_paged(&mV, c.v, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.v_row, s.v_head, s.v_page, a.box_rows);
-    if (!rc) rc = c.heads.dim <= 64 ? launch<64>(c, mK, mV, a, st) : launch<128>(c, mK, mV, a, st);
+    mQ = mO = mK;
+    a.q_boxes = 128 % c.heads.group == 0 && s.q_head > 0 && s.q_token > 0 && s.q_head < 1ll << 39 && s.q_token < 1ll << 39;
+    if (!rc && a.q_boxes) rc = make_map_packed(&mQ, c.q, c.heads.dim, c.heads.q_heads, c.batch.tokens, s.q_head, s.q_token, c.heads.group, 128 / c.heads.group);
+    if (!rc && a.q_boxes)
+        rc = make_map_packed(&mO, c.o, c.heads.dim, c.heads.q_heads, c.batch.tokens, c.heads.dim, (int64_t)c.heads.q_heads * c.heads.dim, c.heads.group, 128 / c.heads.group);
+    if (!rc) rc = c.heads.dim <= 64 ? launch<64>(c, mK, mV, mQ, mO, a, st) : launch<128>(c, mK, mV, mQ, mO, a, st);
     if (rc || splits == 1) return rc;
     return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, splits, a.part_o, a.part_ml, c.o, c.lse, c.bf16}, st);
 }

@@ -79,6 +79,17 @@ int make_map_paged(CUtensorMap* m, const void* ptr, uint64_t dim, uint64_t rows,
     return r == CUDA_SUCCESS ? KDA_OK : KDA_ERR_CUDA;
 }
 
+// Packed rows [tokens][heads][dim] at the strides given; a box is 64 values of box_heads heads of box_tokens tokens.
+int make_map_packed(CUtensorMap* m, const void* ptr, uint64_t dim, uint64_t heads, uint64_t tokens, int64_t head_ld, int64_t token_ld, uint32_t box_heads,
+                    uint32_t box_tokens) {
+    EncodeFn enc = encode_fn();
+    if (!enc) return KDA_ERR_CUDA;
+    const cuuint64_t dims[3] = {dim, heads, tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)head_ld * 2, (cuuint64_t)token_ld * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_tokens}, es[3] = {1, 1, 1};
+    return encode(enc, m, 3, ptr, dims, strides, box, es) == CUDA_SUCCESS ? KDA_OK : KDA_ERR_CUDA;
+}
+
 // ---------------------------------------------------------------------------------------------
 // self-test of the bounded wait every tensor-core-lane kernel relies on: one warp waits, with a short limit, on a
 // barrier that nothing ever arrives at.  The wait must give up, record its code in the status word and let the kernel

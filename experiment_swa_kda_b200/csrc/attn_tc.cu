@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::kBars);
-    uint64_t *bar_q = bar, *bar_s = bar + 1, *bar_p = bar + 3, *bar_o = bar + 5, *bar_end = bar + 7, *bar_full = bar + 8, *bar_free = bar_full + L::kStages,
+    uint64_t *bar_q = bar, *bar_s = bar + 1, *bar_p = bar + 3, *bar_o = bar + 7, *bar_end = bar + 9, *bar_full = bar + 10, *bar_free = bar_full + L::kStages,
              *bar_part = bar_free + L::kStages;
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bar + 60);
     volatile int& abort_flag = *reinterpret_cast<volatile int*>(bar + 61);
@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         mbar_init(bar_end, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(bar_s + t, 1);
-            mbar_init(bar_p + t, 4);
+            mbar_init(bar_p + 2 * t, 4);      // P of keys [0, 64) and [64, 128)
+            mbar_init(bar_p + 2 * t + 1, 4);
             mbar_init(bar_o + t, 1);
         }
         for (int s = 0; s < L::kStages; ++s) {
@@ -280,12 +281,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     p[e] = f2_to_bf16(y);
                 }
                 tmem_st32(tS + 32 * h, p);
+                tmem_st_wait();
+                tc_fence_before();
+                warp_arrive(bar_p + 2 * t + h, lane);      // its product starts
             }
             const float2 both = f2_get(f2_add(sum[0], sum[1]));
             l += both.x + both.y;
-            tmem_st_wait();
-            tc_fence_before();
-            warp_arrive(bar_p + t, lane);
         }
         // ------------------------------------------------------------------ O / l
         const int n = r.end - r.begin;
@@ -415,13 +416,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     for (int t = 0; t < 2 && ok; ++t) {
                         if (in(t, j)) {
                             const int i = j - range[t].begin;
-                            ok = wait(bar_p + t, i & 1);
-                            if (!ok) break;
-                            tc_fence_after();
                             const UmmaDesc v = umma_smem_desc_sw128(s0 + L::kRing + stage(iv) * L::kTile, 16384, 1024);
+                            for (int h = 0; h < 2 && ok; ++h) {      // O_t += P_t V_j, half of the keys as soon as their weights are there
+                                ok = wait(bar_p + 2 * t + h, i & 1);
+                                if (!ok) break;
+                                tc_fence_after();
 #pragma unroll
-                            for (int x = 0; x < 8; ++x)      // O_t += P_t V_j
-                                umma_bf16_ts(tmem + cO + DP * t, tmem + cS + 128 * t + 8 * x, v + (x * 2048), idO, i > 0 || x > 0);
+                                for (int x = 0; x < 4; ++x)
+                                    umma_bf16_ts(tmem + cO + DP * t, tmem + cS + 128 * t + 32 * h + 8 * x, v + (h * 8192 + x * 2048), idO, i > 0 || h > 0 || x > 0);
+                            }
+                            if (!ok) break;
                             umma_commit(bar_o + t);
                         }
                         if (j + 1 < t_end && in(t, j + 1)) scores(t, j + 1, ik);

@@ -21,8 +21,8 @@ int check(const KdaPagedShape* s, bool packed) {
 }
 
 // Parts a row's keys are cut into where its blocks alone leave SMs idle.  What a row sees is known on the device alone, so the
-// bound is the table's; a part has two key tiles at least.
-int split_count(const KdaPagedShape& s, bool packed, int rows, int keys, int resident) {
+// bound is the table's.
+int split_count(const KdaPagedShape& s, bool packed, int rows, int keys, int resident, int least) {      // a part has `least` key tiles
     int per_seq;
     const int group = s.q_heads / s.kv_heads;
     const int max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
@@ -31,11 +31,11 @@ int split_count(const KdaPagedShape& s, bool packed, int rows, int keys, int res
     if (s.window > 0 && max_q > 0 && reach > (long long)s.window + max_q) reach = (long long)s.window + max_q;
     const long long tiles = (reach + keys - 1) / keys;
     long long n = resident / (blocks > 0 ? blocks : 1);
-    if (n > tiles / 2) n = tiles / 2;
+    if (n > tiles / least) n = tiles / least;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
-int general_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 64, 64, 2 * 148); }
-int tc_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 256, 128, 148); }
+int general_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 64, 64, 2 * 148, 1); }
+int tc_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 256, 128, 148, 2); }
 
 }  // namespace
 

@@ -3,7 +3,9 @@
 // running maximum m and sum.
 //
 // A block holds 64 rows (token-major, the query heads of one kv head side by side, so that a key tile serves them all) and
-// goes through its keys in tiles of 64.  Both products are 4 x 4 outputs a thread from 16-byte shared-memory reads.
+// goes through its keys in tiles of 64.  Both products are 4 x 4 outputs a thread from 16-byte shared-memory reads: bound by
+// the multiply-add pipes once there is work for every SM, by the way to memory before that.  Four threads fetch a row, one look at the
+// table each, in 16-byte pieces where the addresses allow it.
 
 #include "attn.cuh"
 
@@ -22,13 +24,49 @@ struct Smem {
     int bad;      // a value in the tile is not finite
 };
 
-template <int DP>
+// A quarter of a row of `width` values from src[at] on to shared memory, as float32 and with zeros behind it; false if a value is
+// not finite.  VEC: pieces of 16 bytes.
+template <int DP, bool VEC>
+__device__ __forceinline__ bool fetch(float* dst, const void* src, long long at, int width, int part, int bf16) {
+    bool fine = true;
+    if (!VEC) {
+        for (int d = part; d < DP; d += 4) {
+            const float x = d < width ? ld_io(src, (size_t)(at + d), bf16) : 0.f;
+            fine &= isfinite(x);
+            dst[d] = x;
+        }
+    } else if (bf16) {
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+            const int d = 8 * part + 32 * i;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (d < width) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(src) + at + d));
+            const float2 f0 = f2_get(f2_from_bf16(x.x)), f1 = f2_get(f2_from_bf16(x.y)), f2_ = f2_get(f2_from_bf16(x.z)), f3 = f2_get(f2_from_bf16(x.w));
+            fine &= isfinite(f0.x) && isfinite(f0.y) && isfinite(f1.x) && isfinite(f1.y) && isfinite(f2_.x) && isfinite(f2_.y) && isfinite(f3.x) && isfinite(f3.y);
+            *reinterpret_cast<float4*>(dst + d) = make_float4(f0.x, f0.y, f1.x, f1.y);
+            *reinterpret_cast<float4*>(dst + d + 4) = make_float4(f2_.x, f2_.y, f3.x, f3.y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) {
+            const int d = 4 * part + 16 * i;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (d < width) x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(src) + at + d));
+            fine &= isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w);
+            *reinterpret_cast<float4*>(dst + d) = x;
+        }
+    }
+    return fine;
+}
+
+template <int DP, bool VEC>
 __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles tiles, int splits, float* part_o, float2* part_ml) {
     extern __shared__ float4 raw[];
     Smem<DP>& sm = *reinterpret_cast<Smem<DP>*>(raw);
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int hk = blockIdx.y, z = blockIdx.z, g = c.heads.group, D = c.heads.dim;
     const Batch& b = c.batch;
+    dependents_go();
     Unit u;
     if (!make_unit(b, tiles, blockIdx.x, c.window, u)) {
         int n, tile;
@@ -41,11 +79,11 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
 
     auto token_of = [&](int r) { return u.first + (u.row0 + r) / g; };
     auto head_of = [&](int r) { return hk * g + (u.row0 + r) % g; };
-    for (int e = tid; e < kRows * DP; e += kThreads) {
-        const int r = e / DP, d = e - r * DP;
-        float x = 0.f;
-        if (r < u.rows && d < D) x = ld_io(c.q, (size_t)(token_of(r) * c.strides.q_token + head_of(r) * c.strides.q_head + d), c.bf16);
-        sm.q[r][d] = x;
+    const int f_row = tid >> 2, f_part = tid & 3;      // the row this thread fetches, and its part
+    {
+        const bool is = f_row < u.rows;
+        const long long at = is ? token_of(f_row) * c.strides.q_token + head_of(f_row) * c.strides.q_head : 0;
+        fetch<DP, VEC>(sm.q[f_row], c.q, at, is ? D : 0, f_part, c.bf16);
     }
     // the keys each of this thread's rows sees
     int last[4], first[4];
@@ -68,23 +106,21 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
         __syncthreads();
         if (tid == 0) sm.bad = 0;
         __syncthreads();
-        bool bad = false;
-        for (int e = tid; e < kKeys * DP; e += kThreads) {
-            const int r = e / DP, d = e - r * DP, key = t * kKeys + r;
-            float x = 0.f, y = 0.f;
-            if (d < D && key >= u.lo && key < u.hi) {
-                const int page = b.page(u.n, key / b.page_size), row = key % b.page_size;
-                if (page >= 0) {
-                    x = ld_io(c.k, (size_t)(page * c.strides.k_page + row * c.strides.k_row + hk * c.strides.k_head + d), c.bf16);
-                    y = ld_io(c.v, (size_t)(page * c.strides.v_page + row * c.strides.v_row + hk * c.strides.v_head + d), c.bf16);
-                } else if (d == 0) {
-                    b.tell(KDA_ERR_BLOCK_TABLE);
-                }
+        const int key = t * kKeys + f_row;
+        long long k_at = 0, v_at = 0;
+        int width = 0;
+        if (key >= u.lo && key < u.hi) {
+            const int page = b.page(u.n, key / b.page_size), row = key % b.page_size;
+            if (page >= 0) {
+                width = D;
+                k_at = page * c.strides.k_page + row * c.strides.k_row + hk * c.strides.k_head;
+                v_at = page * c.strides.v_page + row * c.strides.v_row + hk * c.strides.v_head;
+            } else if (f_part == 0) {
+                b.tell(KDA_ERR_BLOCK_TABLE);
             }
-            sm.k[r][d] = x;
-            sm.v[r][d] = y;
-            bad |= !isfinite(y);
         }
+        fetch<DP, VEC>(sm.k[f_row], c.k, k_at, width, f_part, c.bf16);
+        const bool bad = !fetch<DP, VEC>(sm.v[f_row], c.v, v_at, width, f_part, c.bf16);
         if (bad) sm.bad = 1;
         __syncthreads();
 
@@ -210,20 +246,23 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= rows) return;
+    dependency_wait();
     float m = -INFINITY;
-    for (int z = lane; z < c.splits; z += 32) m = fmaxf(m, c.part_ml[z * rows + row].x);
+    for (int z = lane; z < c.splits; z += 32) m = fmaxf(m, ld_after_f32(&c.part_ml[z * rows + row].x));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float acc[8] = {}, l = 0.f;
+#pragma unroll 4
     for (int z = 0; z < c.splits; ++z) {
-        const float2 ml = c.part_ml[z * rows + row];
-        if (ml.x == -INFINITY) continue;
-        const float w = exp2f(ml.x - m);
-        l += ml.y * w;
+        const uint2 ml = ld_after8(c.part_ml + z * rows + row);
+        const float x = __uint_as_float(ml.x);
+        if (x == -INFINITY) continue;
+        const float w = exp2f(x - m);
+        l += __uint_as_float(ml.y) * w;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const int d = lane + 32 * x;
-            if (d < c.dim) acc[x] = fmaf(w, c.part_o[(z * rows + row) * c.dim + d], acc[x]);
+        for (int i = 0; i < 8; ++i) {
+            const int d = lane + 32 * i;
+            if (d < c.dim) acc[i] = fmaf(w, ld_after_f32(c.part_o + (z * rows + row) * c.dim + d), acc[i]);
         }
     }
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
@@ -238,8 +277,13 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
 template <int DP>
 int launch(const Call& c, const Tiles& t, dim3 grid, int splits, float* part_o, float2* part_ml, cudaStream_t st) {
     const size_t smem = sizeof(Smem<DP>);
-    if (int rc = set_smem_limit(attn_general_kernel<DP>, smem)) return rc;
-    KDA_LAUNCH("attn_general_kernel", st, attn_general_kernel<DP><<<grid, kThreads, smem, st>>>(c, t, splits, part_o, part_ml));
+    const Strides& s = c.strides;
+    const int unit = c.bf16 ? 8 : 4;      // values in 16 bytes
+    const long long all = s.q_token | s.q_head | s.k_page | s.k_row | s.k_head | s.v_page | s.v_row | s.v_head | c.heads.dim;
+    const bool vec = all % unit == 0 && (reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % 16 == 0;
+    auto kern = vec ? attn_general_kernel<DP, true> : attn_general_kernel<DP, false>;
+    if (int rc = set_smem_limit(kern, smem)) return rc;
+    KDA_LAUNCH("attn_general_kernel", st, kern<<<grid, kThreads, smem, st>>>(c, t, splits, part_o, part_ml));
     return launch_status();
 }
 
@@ -247,8 +291,9 @@ int launch(const Call& c, const Tiles& t, dim3 grid, int splits, float* part_o, 
 
 int combine(const Combine& c, cudaStream_t st) {
     const long long rows = (long long)c.tokens * c.q_heads;
-    KDA_LAUNCH("attn_combine_kernel", st, attn_combine_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(c));
-    return launch_status();
+    cudaError_t e = cudaSuccess;
+    KDA_LAUNCH("attn_combine_kernel", st, e = launch_early(attn_combine_kernel, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, 1, c));
+    return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 int general(const Call& c, int splits, cudaStream_t st) {

@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, hk = blockIdx.y, z = blockIdx.z, window = a.c.window;
+    dependents_go();
     // a sequence's last rows see the most keys: they start first
     const int slot = a.slots - 1 - (int)blockIdx.x;
     Unit u;

@@ -20,12 +20,7 @@ namespace attn {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-#ifndef V_BG
-#define V_BG 2
-#define V_FG 3
-#endif
-constexpr int kFwdBlocks = V_FG;
-constexpr int kBwdBlocks = V_BG;      // blocks an SM of the backward: each leaves one part of the weights' gradients
+constexpr int kBlocks = 2;      // blocks an SM of the kernels that go by rows (three: 80 registers, spilled, 640 us where two take 336)
 
 struct Rope {
     KdaRotaryShape s;
@@ -39,7 +34,7 @@ struct Rope {
     Batch batch;                    // append
     Strides cache;
     int* mirror;
-    int slice, slices;              // norm_rope_rows_*: heads of a token a group of lanes takes, and groups a token has
+    int run;                        // norm_rope_rows_*: pieces of a token or of the next that a group of lanes takes one after the other
 };
 
 // Where a token goes: its position, and the cache rows of its key and value (append).
@@ -222,51 +217,102 @@ __global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(Rope p) {
     }
 }
 
-#ifndef V_FB
-#define V_FB 3
-#define V_BB 2
-#endif
 // ---------------------------------------------------------------------------------------------- eight values a lane
 // LANES lanes a row, and both members of a pair in one lane: two pieces of four adjacent values, half the rotated width apart in the
-// split order.  A group of lanes takes a token's heads one after the other - all of them, or a slice where there are too few
-// tokens to fill the machine -, so that the token's place, its cosines and sines and the weights are read once for all of them.
-// What bounds such a loop after memory is issue and the shuffles of the rows' sums, so rows go four at a time (backward two, with
-// two sums each) and their four sums are reduced together: 5 shuffles, not 16, and 4 that hand them out.
+// split order.  What bounds such a loop after memory is issue and the shuffles of the rows' sums, so rows go four at a time (backward
+// two, with two sums each) and their four sums are reduced together: 5 shuffles, not 16, and 4 that hand them out.
+//
+// Such a piece of rows - of one token, and of q, k or (append) v - is what a group of lanes works on at a time, and it takes runs of
+// them, so that a token's place, its cosines and sines and the weights are read once for all of them.  Each lane copies its own
+// values through a ring in shared memory that runs ahead by kStages - 1 pieces: rows held in registers would be waited for
+// by all of a piece's arithmetic, and with 16 to 24 warps an SM too few were on their way (65,536 tokens of 20 heads, forward and
+// backward: 397 us).
 
-// values [0..3], [4..7] of a lane
+// values [0..3], [4..7] of a lane: 8 or 16 bytes each
 template <bool BF16>
-struct Vec8;
-template <>
-struct Vec8<true> {
-    uint2 a, b;
-    __device__ __forceinline__ void load(const void* p, long long at0, long long at1) {
-        a = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + at0));
-        b = __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(p) + at1));
+struct Vec8 {
+    static constexpr int kBytes = BF16 ? 8 : 16;
+    static constexpr int kValue = BF16 ? 2 : 4;
+    static __device__ __forceinline__ void copy(uint32_t dst, const char* src) {
+        if (BF16) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+        else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     }
-    __device__ __forceinline__ void zero() { a = b = make_uint2(0, 0); }
-    __device__ __forceinline__ void get(f2 (&x)[4]) const {
-        x[0] = f2_from_bf16(a.x); x[1] = f2_from_bf16(a.y); x[2] = f2_from_bf16(b.x); x[3] = f2_from_bf16(b.y);
+    static __device__ __forceinline__ void get(const char* p, f2& a, f2& b) {
+        if (BF16) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            a = f2_from_bf16(v.x);
+            b = f2_from_bf16(v.y);
+        } else {
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            a = f2_make(v.x, v.y);
+            b = f2_make(v.z, v.w);
+        }
     }
-    static __device__ __forceinline__ void store(void* p, long long at0, long long at1, const f2 (&x)[4]) {
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + at0) = make_uint2(f2_to_bf16(x[0]), f2_to_bf16(x[1]));
-        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p) + at1) = make_uint2(f2_to_bf16(x[2]), f2_to_bf16(x[3]));
+    static __device__ __forceinline__ void store(char* p, f2 a, f2 b) {
+        if (BF16) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(f2_to_bf16(a), f2_to_bf16(b));
+        } else {
+            const float2 x = f2_get(a), y = f2_get(b);
+            *reinterpret_cast<float4*>(p) = make_float4(x.x, x.y, y.x, y.y);
+        }
     }
 };
-template <>
-struct Vec8<false> {
-    float4 a, b;
-    __device__ __forceinline__ void load(const void* p, long long at0, long long at1) {
-        a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at0));
-        b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at1));
+// The ring: [stage][8 values' worth of pieces of four][thread].
+template <bool BF16>
+struct Ring {
+    static constexpr int kStages = BF16 ? 4 : 2, kPiece = kThreads * Vec8<BF16>::kBytes, kStage = 8 * kPiece, kBytes = kStages * kStage;
+    char* mine;                 // this thread's place of the first piece
+    uint32_t address;
+    int in = 0, out = 0;        // stages to fill and to empty, as offsets
+    __device__ __forceinline__ explicit Ring(char* smem) : mine(smem + threadIdx.x * Vec8<BF16>::kBytes), address((uint32_t)__cvta_generic_to_shared(mine)) {}
+    __device__ __forceinline__ uint32_t to(int piece) const { return address + in + piece * kPiece; }
+    __device__ __forceinline__ const char* from(int piece) const { return mine + out + piece * kPiece; }
+    static __device__ __forceinline__ int after(int stage) { return stage + kStage == kBytes ? 0 : stage + kStage; }
+    static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }      // the oldest is there
+};
+
+// The pieces of a token: ROWS rows each of q's heads, then k's, then v's.  A group goes through runs of `run` pieces, the next one
+// `stride` pieces behind the one before; counted, since a division a piece costs as much as its rows.
+template <int ROWS>
+struct Pieces {
+    int each, of_q, of_k;       // pieces of a token, of q and k
+    int at, all, left;          // this piece of all the batch's; pieces left of the run
+    int t, n, which, h, rows;   // token, piece of the token; q, k or v; first head, heads
+
+    __device__ __forceinline__ Pieces(const KdaRotaryShape& s, bool values, int first, int run) {
+        of_q = (s.q_heads + ROWS - 1) / ROWS;
+        of_k = (s.kv_heads + ROWS - 1) / ROWS;
+        each = of_q + of_k + (values ? of_k : 0);
+        all = s.tokens * each;
+        set(s, first, run);
     }
-    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ __forceinline__ void get(f2 (&x)[4]) const {
-        x[0] = f2_make(a.x, a.y); x[1] = f2_make(a.z, a.w); x[2] = f2_make(b.x, b.y); x[3] = f2_make(b.z, b.w);
+    __device__ __forceinline__ bool more() const { return at < all; }
+    __device__ __forceinline__ void set(const KdaRotaryShape& s, int i, int run) {
+        at = i;
+        left = run;
+        t = i / each;
+        n = i - t * each;
+        place(s);
     }
-    static __device__ __forceinline__ void store(void* p, long long at0, long long at1, const f2 (&x)[4]) {
-        const float2 a = f2_get(x[0]), b = f2_get(x[1]), c = f2_get(x[2]), e = f2_get(x[3]);
-        *reinterpret_cast<float4*>(static_cast<float*>(p) + at0) = make_float4(a.x, a.y, b.x, b.y);
-        *reinterpret_cast<float4*>(static_cast<float*>(p) + at1) = make_float4(c.x, c.y, e.x, e.y);
+    __device__ __forceinline__ void place(const KdaRotaryShape& s) {
+        which = n < of_q ? 0 : n < of_q + of_k ? 1 : 2;
+        h = ROWS * (n - (which == 0 ? 0 : which == 1 ? of_q : of_q + of_k));
+        rows = min(ROWS, (which ? s.kv_heads : s.q_heads) - h);
+    }
+    __device__ __forceinline__ void next(const KdaRotaryShape& s, int run, int stride) {
+        if (--left > 0) {
+            ++at;
+            if (++n == each) {
+                n = 0;
+                ++t;
+            }
+            place(s);
+        } else {
+            const long long to = (long long)at + 1 + stride - run;
+            if (to < all) set(s, (int)to, run);
+            else at = all;
+        }
     }
 };
 
@@ -357,83 +403,98 @@ struct Lane {
     }
 };
 
-// `heads` rows of one token from `from` on, from_stride apart, to `to`, to_stride apart: y = r (x a + x_other b)
-template <int LANES, bool BF16, bool INTER>
-__device__ __forceinline__ void turn_rows(const Lane<LANES, INTER>& ln, const KdaRotaryShape& sh, const void* src, long long from, long long from_stride, void* dst,
-                                          long long to, long long to_stride, int heads, const f2 (&a)[4], const f2 (&b)[4]) {
-    const bool all_turned = sh.rotary_dim == sh.head_dim;
-    const float inv = 1.f / sh.head_dim;
-    for (int h = 0; h < heads; h += 4) {
-        Vec8<BF16> v[4];
-        f2 x[4][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i].zero();
-            if (ln.on && h + i < heads) v[i].load(src, from + (h + i) * from_stride + ln.d0, from + (h + i) * from_stride + ln.d1);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i].get(x[i]);
-        const float r = rsqrtf(fmaf(sum4<LANES>(f2_dot(x[0], x[0]), f2_dot(x[1], x[1]), f2_dot(x[2], x[2]), f2_dot(x[3], x[3]), ln.l, ln.mask), inv, sh.eps));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const f2 r2 = f2_all(__shfl_sync(ln.mask, r, i, LANES));
-            f2 o[4], y[4];
-            ln.other(x[i], o, all_turned);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) y[k] = f2_mul(f2_fma(x[i][k], a[k], f2_mul(o[k], b[k])), r2);
-            if (ln.on && h + i < heads) Vec8<BF16>::store(dst, to + (h + i) * to_stride + ln.d0, to + (h + i) * to_stride + ln.d1, y);
-        }
-    }
-}
-
 template <int LANES, bool BF16, bool INTER, bool APPEND>
-__global__ void __launch_bounds__(kThreads, V_FB) norm_rope_rows_kernel(Rope p) {
+__global__ void __launch_bounds__(kThreads, kBlocks) norm_rope_rows_kernel(Rope p) {
+    extern __shared__ __align__(16) char smem[];
+    using V = Vec8<BF16>;
+    using R = Ring<BF16>;
+    R ring(smem);
     constexpr int kGroups = kThreads / LANES;
     const Lane<LANES, INTER> ln(p.s);
-    const int Hq = p.s.q_heads, Hk = p.s.kv_heads, all = Hq + Hk + (APPEND ? Hk : 0), D = p.s.head_dim;
-    const long long units = (long long)p.s.tokens * p.slices;
-    for (long long unit = (long long)blockIdx.x * kGroups + threadIdx.x / LANES; unit < units; unit += (long long)gridDim.x * kGroups) {
-        const int t = (int)(unit / p.slices), h0 = (int)(unit - (long long)t * p.slices) * p.slice, h1 = min(h0 + p.slice, all);
-        const Place at = place_of<APPEND, LANES>(p, t, ln.l, ln.mask);
-        f2 c[4], s[4];
-        ln.angles(p, max(at.pos, 0), c, s);
-        // u_e c + u_other s with u = x r w: a = w_e c, b = w_other s
-        auto coefficients = [&](const float* w, f2 (&a)[4], f2 (&b)[4]) {
-            f2 own[4];
-            ln.weights(w, own);
+    const int Hq = p.s.q_heads, Hk = p.s.kv_heads, D = p.s.head_dim, piece_gap = (ln.d1 - ln.d0) * V::kValue;
+    const bool all_turned = p.s.rotary_dim == D;
+    const float inv = 1.f / D;
+    const int stride = gridDim.x * kGroups * p.run;
+    Pieces<4> ahead(p.s, APPEND, (blockIdx.x * kGroups + threadIdx.x / LANES) * p.run, p.run);
+    Pieces<4> w = ahead;
+    auto copy = [&]() {
+        if (ahead.more()) {
+            const void* src = ahead.which == 0 ? p.q : ahead.which == 1 ? p.k : p.v;
+            const long long ts = ahead.which == 0 ? p.s.q_token_stride : ahead.which == 1 ? p.s.k_token_stride : p.s.v_token_stride;
+            const long long hs = ahead.which == 0 ? p.s.q_head_stride : ahead.which == 1 ? p.s.k_head_stride : p.s.v_head_stride;
+            const char* from = static_cast<const char*>(src) + (ahead.t * ts + ahead.h * hs + ln.d0) * V::kValue;
+            const long long step = hs * V::kValue;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (ln.on && i < ahead.rows) {
+                    V::copy(ring.to(2 * i), from + i * step);
+                    V::copy(ring.to(2 * i + 1), from + i * step + piece_gap);
+                }
+            ahead.next(p.s, p.run, stride);
+        }
+        R::commit();
+        ring.in = R::after(ring.in);
+    };
+#pragma unroll
+    for (int i = 0; i < R::kStages - 1; ++i) copy();
+    Place at = {};
+    f2 c[4], s[4], a[4], b[4];
+    int token = -1, kind = -1;
+    for (; w.more(); w.next(p.s, p.run, stride)) {
+        copy();
+        if (w.t != token) {
+            token = w.t;
+            kind = -1;
+            at = place_of<APPEND, LANES>(p, token, ln.l, ln.mask);
+            ln.angles(p, max(at.pos, 0), c, s);
+        }
+        if (w.which != kind && w.which < 2) {
+            kind = w.which;
+            f2 own[4];      // u_e c + u_other s with u = x r w: a = w_e c, b = w_other s
+            ln.weights(kind ? p.k_weight : p.q_weight, own);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 a[i] = f2_mul(own[i], c[i]);
                 b[i] = f2_mul(INTER ? swapped(own[i]) : own[i ^ 2], s[i]);
             }
-        };
-        f2 a[4], b[4];
-        if (h0 < Hq) {
-            const int n = min(h1, Hq) - h0;
-            const long long to = ((long long)t * Hq + h0) * D;
-            if (APPEND && at.pos < 0) {
-                const f2 none[4] = {f2_all(0.f), f2_all(0.f), f2_all(0.f), f2_all(0.f)};
-                for (int h = 0; h < n; ++h)
-                    if (ln.on) Vec8<BF16>::store(p.q_out, to + (long long)h * D + ln.d0, to + (long long)h * D + ln.d1, none);
+        }
+        R::wait();
+        f2 x[4][4];
+        float ss[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            V::get(ring.from(2 * i), x[i][0], x[i][1]);
+            V::get(ring.from(2 * i + 1), x[i][2], x[i][3]);
+            ss[i] = ln.on ? f2_dot(x[i], x[i]) : 0.f;
+        }
+        ring.out = R::after(ring.out);
+        void* dst = w.which == 0 ? p.q_out : w.which == 1 ? p.k_out : p.v_out;
+        long long to = ((long long)w.t * (w.which ? Hk : Hq) + w.h) * D, hs = D;
+        if (APPEND && w.which) {
+            if (at.pos < 0 || at.k_at < 0) continue;
+            hs = w.which == 1 ? p.cache.k_head : p.cache.v_head;
+            to = (w.which == 1 ? at.k_at : at.v_at) + w.h * hs;
+        }
+        char* into = static_cast<char*>(dst) + (to + ln.d0) * V::kValue;
+        const long long step = hs * V::kValue;
+        const float r = rsqrtf(fmaf(sum4<LANES>(ss[0], ss[1], ss[2], ss[3], ln.l, ln.mask), inv, p.s.eps));
+        const bool none = APPEND && at.pos < 0;      // padding
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f2 r2 = f2_all(__shfl_sync(ln.mask, r, i, LANES));
+            f2 y[4];
+            if (APPEND && w.which == 2) {      // values go as they are
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = x[i][k];
             } else {
-                coefficients(p.q_weight, a, b);
-                turn_rows<LANES, BF16>(ln, p.s, p.q, t * p.s.q_token_stride + h0 * p.s.q_head_stride, p.s.q_head_stride, p.q_out, to, D, n, a, b);
+                f2 o[4];
+                ln.other(x[i], o, all_turned);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) y[k] = none ? f2_all(0.f) : f2_mul(f2_fma(x[i][k], a[k], f2_mul(o[k], b[k])), r2);
             }
-        }
-        if (APPEND && (at.pos < 0 || at.k_at < 0)) continue;
-        const int k0 = max(h0 - Hq, 0), k1 = min(h1 - Hq, Hk);
-        if (k0 < k1) {
-            coefficients(p.k_weight, a, b);
-            turn_rows<LANES, BF16>(ln, p.s, p.k, t * p.s.k_token_stride + k0 * p.s.k_head_stride, p.s.k_head_stride, p.k_out,
-                                   APPEND ? at.k_at + k0 * p.cache.k_head : ((long long)t * Hk + k0) * D, APPEND ? p.cache.k_head : D, k1 - k0, a, b);
-        }
-        if (APPEND && ln.on) {      // values go as they are
-            for (int v = max(h0 - Hq - Hk, 0); v < h1 - Hq - Hk; ++v) {
-                Vec8<BF16> x;
-                f2 y[4];
-                x.load(p.v, t * p.s.v_token_stride + v * p.s.v_head_stride + ln.d0, t * p.s.v_token_stride + v * p.s.v_head_stride + ln.d1);
-                x.get(y);
-                Vec8<BF16>::store(p.v_out, at.v_at + v * p.cache.v_head + ln.d0, at.v_at + v * p.cache.v_head + ln.d1, y);
+            if (ln.on && i < w.rows) {
+                V::store(into + i * step, y[0], y[1]);
+                V::store(into + i * step + piece_gap, y[2], y[3]);
             }
         }
     }
@@ -442,92 +503,113 @@ __global__ void __launch_bounds__(kThreads, V_FB) norm_rope_rows_kernel(Rope p) 
 // The same rows backward; each lane sums its weights' gradients over all rows it meets, a block over its lanes, and
 // norm_rope_dw_kernel over the blocks, all in a fixed order.
 template <int LANES, bool BF16, bool INTER>
-__global__ void __launch_bounds__(kThreads, V_BB) norm_rope_rows_bwd_kernel(Rope p) {
+__global__ void __launch_bounds__(kThreads, kBlocks) norm_rope_rows_bwd_kernel(Rope p) {
+    extern __shared__ __align__(16) char smem[];
+    using V = Vec8<BF16>;
+    using R = Ring<BF16>;
+    R ring(smem);
     constexpr int kGroups = kThreads / LANES;
     dependents_go();
     const Lane<LANES, INTER> ln(p.s);
-    const int Hq = p.s.q_heads, Hk = p.s.kv_heads, all = Hq + Hk, D = p.s.head_dim;
+    const int Hq = p.s.q_heads, Hk = p.s.kv_heads, D = p.s.head_dim, piece_gap = (ln.d1 - ln.d0) * V::kValue;
     const bool all_turned = p.s.rotary_dim == D;
     const float inv = 1.f / D;
-    const long long units = (long long)p.s.tokens * p.slices;
-    f2 dw[2][4];
+    const int stride = gridDim.x * kGroups * p.run;
+    Pieces<2> ahead(p.s, false, (blockIdx.x * kGroups + threadIdx.x / LANES) * p.run, p.run);
+    Pieces<2> w = ahead;
+    auto copy = [&]() {
+        if (ahead.more()) {
+            const void *src = ahead.which ? p.k : p.q, *grad = ahead.which ? p.d_k : p.d_q;
+            const long long hs = ahead.which ? p.s.k_head_stride : p.s.q_head_stride;
+            const char* from = static_cast<const char*>(src) + (ahead.t * (ahead.which ? p.s.k_token_stride : p.s.q_token_stride) + ahead.h * hs + ln.d0) * V::kValue;
+            const char* to = static_cast<const char*>(grad) + ((long long)(ahead.t * (ahead.which ? Hk : Hq) + ahead.h) * D + ln.d0) * V::kValue;
+            const long long step = hs * V::kValue;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (ln.on && i < ahead.rows) {
+                    V::copy(ring.to(4 * i), from + i * step);
+                    V::copy(ring.to(4 * i + 1), from + i * step + piece_gap);
+                    V::copy(ring.to(4 * i + 2), to + i * D * V::kValue);
+                    V::copy(ring.to(4 * i + 3), to + i * D * V::kValue + piece_gap);
+                }
+            ahead.next(p.s, p.run, stride);
+        }
+        R::commit();
+        ring.in = R::after(ring.in);
+    };
+#pragma unroll
+    for (int i = 0; i < R::kStages - 1; ++i) copy();
+    f2 dw[2][4], c[4], s[4], own[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[0][i] = dw[1][i] = f2_all(0.f);
-    for (long long unit = (long long)blockIdx.x * kGroups + threadIdx.x / LANES; unit < units; unit += (long long)gridDim.x * kGroups) {
-        const int t = (int)(unit / p.slices), h0 = (int)(unit - (long long)t * p.slices) * p.slice, h1 = min(h0 + p.slice, all);
-        const Place at = place_of<false>(p, t);
-        f2 c[4], s[4];
-        ln.angles(p, at.pos, c, s);
+    int token = -1, kind = -1;
+    for (; w.more(); w.next(p.s, p.run, stride)) {
+        copy();
+        if (w.t != token) {
+            token = w.t;
+            const Place at = place_of<false>(p, token);
+            ln.angles(p, at.pos, c, s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = f2_mul(s[i], f2_all(-1.f));      // the transposed rotation
+            for (int i = 0; i < 4; ++i) s[i] = f2_mul(s[i], f2_all(-1.f));      // the transposed rotation
+        }
+        if (w.which != kind) {
+            kind = w.which;
+            ln.weights(kind ? p.k_weight : p.q_weight, own);
+        }
+        R::wait();
+        f2 x[2][4], du[2][4];
+        float ss[2], dot[2];
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const int H = which ? Hk : Hq, a0 = which ? max(h0 - Hq, 0) : h0, a1 = which ? h1 - Hq : min(h1, Hq);
-            if (a0 >= a1) continue;
-            const long long hs = which ? p.s.k_head_stride : p.s.q_head_stride;
-            const long long from = t * (which ? p.s.k_token_stride : p.s.q_token_stride), to = (long long)t * H * D;
-            const void *src = which ? p.k : p.q, *grad = which ? p.d_k : p.d_q;
-            void* dst = which ? p.k_out : p.q_out;
-            f2 own[4];
-            ln.weights(which ? p.k_weight : p.q_weight, own);
-            for (int h = a0; h < a1; h += 2) {
-                Vec8<BF16> xv[2], gv[2];
-                f2 x[2][4], du[2][4];
-                float ss[2], dot[2];
+        for (int i = 0; i < 2; ++i) {
+            f2 g[4], o[4], sum = f2_all(0.f);
+            V::get(ring.from(4 * i), x[i][0], x[i][1]);
+            V::get(ring.from(4 * i + 1), x[i][2], x[i][3]);
+            V::get(ring.from(4 * i + 2), g[0], g[1]);
+            V::get(ring.from(4 * i + 3), g[2], g[3]);
+            ln.other(g, o, all_turned);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    xv[i].zero();
-                    gv[i].zero();
-                    if (ln.on && h + i < a1) {
-                        xv[i].load(src, from + (h + i) * hs + ln.d0, from + (h + i) * hs + ln.d1);
-                        gv[i].load(grad, to + (long long)(h + i) * D + ln.d0, to + (long long)(h + i) * D + ln.d1);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    f2 o[4];
-                    xv[i].get(x[i]);
-                    gv[i].get(du[i]);
-                    ln.other(du[i], o, all_turned);
-                    ss[i] = f2_dot(x[i], x[i]);
-                    f2 sum = f2_all(0.f);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const f2 d = f2_fma(o[k], s[k], f2_mul(du[i][k], c[k]));
-                        sum = f2_fma(f2_mul(d, own[k]), x[i][k], sum);
-                        du[i][k] = d;
-                    }
-                    const float2 t2 = f2_get(sum);
-                    dot[i] = t2.x + t2.y;
-                }
-                const float mean = sum4<LANES>(ss[0], ss[1], dot[0], dot[1], ln.l, ln.mask) * inv;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float r = rsqrtf(__shfl_sync(ln.mask, mean, i, LANES) + p.s.eps), f = -r * r * __shfl_sync(ln.mask, mean, 2 + i, LANES);
-                    const f2 r2 = f2_all(r), g2 = f2_all(f);
-                    f2 y[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        dw[which][k] = f2_fma(f2_mul(du[i][k], x[i][k]), r2, dw[which][k]);
-                        y[k] = f2_mul(f2_fma(x[i][k], g2, f2_mul(du[i][k], own[k])), r2);
-                    }
-                    if (ln.on && h + i < a1) Vec8<BF16>::store(dst, to + (long long)(h + i) * D + ln.d0, to + (long long)(h + i) * D + ln.d1, y);
-                }
+            for (int k = 0; k < 4; ++k) {
+                du[i][k] = f2_fma(o[k], s[k], f2_mul(g[k], c[k]));
+                sum = f2_fma(f2_mul(du[i][k], own[k]), x[i][k], sum);
             }
+            const float2 t2 = f2_get(sum);
+            ss[i] = ln.on ? f2_dot(x[i], x[i]) : 0.f;
+            dot[i] = ln.on ? t2.x + t2.y : 0.f;
+        }
+        ring.out = R::after(ring.out);
+        char* into = static_cast<char*>(w.which ? p.k_out : p.q_out) + ((long long)(w.t * (w.which ? Hk : Hq) + w.h) * D + ln.d0) * V::kValue;
+        const float mean = sum4<LANES>(ss[0], ss[1], dot[0], dot[1], ln.l, ln.mask) * inv;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float r = rsqrtf(__shfl_sync(ln.mask, mean, i, LANES) + p.s.eps), f = -r * r * __shfl_sync(ln.mask, mean, 2 + i, LANES);
+            if (!ln.on || i >= w.rows) continue;
+            const f2 r2 = f2_all(r), g2 = f2_all(f);
+            f2 y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const f2 t = f2_mul(f2_mul(du[i][k], x[i][k]), r2);
+                if (w.which) dw[1][k] = f2_add(dw[1][k], t);
+                else dw[0][k] = f2_add(dw[0][k], t);
+                y[k] = f2_mul(f2_fma(x[i][k], g2, f2_mul(du[i][k], own[k])), r2);
+            }
+            V::store(into + i * D * V::kValue, y[0], y[1]);
+            V::store(into + i * D * V::kValue + piece_gap, y[2], y[3]);
         }
     }
     if (p.part == nullptr) return;
-    __shared__ float sum[kGroups][8 * LANES];
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    float* sum = reinterpret_cast<float*>(smem);      // [groups][8 LANES]
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < 4; ++k) *reinterpret_cast<float2*>(&sum[threadIdx.x / LANES][(k < 2 ? ln.d0 : ln.d1 - 4) + 2 * k]) = f2_get(dw[which][k]);
+        for (int k = 0; k < 4; ++k)
+            *reinterpret_cast<float2*>(sum + threadIdx.x / LANES * 8 * LANES + (k < 2 ? ln.d0 : ln.d1 - 4) + 2 * k) = f2_get(dw[which][k]);
         __syncthreads();
         for (int d = threadIdx.x; d < D; d += kThreads) {
             float v = 0.f;
 #pragma unroll
-            for (int k = 0; k < kGroups; ++k) v += sum[k][d];
+            for (int k = 0; k < kGroups; ++k) v += sum[k * 8 * LANES + d];
             p.part[((size_t)blockIdx.x * 2 + which) * D + d] = v;
         }
     }
@@ -582,39 +664,44 @@ bool rows8(const Rope& p, std::initializer_list<long long> strides) {
            on16({p.q, p.k, p.v, p.cos, p.sin, p.q_weight, p.k_weight, p.q_out, p.k_out, p.v_out, p.d_q, p.d_k});
 }
 int lanes_for(int dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
-// Heads of a token a group takes: all of them while that still gives every SM its threads, a part otherwise.
-void slice_heads(Rope& p, int heads, int lanes) {
-    const long long groups = 148ll * 2048 / lanes;
-    long long n = groups / (p.s.tokens > 0 ? p.s.tokens : 1);
-    if (n < 1) n = 1;
-    if (n > heads) n = heads;
-    p.slice = (int)((heads + n - 1) / n);
-    p.slices = (heads + p.slice - 1) / p.slice;
+// How many pieces a group takes in a row, and the blocks: a token's while the machine is full all the same, one where it is not.
+int runs_for(Rope& p, int each, int lanes) {
+    const long long pieces = (long long)p.s.tokens * each, groups = 148ll * kBlocks * (kThreads / lanes);
+    p.run = (int)(pieces >= groups * each ? each : pieces > groups ? pieces / groups : 1);
+    const long long runs = (pieces + p.run - 1) / p.run, blocks = (runs + kThreads / lanes - 1) / (kThreads / lanes);
+    return (int)(blocks < 148 * kBlocks ? blocks : 148 * kBlocks);
+}
+int pieces_of(int heads, int rows) { return (heads + rows - 1) / rows; }
+template <class K>
+int run_rows(K kern, bool bf16, const Rope& p, int blocks, cudaStream_t st) {
+    const size_t bytes = bf16 ? Ring<true>::kBytes : Ring<false>::kBytes;
+    if (int rc = set_smem_limit(kern, bytes)) return rc;
+    kern<<<blocks, kThreads, bytes, st>>>(p);
+    return KDA_OK;
 }
 template <template <int, bool, bool> class K>
-void by_shape(const Rope& p, int blocks, cudaStream_t st) {
+int by_shape(const Rope& p, int blocks, cudaStream_t st) {
     const bool bf = p.s.io_dtype == KDA_DTYPE_BF16, in = p.s.interleaved != 0;
     const int lanes = lanes_for(p.s.head_dim);
-#define KDA_ROPE_CASE(L)                                                                                             \
-    if (lanes == L) {                                                                                                \
-        if (bf) in ? K<L, true, true>::run(p, blocks, st) : K<L, true, false>::run(p, blocks, st);                   \
-        else in ? K<L, false, true>::run(p, blocks, st) : K<L, false, false>::run(p, blocks, st);                    \
-    }
+#define KDA_ROPE_CASE(L)                                                                                                                            \
+    if (lanes == L)                                                                                                                                 \
+        return bf ? (in ? run_rows(K<L, true, true>::kernel(), true, p, blocks, st) : run_rows(K<L, true, false>::kernel(), true, p, blocks, st))   \
+                  : (in ? run_rows(K<L, false, true>::kernel(), false, p, blocks, st) : run_rows(K<L, false, false>::kernel(), false, p, blocks, st));
     KDA_ROPE_CASE(8) KDA_ROPE_CASE(16) KDA_ROPE_CASE(32)
 #undef KDA_ROPE_CASE
-
+    return KDA_ERR_UNSUPPORTED;
 }
 template <int L, bool B, bool I>
-struct RunForward {
-    static void run(const Rope& p, int blocks, cudaStream_t st) { norm_rope_rows_kernel<L, B, I, false><<<blocks, kThreads, 0, st>>>(p); }
+struct Forward {
+    static auto kernel() { return norm_rope_rows_kernel<L, B, I, false>; }
 };
 template <int L, bool B, bool I>
-struct RunAppend {
-    static void run(const Rope& p, int blocks, cudaStream_t st) { norm_rope_rows_kernel<L, B, I, true><<<blocks, kThreads, 0, st>>>(p); }
+struct Append {
+    static auto kernel() { return norm_rope_rows_kernel<L, B, I, true>; }
 };
 template <int L, bool B, bool I>
-struct RunBackward {
-    static void run(const Rope& p, int blocks, cudaStream_t st) { norm_rope_rows_bwd_kernel<L, B, I><<<blocks, kThreads, 0, st>>>(p); }
+struct Backward {
+    static auto kernel() { return norm_rope_rows_bwd_kernel<L, B, I>; }
 };
 
 Rope fill(const KdaRotaryShape& s, const void* q, const void* k, const float* cos, const float* sin, const void* positions, const float* qw, const float* kw) {
@@ -642,11 +729,10 @@ extern "C" int kda_norm_rope_fwd(const KdaRotaryShape* s, const void* q, const v
     p.q_out = q_out; p.k_out = k_out;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride})) {
-        const int lanes = lanes_for(s->head_dim);
-        slice_heads(p, s->q_heads + s->kv_heads, lanes);
-        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, kFwdBlocks);
-        KDA_LAUNCH("norm_rope_rows_kernel", st, by_shape<RunForward>(p, blocks, st));
-        return launch_status();
+        const int blocks = runs_for(p, pieces_of(s->q_heads, 4) + pieces_of(s->kv_heads, 4), lanes_for(s->head_dim));
+        int rc = KDA_OK;
+        KDA_LAUNCH("norm_rope_rows_kernel", st, rc = by_shape<Forward>(p, blocks, st));
+        return rc ? rc : launch_status();
     }
     const int blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), kWarps, 8);
     KDA_LAUNCH("norm_rope_kernel", st, norm_rope_kernel<false><<<blocks, kThreads, 0, st>>>(p));
@@ -655,7 +741,7 @@ extern "C" int kda_norm_rope_fwd(const KdaRotaryShape* s, const void* q, const v
 
 extern "C" size_t kda_norm_rope_bwd_scratch_bytes(const KdaRotaryShape* s) {
     if (check(s)) return 0;
-    return align_up((size_t)blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), 1, kBwdBlocks) * 2 * s->head_dim * sizeof(float), 256);
+    return align_up((size_t)blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), 1, kBlocks) * 2 * s->head_dim * sizeof(float), 256);
 }
 
 extern "C" int kda_norm_rope_bwd(const KdaRotaryShape* s, const void* q, const void* k, const float* cos, const float* sin, const void* positions,
@@ -674,12 +760,12 @@ extern "C" int kda_norm_rope_bwd(const KdaRotaryShape* s, const void* q, const v
     p.part = sums ? static_cast<float*>(scratch) : nullptr;
     int blocks;
     if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride})) {
-        const int lanes = lanes_for(s->head_dim);
-        slice_heads(p, s->q_heads + s->kv_heads, lanes);
-        blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, kBwdBlocks);
-        KDA_LAUNCH("norm_rope_rows_bwd_kernel", st, by_shape<RunBackward>(p, blocks, st));
+        blocks = runs_for(p, pieces_of(s->q_heads, 2) + pieces_of(s->kv_heads, 2), lanes_for(s->head_dim));
+        int rc = KDA_OK;
+        KDA_LAUNCH("norm_rope_rows_bwd_kernel", st, rc = by_shape<Backward>(p, blocks, st));
+        if (rc) return rc;
     } else {
-        blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), kWarps, kBwdBlocks);
+        blocks = blocks_for((long long)s->tokens * (s->q_heads + s->kv_heads), kWarps, kBlocks);
         KDA_LAUNCH("norm_rope_bwd_kernel", st, norm_rope_bwd_kernel<<<blocks, kThreads, 0, st>>>(p));
     }
     if (int rc = launch_status()) return rc;
@@ -710,11 +796,10 @@ extern "C" int kda_norm_rope_append(const KdaRotaryShape* s, const KdaPagedShape
     cudaStream_t st = (cudaStream_t)stream;
     if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride, s->v_token_stride, s->v_head_stride, g->k_page_stride, g->k_row_stride,
                   g->k_head_stride, g->v_page_stride, g->v_row_stride, g->v_head_stride})) {
-        const int lanes = lanes_for(s->head_dim);
-        slice_heads(p, s->q_heads + 2 * s->kv_heads, lanes);
-        const int blocks = blocks_for((long long)s->tokens * p.slices, kThreads / lanes, kFwdBlocks);
-        KDA_LAUNCH("norm_rope_append_rows_kernel", st, by_shape<RunAppend>(p, blocks, st));
-        return launch_status();
+        const int blocks = runs_for(p, pieces_of(s->q_heads, 4) + 2 * pieces_of(s->kv_heads, 4), lanes_for(s->head_dim));
+        int rc = KDA_OK;
+        KDA_LAUNCH("norm_rope_append_rows_kernel", st, rc = by_shape<Append>(p, blocks, st));
+        return rc ? rc : launch_status();
     }
     const int blocks = blocks_for((long long)s->tokens * (s->q_heads + 2 * s->kv_heads), kWarps, 8);
     KDA_LAUNCH("norm_rope_append_kernel", st, norm_rope_kernel<true><<<blocks, kThreads, 0, st>>>(p));

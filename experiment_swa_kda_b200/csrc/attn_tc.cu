@@ -298,7 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (ok && 128 * t + 32 * (warp & 3) < u.rows) {
             tc_fence_after();
             const bool mine = row < u.rows;
-            if (m == kLowest) l = 0.f;                  // nothing but -inf: 0 / 0
+            const bool dead = m == kLowest;             // nothing but -inf: 0 / 0 (ex2_pair ends at 2^-125)
+            if (dead) l = 0.f;
             if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);      // a NaN or +inf among the scores, which ex2_pair does not pass on
             const int tok = u.first + prow / g, head = hk * g + prow % g;
             const size_t out = (size_t)tok * a.c.heads.q_heads + head;
@@ -320,6 +321,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         for (int e = 0; e < 32; ++e) o[y][e] = 0;
                 }
                 tmem_ld_wait();
+                if (dead)
+#pragma unroll
+                    for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0;
                 if (odd_values && n > 0) {
                     // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
 #pragma unroll 1

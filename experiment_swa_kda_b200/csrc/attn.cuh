@@ -185,6 +185,7 @@ struct Call {
 int general(const Call& c, int splits, cudaStream_t st);
 bool tc_takes(const Call& c);      // bf16, head width, page size and strides that the tensor-core kernel can load
 int tc(const Call& c, int splits, cudaStream_t st);
+size_t tc_workspace(long long slots, int kv_heads, int splits, int dim);
 bool decode_takes(const Call& c);      // ... and at most 16 rows a sequence and kv head
 size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim);
 int decode(const Call& c, cudaStream_t st);

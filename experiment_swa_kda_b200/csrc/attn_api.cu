@@ -20,7 +20,7 @@ int check(const KdaPagedShape* s, bool packed) {
     return KDA_OK;
 }
 
-// Parts a row's keys are cut into where its blocks alone leave SMs idle.  What a row sees is known on the device alone, so the
+// Parts a row's keys may be cut into where its blocks alone leave SMs idle.  What a row sees is known on the device alone, so the
 // bound is the table's.
 int split_count(const KdaPagedShape& s, bool packed, int rows, int keys, int resident, int least) {      // a part has `least` key tiles
     int per_seq;
@@ -35,7 +35,13 @@ int split_count(const KdaPagedShape& s, bool packed, int rows, int keys, int res
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 int general_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 64, 64, 2 * 148, 1); }
-int tc_splits(const KdaPagedShape& s, bool packed) { return split_count(s, packed, 256, 128, 148, 2); }
+// The tensor-core kernel finds on the device how long a part should be, with a thread for each row tile; blocks without a part end at once,
+// so there may be more of them than SMs.
+int tc_splits(const KdaPagedShape& s, bool packed) {
+    int per_seq;
+    const int max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
+    return tile_slots(s.tokens, s.n_seq, max_q, s.q_heads / s.kv_heads, 256, packed, per_seq) <= 384 ? split_count(s, packed, 256, 128, 3 * 148, 4) : 1;
+}
 
 }  // namespace
 
@@ -43,11 +49,14 @@ extern "C" size_t kda_paged_attention_workspace_bytes(const KdaPagedShape* s) {
     if (check(s, true)) return 0;
     const size_t rows = (size_t)s->tokens * s->q_heads;
     size_t most = 0;
-    for (int way = 0; way < 4; ++way) {
-        const bool packed = way & 1;
+    for (int packed = 0; packed < 2; ++packed) {      // whether the batch has cu_seqlens is not known here
         if (!packed && s->tokens % s->n_seq != 0) continue;
-        const size_t n = (size_t)(way & 2 ? tc_splits(*s, packed) : general_splits(*s, packed));
-        const size_t need = n > 1 ? align_up(rows * n * sizeof(float2), 256) + rows * n * s->head_dim * sizeof(float) : 0;
+        const size_t n = (size_t)general_splits(*s, packed);
+        size_t need = n > 1 ? align_up(rows * n * sizeof(float2), 256) + rows * n * s->head_dim * sizeof(float) : 0;
+        if (need > most) most = need;
+        int per_seq;
+        const long long slots = tile_slots(s->tokens, s->n_seq, packed ? s->max_q_len : s->tokens / s->n_seq, s->q_heads / s->kv_heads, 256, packed, per_seq);
+        need = tc_workspace(slots, s->kv_heads, tc_splits(*s, packed), s->head_dim);
         if (need > most) most = need;
     }
     const int each = s->tokens / s->n_seq, max_q = s->max_q_len > each ? s->max_q_len : each;

@@ -39,6 +39,7 @@ constexpr int kSoftmaxWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kFixWarp = 10, kTh
 #define KDA_SOFTMAX_REGS "216"
 #define KDA_OTHER_REGS "72"
 constexpr int kPolyOf = 4;            // one pair of weights of so many is made by ex2_pair (8,191 tokens: none 252 us, 1/4 246, 1/2 263; 64-wide heads 229, 206, 231)
+constexpr int kMinPart = 8;           // key tiles of a part at least
 constexpr float kLazy = 8.f;
 constexpr int kStatusWait = 120;      // device status of an expired wait
 
@@ -55,9 +56,18 @@ struct Args {
     Call c;
     Tiles tiles;
     int slots, splits, box_rows, q_boxes;
-    float* part_o;
+    // Where rows are cut into parts: how many each block's have, [slots][kv heads]; of each part, [splits][slots][kv heads], a row's maximum
+    // and sum [256] and its sums [2 row tiles][2 halves of the columns][128][DP / 2], pieces of 16 bytes exchanged within a row as
+    // part_off() says.
+    int* parts;
     float2* part_ml;
+    float* part_o;
 };
+// byte offset of 16-byte piece c of row r in half a row tile's sums
+template <int DP>
+__device__ __forceinline__ int part_off(int r, int c) {
+    return r * DP * 2 + ((c ^ (r & 7)) << 4);
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -126,19 +136,53 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // keys any row of the block sees: [u.lo, u.hi); keys all of them see: [all_lo, all_hi)
     const int first_pos = u.base + u.row0 / g, last_pos = u.base + (u.row0 + u.rows - 1) / g;
     const int all_lo = window > 0 ? max(last_pos - window + 1, 0) : 0, all_hi = first_pos + 1;
-    const int t0 = u.lo / kKeys, nt = max((u.hi + kKeys - 1) / kKeys - t0, 0);
-    const int t_begin = a.splits > 1 ? t0 + nt * z / a.splits : t0, t_end = a.splits > 1 ? t0 + nt * (z + 1) / a.splits : t0 + nt;
+    // Key tiles start at the first box in reach, not at multiples of their size: a window of 1,024 keys and 64 rows is 9 tiles, not 10.
+    const int key0 = u.lo / a.box_rows * a.box_rows, nt = max((u.hi - key0 + kKeys - 1) / kKeys, 0);
+    int t_begin = 0, t_end = nt;
+    bool split = false;
+    if (a.splits > 1) {
+        // The shortest parts with which all blocks run side by side, found by halving; none where they would be little shorter than the
+        // longest row tile's keys (a part costs some 5 tiles of its own, and the join).  The host sees to it that a thread has a slot.
+        int tiles = 0;
+        Unit v;
+        if (tid < a.slots && make_unit(b, a.tiles, tid, window, v)) tiles = max((v.hi - v.lo / a.box_rows * a.box_rows + kKeys - 1) / kKeys, 1);
+        __shared__ int sums[2][kThreads / 32];
+        int turn = 0;
+        auto over = [&](int x, bool most) {
+            x = most ? __reduce_max_sync(0xffffffffu, x) : __reduce_add_sync(0xffffffffu, x);
+            turn ^= 1;
+            if (lane == 0) sums[turn][warp] = x;
+            __syncthreads();
+            int all = 0;
+#pragma unroll
+            for (int i = 0; i < kThreads / 32; ++i) all = most ? max(all, sums[turn][i]) : all + sums[turn][i];
+            return all;
+        };
+        const int longest = over(tiles, true);
+        int lo = kMinPart, hi = longest;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (over((tiles + mid - 1) / mid, false) * a.c.heads.kv_heads <= 148) hi = mid;
+            else lo = mid + 1;
+        }
+        const int part = 4 * lo > 3 * longest ? longest : lo, parts = min(max((nt + part - 1) / part, 1), a.splits);
+        if (z >= parts) return;
+        split = parts > 1;
+        t_begin = nt * z / parts;
+        t_end = nt * (z + 1) / parts;
+        if (z == 0 && tid == 0) a.parts[slot * a.c.heads.kv_heads + hk] = parts;
+    }
     auto range_of = [&](int t) {      // key tiles of row tile t
         const int r0 = u.row0 + 128 * t, r1 = min(r0 + 128, u.row0 + u.rows) - 1;
         if (r0 > r1) return Range{0, 0};
         const int hi = u.base + r1 / g + 1, lo = window > 0 ? max(u.base + r0 / g - window + 1, 0) : 0;
-        Range r{max(t_begin, lo / kKeys), min(t_end, (max(hi, 0) + kKeys - 1) / kKeys)};
+        Range r{max(t_begin, (lo - key0) / kKeys), min(t_end, (max(hi - key0, 0) + kKeys - 1) / kKeys)};
         if (r.end < r.begin) r.end = r.begin;
         return r;
     };
     const Range range[2] = {range_of(0), range_of(1)};
     // the tiles some row sees only in part
-    auto partial = [&](int j) { return j * kKeys < all_lo || (j + 1) * kKeys > all_hi; };
+    auto partial = [&](int j) { return key0 + j * kKeys < all_lo || key0 + (j + 1) * kKeys > all_hi; };
 
     if (warp == 0 && elect_one()) {
         mbar_init(bar_q, a.q_boxes ? 1 : kSoftmaxWarps);
@@ -219,8 +263,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, s[q]);
             tmem_ld_wait();
             float top = kLowest;
-            if (j * kKeys < w_lo || (j + 1) * kKeys > w_hi) {
-                const int from = first - j * kKeys, to = last - j * kKeys;      // of the tile's keys the row sees [from, to]
+            const int k0 = key0 + j * kKeys;
+            if (k0 < w_lo || k0 + kKeys > w_hi) {
+                const int from = first - k0, to = last - k0;      // of the tile's keys the row sees [from, to]
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int lo = min(max(from - 32 * q, 0), 32), hi = min(max(to - 32 * q + 1, 0), 32);
@@ -303,10 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);      // a NaN or +inf among the scores, which ex2_pair does not pass on
             const int tok = u.first + prow / g, head = hk * g + prow % g;
             const size_t out = (size_t)tok * a.c.heads.q_heads + head;
-            const bool split = a.splits > 1;
-            const size_t at = (size_t)z * b.tokens * a.c.heads.q_heads + out;
+            const size_t part = ((size_t)z * a.slots + slot) * a.c.heads.kv_heads + hk;
             const float inv = split ? 1.f : m == -INFINITY ? 0.f : 1.f / l;
-            if (mine && split) a.part_ml[at] = make_float2(m == -INFINITY ? m : max_nan(m * c, kLowest), l);
+            if (mine && split) a.part_ml[part * kRows + row] = make_float2(m == -INFINITY ? m : m < INFINITY ? max_nan(m * c, kLowest) : __int_as_float(0x7fffffff), l);
             if (mine && !split && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m * c + log2f(l)) * kLn2;
             uint8_t* stage_out = sm + t * L::kTile;      // Q has been read; rows as TMA lays them out
             const int x0 = 32 * (warp & 3);
@@ -327,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (odd_values && n > 0) {
                     // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
 #pragma unroll 1
-                    for (int key = max(first, r.begin * kKeys); key <= min(last, r.end * kKeys - 1); ++key) {
+                    for (int key = max(max(first, 0), key0 + r.begin * kKeys); key <= min(last, key0 + r.end * kKeys - 1); ++key) {
                         if (key >= all_lo && key < all_hi) {
                             key = all_hi - 1;
                             continue;
@@ -345,12 +389,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 }
                 if (split) {
-                    float* dst = a.part_o + at * D + 64 * q;
+                    // a warp's rows, half of the columns at a time (64-wide heads: both halves here), as they lie in the workspace
 #pragma unroll
-                    for (int e = 0; e < 64; e += 4)
-                        if (mine && 64 * q + e < D)
-                            *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(o[e >> 5][e & 31]), __uint_as_float(o[e >> 5][(e & 31) + 1]),
-                                                                              __uint_as_float(o[e >> 5][(e & 31) + 2]), __uint_as_float(o[e >> 5][(e & 31) + 3]));
+                    for (int h = 0; h < 128 / DP; ++h) {
+                        constexpr int kCols = DP / 2;
+                        uint8_t* at = stage_out + x0 * DP * 2;
+                        if (q + h > 0) {      // the copy before has read its place
+                            tma_store_wait_read();
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int x = 0; x < kCols / 4; ++x) {
+                            const int e = kCols * h + 4 * x;
+                            *reinterpret_cast<uint4*>(at + part_off<DP>(lane, x)) = make_uint4(o[e >> 5][e & 31], o[e >> 5][(e & 31) + 1], o[e >> 5][(e & 31) + 2], o[e >> 5][(e & 31) + 3]);
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            const float* dst = a.part_o + ((part * 2 + t) * 2 + q + h) * (128 * kCols) + x0 * kCols;
+                            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(at)), "r"(32 * kCols * 4) : "memory");
+                            tma_store_commit();
+                        }
+                    }
                 } else {
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
@@ -362,7 +422,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 }
             }
-            if (!split && a.q_boxes && 128 * (t + 1) <= u.rows) {
+            if (split) {
+                tma_store_wait_read();
+            } else if (a.q_boxes && 128 * (t + 1) <= u.rows) {
                 // a full tile leaves by TMA, as Q came
                 fence_async_smem();
                 asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory");
@@ -374,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     tma_store_commit();
                     tma_store_wait_read();
                 }
-            } else if (!split) {
+            } else {
                 __syncwarp();
                 constexpr int kLanes = DP / 8;      // lanes that hold a row
                 __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.c.o);
@@ -452,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             bool ok = true;
             const int total = 2 * (t_end - t_begin);
             auto look = [&](int j, int& row) {      // page of this lane's box, -1: nothing to load
-                const int key = j * kKeys + box * a.box_rows;
+                const int key = key0 + j * kKeys + box * a.box_rows;
                 if (box >= boxes || j >= t_end || key >= u.hi || key + a.box_rows <= u.lo) return -1;
                 const int col = key / b.page_size;
                 row = key - col * b.page_size;
@@ -515,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 uint8_t* v = sm + L::kRing + s * L::kTile;
                 // keys [0, head) and [tail, 128) of the tile; a piece of eight values a thread, DP / 8 threads a row
                 constexpr int kChunks = DP / 8, kStep = 64 / kChunks;
-                const int k0 = j * kKeys, head = min(max(all_lo - k0, 0), kKeys), tail = max(min(max(all_hi - k0, 0), kKeys), head);
+                const int k0 = key0 + j * kKeys, head = min(max(all_lo - k0, 0), kKeys), tail = max(min(max(all_hi - k0, 0), kKeys), head);
                 const int x = tid - kFixWarp * 32, ch = x % kChunks;
 #pragma unroll 4
                 for (int y = x / kChunks; y < head + kKeys - tail; y += kStep) {
@@ -549,12 +611,72 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
+// Joins the parts of 32 rows: a warp four of them, eight lanes a row.
+template <int DP>
+__global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant__ Args a) {
+    const Batch& b = a.c.batch;
+    const int slot = blockIdx.x >> 3, hk = blockIdx.y, g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads;
+    const int lane = threadIdx.x & 31, l8 = lane & 7, row = 32 * (blockIdx.x & 7) + 4 * (threadIdx.x >> 5) + (lane >> 3);
+    Unit u;
+    if (!make_unit(b, a.tiles, slot, a.c.window, u) || 32 * (int)(blockIdx.x & 7) >= u.rows) return;
+    dependency_wait();
+    int parts;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(parts) : "l"(a.parts + slot * Hk + hk) : "memory");
+    if (parts < 2) return;
+    const size_t step = (size_t)a.slots * Hk, unit = (size_t)slot * Hk + hk;
+    float m = -INFINITY, l = 0.f;
+    for (int z = l8; z < parts; z += 8) m = max_nan(m, ld_after_f32(&a.part_ml[(unit + z * step) * kRows + row].x));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    constexpr int kPieces = DP / 32;      // pieces of four values a lane: l8, l8 + 8, ... of the row's
+    f2 acc[kPieces][2];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) acc[i][0] = acc[i][1] = f2_all(0.f);
+    const int r = row & 127;
+#pragma unroll 4
+    for (int z = 0; z < parts; ++z) {
+        const size_t part = unit + z * step;
+        const uint2 ml = ld_after8(a.part_ml + part * kRows + row);
+        const char* src = reinterpret_cast<const char*>(a.part_o + (part * 2 + (row >> 7)) * (128 * DP));
+        uint4 v[kPieces];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            const int piece = l8 + 8 * i, half = piece / (DP / 8), c = piece % (DP / 8);
+            v[i] = ld_after16(src + half * (128 * DP * 2) + part_off<DP>(r, c));
+        }
+        const float x = __uint_as_float(ml.x), f = x == -INFINITY ? 0.f : ex2(x - m);
+        if (x == -INFINITY) continue;      // its sums are 0
+        l = fmaf(__uint_as_float(ml.y), f, l);
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            acc[i][0] = f2_fma(f2_make(__uint_as_float(v[i].x), __uint_as_float(v[i].y)), f2_all(f), acc[i][0]);
+            acc[i][1] = f2_fma(f2_make(__uint_as_float(v[i].z), __uint_as_float(v[i].w)), f2_all(f), acc[i][1]);
+        }
+    }
+    if (row >= u.rows) return;
+    const int pr = u.row0 + row, tok = pr / g;
+    const size_t out = (size_t)(u.first + tok) * a.c.heads.q_heads + hk * g + pr - tok * g;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    if (l8 == 0 && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int d = 4 * (l8 + 8 * i);
+        if (d < D)
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(f2_to_bf16(f2_mul(acc[i][0], f2_all(inv))), f2_to_bf16(f2_mul(acc[i][1], f2_all(inv))));
+    }
+}
+
 template <int DP>
 int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CUtensorMap& mQ, const CUtensorMap& mO, const Args& a, cudaStream_t st) {
     if (int rc = set_smem_limit(attn_tc_kernel<DP>, Layout<DP>::kBytes)) return rc;
     const dim3 grid((unsigned)a.slots, (unsigned)c.heads.kv_heads, (unsigned)a.splits);
     KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
-    return launch_status();
+    if (int rc = launch_status()) return rc;
+    if (a.splits == 1) return KDA_OK;
+    cudaError_t e = cudaSuccess;
+    KDA_LAUNCH("attn_tc_join_kernel", st,
+               e = launch_early(attn_tc_join_kernel<DP>, dim3((unsigned)a.slots * 8, (unsigned)c.heads.kv_heads), 256, 0, st, true, 1, a));
+    return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 }  // namespace
@@ -581,9 +703,16 @@ int tc(const Call& c, int splits, cudaStream_t st) {
     a.slots = (int)tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq);
     a.splits = splits;
     a.box_rows = c.batch.page_size < kKeys ? c.batch.page_size : kKeys;
-    const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
-    a.part_ml = static_cast<float2*>(c.workspace);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * splits * sizeof(float2), 256));
+    a.parts = nullptr;
+    a.part_ml = nullptr;
+    a.part_o = nullptr;
+    if (splits > 1) {
+        const size_t units = (size_t)a.slots * c.heads.kv_heads;
+        char* ws = static_cast<char*>(c.workspace);
+        a.parts = reinterpret_cast<int*>(ws);
+        a.part_ml = reinterpret_cast<float2*>(ws + align_up(units * sizeof(int), 256));
+        a.part_o = reinterpret_cast<float*>(a.part_ml + units * splits * kRows);
+    }
     CUtensorMap mK, mV, mQ, mO;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
@@ -594,8 +723,14 @@ int tc(const Call& c, int splits, cudaStream_t st) {
     if (!rc && a.q_boxes)
         rc = make_map_packed(&mO, c.o, c.heads.dim, c.heads.q_heads, c.batch.tokens, c.heads.dim, (int64_t)c.heads.q_heads * c.heads.dim, c.heads.group, 128 / c.heads.group);
     if (!rc) rc = c.heads.dim <= 64 ? launch<64>(c, mK, mV, mQ, mO, a, st) : launch<128>(c, mK, mV, mQ, mO, a, st);
-    if (rc || splits == 1) return rc;
-    return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, splits, a.part_o, a.part_ml, c.o, c.lse, c.bf16}, st);
+    return rc;
+}
+
+// of a call whose rows are cut into `splits` parts at most
+size_t tc_workspace(long long slots, int kv_heads, int splits, int dim) {
+    if (splits < 2) return 0;
+    const size_t units = (size_t)slots * kv_heads, width = dim <= 64 ? 64 : 128;
+    return align_up(units * sizeof(int), 256) + units * splits * kRows * (sizeof(float2) + width * sizeof(float));
 }
 
 }  // namespace attn

@@ -16,11 +16,14 @@ pages.  These three are read on the device: a decode loop captures the calls in 
 
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
+import torch.nn as nn
 
 from . import _native, ops
+from .kda import Linear
 
 Tensor = torch.Tensor
 
@@ -173,4 +176,60 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     raise RuntimeError("paged_attention: the batch or the block table is too large for one call, or a trace is being recorded")
 
 
-__all__ = ["paged_attention", "qk_norm_rope", "qk_norm_rope_append"]
+# ------------------------------------------------------------------------------------------
+# the layer
+# ------------------------------------------------------------------------------------------
+
+@dataclass
+class PagedCache:
+    """Pages of one attention layer and where the sequences of a serving batch have theirs.  The caller's scheduler owns it: it
+    hands out pages through `block_table`, and sets `kv_lens` before a step to what a sequence will have after it."""
+
+    k: Tensor               # [pages, page_size, Hk, D]
+    v: Tensor
+    block_table: Tensor     # [N, pages of a sequence] int32
+    kv_lens: Tensor         # [N] int32
+
+    @staticmethod
+    def zeros(sequences: int, max_len: int, page_size: int, num_kv_heads: int, head_dim: int, device, dtype=torch.bfloat16) -> "PagedCache":
+        """Room for `max_len` tokens of every sequence, pages dealt out in order."""
+        each = -(-max_len // page_size)
+        pages = lambda: torch.zeros(sequences * each, page_size, num_kv_heads, head_dim, device=device, dtype=dtype)
+        table = torch.arange(sequences * each, device=device, dtype=torch.int32).view(sequences, each)
+        return PagedCache(pages(), pages(), table, torch.zeros(sequences, device=device, dtype=torch.int32))
+
+
+class PagedAttention(nn.Module):
+    """A full (`window` 0) or sliding-window attention layer for serving, the neighbour of `KimiDeltaAttention` in a model that mixes
+    both: projections -> norm, rotation and cache append in one launch -> attention over the pages -> output projection."""
+
+    def __init__(self, hidden_size: int, num_heads: int, num_kv_heads: int, head_dim: int, window: int = 0, max_positions: int = 65536,
+                 rope_base: float = 10000.0, norm_eps: float = 1e-6):
+        super().__init__()
+        if num_kv_heads <= 0 or num_heads % num_kv_heads != 0:
+            raise ValueError("num_kv_heads must divide num_heads")
+        self.num_heads, self.num_kv_heads, self.head_dim, self.window, self.norm_eps = num_heads, num_kv_heads, head_dim, window, norm_eps
+        self.qkv_proj = Linear(hidden_size, (num_heads + 2 * num_kv_heads) * head_dim, bias=False)
+        self.q_norm = nn.Parameter(torch.ones(head_dim))
+        self.k_norm = nn.Parameter(torch.ones(head_dim))
+        self.o_proj = Linear(num_heads * head_dim, hidden_size, bias=False)
+        freq = rope_base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
+        angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq
+        self.register_buffer("cos", angle.cos().float(), persistent=False)
+        self.register_buffer("sin", angle.sin().float(), persistent=False)
+
+    @torch.no_grad()
+    def forward(self, hidden_states: Tensor, cache: PagedCache, cu_seqlens: Optional[Tensor] = None, max_q_len: int = 0) -> Tensor:
+        """hidden_states [B,T,hidden], T new tokens of each of the cache's B sequences, or [1,tokens,hidden], packed, with `cu_seqlens`."""
+        lead = hidden_states.shape[:-1]
+        if cu_seqlens is None:
+            max_q_len = hidden_states.shape[1]
+        qkv = self.qkv_proj(hidden_states).reshape(-1, self.num_heads + 2 * self.num_kv_heads, self.head_dim)
+        q, k, v = qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), 1)
+        place = (cache.k, cache.v, cache.block_table, cache.kv_lens, cu_seqlens)
+        q = qk_norm_rope_append(q, k, v, self.cos, self.sin, *place, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.norm_eps)
+        o = paged_attention(q, *place, max_q_len=max_q_len, window=self.window)
+        return self.o_proj(o.reshape(*lead, -1))
+
+
+__all__ = ["PagedAttention", "PagedCache", "paged_attention", "qk_norm_rope", "qk_norm_rope_append"]

@@ -568,10 +568,17 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Cut cut = find_start<kJoinThreads>(b, Hk, window, a.blocks, id, &start, sums);
-    if (id >= cut.used) return;
+    // No block ends before the stretches have: whoever is launched behind this kernel takes that for the end of both.
+    if (id >= cut.used) {
+        dependency_wait();
+        return;
+    }
     const Seq s = start.s;
     const int unit = cut.begin(id) - (start.tile - s.t0), unit_end = unit + (s.t1 - s.t0);      // of the list
-    if (unit == cut.begin(id) || cut.begin(id - 1) > unit) return;
+    if (unit == cut.begin(id) || cut.begin(id - 1) > unit) {
+        dependency_wait();
+        return;
+    }
     int parts = 1;      // stretches id - 1 .. id - 1 + parts
     while (id + parts < cut.used && cut.begin(id + parts) < unit_end) ++parts;
     const int rows = min(s.count * g, kRows);

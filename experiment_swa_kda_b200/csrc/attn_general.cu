@@ -245,8 +245,8 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
     const long long rows = (long long)c.tokens * c.q_heads;
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
+    dependency_wait();      // in every block: the end of this kernel stands for that of the one before too
     if (row >= rows) return;
-    dependency_wait();
     float m = -INFINITY;
     for (int z = lane; z < c.splits; z += 32) m = fmaxf(m, ld_after_f32(&c.part_ml[z * rows + row].x));
 #pragma unroll

@@ -669,7 +669,7 @@ int runs_for(Rope& p, int each, int lanes) {
     const long long pieces = (long long)p.s.tokens * each, groups = 148ll * kBlocks * (kThreads / lanes);
     p.run = (int)(pieces >= groups * each ? each : pieces > groups ? pieces / groups : 1);
     const long long runs = (pieces + p.run - 1) / p.run, blocks = (runs + kThreads / lanes - 1) / (kThreads / lanes);
-    return (int)(blocks < 148 * kBlocks ? blocks : 148 * kBlocks);
+    return (int)(blocks < 1 ? 1 : blocks < 148 * kBlocks ? blocks : 148 * kBlocks);
 }
 int pieces_of(int heads, int rows) { return (heads + rows - 1) / rows; }
 template <class K>

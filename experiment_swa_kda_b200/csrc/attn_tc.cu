@@ -618,8 +618,9 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
     const int slot = blockIdx.x >> 3, hk = blockIdx.y, g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads;
     const int lane = threadIdx.x & 31, l8 = lane & 7, row = 32 * (blockIdx.x & 7) + 4 * (threadIdx.x >> 5) + (lane >> 3);
     Unit u;
-    if (!make_unit(b, a.tiles, slot, a.c.window, u) || 32 * (int)(blockIdx.x & 7) >= u.rows) return;
-    dependency_wait();
+    const bool some = make_unit(b, a.tiles, slot, a.c.window, u);
+    dependency_wait();      // in every block: the end of this kernel stands for that of the one before too
+    if (!some || 32 * (int)(blockIdx.x & 7) >= u.rows) return;
     int parts;
     asm volatile("ld.global.s32 %0, [%1];" : "=r"(parts) : "l"(a.parts + slot * Hk + hk) : "memory");
     if (parts < 2) return;

@@ -130,8 +130,10 @@ def test_norm_rope_partial_gradients_streams_and_repeats():
         zq, _ = m.qk_norm_rope(q, k, cos, sin, q_weight=w.detach())
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(yq, zq)
-    empty = m.qk_norm_rope(q[:, :0], k[:, :0], cos, sin)
+    empty = m.qk_norm_rope(q[:, :0], k[:, :0], cos, sin, q_weight=w)
     assert empty[0].shape == (2, 0, 4, 128)
+    none, = torch.autograd.grad(empty[0].float().sum(), w)
+    assert torch.equal(none, torch.zeros_like(none))
 
 
 # ---------------------------------------------------------------------------------------------- paged batches
@@ -212,6 +214,37 @@ def test_paged_attention(case, dtype, bound):
     fine = torch.isfinite(wlse)
     assert ((got - wlse)[fine].abs() <= 2e-5 * (1 + wlse[fine].abs())).all()
     assert torch.equal(o, b.attend(max_q_len=max(q_lens) if bound else 0))      # the same bits again, with and without lse
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hk,D,page,window,longest", [(8, 2, 128, 16, 0, 300), (3, 3, 64, 64, 50, 200), (16, 1, 128, 128, 0, 90), (12, 1, 96, 16, 33, 400)])
+def test_token_steps_of_many_sequences(dtype, Hq, Hk, D, page, window, longest):
+    """More sequences than threads of a block, of every length, some empty: stretches begin and end anywhere."""
+    gen = torch.Generator().manual_seed(longest)
+    kv_lens = torch.randint(0, longest, (260,), generator=gen).tolist()
+    b = Batch([1] * 260, kv_lens, Hq, Hk, D, page, dtype, window, seed=longest)
+    o, lse = b.attend(return_lse=True, max_q_len=1)
+    want, wlse, size = b.oracle()
+    close(o, want, size, dtype)
+    assert torch.equal(torch.isinf(lse.cpu()), torch.isinf(wlse))
+
+
+@pytest.mark.parametrize("case", [
+    ([70], [5000], 2, 1, 128, 64, 0),                 # one row tile and long rows: parts
+    ([5, 300, 1, 33], [3000, 300, 2500, 1000], 4, 2, 64, 16, 0),
+    ([200], [4000], 6, 2, 128, 32, 3000),
+    ([40, 2], [1500, 2100], 40, 2, 128, 16, 0),       # groups of 20: rows that are no whole tokens
+    ([300, 300], [700, 320], 16, 16, 128, 16, 130),
+    ([129], [900], 32, 1, 128, 8, 0),
+], ids=lambda c: f"q{max(c[0])}_kv{max(c[1])}_h{c[2]}_{c[3]}_d{c[4]}_p{c[5]}_w{c[6]}")
+@pytest.mark.parametrize("bound", [False, True], ids=["", "max_q_len"])
+def test_long_rows_and_wide_groups(case, bound):
+    q_lens, kv_lens, Hq, Hk, D, page, window = case
+    b = Batch(q_lens, kv_lens, Hq, Hk, D, page, BF16, window, seed=page, heads_first=not bound)
+    o, lse = b.attend(return_lse=True, max_q_len=max(q_lens) if bound else 0)
+    want, wlse, size = b.oracle()
+    close(o, want, size, BF16)
+    assert ((lse.double().cpu() - wlse).abs() <= 2e-5 * (1 + wlse.abs())).all()
 
 
 @pytest.mark.parametrize("q_len", [1, 3, 150])
@@ -298,6 +331,18 @@ def test_offsets_beyond_32_bits():
         o = m.paged_attention(b.dq, k, v, table, b.dlens, b.dcu)
         want, _, size = b.oracle()
         close(o, want, size, BF16)
+
+
+@pytest.mark.parametrize("q_len,Hq,kv", [(1, 8, 3000), (1, 4, 60), (40, 8, 6000), (300, 3, 500)])
+def test_what_follows_finds_the_output(q_len, Hq, kv):
+    """Kernels that start early end behind those before them: the next one in the stream reads whole results, call after call."""
+    b = Batch([q_len] * 4, [kv] * 4, Hq, 1, 128, 16, BF16)
+    first = b.attend(max_q_len=q_len).clone()
+    for _ in range(20):
+        o = b.attend(max_q_len=q_len)
+        seen = o + 0
+        o.zero_()
+        assert torch.equal(seen, first)
 
 
 def test_graph_follows_the_arrays():
@@ -445,6 +490,9 @@ def test_bad_tables_are_reported(q_len):
     b.attend()
     b.dcu.copy_(b.cu)
     report("cu_seqlens")
+    if q_len > 1:
+        b.attend(max_q_len=q_len // 2)      # a bound that is none
+        report("cu_seqlens")
     cos, sin = (t.to(DEV) for t in tables(299, 128))      # one position short
     kv = torch.zeros(q_len, 2, 128, device=DEV, dtype=BF16)
     m.qk_norm_rope_append(b.dq, kv, kv, cos, sin, b.dk.clone(), b.dv.clone(), b.dtable, b.dlens, b.dcu)

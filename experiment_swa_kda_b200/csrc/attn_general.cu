@@ -5,7 +5,9 @@
 // A block holds 64 rows (token-major, the query heads of one kv head side by side, so that a key tile serves them all) and
 // goes through its keys in tiles of 64.  Both products are 4 x 4 outputs a thread from 16-byte shared-memory reads: bound by
 // the multiply-add pipes once there is work for every SM, by the way to memory before that.  Four threads fetch a row, one look at the
-// table each, in 16-byte pieces where the addresses allow it.
+// table each, in 16-byte pieces where the addresses allow it.  Two times 257 tokens over 515, float32, 4 heads of 64 on 2: 27 us
+// (288 blocks of one or two tiles, each the latency of its fetches and of 8,192 cycles of products at two warps a scheduler); tiles fetched
+// ahead into registers took as long.
 
 #include "attn.cuh"
 

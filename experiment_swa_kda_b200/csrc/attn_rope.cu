@@ -8,7 +8,8 @@
 // Everything is float32 between the load and the one rounding of the store.  r is formed again in the backward: it costs a sum
 // over values that are in registers anyway, a saved one would be read.
 //
-// Bound by memory.  Two forms each way: norm_rope_rows_* for widths, strides and addresses that allow wide accesses, and
+// Bound by memory, and close behind it by issue: 65,536 tokens of 16 + 4 heads take 122 us forward (5.5 TB/s, 0.84 of the copy
+// rate) and 225 backward (4.5 TB/s, 63 % of the issue slots); 8,191 tokens into the cache 29.  Two forms each way: norm_rope_rows_* for widths, strides and addresses that allow wide accesses, and
 // norm_rope_kernel / norm_rope_bwd_kernel for all others.
 
 #include <initializer_list>

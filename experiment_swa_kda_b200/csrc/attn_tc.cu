@@ -582,28 +582,44 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (!ok) break;
                 phase ^= 1u << s;
                 uint8_t* v = sm + L::kRing + s * L::kTile;
-                // keys [0, head) and [tail, 128) of the tile; a piece of eight values a thread, DP / 8 threads a row
+                // Keys [0, head) and [tail, 128) of the tile, a piece of eight values a thread, DP / 8 threads a row: those outside of
+                // [u.lo, u.hi) are blanked, the others looked through.  The product of the tile waits for this.
                 constexpr int kChunks = DP / 8, kStep = 64 / kChunks;
                 const int k0 = key0 + j * kKeys, head = min(max(all_lo - k0, 0), kKeys), tail = max(min(max(all_hi - k0, 0), kKeys), head);
-                const int x = tid - kFixWarp * 32, ch = x % kChunks;
-#pragma unroll 4
-                for (int y = x / kChunks; y < head + kKeys - tail; y += kStep) {
-                    const int r = y < head ? y : y - head + tail, key = k0 + r;
-                    uint4* at = reinterpret_cast<uint4*>(v + (ch >> 3) * 16384 + sw128_off(r, ch & 7));
-                    uint4 w = *at;
-                    uint32_t* p = reinterpret_cast<uint32_t*>(&w);
-                    const bool out = key < u.lo || key >= u.hi;
-                    bool here = out;
+                const int x = tid - kFixWarp * 32, ch = x % kChunks, y0 = x / kChunks;
+                auto place = [&](int r) { return reinterpret_cast<uint4*>(v + (ch >> 3) * 16384 + sw128_off(r, ch & 7)); };
+                auto through = [&](int from, int to) {
+                    constexpr int kAhead = 8;
+                    for (int r = from + y0; r < to; r += kAhead * kStep) {
+                        uint4 w[kAhead];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t keep = 0xffffffffu;
-                        if ((p[k] & 0x7f80u) == 0x7f80u) keep = 0xffff0000u;
-                        if ((p[k] & 0x7f800000u) == 0x7f800000u) keep &= 0xffffu;
-                        if (keep != 0xffffffffu && !out) here = odd = true;
-                        p[k] = out ? 0u : p[k] & keep;
+                        for (int k = 0; k < kAhead; ++k) w[k] = *place(min(r + k * kStep, kKeys - 1));
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k) {
+                            // an exponent of ones and one more is the sign's bit
+                            auto ones = [](uint32_t z) { return ((z & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };
+                            if (r + k * kStep >= to || (ones(w[k].x) | ones(w[k].y) | ones(w[k].z) | ones(w[k].w)) == 0) continue;
+                            odd = true;
+                            uint32_t* p = reinterpret_cast<uint32_t*>(&w[k]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if ((p[i] & 0x7f80u) == 0x7f80u) p[i] &= 0xffff0000u;
+                                if ((p[i] & 0x7f800000u) == 0x7f800000u) p[i] &= 0xffffu;
+                            }
+                            *place(r + k * kStep) = w[k];
+                        }
                     }
-                    if (here) *at = w;
-                }
+                };
+                auto blank = [&](int from, int to) {
+                    for (int r = from + y0; r < to; r += kStep) *place(r) = make_uint4(0, 0, 0, 0);
+                };
+                const int lo = min(max(u.lo - k0, 0), kKeys), hi = min(max(u.hi - k0, 0), kKeys);      // keys in reach
+                blank(0, min(lo, head));
+                through(min(lo, head), min(head, hi));
+                blank(hi, head);
+                blank(tail, lo);
+                through(max(tail, lo), hi);
+                blank(max(tail, hi), kKeys);
                 if (odd) odd_values = 1;
                 __threadfence_block();
                 fence_async_smem();

@@ -136,6 +136,26 @@ def test_norm_rope_partial_gradients_streams_and_repeats():
     assert torch.equal(none, torch.zeros_like(none))
 
 
+def test_norm_rope_trace_and_weight_types():
+    import experiment_swa_kda_b200 as m
+    gen = torch.Generator().manual_seed(6)
+    q, k = (torch.randn(1, 20, h, 64, generator=gen).to(BF16).to(DEV) for h in (2, 1))
+    cos, sin = (t.to(DEV) for t in tables(20, 64))
+    w = (1 + 0.1 * torch.randn(64, generator=gen)).to(BF16).to(DEV)
+    traced = torch.jit.trace(lambda q, k, w: m.qk_norm_rope(q, k, cos, sin, k_weight=w), (q, k, w), check_trace=False)
+    for a, b in zip(traced(q, k, w), m.qk_norm_rope(q, k, cos, sin, k_weight=w)):
+        assert torch.equal(a, b)
+    wanted = w.clone().requires_grad_(True)      # a bf16 weight gets a bf16 gradient, rounded once
+    yk = m.qk_norm_rope(q, k, cos, sin, k_weight=wanted)[1]
+    got, = torch.autograd.grad(yk.sum(), wanted)
+    _, dw = A.norm_rope_backward(k.cpu(), torch.ones(k.shape), cos.cpu(), sin.cpu(), w.cpu(), 1e-6, False)
+    assert got.dtype == BF16
+    assert ((got.double().cpu() - dw).abs() <= U * dw.abs() + 1e-5 * 20).all()
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        with torch.autograd.forward_ad.dual_level():
+            m.qk_norm_rope(torch.autograd.forward_ad.make_dual(q, q), k, cos, sin)
+
+
 # ---------------------------------------------------------------------------------------------- paged batches
 
 class Batch:

@@ -254,17 +254,25 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float acc[8] = {}, l = 0.f;
-#pragma unroll 4
-    for (int z = 0; z < c.splits; ++z) {
-        const uint2 ml = ld_after8(c.part_ml + z * rows + row);
-        const float x = __uint_as_float(ml.x);
-        if (x == -INFINITY) continue;
-        const float w = exp2f(x - m);
-        l += __uint_as_float(ml.y) * w;
+    constexpr int kAhead = 4;
+    for (int z0 = 0; z0 < c.splits; z0 += kAhead) {
+        uint2 ml[kAhead];
+        float v[kAhead][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = lane + 32 * i;
-            if (d < c.dim) acc[i] = fmaf(w, ld_after_f32(c.part_o + (z * rows + row) * c.dim + d), acc[i]);
+        for (int k = 0; k < kAhead; ++k) {
+            const long long at = (long long)min(z0 + k, c.splits - 1) * rows + row;
+            ml[k] = ld_after8(c.part_ml + at);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = lane + 32 * i < c.dim ? ld_after_f32(c.part_o + at * c.dim + lane + 32 * i) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const float x = __uint_as_float(ml[k].x);
+            if (z0 + k >= c.splits || x == -INFINITY) continue;      // without a key its sums are 0
+            const float w = exp2f(x - m);
+            l += __uint_as_float(ml[k].y) * w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[k][i], acc[i]);
         }
     }
     const float inv = m == -INFINITY ? 0.f : 1.f / l;

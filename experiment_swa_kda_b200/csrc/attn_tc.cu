@@ -148,31 +148,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     int t_begin = 0, t_end = nt;
     bool split = false;
     if (a.splits > 1) {
-        // The shortest parts with which all blocks run side by side, found by halving; none where they would be little shorter than the
-        // longest row tile's keys (a part costs some 5 tiles of its own, and the join).  The host sees to it that a thread has a slot.
+        // The shortest parts with which all blocks run side by side, looked for by one length a warp, twice; none where they would be
+        // little shorter than the longest row tile's keys (a part costs some 5 tiles of its own, and the join).  The host sees to it
+        // that a thread has a slot.
+        constexpr int kTries = kThreads / 32;
+        int *tiles_of = reinterpret_cast<int*>(sm), *blocks_of = tiles_of + kThreads;      // nothing else is there yet
         int tiles = 0;
         Unit v;
         if (tid < a.slots && make_unit(b, a.tiles, tid, window, v)) tiles = max((v.hi - v.lo / a.box_rows * a.box_rows + kKeys - 1) / kKeys, 1);
-        __shared__ int sums[2][kThreads / 32];
-        int turn = 0;
-        auto over = [&](int x, bool most) {
-            x = most ? __reduce_max_sync(0xffffffffu, x) : __reduce_add_sync(0xffffffffu, x);
-            turn ^= 1;
-            if (lane == 0) sums[turn][warp] = x;
-            __syncthreads();
-            int all = 0;
+        tiles_of[tid] = tiles;
+        __syncthreads();
+        int longest = 0;
+        for (int i = lane; i < a.slots; i += 32) longest = max(longest, tiles_of[i]);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        int lo = min(kMinPart, longest), hi = longest;      // hi is long enough, or nothing is
 #pragma unroll
-            for (int i = 0; i < kThreads / 32; ++i) all = most ? max(all, sums[turn][i]) : all + sums[turn][i];
-            return all;
-        };
-        const int longest = over(tiles, true);
-        int lo = kMinPart, hi = longest;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (over((tiles + mid - 1) / mid, false) * a.c.heads.kv_heads <= 148) hi = mid;
-            else lo = mid + 1;
+        for (int round = 0; round < 2; ++round) {
+            const int step = (hi - lo) / kTries + 1, mine = min(lo + warp * step, hi);
+            int sum = 0;
+            for (int i = lane; i < a.slots; i += 32) sum += (tiles_of[i] + mine - 1) / mine;
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == 0) blocks_of[round * kTries + warp] = sum;
+            __syncthreads();
+            int first = 0;
+            while (first < kTries - 1 && blocks_of[round * kTries + first] * a.c.heads.kv_heads > 148) ++first;
+            hi = min(lo + first * step, hi);
+            lo = first > 0 ? min(lo + (first - 1) * step + 1, hi) : hi;
         }
-        const int part = 4 * lo > 3 * longest ? longest : lo, parts = min(max((nt + part - 1) / part, 1), a.splits);
+        const int part = 4 * hi > 3 * longest ? longest : hi, parts = min(max((nt + part - 1) / part, 1), a.splits);
         if (z >= parts) return;
         split = parts > 1;
         t_begin = nt * z / parts;
@@ -646,32 +649,38 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
     if (parts < 2) return;
     const size_t step = (size_t)a.slots * Hk, unit = (size_t)slot * Hk + hk;
     float m = -INFINITY, l = 0.f;
-    for (int z = l8; z < parts; z += 8) m = max_nan(m, ld_after_f32(&a.part_ml[(unit + z * step) * kRows + row].x));
+    for (int z = l8; z < parts; z += 8) m = max_nan(m, a.part_ml[(unit + z * step) * kRows + row].x);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    constexpr int kPieces = DP / 32;      // pieces of four values a lane: l8, l8 + 8, ... of the row's
+    constexpr int kPieces = DP / 32, kAhead = 4;      // pieces of four values a lane: l8, l8 + 8, ... of the row's; parts on their way
     f2 acc[kPieces][2];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) acc[i][0] = acc[i][1] = f2_all(0.f);
     const int r = row & 127;
-#pragma unroll 4
-    for (int z = 0; z < parts; ++z) {
-        const size_t part = unit + z * step;
-        const uint2 ml = ld_after8(a.part_ml + part * kRows + row);
-        const char* src = reinterpret_cast<const char*>(a.part_o + (part * 2 + (row >> 7)) * (128 * DP));
-        uint4 v[kPieces];
+    for (int z0 = 0; z0 < parts; z0 += kAhead) {
+        float2 ml[kAhead];
+        float4 v[kAhead][kPieces];
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int piece = l8 + 8 * i, half = piece / (DP / 8), c = piece % (DP / 8);
-            v[i] = ld_after16(src + half * (128 * DP * 2) + part_off<DP>(r, c));
+        for (int k = 0; k < kAhead; ++k) {
+            const size_t part = unit + min(z0 + k, parts - 1) * step;
+            ml[k] = a.part_ml[part * kRows + row];
+            const char* src = reinterpret_cast<const char*>(a.part_o + (part * 2 + (row >> 7)) * (128 * DP));
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int piece = l8 + 8 * i, half = piece / (DP / 8), c = piece % (DP / 8);
+                v[k][i] = *reinterpret_cast<const float4*>(src + half * (128 * DP * 2) + part_off<DP>(r, c));
+            }
         }
-        const float x = __uint_as_float(ml.x), f = x == -INFINITY ? 0.f : ex2(x - m);
-        if (x == -INFINITY) continue;      // its sums are 0
-        l = fmaf(__uint_as_float(ml.y), f, l);
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            acc[i][0] = f2_fma(f2_make(__uint_as_float(v[i].x), __uint_as_float(v[i].y)), f2_all(f), acc[i][0]);
-            acc[i][1] = f2_fma(f2_make(__uint_as_float(v[i].z), __uint_as_float(v[i].w)), f2_all(f), acc[i][1]);
+        for (int k = 0; k < kAhead; ++k) {
+            if (z0 + k >= parts || ml[k].x == -INFINITY) continue;      // without a key its sums are 0
+            const float f = ex2(ml[k].x - m);
+            l = fmaf(ml[k].y, f, l);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                acc[i][0] = f2_fma(f2_make(v[k][i].x, v[k][i].y), f2_all(f), acc[i][0]);
+                acc[i][1] = f2_fma(f2_make(v[k][i].z, v[k][i].w), f2_all(f), acc[i][1]);
+            }
         }
     }
     if (row >= u.rows) return;

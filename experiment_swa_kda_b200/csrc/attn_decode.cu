@@ -608,21 +608,15 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
     if (of < share) {
         const int r = at / (D / 4), d = 4 * (at - r * (D / 4));
         float o[4] = {};
-        constexpr int kAhead = 8;
-        for (int k0 = of; k0 <= parts; k0 += kAhead * share) {
-            uint4 v[kAhead];
-#pragma unroll
-            for (int x = 0; x < kAhead; ++x) v[x] = ld_after16(a.part_o + place(min(k0 + x * share, parts), r) * D + d);
-#pragma unroll
-            for (int x = 0; x < kAhead; ++x) {
-                const int k = k0 + x * share;
-                const float f = k <= parts ? weight[k * kRows + r] : 0.f;
-                if (f == 0.f) continue;
-                o[0] = fmaf(__uint_as_float(v[x].x), f, o[0]);
-                o[1] = fmaf(__uint_as_float(v[x].y), f, o[1]);
-                o[2] = fmaf(__uint_as_float(v[x].z), f, o[2]);
-                o[3] = fmaf(__uint_as_float(v[x].w), f, o[3]);
-            }
+#pragma unroll 8
+        for (int k = of; k <= parts; k += share) {
+            const uint4 v = ld_after16(a.part_o + place(k, r) * D + d);
+            const float f = weight[k * kRows + r];
+            if (f == 0.f) continue;
+            o[0] = fmaf(__uint_as_float(v.x), f, o[0]);
+            o[1] = fmaf(__uint_as_float(v.y), f, o[1]);
+            o[2] = fmaf(__uint_as_float(v.z), f, o[2]);
+            o[3] = fmaf(__uint_as_float(v.w), f, o[3]);
         }
         acc[tid] = make_float4(o[0], o[1], o[2], o[3]);
     }

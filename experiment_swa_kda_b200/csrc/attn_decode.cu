@@ -36,6 +36,10 @@ using namespace tc;
 
 constexpr int kMaxRows = 16, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
 constexpr int kPerSm = 2;             // blocks an SM: 98 KB each
+// Up to so many tiles a sequence and kv head stay together: they take about as long as two of them and the join, which is a launch less (3
+// conversations of 40 tokens 14.5 us in parts, 8.4 whole; 16 of 100 12.5 and 10.4).  Six where there are sequences for every SM (200 of up
+// to 380 36 and 33), four where parts would have some to themselves (one of 300 12.4 and 13.2 with six).
+constexpr int kWholeTiles = 4, kWholeTilesOfMany = 6;
 constexpr int kMinTiles = 2;          // a stretch has at least these many tiles
 constexpr float kLazy = 8.f;          // as in the kernel for long chunks: sums are rescaled when a maximum grew by 2^8
 constexpr int kStatusWait = 121;
@@ -53,6 +57,7 @@ struct Layout {
 struct Args {
     Call c;
     int blocks, box_rows;
+    int whole;            // stretches begin and end with a sequence and kv head: no parts
     float* part_o;        // [blocks][2][rows][D]
     float2* part_ml;      // [blocks][2][rows]
 };
@@ -93,10 +98,11 @@ struct Start {
     Seq s;                // where a stretch begins
     Raw after;
     int n, hk, tile;
+    int begin, end;       // the stretch, of the list, where it is whole
 };
 // The cut, and where stretch `id` begins.  Called by all THREADS of a block; `sums` has a place for each warp.  The host takes
 // care that the list has less than 2^31 tiles.
-template <int THREADS>
+template <int THREADS, bool whole>
 __device__ __forceinline__ Cut find_start(const Batch& b, int kv_heads, int window, int blocks, int id, Start* start, int* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = (b.n_seq + THREADS - 1) / THREADS, n0 = min(tid * each, b.n_seq), n1 = min(n0 + each, b.n_seq);
@@ -120,18 +126,49 @@ __device__ __forceinline__ Cut find_start(const Batch& b, int kv_heads, int wind
         if (w < warp) upto += sums[w];
         cut.total += sums[w];
     }
-    cut.used = min(blocks, max(cut.total / kMinTiles, 1));
+    cut.used = min(blocks, max(whole ? cut.total : cut.total / kMinTiles, 1));
     cut.each = cut.total / cut.used;
     cut.longer = cut.total - cut.each * cut.used;
-    const int begin = cut.begin(id);
-    int at = upto - mine;
-    if (begin >= at && begin < upto) {
+    if (whole) {
+        if (tid == 0) {
+            start->begin = cut.begin(id);
+            start->end = cut.begin(id + 1);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int side = 0; side <= (whole ? 1 : 0); ++side) {      // whole: both ends move on to the next beginning of a sequence and kv head
+        const int place = cut.begin(id + side);
+        int at = upto - mine;
+        if (place < at || place >= upto) continue;
         for (int n = n0; n < n1; ++n) {
-            const Seq s = seq_at(b, n, window);
-            const int nt = s.t1 - s.t0, here = nt * kv_heads;
-            if (begin < at + here) {
-                const int rest = begin - at, hk = rest / nt;
-                *start = Start{s, raw_at(b, n + 1), n, hk, s.t0 + rest - hk * nt};
+            Seq s = seq_at(b, n, window);
+            int nt = s.t1 - s.t0;
+            const int here = nt * kv_heads;
+            if (place < at + here) {
+                const int rest = place - at;
+                int hk = rest / nt, tile = s.t0 + rest - hk * nt;
+                const int on = whole && tile > s.t0 ? s.t1 - tile : 0;
+                if (side == 1) {
+                    start->end = place + on;
+                    break;
+                }
+                if (on > 0) {
+                    start->begin = place + on;
+                    if (++hk == kv_heads) {
+                        hk = 0;
+                        do {
+                            if (++n >= b.n_seq) break;
+                            s = seq_at(b, n, window);
+                        } while (s.t1 <= s.t0);
+                    }
+                    tile = s.t0;
+                }
+                start->s = s;
+                start->after = raw_at(b, n + 1);
+                start->n = n;
+                start->hk = hk;
+                start->tile = tile;
                 break;
             }
             at += here;
@@ -217,8 +254,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         mbar_fence_init();
     }
     if (tid == 0) flags[0] = flags[1] = flags[2] = 0;
-    const Cut cut = find_start<kThreads>(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
-    const int tiles = cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
+    const Cut cut = a.whole ? find_start<kThreads, true>(b, Hk, window, a.blocks, blockIdx.x, &start, sums)
+                            : find_start<kThreads, false>(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
+    const int tiles = a.whole ? start.end - start.begin : cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
 
     uint8_t* ring = sm + warp * kStages * L::kStage;
     Walk ahead = {}, w = {};
@@ -569,7 +607,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const Cut cut = find_start<kJoinThreads>(b, Hk, window, a.blocks, id, &start, sums);
+    const Cut cut = find_start<kJoinThreads, false>(b, Hk, window, a.blocks, id, &start, sums);
     // No block ends before the stretches have: whoever is launched behind this kernel takes that for the end of both.
     if (id >= cut.used) {
         dependency_wait();
@@ -642,15 +680,18 @@ int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStre
     if (int rc = set_smem_limit(attn_decode_kernel<DP, NR>, kBytes)) return rc;
     KDA_LAUNCH("attn_decode_kernel", st, attn_decode_kernel<DP, NR><<<a.blocks, kThreads, kBytes, st>>>(mK, mV, a));
     if (int rc = launch_status()) return rc;
-    if (a.blocks == 1) return KDA_OK;
+    if (a.blocks == 1 || a.whole) return KDA_OK;
     cudaError_t e = cudaSuccess;
     KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
+bool keeps_whole(int n_seq, int kv_heads, long long reach) {
+    return reach <= ((long long)n_seq * kv_heads >= 148 ? kWholeTilesOfMany : kWholeTiles) * kTile;
+}
 // Stretches: as many as the machine holds, or as the longest batch that fits the table could use.
 int stretches(int n_seq, int kv_heads, long long reach) {
-    const long long tiles = ((reach + kTile - 1) / kTile + 1) * n_seq * kv_heads, n = tiles / kMinTiles;
+    const long long tiles = ((reach + kTile - 1) / kTile + 1) * n_seq * kv_heads, n = keeps_whole(n_seq, kv_heads, reach) ? tiles : tiles / kMinTiles;
     return (int)(n < 1 ? 1 : n < kMaxBlocks ? n : kMaxBlocks);
 }
 long long reach_of(int table_width, int page_size, int window, int max_q) {
@@ -676,6 +717,7 @@ int decode(const Call& c, cudaStream_t st) {
     a.c = c;
     a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
     a.box_rows = c.batch.page_size < 16 ? c.batch.page_size : 16;
+    a.whole = keeps_whole(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
     a.part_ml = static_cast<float2*>(c.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up((size_t)a.blocks * 2 * kMaxRows * sizeof(float2), 256));
     CUtensorMap mK, mV;

@@ -4,9 +4,9 @@
 //   o_i = sum_j 2^(c s_ij - c m_i) v_j / sum_j 2^(c s_ij - c m_i),   s = q k^T,  c = scale / ln 2
 //
 // Bound by the cache's bytes: a key costs 4 D bytes and at most 64 D operations.  All that counts is that every SM has its share of the
-// keys and enough copies in flight.  16 heads on 4: 32 conversations of up to 16,384 tokens 106 us (0.91 of the copy rate), 128 of
+// keys and enough copies in flight.  16 heads on 4: 32 conversations of up to 16,384 tokens 106 to 111 us (0.87 to 0.91 of the copy rate), 128 of
 // them 0.99 to 1.0; 256 with windows of 512 59 us (0.68: 9 tiles a sequence and head, so that start, ends and join count); one of
-// 3 heads and 4,097 tokens 13 us, two launches of a handful of dependent reads each.
+// 3 heads and 4,097 tokens 12 to 14 us, two launches of a handful of dependent reads each.
 //
 // - The tiles (64 keys of one sequence and kv head) of the whole batch are one list, sequence after sequence, and each block
 //   takes an equal stretch of it, whatever the sequences' lengths are.  The list is known on the device alone: every block adds up the

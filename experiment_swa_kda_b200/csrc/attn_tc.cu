@@ -14,13 +14,13 @@
 // 2^kLazy, which costs bf16 nothing: its rounding is relative); after a few tiles that no longer happens.
 // P is rounded to bf16 because the product takes one type and V is bf16; sums and statistics are float32.
 //
-// 8,191 tokens of 16 heads on 4: 238 us (1,156 TFLOP/s, 0.71 of the measured burst rate of a library product; 270 us where calls follow one
-// another and the power cap holds the clock, 0.74 of the sustained one), the tensor pipe busy for 58 % of them.  A pair of row tiles
+// 8,191 tokens of 16 heads on 4: 232 us (1,187 TFLOP/s, 0.73 of the measured burst rate of a library product; 267 us where calls follow one
+// another and the power cap holds the clock, 0.75 of the sustained one), the tensor pipe busy for 58 % of them.  A pair of row tiles
 // takes 2,900 to 3,350 cycles a key tile, of which its products need 2,048 and the special function unit 1,536: a row tile's softmax,
 // 2,000 cycles of two warps a scheduler, and the products behind it, 1,300, follow one another, and the other tile covers most of
 // that, not all.  Measured and left out: the exponentials of the two tiles in turns (270 us), maxima only where sums ask for them (261),
 // P in columns of its own for 64-wide heads (196 -> 248).  A block costs 12,000 to 16,000 cycles besides its tiles - its rows,
-// the first keys, the output -, which shows in windows: four times 2,048 tokens with windows of 1,024 take 115 us, 0.35 of the burst rate.
+// the first keys, the output -, which shows in windows: four times 2,048 tokens with windows of 1,024 take 106 us, 0.38 of the burst rate.
 //
 // K and V come page by page by TMA into one ring (K 0, V 0, K 1, V 1, ...).  A tile that some row sees only in part is masked
 // in registers; in its V tile the keys that no row sees are blanked, since 0 times what lies in an unused slot may be NaN, and

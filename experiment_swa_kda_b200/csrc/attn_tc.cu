@@ -346,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         // ------------------------------------------------------------------ O / l
         const int n = r.end - r.begin;
+        const bool full = !split && a.q_boxes && 128 * (t + 1) <= u.rows;      // the same for the row tile's warps
         if (ok && n > 0) {
             ok = wait(bar_o + t, (n - 1) & 1);
             __syncwarp();
@@ -434,19 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
             if (split) {
                 tma_store_wait_read();
-            } else if (a.q_boxes && 128 * (t + 1) <= u.rows) {
-                // a full tile leaves by TMA, as Q came
-                fence_async_smem();
-                asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory");
-                if ((warp & 3) == 0 && elect_one()) {
-                    for (int h = 0; h < DP / 64; ++h)
-                        asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(&mO), "r"(smem_u32(stage_out + h * 16384)),
-                                     "r"(h * 64), "r"(hk * g), "r"(u.first + (u.row0 + 128 * t) / g)
-                                     : "memory");
-                    tma_store_commit();
-                    tma_store_wait_read();
-                }
-            } else {
+            } else if (!full) {
                 __syncwarp();
                 constexpr int kLanes = DP / 8;      // lanes that hold a row
                 __nv_bfloat16* o = static_cast<__nv_bfloat16*>(a.c.o);
@@ -459,6 +448,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         *reinterpret_cast<uint4*>(o + ((size_t)(u.first + tk) * a.c.heads.q_heads + hk * g + hd) * D + 8 * chunk) = v;
                     for (hd += 32 / kLanes; hd >= g; hd -= g) ++tk;
                 }
+            }
+        }
+        if (full) {
+            // a full tile leaves by TMA, as Q came; its warps meet whatever their waits said
+            fence_async_smem();
+            asm volatile("bar.sync %0, 128;" ::"r"(2 + t) : "memory");
+            if ((warp & 3) == 0 && !abort_flag && elect_one()) {
+                for (int h = 0; h < DP / 64; ++h)
+                    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(&mO),
+                                 "r"(smem_u32(sm + t * L::kTile + h * 16384)), "r"(h * 64), "r"(hk * g), "r"(u.first + (u.row0 + 128 * t) / g)
+                                 : "memory");
+                tma_store_commit();
+                tma_store_wait_read();
             }
         }
     } else {
@@ -580,9 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int j = t_begin; j < t_end; ++j) {
                 if (!partial(j)) continue;
                 const int i = 2 * (j - t_begin) + 1, s = stage(i);
-                bool ok = wait(bar_part + s, (phase >> s) & 1u);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+                const bool ok = __all_sync(0xffffffffu, wait(bar_part + s, (phase >> s) & 1u));
                 phase ^= 1u << s;
                 uint8_t* v = sm + L::kRing + s * L::kTile;
                 // Keys [0, head) and [tail, 128) of the tile, a piece of eight values a thread, DP / 8 threads a row: those outside of
@@ -617,17 +617,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     for (int r = from + y0; r < to; r += kStep) *place(r) = make_uint4(0, 0, 0, 0);
                 };
                 const int lo = min(max(u.lo - k0, 0), kKeys), hi = min(max(u.hi - k0, 0), kKeys);      // keys in reach
-                blank(0, min(lo, head));
-                through(min(lo, head), min(head, hi));
-                blank(hi, head);
-                blank(tail, lo);
-                through(max(tail, lo), hi);
-                blank(max(tail, hi), kKeys);
+                if (ok) {
+                    blank(0, min(lo, head));
+                    through(min(lo, head), min(head, hi));
+                    blank(hi, head);
+                    blank(tail, lo);
+                    through(max(tail, lo), hi);
+                    blank(max(tail, hi), kKeys);
+                }
                 if (odd) odd_values = 1;
                 __threadfence_block();
                 fence_async_smem();
-                asm volatile("bar.sync 1, 64;" ::: "memory");
-                if (tid == kFixWarp * 32) mbar_arrive(bar_full + s);
+                asm volatile("bar.sync 1, 64;" ::: "memory");      // the two warps meet whatever their waits said
+                if (tid == kFixWarp * 32 && !abort_flag) mbar_arrive(bar_full + s);
             }
         }
     }

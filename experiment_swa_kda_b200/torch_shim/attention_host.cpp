@@ -52,7 +52,15 @@ struct NormRopeNode : public HostNode {
     bool has_qw = false, has_kw = false, has_pos = false;
     at::ScalarType qw_type = at::kFloat, kw_type = at::kFloat;
     std::vector<int64_t> q_sizes, k_sizes;
+    c10::Device device = c10::Device(c10::kCUDA, 0);
     std::string name() const override { return "QKNormRopeBackward"; }
+    // A saved tensor.  A saved-tensor hook may hand it back at other strides (one that offloads to the host makes slices dense), so none are
+    // taken from the forward; of another shape, type or device it would be read out of range.
+    Tensor back(const Tensor& t, at::IntArrayRef sizes, at::ScalarType type) const {
+        TORCH_CHECK(t.defined() && t.sizes() == sizes && t.scalar_type() == type && t.device() == device,
+                    "a saved-tensor hook handed a tensor of another shape, type or device back to qk_norm_rope");
+        return t;
+    }
     variable_list apply(variable_list&& grads) override {
         std::vector<Tensor> t;
         {
@@ -60,19 +68,25 @@ struct NormRopeNode : public HostNode {
             for (size_t i = 0; i < saved.size(); ++i) t.push_back(get(i));
         }
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor &q = t[0], &k = t[1], &cos = t[2], &sin = t[3];
+        c10::cuda::CUDAGuard guard(device);
+        watch_status(device.index());
+        const at::ScalarType io = sh.io_dtype == KDA_DTYPE_BF16 ? at::kBFloat16 : at::kFloat;
+        const int64_t table[2] = {sh.table_len, sh.rotary_dim / 2}, place[2] = {q_sizes[0], q_sizes[1]}, width[1] = {sh.head_dim};
+        const Tensor q = rows_of(back(t[0], q_sizes, io)), k = rows_of(back(t[1], k_sizes, io));
+        const Tensor cos = dense(back(t[2], {table, 2}, at::kFloat)), sin = dense(back(t[3], {table, 2}, at::kFloat));
         size_t at_ = 4;
-        const Tensor pos = has_pos ? t[at_++] : Tensor();
-        const Tensor qw = has_qw ? t[at_++] : Tensor(), kw = has_kw ? t[at_++] : Tensor();
-        c10::cuda::CUDAGuard guard(q.device());
-        watch_status(q.device().index());
+        const Tensor pos = has_pos ? dense(back(t[at_++], {place, 2}, sh.positions_64 ? at::kLong : at::kInt)) : Tensor();
+        const Tensor qw = has_qw ? dense(back(t[at_++], {width, 1}, at::kFloat)) : Tensor(), kw = has_kw ? dense(back(t[at_++], {width, 1}, at::kFloat)) : Tensor();
+        KdaRotaryShape s = sh;
+        s.q_token_stride = token_stride(q), s.q_head_stride = q.stride(2);
+        s.k_token_stride = token_stride(k), s.k_head_stride = k.stride(2);
         const Tensor dqo = grads[0].defined() ? dense_as(grads[0], q.scalar_type()) : at::zeros(q_sizes, q.options());
         const Tensor dko = grads[1].defined() ? dense_as(grads[1], k.scalar_type()) : at::zeros(k_sizes, k.options());
         Tensor dq = empty(q_sizes, q.scalar_type(), q), dk = empty(k_sizes, k.scalar_type(), k), dqw, dkw, scr;
         if (has_qw && task_should_compute_output(2)) dqw = empty({sh.head_dim}, at::kFloat, q);
         if (has_kw && task_should_compute_output(3)) dkw = empty({sh.head_dim}, at::kFloat, q);
-        if (dqw.defined() || dkw.defined()) scr = bytes(kda_norm_rope_bwd_scratch_bytes(&sh), q);
-        must(kda_norm_rope_bwd(&sh, q.const_data_ptr(), k.const_data_ptr(), fptr(cos), fptr(sin), has_pos ? pos.const_data_ptr() : nullptr, fptr(qw), fptr(kw),
+        if (dqw.defined() || dkw.defined()) scr = bytes(kda_norm_rope_bwd_scratch_bytes(&s), q);
+        must(kda_norm_rope_bwd(&s, q.const_data_ptr(), k.const_data_ptr(), fptr(cos), fptr(sin), has_pos ? pos.const_data_ptr() : nullptr, fptr(qw), fptr(kw),
                                dqo.const_data_ptr(), dko.const_data_ptr(), dq.data_ptr(), dk.data_ptr(), dqw.defined() ? dqw.data_ptr<float>() : nullptr,
                                dkw.defined() ? dkw.data_ptr<float>() : nullptr, scr.defined() ? scr.data_ptr() : nullptr,
                                scr.defined() ? (size_t)scr.numel() : 0, stream_of(q)),
@@ -120,6 +134,7 @@ TensorPair norm_rope(const Tensor& q_, const Tensor& k_, const Tensor& cos_, con
         auto node = make_node<NormRopeNode>();
         node->set_next_edges(torch::autograd::collect_next_edges(q_, k_, has(qw_) ? *qw_ : none, has(kw_) ? *kw_ : none));
         node->sh = sh;
+        node->device = q.device();
         node->has_pos = pos.defined(), node->has_qw = qw.defined(), node->has_kw = kw.defined();
         if (has(qw_)) node->qw_type = qw_->scalar_type();
         if (has(kw_)) node->kw_type = kw_->scalar_type();

@@ -347,8 +347,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // ------------------------------------------------------------------ O / l
         const int n = r.end - r.begin;
         const bool full = !split && a.q_boxes && 128 * (t + 1) <= u.rows;      // the same for the row tile's warps
+        // The output goes through the queries' place.  With a key, what is read there has been read when the last product ends; without one (a
+        // row tile of padding, or a part behind its keys) its queries may still be on their way there, if anything fetched them.
         if (ok && n > 0) {
             ok = wait(bar_o + t, (n - 1) & 1);
+            __syncwarp();
+        } else if (ok && (!a.q_boxes || t_begin < t_end)) {
+            ok = wait(bar_q, 0);
             __syncwarp();
         }
         if (ok && 128 * t + 32 * (warp & 3) < u.rows) {

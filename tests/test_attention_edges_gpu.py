@@ -3,11 +3,12 @@
 Bounds are those of test_attention_gpu.py."""
 
 import contextlib
+import math
 
 import pytest
 import torch
 
-from test_attention_gpu import BF16, DEV, F32, tables
+from test_attention_gpu import BF16, DEV, F32, Batch, close, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +60,33 @@ def test_a_hook_that_changes_a_saved_tensor_is_refused():
             y, _ = m.qk_norm_rope(x, k, cos, sin)
         with pytest.raises(RuntimeError, match="saved-tensor hook"):
             torch.autograd.grad(y, x, dy[0])
+
+
+# ---------------------------------------------------------------------------------------------- padding
+
+def check_padding(b, o, lse, want, wlse, size):
+    """o = 0 and lse = -inf, bit for bit, where a token is padding; the oracle's values elsewhere."""
+    pad = torch.isinf(wlse)
+    assert torch.equal(o.cpu()[pad], torch.zeros_like(o.cpu()[pad])) and bool((lse.cpu()[pad] == -math.inf).all())
+    close(o.cpu()[~pad], want[~pad], size[~pad], b.dtype)
+    assert ((lse.double().cpu() - wlse)[~pad].abs() <= 2e-5 * (1 + wlse[~pad].abs())).all()
+
+
+@pytest.mark.parametrize("tokens,real", [(130, 0), (130, 1), (130, 90), (512, 0), (512, 1), (512, 90), (64, 20)])
+@pytest.mark.parametrize("Hq,Hk,D", [(4, 1, 128), (16, 4, 64), (3, 1, 128), (12, 4, 96)])
+@pytest.mark.parametrize("fill", [7.0, math.nan])
+def test_row_tiles_of_padding_beside_live_ones(tokens, real, Hq, Hk, D, fill):
+    """Whatever the queries of padding tokens hold, whole row tiles of them too, their outputs are 0, call after call."""
+    b = Batch([tokens, 5, tokens], [real, 3, 0], Hq, Hk, D, 16, BF16, seed=real)
+    pos = torch.cat([torch.arange(n - a, n) for a, n in zip(b.q_lens, b.kv_lens)])
+    b.dq[(pos < 0).to(DEV)] = fill
+    oracle = b.oracle()
+    # also with a table that leaves room for long rows, which are then cut into parts
+    wide = torch.cat((b.dtable, torch.full((3, 400), -7, dtype=torch.int32, device=DEV)), 1)
+    for table in (b.dtable, wide):
+        b.dtable = table
+        for bound in (0, tokens):
+            o, lse = b.attend(return_lse=True, max_q_len=bound)
+            check_padding(b, o, lse, *(oracle[i] for i in (0, 1, 2)))
+            for _ in range(20):
+                assert torch.equal(o, b.attend(max_q_len=bound))

@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         const int part = 4 * hi > 3 * longest ? longest : hi, parts = min(max((nt + part - 1) / part, 1), a.splits);
         if (z >= parts) return;
+        fence_async_smem();      // the list's place is written by copies next
         split = parts > 1;
         t_begin = nt * z / parts;
         t_end = nt * (z + 1) / parts;

@@ -1,0 +1,19 @@
+"""What the attention kernels' sources have to keep where no run can show it."""
+
+import os
+import re
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "experiment_swa_kda_b200", "csrc")
+
+
+def source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return f.read()
+
+
+def test_lists_in_shared_memory_end_before_copies_take_their_place():
+    """The search for a part's length leaves its lists where the queries go; an ordinary access and a bulk copy to the same place are
+    ordered by a fence of the asynchronous proxy and the barrier behind it."""
+    text = source("attn_tc.cu")
+    lists, setup = text.index("blocks_of = tiles_of"), text.index("mbar_init(bar_q")
+    assert lists < text.index("fence_async_smem();", lists) < setup < text.index("__syncthreads();", setup)

@@ -225,6 +225,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         b.tell(kStatusWait);
         return false;
     };
+    // The same for a warp that goes on together: a limit that runs out in some lanes and not in others is every lane's, or those left would
+    // wait in the warp's next collective for lanes that are gone.
+    auto warp_wait = [&](uint64_t* w, uint32_t parity) { return __all_sync(0xffffffffu, wait(w, parity)) != 0; };
     // stage and phase of the ring's i-th tile
     auto stage = [](int i) { return i % L::kStages; };
     auto turn = [](int i) { return (uint32_t)(i / L::kStages) & 1u; };
@@ -265,8 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         bool ok = true;
         for (int j = r.begin; j < r.end; ++j) {
             const int i = j - r.begin;
-            ok = wait(bar_s + t, i & 1);
-            __syncwarp();
+            ok = warp_wait(bar_s + t, i & 1);
             if (!ok) break;
             tc_fence_after();
             uint32_t s[4][32];
@@ -302,8 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (grow) m = next;
                 l *= f;
                 if (i > 0) {      // the sums so far are complete once the product before has ended
-                    ok = wait(bar_o + t, (i - 1) & 1);
-                    __syncwarp();
+                    ok = warp_wait(bar_o + t, (i - 1) & 1);
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll 1
@@ -351,11 +352,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // The output goes through the queries' place.  With a key, what is read there has been read when the last product ends; without one (a
         // row tile of padding, or a part behind its keys) its queries may still be on their way there, if anything fetched them.
         if (ok && n > 0) {
-            ok = wait(bar_o + t, (n - 1) & 1);
-            __syncwarp();
+            ok = warp_wait(bar_o + t, (n - 1) & 1);
         } else if (ok && (!a.q_boxes || t_begin < t_end)) {
-            ok = wait(bar_q, 0);
-            __syncwarp();
+            ok = warp_wait(bar_q, 0);
         }
         if (ok && 128 * t + 32 * (warp & 3) < u.rows) {
             tc_fence_after();
@@ -556,8 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (; i < total; ++i) {
                 const int j = t_begin + (i >> 1), s = stage(i);
                 const bool isv = i & 1;
-                if (i >= L::kStages) ok = wait(bar_free + s, turn(i - L::kStages));
-                ok = __all_sync(0xffffffffu, ok);
+                if (i >= L::kStages) ok = warp_wait(bar_free + s, turn(i - L::kStages));
                 if (!ok) break;
                 if (!isv) next_page = look(j + 1, next_row);
                 uint64_t* f = isv && partial(j) ? bar_part + s : bar_full + s;
@@ -588,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int j = t_begin; j < t_end; ++j) {
                 if (!partial(j)) continue;
                 const int i = 2 * (j - t_begin) + 1, s = stage(i);
-                const bool ok = __all_sync(0xffffffffu, wait(bar_part + s, (phase >> s) & 1u));
+                const bool ok = warp_wait(bar_part + s, (phase >> s) & 1u);
                 phase ^= 1u << s;
                 uint8_t* v = sm + L::kRing + s * L::kTile;
                 // Keys [0, head) and [tail, 128) of the tile, a piece of eight values a thread, DP / 8 threads a row: those outside of

@@ -116,6 +116,9 @@ inline long long tile_slots(int tokens, int n_seq, int max_q_len, int group, int
     return by_tokens;
 }
 
+// The first key that a token at `pos` sees; in this order nothing leaves 32 bits, however negative a padding token's position or wide the window.
+__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+
 // A block's share of one tile: which rows, and which keys any of them sees.
 struct Unit {
     int n, first, count;       // sequence, its first new token and how many it has
@@ -134,7 +137,7 @@ __device__ __forceinline__ bool make_unit(const Batch& b, const Tiles& t, int sl
     u.base = len - u.count;
     const int i0 = u.row0 / t.group, i1 = (u.row0 + u.rows - 1) / t.group;
     u.hi = max(u.base + i1 + 1, 0);
-    u.lo = window > 0 ? max(u.base + i0 - window + 1, 0) : 0;
+    u.lo = first_key(u.base + i0, window);
     return true;
 }
 // What a batch got wrong is reported by the blocks of the first tile of each sequence.

@@ -82,7 +82,7 @@ __device__ __forceinline__ Seq seq_of_raw(const Batch& b, const Raw& r, int wind
     const int len = max(r.len, 0) > room ? (int)room : max(r.len, 0);
     s.base = len - s.count;
     s.hi = s.count > 0 ? len : 0;
-    s.lo = window > 0 ? min(max(s.base - window + 1, 0), s.hi) : 0;
+    s.lo = min(first_key(s.base, window), s.hi);
     s.t0 = s.lo / kTile;
     s.t1 = (s.hi + kTile - 1) / kTile;
     return s;
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             if (tiles - i > w.s.t1 - w.tile) fetch_q(then);
             rows = min(w.s.count * g, kRows);
             unit_begin = w.tile;
-            all_lo = window > 0 ? max(w.s.base + (rows - 1) / g - window + 1, 0) : 0;
+            all_lo = first_key(w.s.base + (rows - 1) / g, window);
             all_hi = w.s.base + 1;
 #pragma unroll
             for (int y = 0; y < NR; ++y) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                 for (int x = 0; x < 2; ++x) {
                     const int r = 8 * y + 2 * c4 + x;
                     last[y][x] = r < rows ? w.s.base + r / g : -1;
-                    first[y][x] = window > 0 ? last[y][x] - window + 1 : 0;
+                    first[y][x] = first_key(last[y][x], window);
                     m[y][x] = -INFINITY;
                     l[y][x] = 0.f;
                 }
@@ -556,9 +556,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                 float o[4] = {oa.x, oa.y, ob.x, ob.y};
                 if (M == kLowest) sum = 0.f;      // nothing but -inf: 0 / 0
                 if (flags[1 + q_buffer]) {
-                    const int to = w.s.base + r / g, from = window > 0 ? to - window + 1 : 0;
+                    const int to = w.s.base + r / g, from = first_key(to, window);
 #pragma unroll 1
-                    for (int key = max(max(from, 0), unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
+                    for (int key = max(from, unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
                         if (key >= all_lo && key < all_hi) continue;
                         const int pg = b.page(w.n, key / b.page_size);
                         if (pg < 0) continue;

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i;
         last[i] = r < u.rows ? u.base + (u.row0 + r) / g : -1;
-        first[i] = c.window > 0 ? last[i] - c.window + 1 : 0;
+        first[i] = first_key(last[i], c.window);
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll

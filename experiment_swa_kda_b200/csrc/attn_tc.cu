@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
     // keys any row of the block sees: [u.lo, u.hi); keys all of them see: [all_lo, all_hi)
     const int first_pos = u.base + u.row0 / g, last_pos = u.base + (u.row0 + u.rows - 1) / g;
-    const int all_lo = window > 0 ? max(last_pos - window + 1, 0) : 0, all_hi = first_pos + 1;
+    const int all_lo = first_key(last_pos, window), all_hi = first_pos + 1;
     // Key tiles start at the first box in reach, not at multiples of their size: a window of 1,024 keys and 64 rows is 9 tiles, not 10.
     const int key0 = u.lo / a.box_rows * a.box_rows, nt = max((u.hi - key0 + kKeys - 1) / kKeys, 0);
     int t_begin = 0, t_end = nt;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     auto range_of = [&](int t) {      // key tiles of row tile t
         const int r0 = u.row0 + 128 * t, r1 = min(r0 + 128, u.row0 + u.rows) - 1;
         if (r0 > r1) return Range{0, 0};
-        const int hi = u.base + r1 / g + 1, lo = window > 0 ? max(u.base + r0 / g - window + 1, 0) : 0;
+        const int hi = u.base + r1 / g + 1, lo = first_key(u.base + r0 / g, window);
         Range r{max(t_begin, (lo - key0) / kKeys), min(t_end, (max(hi - key0, 0) + kKeys - 1) / kKeys)};
         if (r.end < r.begin) r.end = r.begin;
         return r;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t tS = tmem + lanes + cS + 128 * t, tO = tmem + lanes + cO + DP * t;
         const int row = 128 * t + (tid & 127), prow = u.row0 + row;
         const int last = row < u.rows ? u.base + prow / g : last_pos;      // rows behind the last one compute along, unseen
-        const int first = window > 0 ? last - window + 1 : 0;
+        const int first = first_key(last, window);
         // keys all rows of the warp see
         const int w_lo = __reduce_max_sync(0xffffffffu, first), w_hi = __reduce_min_sync(0xffffffffu, last) + 1;
         const float c = a.c.scale * 1.4426950408889634f, lazy = kLazy / c;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (odd_values && n > 0) {
                     // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
 #pragma unroll 1
-                    for (int key = max(max(first, 0), key0 + r.begin * kKeys); key <= min(last, key0 + r.end * kKeys - 1); ++key) {
+                    for (int key = max(first, key0 + r.begin * kKeys); key <= min(last, key0 + r.end * kKeys - 1); ++key) {
                         if (key >= all_lo && key < all_hi) {
                             key = all_hi - 1;
                             continue;

@@ -4,6 +4,7 @@
 
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <tuple>
@@ -168,13 +169,13 @@ bool paged_shape(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
     } else if (T % N != 0) {
         return false;
     }
-    if (max_q < 0 || max_q > kInt || window < 0 || window > kInt) return false;
+    if (max_q < 0 || max_q > kInt || window < 0) return false;
     s = {};
     s.tokens = (int32_t)T, s.n_seq = (int32_t)N, s.max_q_len = (int32_t)max_q;
     s.q_heads = (int32_t)H, s.kv_heads = (int32_t)hk, s.head_dim = (int32_t)D;
     s.io_dtype = dt(q);
     s.n_pages = (int32_t)pages, s.page_size = (int32_t)page, s.table_width = (int32_t)width;
-    s.window = (int32_t)window;
+    s.window = (int32_t)std::min(window, kInt);      // no sequence is longer
     s.scale = 1.f;
     s.table_stride = table.stride(0);
     s.q_token_stride = q.stride(0), s.q_head_stride = q.stride(1);

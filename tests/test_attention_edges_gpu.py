@@ -90,3 +90,19 @@ def test_row_tiles_of_padding_beside_live_ones(tokens, real, Hq, Hk, D, fill):
             check_padding(b, o, lse, *(oracle[i] for i in (0, 1, 2)))
             for _ in range(20):
                 assert torch.equal(o, b.attend(max_q_len=bound))
+
+
+# ---------------------------------------------------------------------------------------------- windows
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 40])
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("q_lens,kv_lens,Hq,Hk", [([9], [3], 1, 1), ([4, 1, 3], [1, 500, 130], 4, 1), ([130, 40], [90, 500], 4, 1), ([300], [297], 6, 2)])
+def test_windows_that_hide_nothing(window, dtype, q_lens, kv_lens, Hq, Hk):
+    """The largest windows there are, padding or not, are the same as none."""
+    b = Batch(q_lens, kv_lens, Hq, Hk, 128, 16, dtype)
+    for bound in (0, max(q_lens)):
+        o, lse = b.attend(return_lse=True, max_q_len=bound)
+        b.window = window
+        p, plse = b.attend(return_lse=True, max_q_len=bound)
+        b.window = 0
+        assert torch.equal(o, p) and torch.equal(lse, plse)

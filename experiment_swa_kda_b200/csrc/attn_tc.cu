@@ -93,18 +93,19 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// 2^x of a pair on the multiply-add pipes: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 whose largest relative
-// error is least there (2.6e-6; degree 3 leaves 7.5e-5, which the sums of few weights show), n added to the exponent.  The special function unit gives 16 values a cycle and SM, the tensor
-// pipe wants 128 x 128 of them every 1,024 cycles, so part of them is made here.
+// 2^x of a pair on the multiply-add pipes: x = n + f with |f| <= 1/2, 2^f by the polynomial of degree 4 with 2^0 = 1 whose largest relative
+// error is least there (2.8e-6; degree 3 leaves 7.5e-5, which the sums of few weights show), n added to the exponent.  -127 and all below it, the -inf of a
+// hidden key too, give f = 0 and n = -127: no bit is left, so a hidden key weighs nothing whatever its value is.  The special function unit gives 16
+// values a cycle and SM, the tensor pipe wants 128 x 128 of them every 1,024 cycles, so part of them is made here.
 __device__ __forceinline__ f2 ex2_pair(f2 x) {
     const float2 v = f2_get(x);
-    x = f2_make(fmaxf(v.x, -125.f), fmaxf(v.y, -125.f));
+    x = f2_make(fmaxf(v.x, -127.f), fmaxf(v.y, -127.f));
     const f2 magic = f2_all(12582912.f);      // 1.5 x 2^23: the sum's low bits are n
     const f2 t = f2_add(x, magic), f = f2_add(x, f2_fma(t, f2_all(-1.f), magic));
-    f2 p = f2_fma(f2_all(0.0095701022f), f, f2_all(0.0559178591f));
-    p = f2_fma(p, f, f2_all(0.2402474433f));
-    p = f2_fma(p, f, f2_all(0.6931217909f));
-    p = f2_fma(p, f, f2_all(0.9999992847f));
+    f2 p = f2_fma(f2_all(0.0095828531f), f, f2_all(0.0559064248f));
+    p = f2_fma(p, f, f2_all(0.2402409864f));
+    p = f2_fma(p, f, f2_all(0.6931241928f));
+    p = f2_fma(p, f, f2_all(1.f));
     const float2 r = f2_get(p), n = f2_get(t);
     return f2_make(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
 }
@@ -359,8 +360,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (ok && 128 * t + 32 * (warp & 3) < u.rows) {
             tc_fence_after();
             const bool mine = row < u.rows;
-            const bool dead = m == kLowest;             // nothing but -inf: 0 / 0 (ex2_pair ends at 2^-125)
-            if (dead) l = 0.f;
             if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);      // a NaN or +inf among the scores, which ex2_pair does not pass on
             const int tok = u.first + prow / g, head = hk * g + prow % g;
             const size_t out = (size_t)tok * a.c.heads.q_heads + head;
@@ -381,9 +380,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         for (int e = 0; e < 32; ++e) o[y][e] = 0;
                 }
                 tmem_ld_wait();
-                if (dead)
-#pragma unroll
-                    for (int e = 0; e < 64; ++e) o[e >> 5][e & 31] = 0;
                 if (odd_values && n > 0) {
                     // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
 #pragma unroll 1

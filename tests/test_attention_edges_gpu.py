@@ -106,3 +106,26 @@ def test_windows_that_hide_nothing(window, dtype, q_lens, kv_lens, Hq, Hk):
         p, plse = b.attend(return_lse=True, max_q_len=bound)
         b.window = 0
         assert torch.equal(o, p) and torch.equal(lse, plse)
+
+
+# ---------------------------------------------------------------------------------------------- values of any size
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("q_len,Hq,D,window", [(4, 2, 128, 0), (200, 4, 128, 0), (200, 4, 64, 120), (60, 6, 96, 30)])
+def test_hidden_keys_weigh_nothing(dtype, q_len, Hq, D, window):
+    """The largest finite values at keys that a row does not see change no bit of its output."""
+    kv = 300
+    b = Batch([q_len], [kv], Hq, 2, D, 16, dtype, window=window)
+    before = b.attend()
+    hidden = torch.zeros(q_len, dtype=torch.bool)
+    last, early = range(kv - min(q_len - 1, 20), kv), range(kv - q_len - window + 1, kv - q_len - window + 9) if window else ()
+    for pos in (*last, *early):
+        at = int(b.table[0, pos // 16]), pos % 16
+        b.dv[at[0], at[1]] = torch.finfo(dtype).max
+        b.dv[at[0], at[1], :, ::3] = torch.finfo(dtype).min
+        i = torch.arange(q_len) + kv - q_len
+        hidden |= (i >= pos) & ((i < pos + window) if window else True)
+    assert not hidden.all()
+    after = b.attend()
+    assert torch.equal(before.cpu()[~hidden], after.cpu()[~hidden])
+    assert not torch.equal(before.cpu()[hidden], after.cpu()[hidden])

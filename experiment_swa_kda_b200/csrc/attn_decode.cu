@@ -650,7 +650,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
         for (int k = of; k <= parts; k += share) {
             const uint4 v = ld_after16(a.part_o + place(k, r) * D + d);
             const float f = weight[k * kRows + r];
-            if (f == 0.f) continue;
             o[0] = fmaf(__uint_as_float(v.x), f, o[0]);
             o[1] = fmaf(__uint_as_float(v.y), f, o[1]);
             o[2] = fmaf(__uint_as_float(v.z), f, o[2]);

@@ -129,3 +129,18 @@ def test_hidden_keys_weigh_nothing(dtype, q_len, Hq, D, window):
     after = b.attend()
     assert torch.equal(before.cpu()[~hidden], after.cpu()[~hidden])
     assert not torch.equal(before.cpu()[hidden], after.cpu()[hidden])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("q_len,Hq,kv", [(1, 2, 6000), (3, 4, 3000), (70, 2, 5000)])
+def test_values_that_are_not_finite_reach_rows_whose_weights_vanish(dtype, q_len, Hq, kv):
+    """A visible NaN is in the sum however small its weight: keys hundreds of units below the others, in parts of their own."""
+    b = Batch([q_len], [kv], Hq, 1, 128, 16, dtype)
+    b.dq.fill_(1.0), b.q.fill_(1.0)
+    for c in (b.k, b.dk):
+        c[b.table[0, :20].long()] = -100.0      # keys 0 .. 319: scores of -100 sqrt(128)
+    for c in (b.v, b.dv):
+        c[int(b.table[0, 3]), 5, 0, 7] = math.nan
+    o, want, size = b.attend(max_q_len=q_len), *b.oracle()[::2]
+    assert torch.isnan(want[..., 7]).all() and torch.isfinite(want[..., 8]).all()
+    close(o, want, size, dtype)

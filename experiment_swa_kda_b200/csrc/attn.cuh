@@ -16,6 +16,8 @@ struct Batch {
     long long table_stride;
     int n_seq, tokens, q_len, n_pages, page_size, table_width;
 
+    // Said by every thread that finds it, as long as the call runs: these calls have no status word of their own in which a first teller could be
+    // known (a captured call has nothing that tells one replay from the next).  The host therefore clears the word behind the stream's work.
     __device__ __forceinline__ void tell(int code) const {
         if (mirror != nullptr) *reinterpret_cast<volatile int*>(mirror) = code;
     }

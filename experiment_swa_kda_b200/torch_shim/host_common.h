@@ -57,7 +57,7 @@ inline size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Device status without a hot-path cost: every device has one page-locked word that the kernels write to only when
 // something failed (an expired bounded wait, an inconsistent cu_seqlens).  watch_status registers the word on the first
-// call on a device and raises if an earlier call left a code in it; the word is cleared by the report.
+// call on a device and raises if an earlier call left a code in it; the report clears the word once the current stream's work has ended.
 void watch_status(int device);
 
 }  // namespace kda_host

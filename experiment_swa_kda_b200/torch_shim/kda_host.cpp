@@ -42,6 +42,12 @@ void watch_status(int device) {
     }
     int32_t* word = status_words.load(std::memory_order_relaxed) + device;
     if (__atomic_load_n(word, __ATOMIC_ACQUIRE) == 0) return;
+    // The call that found something wrong may still run, and more of its blocks may find it: taken away before they are done, their word would
+    // come back and be raised again.  So the stream's work ends first.  (What runs in other streams is not waited for, and a capture cannot wait.)
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess || (capture == cudaStreamCaptureStatusNone && cudaStreamSynchronize(stream) != cudaSuccess))
+        (void)cudaGetLastError();      // what the device reported is raised all the same
     const int32_t bad = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL);
     if (bad == 0) return;
     const int rc = kda_status_word_code(bad);

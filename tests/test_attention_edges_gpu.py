@@ -144,3 +144,29 @@ def test_values_that_are_not_finite_reach_rows_whose_weights_vanish(dtype, q_len
     o, want, size = b.attend(max_q_len=q_len), *b.oracle()[::2]
     assert torch.isnan(want[..., 7]).all() and torch.isfinite(want[..., 8]).all()
     close(o, want, size, dtype)
+
+
+# ---------------------------------------------------------------------------------------------- errors
+
+def test_one_call_reports_its_error_once():
+    """A call that still runs when its error is raised does not raise it again from the next one."""
+    import experiment_swa_kda_b200 as m
+    n, length = 2048, 8192
+    q = torch.zeros(n * 32, 1, 128, device=DEV)
+    cache = torch.zeros(4, 16, 1, 128, device=DEV)
+    table = torch.full((n, length // 16), -1, dtype=torch.int32, device=DEV)      # no page at all, in any sequence
+    lens = torch.full((n,), length, dtype=torch.int32, device=DEV)
+    cos = sin = torch.ones(4, 64, device=DEV)
+    nothing = torch.zeros(1, 0, 1, 128, device=DEV)      # a call that looks at the status and launches nothing
+    m.qk_norm_rope(nothing, nothing, cos, sin)
+    torch.cuda.synchronize()
+    m.paged_attention(q, cache, cache, table, lens)
+    done = torch.cuda.Event()
+    done.record()
+    with pytest.raises(RuntimeError, match="block table"):
+        while True:
+            finished = done.query()
+            m.qk_norm_rope(nothing, nothing, cos, sin)
+            assert not finished, "the error was never reported"
+    torch.cuda.synchronize()
+    m.qk_norm_rope(nothing, nothing, cos, sin)

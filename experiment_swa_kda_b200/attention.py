@@ -213,10 +213,24 @@ class PagedAttention(nn.Module):
         self.q_norm = nn.Parameter(torch.ones(head_dim))
         self.k_norm = nn.Parameter(torch.ones(head_dim))
         self.o_proj = Linear(num_heads * head_dim, hidden_size, bias=False)
-        freq = rope_base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
-        angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * freq
-        self.register_buffer("cos", angle.cos().float(), persistent=False)
-        self.register_buffer("sin", angle.sin().float(), persistent=False)
+        self.max_positions, self.rope_base = max_positions, rope_base
+        for name, table in zip(("cos", "sin"), self._tables(torch.get_default_device())):
+            self.register_buffer(name, table, persistent=False)
+
+    def _tables(self, device) -> Tuple[Tensor, Tensor]:
+        place = {"dtype": torch.float64, "device": "cpu"}
+        freq = self.rope_base ** (-torch.arange(0, self.head_dim, 2, **place) / self.head_dim)
+        angle = torch.arange(self.max_positions, **place)[:, None] * freq
+        return angle.cos().float().to(device), angle.sin().float().to(device)
+
+    def _apply(self, fn, *args, **kwargs):
+        """Casts of the module are its parameters': the rotation's tables stay float32, and are made again where a cast has rounded
+        them or they had no values yet."""
+        had_values = not self.cos.is_meta
+        super()._apply(fn, *args, **kwargs)
+        if self.cos.dtype != torch.float32 or not had_values:
+            self.cos, self.sin = self._tables(self.cos.device)
+        return self
 
     @torch.no_grad()
     def forward(self, hidden_states: Tensor, cache: PagedCache, cu_seqlens: Optional[Tensor] = None, max_q_len: int = 0) -> Tensor:

@@ -170,3 +170,29 @@ def test_one_call_reports_its_error_once():
             assert not finished, "the error was never reported"
     torch.cuda.synchronize()
     m.qk_norm_rope(nothing, nothing, cos, sin)
+
+
+# ---------------------------------------------------------------------------------------------- the layer
+
+@pytest.mark.parametrize("cast", [lambda l: l.bfloat16(), lambda l: l.to(torch.bfloat16), lambda l: l.half().float(), lambda l: l.double().float().bfloat16()])
+def test_layer_keeps_its_tables_through_casts(cast):
+    """The rotation's tables are float32 whatever the parameters' type becomes, and keep their values."""
+    import experiment_swa_kda_b200 as m
+    torch.manual_seed(2)
+    layer = m.PagedAttention(256, 4, 2, 64, max_positions=300).to(DEV)
+    cos, sin = layer.cos.clone(), layer.sin.clone()
+    cast(layer)
+    assert layer.cos.dtype == F32 and torch.equal(layer.cos, cos) and torch.equal(layer.sin, sin) and layer.cos.device == cos.device
+    cache = m.PagedCache.zeros(2, 20, 16, 2, 64, DEV)
+    cache.kv_lens += 20
+    y = layer(torch.randn(2, 20, 256, device=DEV).bfloat16(), cache)
+    assert torch.isfinite(y).all()
+
+
+def test_layer_made_without_memory_gets_its_tables():
+    import experiment_swa_kda_b200 as m
+    with torch.device("meta"):
+        layer = m.PagedAttention(256, 4, 2, 64, max_positions=300)
+    layer = layer.to_empty(device=DEV)
+    want = m.PagedAttention(256, 4, 2, 64, max_positions=300).to(DEV)
+    assert torch.equal(layer.cos, want.cos) and torch.equal(layer.sin, want.sin)

@@ -237,6 +237,9 @@ class PagedAttention(nn.Module):
         """hidden_states [B,T,hidden], T new tokens of each of the cache's B sequences, or [1,tokens,hidden], packed, with `cu_seqlens`."""
         lead = hidden_states.shape[:-1]
         if cu_seqlens is None:
+            sequences = cache.block_table.shape[0]
+            if hidden_states.ndim != 3 or hidden_states.shape[0] != sequences:
+                raise ValueError(f"hidden_states must have shape [B, T, hidden] with the cache's {sequences} sequences, or come with cu_seqlens")
             max_q_len = hidden_states.shape[1]
         qkv = self.qkv_proj(hidden_states).reshape(-1, self.num_heads + 2 * self.num_kv_heads, self.head_dim)
         q, k, v = qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), 1)

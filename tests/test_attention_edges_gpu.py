@@ -196,3 +196,16 @@ def test_layer_made_without_memory_gets_its_tables():
     layer = layer.to_empty(device=DEV)
     want = m.PagedAttention(256, 4, 2, 64, max_positions=300).to(DEV)
     assert torch.equal(layer.cos, want.cos) and torch.equal(layer.sin, want.sin)
+
+
+def test_layer_compares_its_batch_with_the_cache():
+    import experiment_swa_kda_b200 as m
+    layer = m.PagedAttention(256, 4, 2, 64, max_positions=300).to(DEV)
+    cache = m.PagedCache.zeros(3, 32, 16, 2, 64, DEV)
+    cache.kv_lens += 2
+    x = torch.zeros(2, 3, 256, device=DEV).bfloat16()
+    for bad in (x, x[:1], x[0], x.expand(3, 2, 3, 256)):      # 6, 3, 3 and 18 tokens: three sequences could share them
+        with pytest.raises(ValueError, match="the cache's 3 sequences"):
+            layer(bad, cache)
+    assert layer(x.reshape(1, 6, 256), cache, torch.tensor([0, 2, 4, 6], dtype=torch.int32, device=DEV)).shape == (1, 6, 256)
+    assert layer(x.reshape(3, 2, 256), cache).shape == (3, 2, 256)

@@ -158,7 +158,14 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     """Causal attention of new tokens q [tokens,Hq,D] over a paged cache that holds their own keys and values already.
 
     The token at position p sees positions p - window + 1 .. p (window 0: all up to p); Hq / Hk query heads share a kv head.
-    `max_q_len` bounds the new tokens of any sequence (0: unknown); a batch that says so is cut into blocks accordingly.
+    `max_q_len` bounds the new tokens of any sequence (0: unknown).  A batch that says so is cut into blocks accordingly, and
+    where max_q_len * Hq / Hk <= 16 a kernel for token steps takes it: one token of 32 conversations of up to 16,384 tokens took 107 us
+    with the bound, 195 packed without.
+
+    bfloat16 runs on the tensor cores if D is a multiple of 8 up to 128, the page size 8, 16, 32, 64 or a multiple of 128, and the
+    cache lies on 16 bytes at strides of whole 16 bytes.  Everything else (float32, wider heads, other pages) runs on the CUDA
+    cores, 14 times slower and more: take such page sizes where there is a choice.
+
     Returns o [tokens,Hq,D], or (o, lse [tokens,Hq]) with the natural log of each row's sum of exponentials.  A padding token
     (negative position) gets o = 0 and lse = -inf.  Pages that no new token reaches are not touched, and their entries in
     the table may be anything.  Inference only."""

@@ -35,7 +35,7 @@ namespace {
 using namespace tc;
 
 constexpr int kMaxRows = 16, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
-constexpr int kPerSm = 2;             // blocks an SM: 98 KB each
+constexpr int kPerSm = 2;             // blocks an SM: 102 KB each, 106 with more than 8 rows
 // Up to so many tiles a sequence and kv head stay together: they take about as long as two of them and the join, which is a launch less (3
 // conversations of 40 tokens 14.5 us in parts, 8.4 whole; 16 of 100 12.5 and 10.4).  Six where there are sequences for every SM (200 of up
 // to 380 36 and 33), four where parts would have some to themselves (one of 300 12.4 and 13.2 with six).

@@ -8,22 +8,22 @@
 // two row tiles take turns: while one's scores are turned into weights by its four warps, the other's products run.  S and O
 // live in tensor memory, P (bf16) takes S's place there and is the A operand of its product, so nothing but K and V goes through
 // shared memory.  A thread owns a row: maximum and sum need no exchange.  (Two threads a row, with twice the warps to cover each other's
-// waits, took as long: what the exchange of "a maximum has grown" costs is what they gain.  8,191 tokens 265 us.)
+// waits, took as long: what the exchange of "a maximum has grown" costs is what they gain.)
 //
 // O is rescaled only when a row's maximum has grown by more than 2^kLazy since the last time (the weights are then at most
 // 2^kLazy, which costs bf16 nothing: its rounding is relative); after a few tiles that no longer happens.
 // P is rounded to bf16 because the product takes one type and V is bf16; sums and statistics are float32.
 //
-// 8,191 tokens of 16 heads on 4: 232 us (1,187 TFLOP/s, 0.73 of the measured burst rate of a library product; 267 us where calls follow one
-// another and the power cap holds the clock, 0.75 of the sustained one), the tensor pipe busy for 58 % of them.  A pair of row tiles
+// 8,191 tokens of 16 heads on 4, calls one behind the other: 268 to 271 us (1,020 TFLOP/s, 0.74 of the measured sustained rate of a library
+// product, 0.62 of its burst rate), under the power cap; 235 in runs too short for it.  The tensor pipe is busy for 55 % of them.  A pair of row tiles
 // takes 2,900 to 3,350 cycles a key tile, of which its products need 2,048 and the special function unit 1,536: a row tile's softmax,
 // 2,000 cycles of two warps a scheduler, and the products behind it, 1,300, follow one another, and the other tile covers most of
-// that, not all.  Measured and left out: the exponentials of the two tiles in turns (270 us), maxima only where sums ask for them (261),
-// P in columns of its own for 64-wide heads (196 -> 248).  A block costs 12,000 to 16,000 cycles besides its tiles - its rows,
-// the first keys, the output -, which shows in windows: four times 2,048 tokens with windows of 1,024 take 106 us, 0.38 of the burst rate.
+// that, not all.  Measured and left out (short runs, where this took 232 to 241): the exponentials of the two tiles in turns (270 us), maxima only
+// where sums ask for them (261), two threads a row (265), P in columns of its own for 64-wide heads (196 -> 248).  A block costs 12,000 to 16,000 cycles besides its tiles - its rows,
+// the first keys, the output -, which shows in windows: four times 2,048 tokens with windows of 1,024 take 107 us, 0.37 of the burst rate.
 //
 // K and V come page by page by TMA into one ring (K 0, V 0, K 1, V 1, ...).  A tile that some row sees only in part is masked
-// in registers; in its V tile the keys that no row sees are blanked, since 0 times what lies in an unused slot may be NaN, and
+// in registers, to weights of exactly 0; in its V tile the keys that no row sees are blanked, since 0 times what lies in an unused slot may be NaN, and
 // so are values that are not finite at keys only some rows see: these are added by the rows that see them at the end.
 
 #include "attn.cuh"

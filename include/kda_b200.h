@@ -414,7 +414,9 @@ int kda_norm_rope_append(const KdaRotaryShape* rotary, const KdaPagedShape* page
                          const float* cos, const float* sin, const float* q_weight, const float* k_weight, const int32_t* block_table,
                          const int32_t* kv_lens, const int32_t* cu_seqlens, void* q_out, void* k_cache, void* v_cache, void* stream);
 /* o [tokens, q_heads, head_dim] dense, lse [tokens, q_heads] float32 (log of the sum of exponentials) or NULL.  Query
- * heads h*g .. h*g + g - 1 share kv head h.  Padding tokens: o = 0, lse = -inf. */
+ * heads h*g .. h*g + g - 1 share kv head h.  Padding tokens: o = 0, lse = -inf.  Tensor cores: bf16, head_dim a multiple of 8
+ * up to 128, page_size 8, 16, 32, 64 or a multiple of 128, q, o and the cache on 16 bytes at strides of multiples of 8 elements (the cache's
+ * positive); CUDA cores otherwise. */
 size_t kda_paged_attention_workspace_bytes(const KdaPagedShape* shape);
 int kda_paged_attention(const KdaPagedShape* shape, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
                         const int32_t* kv_lens, const int32_t* cu_seqlens, void* o, float* lse, void* workspace, size_t workspace_bytes,

@@ -487,9 +487,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                     const float p0 = ex2(fmaf(sc[y][2 * t], c, -mc[0])), p1 = ex2(fmaf(sc[y][2 * t + 1], c, -mc[1]));
                     l[y][0] += p0;
                     l[y][1] += p1;
-                    const uint32_t h = pack_bf16(p0, p1);
+                    // hi cut, not rounded, and lo at least 2^-20 of the weight: both of one sign, neither 0, or their sum with an infinite value were NaN
+                    const uint32_t h = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
                     hi[y][t] = turned(h);
-                    lo[y][t] = turned(pack_bf16(p0 - __uint_as_float(h << 16), p1 - __uint_as_float(h & 0xffff0000u)));
+                    lo[y][t] = turned(pack_bf16(fmaxf(p0 - __uint_as_float(h << 16), p0 * 0x1p-20f), fmaxf(p1 - __uint_as_float(h & 0xffff0000u), p1 * 0x1p-20f)));
                 }
             }
 #pragma unroll

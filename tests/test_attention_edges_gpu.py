@@ -146,6 +146,25 @@ def test_values_that_are_not_finite_reach_rows_whose_weights_vanish(dtype, q_len
     close(o, want, size, dtype)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("q_lens,Hq,D,window", [([1, 1, 1], 2, 128, 0), ([1, 1, 1], 16, 64, 200), ([4, 2, 1], 4, 96, 0), ([150, 70, 3], 4, 128, 0)])
+def test_infinite_values_that_are_seen(dtype, q_lens, Hq, D, window):
+    """A visible infinite value is the row's sum, with its sign; two of opposite signs, or a NaN, make it NaN."""
+    b = Batch(q_lens, [400, 333, 270], Hq, 1, D, 16, dtype, window=window)
+    for n, pos, d, x in ((0, 330, 0, math.inf), (0, 341, 1, -math.inf), (1, 240, 2, math.inf), (1, 250, 2, -math.inf), (1, 240, 3, -math.inf), (1, 250, 3, -math.inf),
+                         (2, 200, 4, math.nan), (2, 200, 5, math.inf)):
+        at = int(b.table[n, pos // 16]), pos % 16
+        for c in (b.v, b.dv):
+            c[at[0], at[1], 0, d] = x
+    o, want, size = b.attend(max_q_len=max(q_lens)), *b.oracle()[::2]
+    last = [sum(q_lens[:n + 1]) - 1 for n in range(3)]      # the last tokens see all of them
+    assert want[last[0], 0, :2].tolist() == [math.inf, -math.inf] and torch.isnan(want[last[1], 0, 2]) and want[last[1], 0, 3] == -math.inf
+    assert torch.isnan(want[last[2], 0, 4]) and want[last[2], 0, 5] == math.inf
+    close(o, want, size, dtype)
+    inf = torch.isinf(want)
+    assert torch.equal(o.double().cpu()[inf], want[inf])
+
+
 # ---------------------------------------------------------------------------------------------- errors
 
 def test_one_call_reports_its_error_once():

@@ -40,19 +40,19 @@ def test_pairs_of_weights_on_the_multiply_add_pipes():
     lowest, = set(re.findall(r"fmaxf\(v\.[xy], (-[\d.]+)f\)", body))
     c4, c3 = map(float, re.search(r"f2 p = f2_fma\(f2_all\(([\d.]+)f\), f, f2_all\(([\d.]+)f\)\)", body).groups())
     c2, c1, c0 = map(float, re.findall(r"p = f2_fma\(p, f, f2_all\(([\d.]+)f\)\)", body))
-    f32, fma = np.float32, lambda a, b, c: (a.astype(np.float64) * np.float64(b) + np.float64(c)).astype(np.float32)
+    f32, fma = np.float32, lambda a, b, c: (a.astype(np.float64) * b + c).astype(np.float32)
 
     def ex2_pair(x):
         x, magic = np.fmax(x, f32(lowest)), f32(12582912.0)
         t = x + magic
-        f = x + fma(t, -1.0, magic)
+        f = x + fma(t, -1.0, float(magic))
         p = np.full_like(f, f32(c4))
         for c in (c3, c2, c1, c0):
-            p = fma(p, f, f32(c))
+            p = fma(p, f, float(f32(c)))
         return (p.view(np.uint32) + (t.view(np.uint32) << np.uint32(23))).view(np.float32)
 
     x = np.concatenate([np.linspace(-125, 9, 400_001), np.linspace(-1, 1, 400_001)]).astype(f32)
     assert np.abs(ex2_pair(x) / np.exp2(x.astype(np.float64)) - 1).max() <= 3e-6
     small = ex2_pair(np.linspace(-140, -124, 400_001).astype(f32))
     assert (small >= 0).all() and (small <= f32(2.0 ** -124 * 1.001)).all()
-    assert ex2_pair(np.array([-np.inf, -1e30, -127.0], f32)).tolist() == [0.0, 0.0, 0.0] and ex2_pair(np.zeros(1, f32))[0] == 1.0
+    assert ex2_pair(np.array([-np.inf, -1e30, -127.0], f32)).tolist() == [0.0, 0.0, 0.0] and ex2_pair(np.zeros(1, f32)).tolist() == [1.0]

@@ -17,7 +17,7 @@
 //   four times the parts to join and took longer: 32 x 16 heads 118 us, one conversation 22.)
 // - Products are mma.sync m16n8k16 with the keys as their 16 rows and the query rows as their 8 columns: S^T = K Q^T and O^T = V^T P^T
 //   (P^T comes from S^T's registers by movmatrix).  Up to 8 rows take half the products that rows of queries would.  The weights
-//   go as two bf16 terms, p = hi + lo, which leaves the output with the error of its own rounding.
+//   go as two bf16 terms, p = hi + lo to 2^-16, which leaves the output with the error of its own rounding.
 // - What runs once a sequence (its queries, the join of the warps' sums) is kept short in code: unrolled it was fetched anew every time
 //   and took 5 us.
 

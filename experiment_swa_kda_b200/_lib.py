@@ -36,6 +36,10 @@ class PagedShape(C.Structure):
                                  "v_row_stride", "v_head_stride")]
 
 
+class PlanShape(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("rows", "width", "page_size", "n_pages", "max_tokens")] + [("table_stride", C.c_int64)]
+
+
 _P = C.c_void_p
 _SIGNATURES = {
     "kda_error_string": (C.c_char_p, [C.c_int]),
@@ -86,6 +90,8 @@ _SIGNATURES = {
     "kda_norm_rope_append": (C.c_int, [C.POINTER(RotaryShape), C.POINTER(PagedShape)] + [_P] * 14),
     "kda_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedShape)]),
     "kda_paged_attention": (C.c_int, [C.POINTER(PagedShape)] + [_P] * 9 + [C.c_size_t, _P]),
+    "kda_plan_pages_workspace_bytes": (C.c_size_t, [C.POINTER(PlanShape)]),
+    "kda_plan_pages": (C.c_int, [C.POINTER(PlanShape)] + [_P] * 9 + [C.c_size_t, _P]),
     "kda_launch_count": (C.c_ulonglong, []),
     "kda_profile_enable": (None, [C.c_int]),
     "kda_profile_report": (C.c_int, [C.c_char_p, C.c_size_t]),

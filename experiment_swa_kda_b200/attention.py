@@ -8,6 +8,7 @@ kernels of this package:
     qk_norm_rope         training and prefill: norm + rotation, differentiable
     qk_norm_rope_append  serving: the same, keys and values written to the pages of a cache
     paged_attention      serving: a chunk of new tokens, or one token, of every sequence of a batch over that cache
+    plan_pages           serving: block tables and slots of a step from the lengths of its requests
 
 A batch of new tokens is packed, [tokens, heads, D], with `cu_seqlens` [N+1] as in `chunk_kda`, or without it when every
 sequence has as many.  `kv_lens` [N] counts a sequence's tokens, the new ones among them; `block_table` [N, P] names their
@@ -183,6 +184,45 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     raise RuntimeError("paged_attention: the batch or the block table is too large for one call, or a trace is being recorded")
 
 
+def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens: Tensor, *, page_size: int, max_tokens: int,
+               starts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """Deals out the pages of a step and maps its new tokens to them; returns (cu_seqlens [N+1], positions [max_tokens], slots [max_tokens]).
+
+    The caller sets `kv_lens` [N] to what its requests shall have after the step, `new_lens` [N] of these being new; a row whose
+    request has ended has length 0, one that takes back rejected tokens a smaller length.  IN PLACE the rows of `block_table` [N,P]
+    then hold exactly the columns from starts[n] / page_size (None: 0) up to their length: what they held besides goes back to the
+    pool `page_free` [pages] bool, and what they lack takes the lowest free pages, rows in order.  `starts` is where a row's own pages
+    begin: behind a prefix it shares, or where a sliding window has left off.
+
+    A row is served if the pages lacking up to and with it are there and the new tokens up to and with it are at most `max_tokens`.  One
+    that is not waits: IN PLACE its length is less by its new tokens, none of which cu_seqlens counts.
+
+    positions [max_tokens] int32 are the new tokens' places in their sequences, slots [max_tokens] int64 those in a cache of
+    [pages * page_size] rows; -1 behind the last.  Nothing synchronises; a captured graph follows the arrays.  A pool starts out with all
+    pages free and a table of -1."""
+    out = None
+    if block_table.is_cuda:
+        out = _native.load().plan(block_table, kv_lens, page_free, new_lens, starts, page_size, max_tokens)
+    if out is not None:
+        return out
+    if block_table.ndim != 2 or block_table.dtype != torch.int32 or 0 in block_table.shape:
+        raise ValueError("block_table must be int32 with shape [N, pages of a sequence]")
+    rows, width = block_table.shape
+    for name, t in (("kv_lens", kv_lens), ("new_lens", new_lens), ("starts", starts)):
+        if t is not None and (tuple(t.shape) != (rows,) or t.dtype != torch.int32):
+            raise ValueError(f"{name} must be int32 with shape {(rows,)}")
+    if page_free.ndim != 1 or page_free.dtype != torch.bool:
+        raise ValueError("page_free must be bool with shape [pages]")
+    if page_size < 1 or max_tokens < 0:
+        raise ValueError("page_size must be positive and max_tokens not negative")
+    _same_device(block_table, kv_lens, page_free, new_lens, starts)
+    if (width > 1 and block_table.stride(1) != 1) or (rows > 1 and block_table.stride(0) < width):
+        raise ValueError("block_table must have adjacent values along its last dimension, and rows that do not overlap")
+    if not all(t.is_contiguous() for t in (kv_lens, page_free, new_lens, starts) if t is not None):
+        raise ValueError("kv_lens, page_free, new_lens and starts must be contiguous")
+    raise RuntimeError("plan_pages: the batch, the table or the pool is too large for one call, or a trace is being recorded")
+
+
 # ------------------------------------------------------------------------------------------
 # the layer
 # ------------------------------------------------------------------------------------------
@@ -196,6 +236,7 @@ class PagedCache:
     v: Tensor
     block_table: Tensor     # [N, pages of a sequence] int32
     kv_lens: Tensor         # [N] int32
+    page_free: Optional[Tensor] = None      # [pages] bool: the pool of `plan`
 
     @staticmethod
     def zeros(sequences: int, max_len: int, page_size: int, num_kv_heads: int, head_dim: int, device, dtype=torch.bfloat16) -> "PagedCache":
@@ -204,6 +245,20 @@ class PagedCache:
         pages = lambda: torch.zeros(sequences * each, page_size, num_kv_heads, head_dim, device=device, dtype=dtype)
         table = torch.arange(sequences * each, device=device, dtype=torch.int32).view(sequences, each)
         return PagedCache(pages(), pages(), table, torch.zeros(sequences, device=device, dtype=torch.int32))
+
+    @staticmethod
+    def pool(sequences: int, max_len: int, pages: int, page_size: int, num_kv_heads: int, head_dim: int, device, dtype=torch.bfloat16) -> "PagedCache":
+        """`pages` pages for all sequences together, none dealt out yet: `plan` does that step by step, up to `max_len` tokens of a sequence."""
+        store = lambda: torch.zeros(pages, page_size, num_kv_heads, head_dim, device=device, dtype=dtype)
+        table = torch.full((sequences, -(-max_len // page_size)), -1, device=device, dtype=torch.int32)
+        return PagedCache(store(), store(), table, torch.zeros(sequences, device=device, dtype=torch.int32),
+                          torch.ones(pages, device=device, dtype=torch.bool))
+
+    def plan(self, new_lens: Tensor, max_tokens: int, starts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+        """`plan_pages` of this cache, whose `kv_lens` the caller has set for the step."""
+        if self.page_free is None:
+            raise RuntimeError("this cache's pages are dealt out already; PagedCache.pool makes one whose pages are planned")
+        return plan_pages(self.block_table, self.kv_lens, self.page_free, new_lens, page_size=self.k.shape[1], max_tokens=max_tokens, starts=starts)
 
 
 class PagedAttention(nn.Module):
@@ -256,4 +311,4 @@ class PagedAttention(nn.Module):
         return self.o_proj(o.reshape(*lead, -1))
 
 
-__all__ = ["PagedAttention", "PagedCache", "paged_attention", "qk_norm_rope", "qk_norm_rope_append"]
+__all__ = ["PagedAttention", "PagedCache", "paged_attention", "plan_pages", "qk_norm_rope", "qk_norm_rope_append"]

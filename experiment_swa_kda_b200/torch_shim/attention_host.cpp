@@ -251,6 +251,38 @@ AttentionOut attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
     return std::make_tuple(o, lse);
 }
 
+// ------------------------------------------------------------------------------------------------ pages of a step
+
+using PlanOut = c10::optional<std::tuple<Tensor, Tensor, Tensor>>;
+
+PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const Tensor& news, const OptTensor& starts, int64_t page, int64_t max_tokens) {
+    constexpr int64_t kRows = 16384, kMost = 1 << 30;
+    if (tracing() || !table.is_cuda() || table.dim() != 2 || table.scalar_type() != at::kInt) return c10::nullopt;
+    const int64_t N = table.size(0), width = table.size(1), pages = free.numel();
+    if (N < 1 || N > kRows || width < 1 || width > kInt || (width > 1 && table.stride(1) != 1) || (N > 1 && table.stride(0) < width)) return c10::nullopt;
+    for (const Tensor* t : {&lens, &news})
+        if (t->dim() != 1 || t->numel() != N || t->scalar_type() != at::kInt || !on(*t, table) || !t->is_contiguous()) return c10::nullopt;
+    if (has(starts) && (starts->dim() != 1 || starts->numel() != N || starts->scalar_type() != at::kInt || !on(*starts, table) || !starts->is_contiguous()))
+        return c10::nullopt;
+    if (free.dim() != 1 || free.scalar_type() != at::kBool || !on(free, table) || !free.is_contiguous() || pages > kMost) return c10::nullopt;
+    if (page < 1 || page > kInt || width > kInt / page || width * N > kInt || max_tokens < 0 || max_tokens > kMost) return c10::nullopt;
+    c10::cuda::CUDAGuard guard(table.device());
+    watch_status(table.device().index());
+    at::AutoDispatchBelowADInplaceOrView below;
+    KdaPlanShape s = {};
+    s.rows = (int32_t)N, s.width = (int32_t)width, s.page_size = (int32_t)page, s.n_pages = (int32_t)pages, s.max_tokens = (int32_t)max_tokens;
+    s.table_stride = table.stride(0);
+    Tensor cu = empty({N + 1}, at::kInt, table), positions = empty({max_tokens}, at::kInt, table), slots = empty({max_tokens}, at::kLong, table);
+    const size_t need = kda_plan_pages_workspace_bytes(&s);
+    Tensor ws = bytes(need, table);
+    must(kda_plan_pages(&s, table.mutable_data_ptr<int32_t>(), lens.mutable_data_ptr<int32_t>(), static_cast<uint8_t*>(free.mutable_data_ptr()),
+                        news.const_data_ptr<int32_t>(), iptr(starts), cu.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
+                        ws.data_ptr(), need, stream_of(table)),
+         "kda_plan_pages");
+    for (const Tensor* t : {&table, &lens, &free}) t->unsafeGetTensorImpl()->bump_version();
+    return std::make_tuple(cu, positions, slots);
+}
+
 }  // namespace
 
 void bind_attention(pybind11::module_& m) {
@@ -259,6 +291,7 @@ void bind_attention(pybind11::module_& m) {
     m.def("norm_rope", &norm_rope, nogil());
     m.def("append", &append, nogil());
     m.def("attention", &attention, nogil());
+    m.def("plan", &plan, nogil());
 }
 
 }  // namespace kda_host

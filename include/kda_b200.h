@@ -422,6 +422,26 @@ int kda_paged_attention(const KdaPagedShape* shape, const void* q, const void* k
                         const int32_t* kv_lens, const int32_t* cu_seqlens, void* o, float* lse, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* Pages of such a cache dealt out and the slots of new tokens mapped, from the lengths of a step's requests; no counterpart in the
+ * reference.  Row n of block_table [rows, width] (rows table_stride >= width apart) is to hold columns [starts[n] / page_size,
+ * ceil(kv_lens[n] / page_size)), starts clamped to the length (NULL: 0).  Entries outside go back to the pool (entry -1, page_free[page] = 1);
+ * entries that name no page in [0, n_pages) are missing, and in the order of rows and columns take the pages with page_free != 0 in
+ * ascending order.  A row is served if the entries missing up to and with it are at most the free pages and the new tokens up to and
+ * with it at most max_tokens, or if it lacks nothing and asks for nothing; of one that is not, kv_lens[n] -= new_lens[n], and columns that
+ * this leaves unneeded go back, too late for this call.  cu_seqlens [rows + 1]: new tokens of the rows served.  positions, slots
+ * [max_tokens]: of each of them its place in its sequence, kv_len - new + i, and in the cache, page * page_size + place in the page;
+ * -1 behind the last.  kv_lens count the new tokens, as in kda_paged_attention.  A negative length or one the table has no room for, and an
+ * entry past n_pages, are told as KDA_ERR_BLOCK_TABLE, new_lens outside of [0, kv_len] as KDA_ERR_CU_SEQLENS; such a row's new tokens are
+ * left out or cut.  At most 16,384 rows. */
+typedef struct KdaPlanShape {
+    int32_t rows, width, page_size, n_pages, max_tokens;
+    int64_t table_stride;
+} KdaPlanShape;
+size_t kda_plan_pages_workspace_bytes(const KdaPlanShape* shape);
+int kda_plan_pages(const KdaPlanShape* shape, int32_t* block_table, int32_t* kv_lens, uint8_t* page_free, const int32_t* new_lens,
+                   const int32_t* starts, int32_t* cu_seqlens, int32_t* positions, int64_t* slots, void* workspace, size_t workspace_bytes,
+                   void* stream);
+
 #ifdef __cplusplus
 }
 #endif

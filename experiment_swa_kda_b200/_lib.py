@@ -36,6 +36,10 @@ class PagedShape(C.Structure):
                                  "v_row_stride", "v_head_stride")]
 
 
+class PrefixShape(C.Structure):
+    _fields_ = [("n_groups", C.c_int32), ("table_width", C.c_int32), ("table_stride", C.c_int64)]
+
+
 class PlanShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("rows", "width", "page_size", "n_pages", "max_tokens")] + [("table_stride", C.c_int64)]
 
@@ -90,6 +94,8 @@ _SIGNATURES = {
     "kda_norm_rope_append": (C.c_int, [C.POINTER(RotaryShape), C.POINTER(PagedShape)] + [_P] * 14),
     "kda_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedShape)]),
     "kda_paged_attention": (C.c_int, [C.POINTER(PagedShape)] + [_P] * 9 + [C.c_size_t, _P]),
+    "kda_shared_prefix_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedShape), C.POINTER(PrefixShape)]),
+    "kda_shared_prefix_attention": (C.c_int, [C.POINTER(PagedShape), C.POINTER(PrefixShape)] + [_P] * 12 + [C.c_size_t, _P]),
     "kda_plan_pages_workspace_bytes": (C.c_size_t, [C.POINTER(PlanShape)]),
     "kda_plan_pages": (C.c_int, [C.POINTER(PlanShape)] + [_P] * 9 + [C.c_size_t, _P]),
     "kda_launch_count": (C.c_ulonglong, []),

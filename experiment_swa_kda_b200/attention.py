@@ -8,6 +8,7 @@ kernels of this package:
     qk_norm_rope         training and prefill: norm + rotation, differentiable
     qk_norm_rope_append  serving: the same, keys and values written to the pages of a cache
     paged_attention      serving: a chunk of new tokens, or one token, of every sequence of a batch over that cache
+    shared_prefix_attention   the same for sequences that start with a common text, which is read once
     plan_pages           serving: block tables and slots of a step from the lengths of its requests
 
 A batch of new tokens is packed, [tokens, heads, D], with `cu_seqlens` [N+1] as in `chunk_kda`, or without it when every
@@ -184,6 +185,52 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     raise RuntimeError("paged_attention: the batch or the block table is too large for one call, or a trace is being recorded")
 
 
+def shared_prefix_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kv_lens: Tensor, prefix_table: Tensor, prefix_lens: Tensor,
+                            cu_groups: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None, *, max_q_len: int = 0,
+                            scale: Optional[float] = None, return_lse: bool = False):
+    """`paged_attention` of sequences that start with a common text: its keys and values are in the cache once, and read once for all of
+    the sequences.
+
+    Sequences cu_groups[g] .. cu_groups[g+1] - 1 are group g (`cu_groups` [G+1] int32, or None: N / G each); its text is `prefix_lens`[g] tokens
+    in the pages `prefix_table`[g] ([G,W] int32, [G] int32).  `kv_lens` count the prefix too.  A sequence shares it if its new tokens all lie
+    behind it: its own row of `block_table` then names the pages of positions from prefix_lens[g] on - by position / page_size, as in
+    `paged_attention` -, and the entries before that are not looked at.  The page in which the prefix ends is the sequence's own where its own
+    tokens go on in it.  A sequence whose new tokens do not all lie behind the prefix (padding, a shorter text) or that is in no group
+    has all of its keys in its own pages.
+
+    bfloat16 under the conditions of `paged_attention` runs on the tensor cores, where the new tokens of all sequences of a group share each
+    key tile of the prefix.  Returns o, or (o, lse), as `paged_attention` does.  There is no window: a sliding-window layer sees little of
+    a prefix.  Inference only."""
+    out = None
+    if q.is_cuda:
+        out = _native.load().shared_attention(q, k_cache, v_cache, block_table, kv_lens, prefix_table, prefix_lens, cu_groups, cu_seqlens, max_q_len, scale,
+                                              bool(return_lse))
+    if out is not None:
+        return out if return_lse else out[0]
+    _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
+    if prefix_table.ndim != 2 or prefix_table.dtype != torch.int32 or not 1 <= prefix_table.shape[0] <= block_table.shape[0]:
+        raise ValueError("prefix_table must be int32 with shape [G, pages of a prefix], with a group for one sequence at least")
+    groups = prefix_table.shape[0]
+    if tuple(prefix_lens.shape) != (groups,) or prefix_lens.dtype != torch.int32:
+        raise ValueError(f"prefix_lens must be int32 with shape {(groups,)}")
+    if cu_groups is None:
+        if block_table.shape[0] % groups != 0:
+            raise ValueError("without cu_groups every group has the same number of sequences")
+    elif tuple(cu_groups.shape) != (groups + 1,) or cu_groups.dtype != torch.int32:
+        raise ValueError(f"cu_groups must be int32 with shape {(groups + 1,)}")
+    _same_device(q, prefix_table, prefix_lens, cu_groups)
+    if prefix_table.shape[1] > 1 and prefix_table.stride(1) != 1:
+        raise ValueError("prefix_table must have adjacent values along its last dimension")
+    if not prefix_lens.is_contiguous() or (cu_groups is not None and not cu_groups.is_contiguous()):
+        raise ValueError("prefix_lens and cu_groups must be contiguous")
+    if max_q_len < 0:
+        raise ValueError("max_q_len must not be negative")
+    if scale is not None and not (0 < scale < float("inf")):
+        raise ValueError("scale must be positive and finite")
+    _no_grad("shared_prefix_attention", q, k_cache, v_cache)
+    raise RuntimeError("shared_prefix_attention: the batch or a block table is too large for one call, or a trace is being recorded")
+
+
 def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens: Tensor, *, page_size: int, max_tokens: int,
                starts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """Deals out the pages of a step and maps its new tokens to them; returns (cu_seqlens [N+1], positions [max_tokens], slots [max_tokens]).
@@ -237,6 +284,9 @@ class PagedCache:
     block_table: Tensor     # [N, pages of a sequence] int32
     kv_lens: Tensor         # [N] int32
     page_free: Optional[Tensor] = None      # [pages] bool: the pool of `plan`
+    prefix_table: Optional[Tensor] = None   # texts that sequences share (`shared_prefix_attention`)
+    prefix_lens: Optional[Tensor] = None
+    cu_groups: Optional[Tensor] = None
 
     @staticmethod
     def zeros(sequences: int, max_len: int, page_size: int, num_kv_heads: int, head_dim: int, device, dtype=torch.bfloat16) -> "PagedCache":
@@ -298,6 +348,8 @@ class PagedAttention(nn.Module):
     def forward(self, hidden_states: Tensor, cache: PagedCache, cu_seqlens: Optional[Tensor] = None, max_q_len: int = 0) -> Tensor:
         """hidden_states [B,T,hidden], T new tokens of each of the cache's B sequences, or [1,tokens,hidden], packed, with `cu_seqlens`."""
         lead = hidden_states.shape[:-1]
+        if self.window and cache.prefix_table is not None:
+            raise ValueError("a sliding-window layer does not share a prefix: its cache must not have one")
         if cu_seqlens is None:
             sequences = cache.block_table.shape[0]
             if hidden_states.ndim != 3 or hidden_states.shape[0] != sequences:
@@ -307,8 +359,11 @@ class PagedAttention(nn.Module):
         q, k, v = qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), 1)
         place = (cache.k, cache.v, cache.block_table, cache.kv_lens, cu_seqlens)
         q = qk_norm_rope_append(q, k, v, self.cos, self.sin, *place, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.norm_eps)
-        o = paged_attention(q, *place, max_q_len=max_q_len, window=self.window)
+        if cache.prefix_table is None:
+            o = paged_attention(q, *place, max_q_len=max_q_len, window=self.window)
+        else:
+            o = shared_prefix_attention(q, *place[:4], cache.prefix_table, cache.prefix_lens, cache.cu_groups, cu_seqlens, max_q_len=max_q_len)
         return self.o_proj(o.reshape(*lead, -1))
 
 
-__all__ = ["PagedAttention", "PagedCache", "paged_attention", "plan_pages", "qk_norm_rope", "qk_norm_rope_append"]
+__all__ = ["PagedAttention", "PagedCache", "paged_attention", "plan_pages", "qk_norm_rope", "qk_norm_rope_append", "shared_prefix_attention"]

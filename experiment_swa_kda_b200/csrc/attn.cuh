@@ -21,6 +21,9 @@ struct Batch {
     __device__ __forceinline__ void tell(int code) const {
         if (mirror != nullptr) *reinterpret_cast<volatile int*>(mirror) = code;
     }
+    __device__ __forceinline__ int many() const { return n_seq; }
+    // first new token of sequence n of a packed batch
+    __device__ __forceinline__ int edge(int n) const { return min(max(__ldg(cu + n), 0), tokens); }
     // new tokens [first, first + count) of sequence n
     __device__ __forceinline__ void span(int n, int& first, int& count) const {
         if (cu == nullptr) {
@@ -82,26 +85,97 @@ struct Batch {
     }
 };
 
+// Sequences that start with the same text.  Sequences [groups[g], groups[g + 1]) are group g (null: `each` a group), whose text is lens[g]
+// tokens in the pages of the table's row g.  A sequence shares it if all its new tokens lie behind it; it then has own keys from there on.
+// One that does not - a place in the batch without a request, a shorter text - has all its keys to itself.
+struct Prefix {
+    const int* table;
+    const int* lens;
+    const int* groups;
+    long long table_stride;
+    int n, width, each;
+};
+
+// A batch of which every sequence sees its own keys only: those behind its prefix.
+struct OwnView : Batch {
+    Prefix p;
+    __device__ __forceinline__ int group_edge(int g) const { return p.groups == nullptr ? g * p.each : min(max(__ldg(p.groups + g), 0), n_seq); }
+    // the group of sequence n, or -1
+    __device__ __forceinline__ int group_of(int n) const {
+        if (p.groups == nullptr) return n / p.each;
+        int lo = 0, hi = p.n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (group_edge(mid) <= n) lo = mid;
+            else hi = mid;
+        }
+        return n >= group_edge(lo) && n < group_edge(lo + 1) ? lo : -1;
+    }
+    __device__ __forceinline__ int prefix_len(int g) const {
+        const long long room = (long long)p.width * page_size;
+        const int len = max(__ldg(p.lens + g), 0);
+        return (long long)len > room ? (int)room : len;
+    }
+    // the prefix of sequence n's group, whether or not the sequence shares it
+    __device__ __forceinline__ int prefix_of(int n) const {
+        const int g = group_of(n);
+        return g < 0 ? 0 : prefix_len(g);
+    }
+    __device__ __forceinline__ bool groups_ok(int g) const {
+        if (p.groups != nullptr) {
+            const int a = __ldg(p.groups + g), b = __ldg(p.groups + g + 1);
+            if (a < 0 || a > b || b > n_seq) return false;
+        }
+        return true;
+    }
+    __device__ __forceinline__ bool prefix_ok(int g) const {
+        const int len = __ldg(p.lens + g);
+        return len >= 0 && (long long)len <= (long long)p.width * page_size;
+    }
+};
+
+// The same batch with each group as one sequence: all new tokens of the group see the whole prefix, and nothing else.
+struct GroupView : OwnView {
+    __device__ __forceinline__ int many() const { return p.n; }
+    __device__ __forceinline__ int edge(int g) const {
+        const int s = group_edge(g);
+        return cu == nullptr ? s * q_len : min(max(__ldg(cu + s), 0), tokens);
+    }
+    __device__ __forceinline__ void span(int g, int& first, int& count) const {
+        first = edge(g);
+        count = max(edge(g + 1) - first, 0);
+    }
+    __device__ __forceinline__ int page(int g, int col) const {
+        const int at = __ldg(p.table + g * p.table_stride + col);
+        return (unsigned)at < (unsigned)n_pages ? at : -1;
+    }
+};
+
 // Tiles of `rows` packed rows (token-major, the query heads of one kv head beside each other) of all sequences.  With a bound
 // on the tokens of a sequence every sequence has tiles_per_seq slots; without one sequence n starts at slot
 // first * group / rows + n, which leaves room for its last, partial tile and needs no sum over the sequences before it.
 struct Tiles {
     int rows, group, per_seq;
-    __device__ __forceinline__ bool find(const Batch& b, int slot, int& n, int& tile) const {
+    template <class B>
+    __device__ __forceinline__ int start(const B& b, int i) const {
+        return per_seq > 0 ? i * per_seq : (int)((long long)b.edge(i) * group / rows) + i;
+    }
+    template <class B>
+    __device__ __forceinline__ bool find(const B& b, int slot, int& n, int& tile) const {
+        const int many = b.many();
         if (per_seq > 0) {
             n = slot / per_seq;
             tile = slot - n * per_seq;
-            return n < b.n_seq;
+            return n < many;
         }
-        auto start = [&](int i) { return (int)((long long)min(max(__ldg(b.cu + i), 0), b.tokens) * group / rows) + i; };
-        int lo = 0, hi = b.n_seq;
+        int lo = 0, hi = many;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (start(mid) <= slot) lo = mid;
+            if (start(b, mid) <= slot) lo = mid;
             else hi = mid;
         }
         n = lo;
-        tile = slot - start(lo);
+        tile = slot - start(b, lo);
         return tile >= 0;
     }
 };
@@ -118,6 +192,13 @@ inline long long tile_slots(int tokens, int n_seq, int max_q_len, int group, int
     return by_tokens;
 }
 
+inline long long group_slots(const GroupView& b, int group, int rows, int& per_group) {
+    per_group = 0;
+    if (b.p.n > 1) return (long long)b.tokens * group / rows + b.p.n;
+    per_group = (int)(((long long)b.tokens * group + rows - 1) / rows);
+    return per_group;
+}
+
 // The first key that a token at `pos` sees; in this order nothing leaves 32 bits, however negative a padding token's position or wide the window.
 __device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 
@@ -127,8 +208,27 @@ struct Unit {
     int row0, rows;            // packed rows [row0, row0 + rows) of the sequence
     int base;                  // position of its first new token (negative: padding)
     int lo, hi;                // keys in reach of the tile
+    int from;                  // no row sees a key before this one
 };
-__device__ __forceinline__ bool make_unit(const Batch& b, const Tiles& t, int slot, int window, Unit& u) {
+__device__ __forceinline__ bool make_unit(const GroupView& b, const Tiles& t, int slot, int, Unit& u) {
+    int tile;
+    if (!t.find(b, slot, u.n, tile)) return false;
+    b.span(u.n, u.first, u.count);
+    u.row0 = tile * t.rows;
+    u.rows = min(t.rows, u.count * t.group - u.row0);
+    if (u.rows <= 0) return false;
+    u.base = 0;
+    u.lo = u.from = 0;
+    u.hi = b.prefix_len(u.n);
+    return true;
+}
+__device__ __forceinline__ int own_from(const Batch&, const Unit&) { return 0; }
+__device__ __forceinline__ int own_from(const OwnView& b, const Unit& u) {
+    const int p = b.prefix_of(u.n);
+    return u.base >= p ? p : 0;
+}
+template <class B>
+__device__ __forceinline__ bool make_unit(const B& b, const Tiles& t, int slot, int window, Unit& u) {
     int tile;
     if (!t.find(b, slot, u.n, tile)) return false;
     b.span(u.n, u.first, u.count);
@@ -139,10 +239,16 @@ __device__ __forceinline__ bool make_unit(const Batch& b, const Tiles& t, int sl
     u.base = len - u.count;
     const int i0 = u.row0 / t.group, i1 = (u.row0 + u.rows - 1) / t.group;
     u.hi = max(u.base + i1 + 1, 0);
-    u.lo = first_key(u.base + i0, window);
+    u.from = own_from(b, u);
+    u.lo = max(first_key(u.base + i0, window), u.from);
     return true;
 }
 // What a batch got wrong is reported by the blocks of the first tile of each sequence.
+__device__ __forceinline__ void check_batch(const GroupView& b, const Tiles&, int g, int tile) {
+    if (tile != 0) return;
+    if (!b.groups_ok(g)) b.tell(KDA_ERR_CU_SEQLENS);
+    if (!b.prefix_ok(g)) b.tell(KDA_ERR_BLOCK_TABLE);
+}
 __device__ __forceinline__ void check_batch(const Batch& b, const Tiles& t, int n, int tile) {
     if (tile != 0) return;
     if (!b.span_ok(n)) b.tell(KDA_ERR_CU_SEQLENS);
@@ -166,6 +272,21 @@ struct Strides {
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Which keys a pass goes through.
+enum Keys { kAllKeys, kPrefixKeys, kOwnKeys };
+template <int KEYS>
+struct ViewOf {
+    using type = Batch;
+};
+template <>
+struct ViewOf<kPrefixKeys> {
+    using type = GroupView;
+};
+template <>
+struct ViewOf<kOwnKeys> {
+    using type = OwnView;
+};
+
 struct Combine {
     int tokens, q_heads, dim, splits;
     const float* part_o;      // [splits][tokens * q_heads][dim], not divided by the sum
@@ -173,11 +294,12 @@ struct Combine {
     void* o;
     float* lse;
     int bf16;
+    int prefix_splits;        // of them parts of a prefix
+    GroupView batch;
 };
-int combine(const Combine& c, cudaStream_t st);
 
 struct Call {
-    Batch batch;
+    GroupView batch;
     Heads heads;
     Strides strides;
     const void *q, *k, *v;
@@ -187,6 +309,10 @@ struct Call {
     int window, bf16, max_q_len;
     void* workspace;
 };
+template <int KEYS>
+__device__ __forceinline__ const typename ViewOf<KEYS>::type& view(const Call& c) {
+    return c.batch;
+}
 int general(const Call& c, int splits, cudaStream_t st);
 bool tc_takes(const Call& c);      // bf16, head width, page size and strides that the tensor-core kernel can load
 int tc(const Call& c, int splits, cudaStream_t st);
@@ -194,6 +320,15 @@ size_t tc_workspace(long long slots, int kv_heads, int splits, int dim);
 bool decode_takes(const Call& c);      // ... and at most 16 rows a sequence and kv head
 size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim);
 int decode(const Call& c, cudaStream_t st);
+// The passes of attention behind a shared prefix; their sums stay in the workspace, undivided, for a join.
+int general_shared(const Call& c, int prefix_splits, int own_splits, cudaStream_t st);
+size_t general_shared_workspace(size_t rows, int parts, int dim);
+int tc_prefix(const Call& c, int splits, cudaStream_t st);
+int tc_own(const Call& c, int splits, cudaStream_t st);
+size_t tc_parts_bytes(long long slots, int kv_heads, int splits, int dim);
+int decode_own(const Call& c, float* row_o, float2* row_ml, cudaStream_t st);
+// Own keys of each row: as tc_own left them in own.workspace (row_o null), or one sum a row.
+int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const float* row_o, const float2* row_ml, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace kda

@@ -79,7 +79,9 @@ extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const 
     const bool packed = cu_seqlens != nullptr;
     const int q_len = packed ? 0 : s->tokens / s->n_seq;
     Call c;
-    c.batch = Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width};
+    c.batch = GroupView{};
+    static_cast<Batch&>(c.batch) =
+        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width};
     c.heads = Heads{s->q_heads, s->kv_heads, s->q_heads / s->kv_heads, s->head_dim};
     c.strides = Strides{s->q_token_stride, s->q_head_stride, s->k_page_stride, s->k_row_stride, s->k_head_stride, s->v_page_stride, s->v_row_stride, s->v_head_stride};
     c.q = q; c.k = k_cache; c.v = v_cache; c.o = o; c.lse = lse;
@@ -90,4 +92,116 @@ extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const 
     c.workspace = workspace;
     if (decode_takes(c)) return decode(c, (cudaStream_t)stream);
     return tc_takes(c) ? tc(c, tc_splits(*s, packed), (cudaStream_t)stream) : general(c, general_splits(*s, packed), (cudaStream_t)stream);
+}
+
+// ------------------------------------------------------------------------------------------------ behind a shared prefix
+
+namespace {
+
+int check_prefix(const KdaPagedShape* s, const KdaPrefixShape* p, bool packed, bool grouped) {
+    if (int rc = check(s, packed)) return rc;
+    if (!p) return KDA_ERR_NULL;
+    if (p->n_groups <= 0 || p->n_groups > s->n_seq || p->table_width < 0 || s->window != 0) return KDA_ERR_BAD_SHAPE;
+    if (!grouped && s->n_seq % p->n_groups != 0) return KDA_ERR_BAD_SHAPE;
+    if ((long long)p->table_width * s->page_size >= 1ll << 31) return KDA_ERR_BAD_SHAPE;
+    return KDA_OK;
+}
+
+GroupView groups_of(const KdaPagedShape& s, const KdaPrefixShape& p) {
+    GroupView v = {};
+    v.n_seq = s.n_seq;
+    v.tokens = s.tokens;
+    v.p.n = p.n_groups;
+    return v;
+}
+// Parts of a prefix where its row tiles leave SMs idle, as in split_count; a part has `least` key tiles.
+int prefix_split_count(const KdaPagedShape& s, const KdaPrefixShape& p, int rows, int keys, int resident, int least) {
+    int per;
+    const long long blocks = group_slots(groups_of(s, p), s.q_heads / s.kv_heads, rows, per) * s.kv_heads;
+    const long long tiles = ((long long)p.table_width * s.page_size + keys - 1) / keys;
+    long long n = resident / (blocks > 0 ? blocks : 1);
+    if (n > tiles / least) n = tiles / least;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+int tc_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) {
+    int per;
+    const long long slots = group_slots(groups_of(s, p), s.q_heads / s.kv_heads, 256, per);
+    return slots <= 384 && slots * s.kv_heads <= 148 / 2 ? prefix_split_count(s, p, 256, 128, 3 * 148, 1) : 1;
+}
+int general_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) { return prefix_split_count(s, p, 64, 64, 2 * 148, 1); }
+
+// The shares of a workspace on the tensor cores.
+struct SharedSpace {
+    size_t prefix, own, rows_ml, rows_o, all;
+};
+SharedSpace shared_space(const KdaPagedShape& s, const KdaPrefixShape& p, bool packed, bool few) {
+    SharedSpace w;
+    int per;
+    const int group = s.q_heads / s.kv_heads, max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
+    const size_t rows = (size_t)s.tokens * s.q_heads;
+    w.prefix = align_up(tc_parts_bytes(group_slots(groups_of(s, p), group, 256, per), s.kv_heads, tc_prefix_splits(s, p), s.head_dim), 256);
+    w.own = few ? decode_workspace(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, max_q, s.head_dim)
+                : tc_parts_bytes(tile_slots(s.tokens, s.n_seq, max_q, group, 256, packed, per), s.kv_heads, tc_splits(s, packed), s.head_dim);
+    w.own = align_up(w.own, 256);
+    w.rows_ml = few ? align_up(rows * sizeof(float2), 256) : 0;
+    w.rows_o = few ? align_up(rows * s.head_dim * sizeof(float), 256) : 0;
+    w.all = w.prefix + w.own + w.rows_ml + w.rows_o;
+    return w;
+}
+
+}  // namespace
+
+extern "C" size_t kda_shared_prefix_attention_workspace_bytes(const KdaPagedShape* s, const KdaPrefixShape* p) {
+    if (check_prefix(s, p, true, true)) return 0;
+    size_t most = general_shared_workspace((size_t)s->tokens * s->q_heads, general_prefix_splits(*s, *p) + general_splits(*s, true), s->head_dim);
+    for (int packed = 0; packed < 2; ++packed) {      // whether the batch has cu_seqlens is not known here
+        if (!packed && s->tokens % s->n_seq != 0) continue;
+        const size_t g = general_shared_workspace((size_t)s->tokens * s->q_heads, general_prefix_splits(*s, *p) + general_splits(*s, packed), s->head_dim);
+        if (g > most) most = g;
+        for (int few = 0; few < 2; ++few) {
+            const size_t n = shared_space(*s, *p, packed, few).all;
+            if (n > most) most = n;
+        }
+    }
+    return align_up(most, 256);
+}
+
+extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPrefixShape* p, const void* q, const void* k_cache, const void* v_cache,
+                                           const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, const int32_t* prefix_table,
+                                           const int32_t* prefix_lens, const int32_t* cu_groups, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                                           void* stream) {
+    if (int rc = check_prefix(s, p, cu_seqlens != nullptr, cu_groups != nullptr)) return rc;
+    if (s->tokens == 0) return KDA_OK;
+    if (!q || !kv_lens || !o || !prefix_lens) return KDA_ERR_NULL;
+    if (s->n_pages > 0 && ((s->table_width > 0 && !block_table) || (p->table_width > 0 && !prefix_table) || !k_cache || !v_cache)) return KDA_ERR_NULL;
+    const size_t need = kda_shared_prefix_attention_workspace_bytes(s, p);
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need) return KDA_ERR_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool packed = cu_seqlens != nullptr;
+    const int q_len = packed ? 0 : s->tokens / s->n_seq;
+    Call c;
+    c.batch = GroupView{};
+    static_cast<Batch&>(c.batch) =
+        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width};
+    c.batch.p = Prefix{prefix_table, prefix_lens, cu_groups, p->table_stride, p->n_groups, p->table_width, s->n_seq / p->n_groups};
+    c.heads = Heads{s->q_heads, s->kv_heads, s->q_heads / s->kv_heads, s->head_dim};
+    c.strides = Strides{s->q_token_stride, s->q_head_stride, s->k_page_stride, s->k_row_stride, s->k_head_stride, s->v_page_stride, s->v_row_stride, s->v_head_stride};
+    c.q = q; c.k = k_cache; c.v = v_cache; c.o = o; c.lse = lse;
+    c.scale = s->scale;
+    c.window = 0;
+    c.bf16 = s->io_dtype == KDA_DTYPE_BF16;
+    c.max_q_len = packed ? s->max_q_len : q_len;
+    c.workspace = workspace;
+    if (!tc_takes(c)) return general_shared(c, general_prefix_splits(*s, *p), general_splits(*s, packed), st);
+    const bool few = decode_takes(c);
+    const SharedSpace w = shared_space(*s, *p, packed, few);
+    char* ws = static_cast<char*>(workspace);
+    const int prefix_splits = tc_prefix_splits(*s, *p), own_splits = tc_splits(*s, packed);
+    if (int rc = tc_prefix(c, prefix_splits, st)) return rc;
+    Call own = c;
+    own.workspace = ws + w.prefix;
+    float2* row_ml = reinterpret_cast<float2*>(ws + w.prefix + w.own);
+    float* row_o = reinterpret_cast<float*>(ws + w.prefix + w.own + w.rows_ml);
+    if (int rc = few ? decode_own(own, row_o, row_ml, st) : tc_own(own, own_splits, st)) return rc;
+    return tc_shared_join(c, prefix_splits, own, own_splits, few ? row_o : nullptr, row_ml, st);
 }

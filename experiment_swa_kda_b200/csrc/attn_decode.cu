@@ -60,21 +60,30 @@ struct Args {
     int whole;            // stretches begin and end with a sequence and kv head: no parts
     float* part_o;        // [blocks][2][rows][D]
     float2* part_ml;      // [blocks][2][rows]
+    float* row_o;         // own keys only: [tokens * q_heads][D], not divided by the sums, and (maximum, sum) of each row
+    float2* row_ml;
 };
 
 // One sequence's tiles and rows.
 struct Seq {
     int first, count, base, lo, hi, t0, t1;
 };
-// what a sequence is read from: the ends of its new tokens and its length, as they stand in memory
+// what a sequence is read from: the ends of its new tokens and its length, as they stand in memory, and its group's prefix
 struct Raw {
-    int a, b, len;
+    int a, b, len, prefix;
 };
-__device__ __forceinline__ Raw raw_at(const Batch& b, int n) {
-    if (n >= b.n_seq) return Raw{0, 0, 0};
-    return b.cu != nullptr ? Raw{__ldg(b.cu + n), __ldg(b.cu + n + 1), __ldg(b.kv_lens + n)} : Raw{n * b.q_len, (n + 1) * b.q_len, __ldg(b.kv_lens + n)};
+__device__ __forceinline__ int prefix_at(const Batch&, int) { return 0; }
+__device__ __forceinline__ int prefix_at(const OwnView& b, int n) { return b.prefix_of(n); }
+__device__ __forceinline__ int own_key(const Batch&, const Raw&, int) { return 0; }
+__device__ __forceinline__ int own_key(const OwnView&, const Raw& r, int base) { return base >= r.prefix ? r.prefix : 0; }
+template <class B>
+__device__ __forceinline__ Raw raw_at(const B& b, int n) {
+    if (n >= b.n_seq) return Raw{0, 0, 0, 0};
+    const int p = prefix_at(b, n);
+    return b.cu != nullptr ? Raw{__ldg(b.cu + n), __ldg(b.cu + n + 1), __ldg(b.kv_lens + n), p} : Raw{n * b.q_len, (n + 1) * b.q_len, __ldg(b.kv_lens + n), p};
 }
-__device__ __forceinline__ Seq seq_of_raw(const Batch& b, const Raw& r, int window) {
+template <class B>
+__device__ __forceinline__ Seq seq_of_raw(const B& b, const Raw& r, int window) {
     Seq s;
     s.first = min(max(r.a, 0), b.tokens);
     s.count = min(max(r.b, s.first), b.tokens) - s.first;
@@ -82,12 +91,13 @@ __device__ __forceinline__ Seq seq_of_raw(const Batch& b, const Raw& r, int wind
     const int len = max(r.len, 0) > room ? (int)room : max(r.len, 0);
     s.base = len - s.count;
     s.hi = s.count > 0 ? len : 0;
-    s.lo = min(first_key(s.base, window), s.hi);
+    s.lo = min(max(first_key(s.base, window), own_key(b, r, s.base)), s.hi);
     s.t0 = s.lo / kTile;
     s.t1 = (s.hi + kTile - 1) / kTile;
     return s;
 }
-__device__ __forceinline__ Seq seq_at(const Batch& b, int n, int window) { return seq_of_raw(b, raw_at(b, n), window); }
+template <class B>
+__device__ __forceinline__ Seq seq_at(const B& b, int n, int window) { return seq_of_raw(b, raw_at(b, n), window); }
 
 // How the list is cut: the first `longer` stretches have `each` + 1 tiles, the others `each`.
 struct Cut {
@@ -102,8 +112,8 @@ struct Start {
 };
 // The cut, and where stretch `id` begins.  Called by all THREADS of a block; `sums` has a place for each warp.  The host takes
 // care that the list has less than 2^31 tiles.
-template <int THREADS, bool whole>
-__device__ __forceinline__ Cut find_start(const Batch& b, int kv_heads, int window, int blocks, int id, Start* start, int* sums) {
+template <int THREADS, bool whole, class B>
+__device__ __forceinline__ Cut find_start(const B& b, int kv_heads, int window, int blocks, int id, Start* start, int* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = (b.n_seq + THREADS - 1) / THREADS, n0 = min(tid * each, b.n_seq), n1 = min(n0 + each, b.n_seq);
     int mine = 0;
@@ -190,7 +200,8 @@ struct Walk {
         hk = at.hk;
         tile = at.tile;
     }
-    __device__ __forceinline__ void next(const Batch& b, int kv_heads, int window) {
+    template <class B>
+    __device__ __forceinline__ void next(const B& b, int kv_heads, int window) {
         if (++tile < s.t1) return;
         if (++hk == kv_heads) {
             hk = 0;
@@ -231,7 +242,7 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {      // an 8 x 8 tile o
     return y;
 }
 
-template <int DP, int NR>
+template <int DP, int NR, int KEYS>
 __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                                        const __grid_constant__ Args a) {
     using L = Layout<DP, NR>;
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
     volatile int* flags = reinterpret_cast<volatile int*>(sums + kWarps);      // [0] an expired wait, [1], [2] values that are not finite (of sequences in turn)
     float2* row_ml = reinterpret_cast<float2*>(bars + 64);                     // [warps][rows]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, c4 = lane & 3, r8 = lane >> 2;
-    const Batch& b = a.c.batch;
+    const auto& b = view<KEYS>(a.c);
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window;
 
     uint64_t* bar = bars + warp * kStages;
@@ -332,11 +343,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         }
         if (s.t1 > s.t0) continue;
         const size_t r0 = (size_t)s.first * Hq;
-        for (long long e = tid; e < (long long)s.count * Hq * D; e += kThreads) static_cast<__nv_bfloat16*>(a.c.o)[r0 * D + e] = __float2bfloat16(0.f);
-        if (a.c.lse != nullptr)
-            for (int e = tid; e < s.count * Hq; e += kThreads) a.c.lse[r0 + e] = -INFINITY;
+        if constexpr (KEYS == kOwnKeys) {
+            for (int e = tid; e < s.count * Hq; e += kThreads) a.row_ml[r0 + e] = make_float2(-INFINITY, 0.f);
+        } else {
+            for (long long e = tid; e < (long long)s.count * Hq * D; e += kThreads) static_cast<__nv_bfloat16*>(a.c.o)[r0 * D + e] = __float2bfloat16(0.f);
+            if (a.c.lse != nullptr)
+                for (int e = tid; e < s.count * Hq; e += kThreads) a.c.lse[r0 + e] = -INFINITY;
+        }
     }
-    if (tiles <= 0) return;
+    if (tiles <= 0) {
+        if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too
+        return;
+    }
     put_q(0);
     __syncthreads();
 
@@ -361,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             if (tiles - i > w.s.t1 - w.tile) fetch_q(then);
             rows = min(w.s.count * g, kRows);
             unit_begin = w.tile;
-            all_lo = first_key(w.s.base + (rows - 1) / g, window);
+            all_lo = KEYS == kOwnKeys ? w.s.lo : first_key(w.s.base + (rows - 1) / g, window);
             all_hi = w.s.base + 1;
 #pragma unroll
             for (int y = 0; y < NR; ++y) {
@@ -369,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                 for (int x = 0; x < 2; ++x) {
                     const int r = 8 * y + 2 * c4 + x;
                     last[y][x] = r < rows ? w.s.base + r / g : -1;
-                    first[y][x] = first_key(last[y][x], window);
+                    first[y][x] = KEYS == kOwnKeys ? w.s.lo : first_key(last[y][x], window);
                     m[y][x] = -INFINITY;
                     l[y][x] = 0.f;
                 }
@@ -557,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                 float o[4] = {oa.x, oa.y, ob.x, ob.y};
                 if (M == kLowest) sum = 0.f;      // nothing but -inf: 0 / 0
                 if (flags[1 + q_buffer]) {
-                    const int to = w.s.base + r / g, from = first_key(to, window);
+                    const int to = w.s.base + r / g, from = KEYS == kOwnKeys ? w.s.lo : first_key(to, window);
 #pragma unroll 1
                     for (int key = max(from, unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
                         if (key >= all_lo && key < all_hi) continue;
@@ -578,6 +596,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                     continue;
                 }
                 const size_t out = (size_t)(w.s.first + r / g) * Hq + w.hk * g + r % g;
+                if constexpr (KEYS == kOwnKeys) {
+                    if (d == 0) a.row_ml[out] = make_float2(M == -INFINITY ? M : max_nan(M * c, kLowest), sum);
+                    *reinterpret_cast<float4*>(a.row_o + out * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                    continue;
+                }
                 const float inv = M == -INFINITY ? 0.f : 1.f / sum;
                 if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = M == -INFINITY ? -INFINITY : (M * c + log2f(sum)) * kLn2;
                 *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
@@ -592,20 +615,21 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
     }
     if (flags[0])      // no copy may be in flight when the block ends
         for (int s = 0; s < kStages; ++s) mbar_poll(bar + s, (phases >> s) & 1u, kSpinLimit / 8);
+    if (KEYS == kOwnKeys) dependency_wait();
 }
 
 // Joins the parts of a sequence's kv head that more than one stretch has worked on.  Block i looks at the place where stretch i + 1
 // begins; the first such place inside a sequence takes all its parts.  Four values a thread; with few rows several threads share the
 // parts of one place and add up through shared memory.
 constexpr int kJoinThreads = 512, kMaxBlocks = 148 * kPerSm;
-template <int NR>
+template <int NR, int KEYS>
 __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __grid_constant__ Args a) {
     constexpr int kRows = 8 * NR;
     __shared__ Start start;
     __shared__ int sums[kJoinThreads / 32];
     __shared__ float weight[kMaxBlocks * kRows], row_l[kRows], row_m[kRows];
     __shared__ float4 acc[kJoinThreads];
-    const Batch& b = a.c.batch;
+    const auto& b = view<KEYS>(a.c);
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Cut cut = find_start<kJoinThreads, false>(b, Hk, window, a.blocks, id, &start, sums);
@@ -668,21 +692,31 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
             o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
         }
         const size_t out = (size_t)(s.first + r / g) * Hq + start.hk * g + r % g;
+        if constexpr (KEYS == kOwnKeys) {
+            if (d == 0) a.row_ml[out] = make_float2(row_m[r], row_l[r]);
+            *reinterpret_cast<float4*>(a.row_o + out * D + d) = o;
+            return;
+        }
         const float m = row_m[r], l = row_l[r], inv = m == -INFINITY ? 0.f : 1.f / l;
         if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
     }
 }
 
-template <int DP, int NR>
+template <int DP, int NR, int KEYS>
 int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStream_t st) {
     constexpr int kBytes = Layout<DP, NR>::kBytes;
-    if (int rc = set_smem_limit(attn_decode_kernel<DP, NR>, kBytes)) return rc;
-    KDA_LAUNCH("attn_decode_kernel", st, attn_decode_kernel<DP, NR><<<a.blocks, kThreads, kBytes, st>>>(mK, mV, a));
+    if (int rc = set_smem_limit(attn_decode_kernel<DP, NR, KEYS>, kBytes)) return rc;
+    cudaError_t e = cudaSuccess;
+    if constexpr (KEYS == kOwnKeys) {      // beside the pass over the prefix
+        KDA_LAUNCH("attn_decode_kernel", st, e = launch_early(attn_decode_kernel<DP, NR, KEYS>, dim3(a.blocks), kThreads, kBytes, st, true, 1, mK, mV, a));
+        if (e != cudaSuccess) return KDA_ERR_CUDA;
+    } else {
+        KDA_LAUNCH("attn_decode_kernel", st, attn_decode_kernel<DP, NR, KEYS><<<a.blocks, kThreads, kBytes, st>>>(mK, mV, a));
+    }
     if (int rc = launch_status()) return rc;
     if (a.blocks == 1 || a.whole) return KDA_OK;
-    cudaError_t e = cudaSuccess;
-    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
+    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR, KEYS>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
@@ -712,7 +746,10 @@ size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size,
     return align_up(rows * sizeof(float2), 256) + rows * dim * sizeof(float);
 }
 
-int decode(const Call& c, cudaStream_t st) {
+namespace {
+
+template <int KEYS>
+int pass(const Call& c, float* row_o, float2* row_ml, cudaStream_t st) {
     Args a;
     a.c = c;
     a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
@@ -720,15 +757,22 @@ int decode(const Call& c, cudaStream_t st) {
     a.whole = keeps_whole(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
     a.part_ml = static_cast<float2*>(c.workspace);
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up((size_t)a.blocks * 2 * kMaxRows * sizeof(float2), 256));
+    a.row_o = row_o;
+    a.row_ml = row_ml;
     CUtensorMap mK, mV;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
     if (!rc) rc = make_map_paged(&mV, c.v, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.v_row, s.v_head, s.v_page, a.box_rows);
     if (rc) return rc;
     const bool few = c.max_q_len * c.heads.group <= 8;
-    if (c.heads.dim <= 64) return few ? launch<64, 1>(mK, mV, a, st) : launch<64, 2>(mK, mV, a, st);
-    return few ? launch<128, 1>(mK, mV, a, st) : launch<128, 2>(mK, mV, a, st);
+    if (c.heads.dim <= 64) return few ? launch<64, 1, KEYS>(mK, mV, a, st) : launch<64, 2, KEYS>(mK, mV, a, st);
+    return few ? launch<128, 1, KEYS>(mK, mV, a, st) : launch<128, 2, KEYS>(mK, mV, a, st);
 }
+
+}  // namespace
+
+int decode(const Call& c, cudaStream_t st) { return pass<kAllKeys>(c, nullptr, nullptr, st); }
+int decode_own(const Call& c, float* row_o, float2* row_ml, cudaStream_t st) { return pass<kOwnKeys>(c, row_o, row_ml, st); }
 
 }  // namespace attn
 }  // namespace kda

@@ -63,13 +63,13 @@ __device__ __forceinline__ bool fetch(float* dst, const void* src, long long at,
     return fine;
 }
 
-template <int DP, bool VEC>
+template <int DP, bool VEC, int KEYS>
 __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles tiles, int splits, float* part_o, float2* part_ml) {
     extern __shared__ float4 raw[];
     Smem<DP>& sm = *reinterpret_cast<Smem<DP>*>(raw);
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int hk = blockIdx.y, z = blockIdx.z, g = c.heads.group, D = c.heads.dim;
-    const Batch& b = c.batch;
+    const auto& b = view<KEYS>(c);
     dependents_go();
     Unit u;
     if (!make_unit(b, tiles, blockIdx.x, c.window, u)) {
@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = ty + 16 * i;
-        last[i] = r < u.rows ? u.base + (u.row0 + r) / g : -1;
-        first[i] = first_key(last[i], c.window);
+        last[i] = r >= u.rows ? -1 : KEYS == kPrefixKeys ? u.hi - 1 : u.base + (u.row0 + r) / g;
+        first[i] = KEYS == kAllKeys ? first_key(last[i], c.window) : u.from;
         m[i] = -INFINITY;
         l[i] = 0.f;
 #pragma unroll
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
         const int r = ty + 16 * i;
         if (r >= u.rows) continue;
         const size_t row = (size_t)token_of(r) * c.heads.q_heads + head_of(r);
-        if (splits > 1) {
+        if (splits > 1 || KEYS != kAllKeys) {
             const size_t at = (size_t)z * b.tokens * c.heads.q_heads + row;
             if (tx == 0) part_ml[at] = make_float2(m[i], l[i]);
 #pragma unroll
@@ -244,20 +244,29 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
     }
 }
 
-// Joins the parts of a row: a warp a row.
+// Joins the parts of a row: a warp a row.  SHARED: those of the prefix, which come first, only where the row's sequence shares it.
+template <bool SHARED>
 __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
     const long long rows = (long long)c.tokens * c.q_heads;
     const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     dependency_wait();      // in every block: the end of this kernel stands for that of the one before too
     if (row >= rows) return;
+    int z_first = 0;
+    if (SHARED) {
+        const int n = c.batch.seq_of<32>((int)(row / c.q_heads), lane, 0xffffffffu);
+        int first, count;
+        c.batch.OwnView::span(n, first, count);
+        const int prefix = c.batch.prefix_of(n);
+        if (prefix == 0 || c.batch.kv_len(n) - count < prefix) z_first = c.prefix_splits;
+    }
     float m = -INFINITY;
-    for (int z = lane; z < c.splits; z += 32) m = fmaxf(m, ld_after_f32(&c.part_ml[z * rows + row].x));
+    for (int z = z_first + lane; z < c.splits; z += 32) m = fmaxf(m, ld_after_f32(&c.part_ml[z * rows + row].x));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float acc[8] = {}, l = 0.f;
     constexpr int kAhead = 4;
-    for (int z0 = 0; z0 < c.splits; z0 += kAhead) {
+    for (int z0 = z_first; z0 < c.splits; z0 += kAhead) {
         uint2 ml[kAhead];
         float v[kAhead][8];
 #pragma unroll
@@ -286,41 +295,59 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
     }
 }
 
-template <int DP>
+template <int DP, int KEYS>
 int launch(const Call& c, const Tiles& t, dim3 grid, int splits, float* part_o, float2* part_ml, cudaStream_t st) {
     const size_t smem = sizeof(Smem<DP>);
     const Strides& s = c.strides;
     const int unit = c.bf16 ? 8 : 4;      // values in 16 bytes
     const long long all = s.q_token | s.q_head | s.k_page | s.k_row | s.k_head | s.v_page | s.v_row | s.v_head | c.heads.dim;
     const bool vec = all % unit == 0 && (reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % 16 == 0;
-    auto kern = vec ? attn_general_kernel<DP, true> : attn_general_kernel<DP, false>;
+    auto kern = vec ? attn_general_kernel<DP, true, KEYS> : attn_general_kernel<DP, false, KEYS>;
     if (int rc = set_smem_limit(kern, smem)) return rc;
     KDA_LAUNCH("attn_general_kernel", st, kern<<<grid, kThreads, smem, st>>>(c, t, splits, part_o, part_ml));
     return launch_status();
 }
 
-}  // namespace
-
-int combine(const Combine& c, cudaStream_t st) {
+template <int KEYS>
+int pass(const Call& c, int splits, float* part_o, float2* part_ml, cudaStream_t st) {
+    Tiles t{kRows, c.heads.group, 0};
+    const long long slots = KEYS == kPrefixKeys ? group_slots(c.batch, t.group, kRows, t.per_seq)
+                                                : tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, t.group, kRows, c.batch.cu != nullptr, t.per_seq);
+    const dim3 grid((unsigned)slots, (unsigned)c.heads.kv_heads, (unsigned)splits);
+    if (c.heads.dim <= 64) return launch<64, KEYS>(c, t, grid, splits, part_o, part_ml, st);
+    if (c.heads.dim <= 128) return launch<128, KEYS>(c, t, grid, splits, part_o, part_ml, st);
+    return launch<256, KEYS>(c, t, grid, splits, part_o, part_ml, st);
+}
+int combine(const Combine& c, bool shared, cudaStream_t st) {
     const long long rows = (long long)c.tokens * c.q_heads;
     cudaError_t e = cudaSuccess;
-    KDA_LAUNCH("attn_combine_kernel", st, e = launch_early(attn_combine_kernel, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, 1, c));
+    KDA_LAUNCH("attn_combine_kernel", st,
+               e = launch_early(shared ? attn_combine_kernel<true> : attn_combine_kernel<false>, dim3((unsigned)((rows + 3) / 4)), 128, 0, st, true, 1, c));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
+}  // namespace
+
 int general(const Call& c, int splits, cudaStream_t st) {
-    Tiles t{kRows, c.heads.group, 0};
-    const long long slots = tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, t.group, kRows, c.batch.cu != nullptr, t.per_seq);
-    const dim3 grid((unsigned)slots, (unsigned)c.heads.kv_heads, (unsigned)splits);
     const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
     float2* part_ml = static_cast<float2*>(c.workspace);
     float* part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * splits * sizeof(float2), 256));
-    int rc;
-    if (c.heads.dim <= 64) rc = launch<64>(c, t, grid, splits, part_o, part_ml, st);
-    else if (c.heads.dim <= 128) rc = launch<128>(c, t, grid, splits, part_o, part_ml, st);
-    else rc = launch<256>(c, t, grid, splits, part_o, part_ml, st);
+    const int rc = pass<kAllKeys>(c, splits, part_o, part_ml, st);
     if (rc || splits == 1) return rc;
-    return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, splits, part_o, part_ml, c.o, c.lse, c.bf16}, st);
+    return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, splits, part_o, part_ml, c.o, c.lse, c.bf16, 0, c.batch}, false, st);
+}
+
+size_t general_shared_workspace(size_t rows, int parts, int dim) {
+    return align_up(rows * parts * sizeof(float2), 256) + align_up(rows * parts * dim * sizeof(float), 256);
+}
+int general_shared(const Call& c, int prefix_splits, int own_splits, cudaStream_t st) {
+    const size_t rows = (size_t)c.batch.tokens * c.heads.q_heads;
+    const int parts = prefix_splits + own_splits;
+    float2* part_ml = static_cast<float2*>(c.workspace);
+    float* part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up(rows * parts * sizeof(float2), 256));
+    if (int rc = pass<kPrefixKeys>(c, prefix_splits, part_o, part_ml, st)) return rc;
+    if (int rc = pass<kOwnKeys>(c, own_splits, part_o + rows * prefix_splits * c.heads.dim, part_ml + rows * prefix_splits, st)) return rc;
+    return combine(Combine{c.batch.tokens, c.heads.q_heads, c.heads.dim, parts, part_o, part_ml, c.o, c.lse, c.bf16, prefix_splits, c.batch}, true, st);
 }
 
 }  // namespace attn

@@ -114,7 +114,7 @@ struct Range {
     int begin, end;
 };
 
-template <int DP>
+template <int DP, int KEYS>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                               const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mO,
                                                               const __grid_constant__ Args a) {
@@ -129,8 +129,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     volatile int& odd_values = *reinterpret_cast<volatile int*>(bar + 62);
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const Batch& b = a.c.batch;
+    const auto& b = view<KEYS>(a.c);
     const int g = a.c.heads.group, D = a.c.heads.dim, hk = blockIdx.y, z = blockIdx.z, window = a.c.window;
+    if (KEYS != kAllKeys) dependents_go();
     // a sequence's last rows see the most keys: they start first
     const int slot = a.slots - 1 - (int)blockIdx.x;
     Unit u;
@@ -142,12 +143,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (!some) return;
 
     // keys any row of the block sees: [u.lo, u.hi); keys all of them see: [all_lo, all_hi)
-    const int first_pos = u.base + u.row0 / g, last_pos = u.base + (u.row0 + u.rows - 1) / g;
-    const int all_lo = first_key(last_pos, window), all_hi = first_pos + 1;
+    auto last_of = [&](int prow) { return KEYS == kPrefixKeys ? u.hi - 1 : u.base + prow / g; };      // a row's last key, and its first one
+    auto first_of = [&](int last) { return KEYS == kAllKeys ? first_key(last, window) : u.from; };
+    const int first_pos = last_of(u.row0), last_pos = last_of(u.row0 + u.rows - 1);
+    const int all_lo = first_of(last_pos), all_hi = first_pos + 1;
     // Key tiles start at the first box in reach, not at multiples of their size: a window of 1,024 keys and 64 rows is 9 tiles, not 10.
     const int key0 = u.lo / a.box_rows * a.box_rows, nt = max((u.hi - key0 + kKeys - 1) / kKeys, 0);
     int t_begin = 0, t_end = nt;
-    bool split = false;
+    bool split = KEYS != kAllKeys;      // the sums of these passes are joined whatever their number of parts
     if (a.splits > 1) {
         // The shortest parts with which all blocks run side by side, looked for by one length a warp, twice; none where they would be
         // little shorter than the longest row tile's keys (a part costs some 5 tiles of its own, and the join).  The host sees to it
@@ -179,15 +182,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int part = 4 * hi > 3 * longest ? longest : hi, parts = min(max((nt + part - 1) / part, 1), a.splits);
         if (z >= parts) return;
         fence_async_smem();      // the list's place is written by copies next
-        split = parts > 1;
+        split |= parts > 1;
         t_begin = nt * z / parts;
         t_end = nt * (z + 1) / parts;
         if (z == 0 && tid == 0) a.parts[slot * a.c.heads.kv_heads + hk] = parts;
+    } else if (KEYS != kAllKeys && tid == 0) {
+        a.parts[slot * a.c.heads.kv_heads + hk] = 1;
     }
     auto range_of = [&](int t) {      // key tiles of row tile t
         const int r0 = u.row0 + 128 * t, r1 = min(r0 + 128, u.row0 + u.rows) - 1;
         if (r0 > r1) return Range{0, 0};
-        const int hi = u.base + r1 / g + 1, lo = first_key(u.base + r0 / g, window);
+        const int hi = last_of(r1) + 1, lo = first_of(last_of(r0));
         Range r{max(t_begin, (lo - key0) / kKeys), min(t_end, (max(hi - key0, 0) + kKeys - 1) / kKeys)};
         if (r.end < r.begin) r.end = r.begin;
         return r;
@@ -259,8 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lanes + cS + 128 * t, tO = tmem + lanes + cO + DP * t;
         const int row = 128 * t + (tid & 127), prow = u.row0 + row;
-        const int last = row < u.rows ? u.base + prow / g : last_pos;      // rows behind the last one compute along, unseen
-        const int first = first_key(last, window);
+        const int last = row < u.rows ? last_of(prow) : last_pos;      // rows behind the last one compute along, unseen
+        const int first = first_of(last);
         // keys all rows of the warp see
         const int w_lo = __reduce_max_sync(0xffffffffu, first), w_hi = __reduce_min_sync(0xffffffffu, last) + 1;
         const float c = a.c.scale * 1.4426950408889634f, lazy = kLazy / c;
@@ -698,13 +703,131 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
     }
 }
 
+struct SharedJoin {
+    Args prefix, own;       // `own` without row_o
+    const float* row_o;     // [tokens * q_heads][D] and (maximum, sum) of each row, or null
+    const float2* row_ml;
+};
+// Joins the parts of the prefix and of the own keys, 32 rows a block: a warp four of them, eight lanes a row.
 template <int DP>
+__global__ void __launch_bounds__(256) attn_shared_join_kernel(const __grid_constant__ SharedJoin j) {
+    const GroupView& groups = j.prefix.c.batch;
+    const OwnView& b = groups;
+    const int g = j.prefix.c.heads.group, D = j.prefix.c.heads.dim, Hk = j.prefix.c.heads.kv_heads, Hq = j.prefix.c.heads.q_heads;
+    const int lane = threadIdx.x & 31, l8 = lane & 7;
+    const long long rows = (long long)b.tokens * Hq, at = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
+    const bool is = at < rows;
+    const size_t row = (size_t)(is ? at : rows - 1);
+    const int tok = (int)(row / Hq), head = (int)(row - (size_t)tok * Hq), hk = head / g;
+    const int n = b.seq_of<8>(tok, l8, 0xffu << (lane & 24));
+    int first, count;
+    b.Batch::span(n, first, count);
+    const int base = b.kv_len(n) - count, group = b.group_of(n), prefix = group < 0 ? 0 : b.prefix_len(group);
+    const bool inside = tok >= first && tok < first + count, shares = inside && prefix > 0 && base >= prefix;
+    // Where a pass over sequences (or groups) that start at token `from` has this row.
+    struct Place {
+        int slot, row;
+    };
+    auto place_in = [&](const Args& a, int start, int from) {
+        const long long r = (long long)(tok - from) * g + (head - hk * g);
+        return Place{start + (int)(r / kRows), (int)(r % kRows)};
+    };
+    Place of_prefix{0, 0}, of_own{0, 0};
+    int n_prefix = 0, n_own = inside ? 1 : 0;
+    if (shares) of_prefix = place_in(j.prefix, j.prefix.tiles.start(groups, group), groups.edge(group));
+    if (inside && j.row_o == nullptr) of_own = place_in(j.own, j.own.tiles.start(b, n), first);
+    dependency_wait();
+    // what the device arrays say is not trusted as an index
+    auto parts_of = [&](const Args& a, const Place& p) {
+        if ((unsigned)p.slot >= (unsigned)a.slots || p.row < 0) return 0;
+        const int parts = __float_as_int(ld_after_f32(reinterpret_cast<const float*>(a.parts + p.slot * Hk + hk)));
+        return min(max(parts, 0), a.splits);
+    };
+    if (shares) n_prefix = parts_of(j.prefix, of_prefix);
+    if (inside && j.row_o == nullptr) n_own = parts_of(j.own, of_own);
+    const int parts = n_prefix + n_own;
+    auto part_at = [&](int k, const Args*& a, const Place*& p, int& z) {
+        const bool of = k < n_prefix;
+        a = of ? &j.prefix : &j.own;
+        p = of ? &of_prefix : &of_own;
+        z = of ? k : k - n_prefix;
+    };
+    auto ml_at = [&](int k) -> const float2* {
+        if (k >= n_prefix && j.row_o != nullptr) return j.row_ml + row;
+        const Args* a;
+        const Place* p;
+        int z;
+        part_at(k, a, p, z);
+        return a->part_ml + (((size_t)z * a->slots + p->slot) * Hk + hk) * kRows + p->row;
+    };
+    float m = -INFINITY, l = 0.f;
+    for (int k = l8; k < parts; k += 8) m = max_nan(m, ld_after_f32(&ml_at(k)->x));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffu << (lane & 24), m, o));
+    constexpr int kPieces = DP / 32, kAhead = 4;      // pieces of four values a lane: l8, l8 + 8, ... of the row's; parts on their way
+    f2 acc[kPieces][2];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) acc[i][0] = acc[i][1] = f2_all(0.f);
+    for (int k0 = 0; k0 < parts; k0 += kAhead) {
+        uint2 ml[kAhead];
+        uint4 v[kAhead][kPieces];
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            const int k = min(k0 + x, parts - 1);
+            ml[x] = ld_after8(ml_at(k));
+            if (k >= n_prefix && j.row_o != nullptr) {
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    const int d = 4 * (l8 + 8 * i);
+                    // a row without a key has no sums there
+                    v[x][i] = d < D && __uint_as_float(ml[x].x) != -INFINITY ? ld_after16(j.row_o + row * D + d) : make_uint4(0, 0, 0, 0);
+                }
+                continue;
+            }
+            const Args* a;
+            const Place* p;
+            int z;
+            part_at(k, a, p, z);
+            const size_t part = ((size_t)z * a->slots + p->slot) * Hk + hk;
+            const char* src = reinterpret_cast<const char*>(a->part_o + (part * 2 + (p->row >> 7)) * (128 * DP));
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int piece = l8 + 8 * i, half = piece / (DP / 8), c = piece % (DP / 8);
+                v[x][i] = ld_after16(src + half * (128 * DP * 2) + part_off<DP>(p->row & 127, c));
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < kAhead; ++x) {
+            const float top = __uint_as_float(ml[x].x);
+            if (k0 + x >= parts || top == -INFINITY) continue;      // without a key its sums are 0
+            const float f = ex2(top - m);
+            l = fmaf(__uint_as_float(ml[x].y), f, l);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                acc[i][0] = f2_fma(f2_make(__uint_as_float(v[x][i].x), __uint_as_float(v[x][i].y)), f2_all(f), acc[i][0]);
+                acc[i][1] = f2_fma(f2_make(__uint_as_float(v[x][i].z), __uint_as_float(v[x][i].w)), f2_all(f), acc[i][1]);
+            }
+        }
+    }
+    if (!is || !inside) return;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    if (l8 == 0 && j.prefix.c.lse != nullptr) j.prefix.c.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int d = 4 * (l8 + 8 * i);
+        if (d < D)
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(j.prefix.c.o) + row * D + d) =
+                make_uint2(f2_to_bf16(f2_mul(acc[i][0], f2_all(inv))), f2_to_bf16(f2_mul(acc[i][1], f2_all(inv))));
+    }
+}
+
+template <int DP, int KEYS>
 int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CUtensorMap& mQ, const CUtensorMap& mO, const Args& a, cudaStream_t st) {
-    if (int rc = set_smem_limit(attn_tc_kernel<DP>, Layout<DP>::kBytes)) return rc;
+    if (int rc = set_smem_limit(attn_tc_kernel<DP, KEYS>, Layout<DP>::kBytes)) return rc;
     const dim3 grid((unsigned)a.slots, (unsigned)c.heads.kv_heads, (unsigned)a.splits);
-    KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
+    KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP, KEYS><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
     if (int rc = launch_status()) return rc;
-    if (a.splits == 1) return KDA_OK;
+    if (a.splits == 1 || KEYS != kAllKeys) return KDA_OK;
     const dim3 joins((unsigned)a.slots * 8, (unsigned)c.heads.kv_heads);
     KDA_LAUNCH("attn_tc_join_kernel", st, attn_tc_join_kernel<DP><<<joins, 256, 0, st>>>(a));
     return launch_status();
@@ -727,23 +850,35 @@ bool tc_takes(const Call& c) {
     return true;
 }
 
-int tc(const Call& c, int splits, cudaStream_t st) {
+namespace {
+
+// Where a pass has its parts in its share of the workspace.
+void place_parts(Args& a, const Call& c) {
+    const size_t units = (size_t)a.slots * c.heads.kv_heads;
+    char* ws = static_cast<char*>(c.workspace);
+    a.parts = reinterpret_cast<int*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(ws + align_up(units * sizeof(int), 256));
+    a.part_o = reinterpret_cast<float*>(a.part_ml + units * a.splits * kRows);
+}
+Args args_of(const Call& c, int keys, int splits) {
     Args a;
     a.c = c;
     a.tiles = Tiles{kRows, c.heads.group, 0};
-    a.slots = (int)tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq);
+    a.slots = (int)(keys == kPrefixKeys ? group_slots(c.batch, c.heads.group, kRows, a.tiles.per_seq)
+                                        : tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq));
     a.splits = splits;
     a.box_rows = c.batch.page_size < kKeys ? c.batch.page_size : kKeys;
+    a.q_boxes = 0;
     a.parts = nullptr;
     a.part_ml = nullptr;
     a.part_o = nullptr;
-    if (splits > 1) {
-        const size_t units = (size_t)a.slots * c.heads.kv_heads;
-        char* ws = static_cast<char*>(c.workspace);
-        a.parts = reinterpret_cast<int*>(ws);
-        a.part_ml = reinterpret_cast<float2*>(ws + align_up(units * sizeof(int), 256));
-        a.part_o = reinterpret_cast<float*>(a.part_ml + units * splits * kRows);
-    }
+    if (splits > 1 || keys != kAllKeys) place_parts(a, c);
+    return a;
+}
+
+template <int KEYS>
+int pass(const Call& c, int splits, cudaStream_t st) {
+    Args a = args_of(c, KEYS, splits);
     CUtensorMap mK, mV, mQ, mO;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
@@ -751,15 +886,37 @@ int tc(const Call& c, int splits, cudaStream_t st) {
     mQ = mO = mK;
     a.q_boxes = 128 % c.heads.group == 0 && s.q_head > 0 && s.q_token > 0 && s.q_head < 1ll << 39 && s.q_token < 1ll << 39;
     if (!rc && a.q_boxes) rc = make_map_packed(&mQ, c.q, c.heads.dim, c.heads.q_heads, c.batch.tokens, s.q_head, s.q_token, c.heads.group, 128 / c.heads.group);
-    if (!rc && a.q_boxes)
+    if (!rc && a.q_boxes && KEYS == kAllKeys)
         rc = make_map_packed(&mO, c.o, c.heads.dim, c.heads.q_heads, c.batch.tokens, c.heads.dim, (int64_t)c.heads.q_heads * c.heads.dim, c.heads.group, 128 / c.heads.group);
-    if (!rc) rc = c.heads.dim <= 64 ? launch<64>(c, mK, mV, mQ, mO, a, st) : launch<128>(c, mK, mV, mQ, mO, a, st);
+    if (!rc) rc = c.heads.dim <= 64 ? launch<64, KEYS>(c, mK, mV, mQ, mO, a, st) : launch<128, KEYS>(c, mK, mV, mQ, mO, a, st);
     return rc;
+}
+
+}  // namespace
+
+int tc(const Call& c, int splits, cudaStream_t st) { return pass<kAllKeys>(c, splits, st); }
+int tc_prefix(const Call& c, int splits, cudaStream_t st) { return pass<kPrefixKeys>(c, splits, st); }
+int tc_own(const Call& c, int splits, cudaStream_t st) { return pass<kOwnKeys>(c, splits, st); }
+
+int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const float* row_o, const float2* row_ml, cudaStream_t st) {
+    SharedJoin j;
+    j.prefix = args_of(prefix, kPrefixKeys, prefix_splits);
+    j.own = row_o == nullptr ? args_of(own, kOwnKeys, own_splits) : j.prefix;
+    j.row_o = row_o;
+    j.row_ml = row_ml;
+    const long long rows = (long long)prefix.batch.tokens * prefix.heads.q_heads;
+    auto kern = prefix.heads.dim <= 64 ? attn_shared_join_kernel<64> : attn_shared_join_kernel<128>;
+    cudaError_t e = cudaSuccess;
+    KDA_LAUNCH("attn_shared_join_kernel", st, e = launch_early(kern, dim3((unsigned)((rows + 31) / 32)), 256, 0, st, true, 1, j));
+    return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 // of a call whose rows are cut into `splits` parts at most
 size_t tc_workspace(long long slots, int kv_heads, int splits, int dim) {
     if (splits < 2) return 0;
+    return tc_parts_bytes(slots, kv_heads, splits, dim);
+}
+size_t tc_parts_bytes(long long slots, int kv_heads, int splits, int dim) {
     const size_t units = (size_t)slots * kv_heads, width = dim <= 64 ? 64 : 128;
     return align_up(units * sizeof(int), 256) + units * splits * kRows * (sizeof(float2) + width * sizeof(float));
 }

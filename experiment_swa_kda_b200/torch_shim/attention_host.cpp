@@ -251,6 +251,43 @@ AttentionOut attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
     return std::make_tuple(o, lse);
 }
 
+AttentionOut shared_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const Tensor& prefix_table,
+                              const Tensor& prefix_lens, const OptTensor& groups, const OptTensor& cu, int64_t max_q, c10::optional<double> scale, bool want_lse) {
+    KdaPagedShape pg;
+    if (tracing() || !paged_shape(q_, kc, vc, table, lens, cu, max_q, 0, pg)) return c10::nullopt;
+    if (prefix_table.dim() != 2 || prefix_table.scalar_type() != at::kInt || !on(prefix_table, q_)) return c10::nullopt;
+    const int64_t G = prefix_table.size(0), width = prefix_table.size(1);
+    if (G < 1 || G > pg.n_seq || width > kInt / pg.page_size || (width > 1 && prefix_table.stride(1) != 1)) return c10::nullopt;
+    if (prefix_lens.dim() != 1 || prefix_lens.numel() != G || prefix_lens.scalar_type() != at::kInt || !on(prefix_lens, q_) || !prefix_lens.is_contiguous())
+        return c10::nullopt;
+    if (has(groups)) {
+        if (groups->dim() != 1 || groups->numel() != G + 1 || groups->scalar_type() != at::kInt || !on(*groups, q_) || !groups->is_contiguous()) return c10::nullopt;
+    } else if (pg.n_seq % G != 0) {
+        return c10::nullopt;
+    }
+    if (at::GradMode::is_enabled() && (q_.requires_grad() || kc.requires_grad() || vc.requires_grad())) return c10::nullopt;
+    pg.scale = scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)pg.head_dim));
+    if (!(pg.scale > 0.f) || !std::isfinite(pg.scale)) return c10::nullopt;
+    refuse_tangents(q_, kc, vc);
+    c10::cuda::CUDAGuard guard(q_.device());
+    watch_status(q_.device().index());
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor q = wide(q_);
+    pg.q_token_stride = q.stride(0), pg.q_head_stride = q.stride(1);
+    KdaPrefixShape px = {};
+    px.n_groups = (int32_t)G, px.table_width = (int32_t)width, px.table_stride = prefix_table.stride(0);
+    Tensor o = empty(q.sizes(), q.scalar_type(), q), ws;
+    OptTensor lse;
+    if (want_lse) lse = empty({q.size(0), q.size(1)}, at::kFloat, q);
+    const size_t need = kda_shared_prefix_attention_workspace_bytes(&pg, &px);
+    ws = bytes(need, q);
+    must(kda_shared_prefix_attention(&pg, &px, q.const_data_ptr(), kc.const_data_ptr(), vc.const_data_ptr(), table.const_data_ptr<int32_t>(),
+                                     lens.const_data_ptr<int32_t>(), iptr(cu), prefix_table.const_data_ptr<int32_t>(), prefix_lens.const_data_ptr<int32_t>(),
+                                     iptr(groups), o.data_ptr(), want_lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr(), need, stream_of(q)),
+         "kda_shared_prefix_attention");
+    return std::make_tuple(o, lse);
+}
+
 // ------------------------------------------------------------------------------------------------ pages of a step
 
 using PlanOut = c10::optional<std::tuple<Tensor, Tensor, Tensor>>;
@@ -291,6 +328,7 @@ void bind_attention(pybind11::module_& m) {
     m.def("norm_rope", &norm_rope, nogil());
     m.def("append", &append, nogil());
     m.def("attention", &attention, nogil());
+    m.def("shared_attention", &shared_attention, nogil());
     m.def("plan", &plan, nogil());
 }
 

@@ -422,6 +422,22 @@ int kda_paged_attention(const KdaPagedShape* shape, const void* q, const void* k
                         const int32_t* kv_lens, const int32_t* cu_seqlens, void* o, float* lse, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* The same for sequences that start with a common text, whose keys and values lie in the cache once and are read once for all of them.
+ * Sequences cu_groups[g] .. cu_groups[g + 1] - 1 (device int32 [n_groups + 1]; NULL: n_seq / n_groups each) share the prefix_lens[g] tokens in
+ * the pages prefix_table[g] [n_groups, table_width], rows table_stride apart.  kv_lens count the prefix too, and a sequence whose new tokens
+ * all lie behind it finds its own keys, from position prefix_lens[g] on, through its row of block_table, whose columns before that are not
+ * looked at; one whose new tokens do not (padding, a shorter text), or that is in no group, has all of its keys there.  shape->window is 0.
+ * No counterpart in the reference. */
+typedef struct KdaPrefixShape {
+    int32_t n_groups, table_width;
+    int64_t table_stride;
+} KdaPrefixShape;
+size_t kda_shared_prefix_attention_workspace_bytes(const KdaPagedShape* shape, const KdaPrefixShape* prefix);
+int kda_shared_prefix_attention(const KdaPagedShape* shape, const KdaPrefixShape* prefix, const void* q, const void* k_cache, const void* v_cache,
+                                const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, const int32_t* prefix_table,
+                                const int32_t* prefix_lens, const int32_t* cu_groups, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
 /* Pages of such a cache dealt out and the slots of new tokens mapped, from the lengths of a step's requests; no counterpart in the
  * reference.  Row n of block_table [rows, width] (rows table_stride >= width apart) is to hold columns [starts[n] / page_size,
  * ceil(kv_lens[n] / page_size)), starts clamped to the length (NULL: 0).  Entries outside go back to the pool (entry -1, page_free[page] = 1);

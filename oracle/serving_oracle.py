@@ -54,3 +54,35 @@ def plan_pages(table, kv_lens, page_free, new_lens, page_size, max_tokens, start
                 table[n][c] = -1
     rest = [-1] * (max_tokens - len(positions))
     return table, kv_lens, page_free, cu, positions + rest, slots + rest
+
+
+def shared_prefix_attention(q, k_cache, v_cache, table, kv_lens, q_lens, prefix_table, prefix_lens, cu_groups, scale=None):
+    """(o, lse, A) in float64 with A = sum_j p_j |v_j|, the scale of what rounding the weights can change."""
+    heads, dim = q.shape[1:]
+    group, page = heads // k_cache.shape[2], k_cache.shape[1]
+    scale = dim ** -0.5 if scale is None else scale
+    o, size = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(2))
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+    t = 0
+    for n, (count, length) in enumerate(zip(q_lens, kv_lens)):
+        shared = 0
+        for g, (a, b) in enumerate(zip(cu_groups, cu_groups[1:])):
+            if a <= n < b and length - count >= prefix_lens[g]:
+                shared, of = prefix_lens[g], prefix_table[g]
+        at = torch.arange(max(length, 0))
+        pages = torch.tensor([int(of[p // page]) if p < shared else int(table[n][p // page]) for p in at.tolist()], dtype=torch.long)
+        k, v = (c[pages, at % page].double().repeat_interleave(group, 1) for c in (k_cache, v_cache))
+        for i in range(count):
+            pos = length - count + i
+            if pos >= 0:
+                logits = torch.einsum("hd,khd->hk", q[t].double(), k[:pos + 1]) * scale
+                top = logits.amax(-1, keepdim=True)
+                p = torch.exp(logits - top)
+                total = p.sum(-1, keepdim=True)
+                p = p / total
+                seen = v[:pos + 1]
+                o[t] = torch.einsum("hk,khd->hd", p, seen)
+                size[t] = torch.einsum("hk,khd->hd", p, seen.abs())
+                lse[t] = (top + total.log())[:, 0]
+            t += 1
+    return o, lse, size

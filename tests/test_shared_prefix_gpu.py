@@ -1,0 +1,299 @@
+"""Attention behind a shared prefix against a float64 restatement (oracle/serving_oracle.py).
+
+Bounds, as for paged attention.  float32: 1e-5 of the relative 2-norm.  bfloat16 (unit roundoff u = 2^-8): one rounding of the
+result, |err| <= u |y|; the softmax weights are rounded too, which moves o by at most u sum_j p_j |v_j|, and the sum they are divided
+by as much again; 2^-12 of that scale covers float32 and second-order terms.  The log of the sums has no such rounding: 1e-4 absolute
+(sums of float32 products of 128 bf16 values, a few units of 2^-24 of scores below 100)."""
+
+import math
+
+import pytest
+import torch
+
+import serving_oracle as S
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U = 2.0 ** -8
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def close(got, want, size, dtype):
+    got = got.detach().double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
+    fine = torch.isfinite(want)
+    got, want, size = got[fine], want[fine], size[fine]
+    if dtype == F32:
+        assert (got - want).norm() <= 1e-5 * want.norm() + 1e-30
+        return
+    room = U * want.abs() + (2 * U + 2.0 ** -12) * size + 1e-30
+    assert bool(((got - want).abs() <= room).all()), float(((got - want).abs() - room).max())
+
+
+class Batch:
+    """Sequences of groups, with garbage wherever nothing may be read."""
+
+    def __init__(self, heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, seed=0, garbage=float("nan"), layout="dense", shares=None):
+        """own[n]: tokens behind the prefix (the new ones among them); shares[n] false: own[n] tokens in all, none of them shared."""
+        gen = torch.Generator().manual_seed(seed)
+        n = len(q_lens)
+        group = [next((g for g in range(len(prefix)) if cu_groups[g] <= i < cu_groups[g + 1]), None) for i in range(n)]
+        shares = [True] * n if shares is None else shares
+        base = [prefix[g] if g is not None and s else 0 for g, s in zip(group, shares)]
+        self.kv_lens = [b + o for b, o in zip(base, own)]
+        self.q_lens, self.prefix, self.cu_groups, self.dtype = list(q_lens), list(prefix), list(cu_groups), dtype
+        width = max(1, max(-(-x // page) for x in self.kv_lens)) + 1
+        pw = max(1, max(-(-x // page) for x in prefix))
+        need = sum(max(0, -(-x // page) - b // page) for x, b in zip(self.kv_lens, base)) + sum(-(-x // page) for x in prefix)
+        pages = need + 3
+        order = torch.randperm(pages, generator=gen).tolist()
+        bad = 2 ** 31 - 1
+        self.table = torch.full((n, width), bad, dtype=torch.int32)
+        self.prefix_table = torch.full((len(prefix), pw), -5, dtype=torch.int32)
+        self.k, self.v = (torch.full((pages, page, kv_heads, dim), garbage) for _ in range(2))
+
+        def put(row, lo, hi):
+            for col in range(lo // page, -(-hi // page)):
+                row[col] = order.pop()
+                a, b = max(lo - col * page, 0), min(hi - col * page, page)
+                for c in (self.k, self.v):
+                    c[row[col], a:b] = torch.randn(b - a, kv_heads, dim, generator=gen)
+        for g, x in enumerate(prefix):
+            put(self.prefix_table[g], 0, x)
+        for i in range(n):
+            put(self.table[i], base[i], self.kv_lens[i])
+        self.k, self.v = self.k.to(dtype), self.v.to(dtype)
+        self.q = (1.5 * torch.randn(sum(q_lens), heads, dim, generator=gen)).to(dtype)
+        self.layout = layout
+
+    def device(self):
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+        q, k, v, table, ptable = (t.to(DEV) for t in (self.q, self.k, self.v, self.table, self.prefix_table))
+        if self.layout == "strided":      # slices of larger buffers: one projection's q, k beside v, columns of wider tables
+            wide = torch.empty(q.shape[0], q.shape[1] + 3, q.shape[2], dtype=q.dtype, device=DEV)
+            wide[:, 1:1 + q.shape[1]] = q
+            q = wide[:, 1:1 + q.shape[1]]
+            both = torch.stack((k, v), 2).contiguous()
+            k, v = both[:, :, 0], both[:, :, 1]
+            table = torch.cat((torch.full_like(table, 7), table), 1)[:, table.shape[1]:]
+            ptable = torch.cat((ptable, ptable), 1)[:, :ptable.shape[1]]
+        return [q, k, v, table, i32(self.kv_lens), ptable, i32(self.prefix), i32(self.cu_groups), i32([0] + self.q_lens).cumsum(0).to(torch.int32)]
+
+    def want(self, scale=None):
+        return S.shared_prefix_attention(self.q, self.k, self.v, self.table, self.kv_lens, self.q_lens, self.prefix_table, self.prefix, self.cu_groups, scale)
+
+    def check(self, out, lse=None, scale=None):
+        o, want_lse, size = self.want(scale)
+        close(out, o, size, self.dtype)
+        if lse is not None:
+            lse = lse.double().cpu()
+            assert torch.equal(torch.isinf(lse), torch.isinf(want_lse)) and not bool(torch.isnan(lse).any())
+            fine = torch.isfinite(want_lse)
+            assert bool(((lse - want_lse).abs()[fine] <= 1e-4).all())
+
+
+CASES = [  # heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups
+    (3, 3, 128, 16, BF16, [1], [1], [1], [0, 1]),
+    (3, 3, 128, 16, BF16, [1] * 5, [1, 2, 17, 300, 16], [129], [0, 5]),
+    (16, 4, 128, 64, BF16, [1] * 9, [5, 64, 65, 1, 127, 128, 1, 1000, 2], [1000], [0, 9]),
+    (16, 16, 128, 16, BF16, [1] * 3, [33, 1, 8], [2049], [0, 3]),
+    (16, 1, 128, 32, BF16, [1] * 20, list(range(1, 21)), [700], [0, 20]),
+    (8, 1, 64, 128, BF16, [2] * 6, [2, 3, 70, 129, 4, 5], [257], [0, 6]),
+    (6, 2, 96, 16, BF16, [5] * 4, [5, 9, 100, 6], [333], [0, 4]),
+    (4, 2, 64, 8, BF16, [7, 1, 30, 1], [7, 40, 30, 1], [100, 5], [0, 2, 4]),
+    (12, 4, 64, 16, BF16, [1] * 23, [(7 * i) % 40 + 1 for i in range(23)], [64, 1, 200, 15], [0, 10, 11, 20, 23]),
+    (16, 4, 128, 64, BF16, [100, 33, 260], [130, 33, 261], [515], [0, 3]),
+    (5, 1, 128, 64, BF16, [90, 1, 17], [100, 1, 20], [130], [0, 3]),
+    (4, 2, 8, 16, BF16, [1, 3], [4, 3], [31], [0, 2]),
+    (4, 4, 128, 48, BF16, [1, 9, 2], [50, 9, 3], [97], [0, 3]),
+    (2, 1, 200, 16, BF16, [1, 20], [10, 20], [70], [0, 2]),
+    (4, 2, 64, 16, F32, [1, 33, 2], [5, 50, 3], [190], [0, 3]),
+    (3, 3, 128, 16, F32, [1] * 7, [1, 9, 70, 3, 3, 3, 200], [300, 17], [0, 4, 7]),
+    (2, 1, 50, 5, F32, [3, 1], [3, 2], [12], [0, 2]),
+    (4, 1, 256, 16, F32, [1, 2], [1, 40], [65], [0, 2]),
+]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,q_lens,own,prefix,cu_groups", CASES)
+@pytest.mark.parametrize("bound", [True, False])
+def test_against_the_restatement(heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, bound):
+    import experiment_swa_kda_b200 as m
+    b = Batch(heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, layout="strided" if bound else "dense")
+    o, lse = m.shared_prefix_attention(*b.device(), max_q_len=max(q_lens) if bound else 0, return_lse=True)
+    b.check(o, lse)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q", [1, 3, 40])
+def test_sequences_that_do_not_share(dtype, q):
+    """Places without a request, texts shorter than the prefix, sequences of no group, a group without sequences, a prefix of nothing."""
+    import experiment_swa_kda_b200 as m
+    n = 13
+    own = [(11 * i) % 60 + q for i in range(n)]
+    shares = [True] * n
+    own[1], shares[1] = 0, False            # padding only
+    own[4], shares[4] = max(q - 1, 0), False      # padding first, then tokens (q = 1: padding only)
+    own[6], shares[6] = 20 + q, False       # shorter than its group's prefix
+    own[9], shares[9] = 49 + q, False       # the prefix would begin behind its first new token
+    b = Batch(4, 2, 64, 16, dtype, [q] * n, own, [50, 50, 0], [2, 8, 8, 12], shares=shares)
+    for max_q in (q, 0):
+        o, lse = m.shared_prefix_attention(*b.device(), max_q_len=max_q, return_lse=True)
+        b.check(o, lse)
+
+
+def test_equal_groups_and_lengths_without_their_tables():
+    import experiment_swa_kda_b200 as m
+    for q in (1, 6):
+        b = Batch(8, 2, 128, 16, BF16, [q] * 6, [q, q + 1, 40, 9, 8, 100], [77, 128, 200], [0, 2, 4, 6])
+        args = b.device()
+        args[7] = args[8] = None
+        o, lse = m.shared_prefix_attention(*args, return_lse=True, scale=0.2)
+        b.check(o, lse, scale=0.2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("q", [1, 24])
+def test_values_that_are_not_finite(dtype, q):
+    """Infinite and undefined values at keys that are seen, in the prefix and behind it; scores of -inf throughout."""
+    import experiment_swa_kda_b200 as m
+    for where in ("prefix_v", "prefix_k", "own_v", "last_v", "minus"):
+        b = Batch(4, 2, 64, 16, dtype, [q] * 5, [q + 3, q, 30 + q, 2 + q, q], [150], [0, 5], seed=3)
+        page = 16
+        at = {"prefix_v": (int(b.prefix_table[0, 3]), 5), "prefix_k": (int(b.prefix_table[0, 9]), 2), "own_v": (int(b.table[2, (160) // page]), 160 % page),
+              "last_v": (int(b.table[0, (b.kv_lens[0] - 1) // page]), (b.kv_lens[0] - 1) % page)}.get(where)
+        if where == "minus":      # every key of the prefix and of sequence 0's first own key scores -inf against row 0
+            b.q[0] = 1.0
+            for p in range(150):
+                b.k[int(b.prefix_table[0, p // page]), p % page] = -math.inf
+            for p in range(150, b.kv_lens[0]):
+                b.k[int(b.table[0, p // page]), p % page] = -math.inf
+        elif where == "prefix_k":
+            b.k[at[0], at[1], 1] = math.nan
+        else:
+            b.v[at[0], at[1], 0, 7], b.v[at[0], at[1], 1, 3], b.v[at[0], at[1], 1, 4] = math.inf, -math.inf, math.nan
+        o = m.shared_prefix_attention(*b.device(), max_q_len=q)
+        want, _, size = b.want()
+        if where == "minus":
+            # rows other than the first have scores of both signs and infinities: NaN in both, as the formula says
+            assert bool(torch.isnan(want[0]).all()) and bool(torch.isnan(o[0]).all())
+            continue
+        close(o, want, size, dtype)
+
+
+def test_equals_paged_attention_where_rows_hold_the_prefix():
+    """Tables whose rows name the prefix's pages themselves: both operators say the same up to rounding."""
+    import experiment_swa_kda_b200 as m
+    b = Batch(16, 4, 128, 64, BF16, [1] * 40, [(37 * i) % 500 + 1 for i in range(40)], [1024], [0, 40])
+    args = b.device()
+    table = args[3].clone()
+    table[:, :16] = args[5][0, :16]
+    one, lse1 = m.shared_prefix_attention(*args, max_q_len=1, return_lse=True)
+    two, lse2 = m.paged_attention(args[0], args[1], args[2], table, args[4], args[8], max_q_len=1, return_lse=True)
+    assert (lse1 - lse2).abs().max() <= 1e-4
+    # one rounding each, and the weights' of the tensor-core kernel
+    assert (one.double() - two.double()).norm() <= 3 * U * two.double().norm()
+
+
+def test_inconsistent_arrays_are_bounded_and_told():
+    import experiment_swa_kda_b200 as m
+    fine = Batch(4, 2, 64, 16, BF16, [1] * 4, [3, 4, 5, 6], [40], [0, 4])
+    for dtype in (BF16, F32):
+        for at, bad, match in ((7, [0, 9], "cu_seqlens"), (7, [3, 1], "cu_seqlens|block table"), (7, [-2, 4], "cu_seqlens"), (6, [-1], "block table"), (6, [10 ** 6], "block table"),
+                               (8, [0, 1, 2, 9, 4], "cu_seqlens"), (8, [0, 1, 2, 3, 3], "cu_seqlens"), (4, [43, 10 ** 6, 45, 46], "block table"),
+                               (5, [[-1, 99, -7]], "block table")):
+            args = Batch(4, 2, 64, 16, dtype, [1] * 4, [3, 4, 5, 6], [40], [0, 4], garbage=0.0).device()
+            args[at] = torch.tensor(bad, dtype=torch.int32, device=DEV)
+            for max_q in (1, 0):
+                m.shared_prefix_attention(*args, max_q_len=max_q)
+                torch.cuda.synchronize()
+                with pytest.raises(RuntimeError, match=match):
+                    m.shared_prefix_attention(*fine.device(), max_q_len=1)
+    o = m.shared_prefix_attention(*fine.device(), max_q_len=1)
+    fine.check(o)
+
+
+def test_captured_on_another_stream_and_two_graphs_at_once():
+    import experiment_swa_kda_b200 as m
+    batches = [Batch(16, 4, 128, 16, BF16, [q] * 12, [(13 * i) % 90 + q for i in range(12)], [600], [0, 12], seed=q) for q in (1, 6)]
+    args = [b.device() for b in batches]
+    wants = [m.shared_prefix_attention(*a, max_q_len=q) for a, q in zip(args, (1, 6))]
+    for b, w in zip(batches, wants):
+        b.check(w)
+    graphs, outs = [], []
+    for a, q in zip(args, (1, 6)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(m.shared_prefix_attention(*a, max_q_len=q))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, wants):
+        assert torch.equal(o, w)
+    # the device arrays are followed: two tokens fewer in one sequence
+    args[0][4][3] -= 2
+    batches[0].kv_lens[3] -= 2
+    graphs[0].replay()
+    batches[0].check(outs[0])
+
+
+def test_refusals():
+    import experiment_swa_kda_b200 as m
+    b = Batch(4, 2, 64, 16, BF16, [1] * 4, [3, 4, 5, 6], [40], [0, 4])
+    for at, bad, match in ((5, torch.zeros(1, 3, device=DEV), "prefix_table"), (5, torch.zeros(5, 3, dtype=torch.int32, device=DEV), "prefix_table"),
+                           (6, torch.zeros(2, dtype=torch.int32, device=DEV), "prefix_lens"), (7, torch.zeros(3, dtype=torch.int32, device=DEV), "cu_groups"),
+                           (6, torch.zeros(1, dtype=torch.int32), "CPU"), (5, torch.zeros(1, 6, dtype=torch.int32, device=DEV)[:, ::2], "adjacent")):
+        args = b.device()
+        args[at] = bad
+        with pytest.raises((ValueError, RuntimeError), match=match):
+            m.shared_prefix_attention(*args, max_q_len=1)
+    args = b.device()
+    with pytest.raises(ValueError, match="scale"):
+        m.shared_prefix_attention(*args, scale=0.0)
+    with pytest.raises(ValueError, match="max_q_len"):
+        m.shared_prefix_attention(*args, max_q_len=-1)
+    args[5], args[6], args[7] = (torch.zeros(3, 3, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV), None)
+    with pytest.raises(ValueError, match="cu_groups"):
+        m.shared_prefix_attention(*args)
+    args = b.device()
+    args[0] = args[0].requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference"):
+        m.shared_prefix_attention(*args)
+    args[0] = args[0].detach()[:0]
+    args[8] = torch.zeros(5, dtype=torch.int32, device=DEV)
+    assert m.shared_prefix_attention(*args).shape == (0, 4, 64)
+
+
+def test_serving_with_a_pool_and_a_prefix():
+    """A step as a scheduler makes it: pages are planned, keys and values appended, attention reads the prefix once."""
+    import experiment_swa_kda_b200 as m
+    torch.manual_seed(5)
+    layer = m.PagedAttention(256, 4, 2, 64, max_positions=512).to(DEV)
+    page, prefix = 16, 101
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    text = torch.randn(1, prefix, 256, device=DEV).bfloat16()
+    # row 3 of the pool's table holds the prefix, rows 0 .. 2 are places for requests
+    pool = m.PagedCache.pool(4, 300, 60, page, 2, 64, DEV)
+    pool.kv_lens.copy_(i32([0, 0, 0, prefix]))
+    cu, _, _ = pool.plan(i32([0, 0, 0, prefix]), prefix)
+    layer(text, pool, cu, max_q_len=prefix)
+    whole = m.PagedCache.zeros(3, 300, page, 2, 64, DEV)
+    whole.kv_lens.fill_(prefix)
+    layer(text.expand(3, -1, -1), whole)
+    serve = m.PagedCache(pool.k, pool.v, pool.block_table[:3], pool.kv_lens[:3], prefix_table=pool.block_table[3:], prefix_lens=pool.kv_lens[3:])
+    lens = [prefix] * 3
+    for new in ([5, 40, 1], [1, 1, 1], [1, 1, 1], [2, 7, 30]):
+        lens = [a + b for a, b in zip(lens, new)]
+        pool.kv_lens.copy_(i32(lens + [prefix]))
+        whole.kv_lens.copy_(i32(lens))
+        cu, positions, slots = pool.plan(i32(new + [0]), sum(new), starts=i32([prefix] * 3 + [0]))
+        x = torch.randn(1, sum(new), 256, device=DEV).bfloat16()
+        got, want = layer(x, serve, cu[:4], max_q_len=max(new)), layer(x, whole, cu[:4], max_q_len=max(new))
+        # two attention outputs of one rounding and one set of rounded weights each, through one projection
+        assert (got.double() - want.double()).norm() <= 1e-2 * want.double().norm()
+    assert int((~pool.page_free).sum()) == -(-prefix // page) + sum(-(-n // page) - prefix // page for n in lens)

@@ -192,6 +192,8 @@ inline long long tile_slots(int tokens, int n_seq, int max_q_len, int group, int
     return by_tokens;
 }
 
+// Rows of a row tile in the tensor-core pass over prefixes.
+inline int prefix_rows(int tokens, int n_groups, int group) { return (long long)tokens * group <= 128ll * n_groups ? 128 : 256; }
 inline long long group_slots(const GroupView& b, int group, int rows, int& per_group) {
     per_group = 0;
     if (b.p.n > 1) return (long long)b.tokens * group / rows + b.p.n;
@@ -273,13 +275,76 @@ constexpr float kLowest = -3.402823466e38f;
 constexpr float kLn2 = 0.6931471805599453f;
 
 // Which keys a pass goes through.
-enum Keys { kAllKeys, kPrefixKeys, kOwnKeys };
+// Own keys of sequence n in tiles of 64.
+__device__ __forceinline__ int own_tiles_of(const OwnView& b, int n) {
+    int first, count;
+    b.Batch::span(n, first, count);
+    const int len = b.kv_len(n), p = b.prefix_of(n);
+    if (count <= 0) return 0;
+    return (len + 63) / 64 - (len - count >= p ? p : 0) / 64;
+}
+
+// Attention behind a prefix is two passes side by side, one over the prefixes and one over own keys, and the SMs are dealt out so that both end
+// together.  What a group's prefix is in work: tiles of 128 keys, and row tiles that go through them.
+struct PrefixWork {
+    int tiles, row_tiles;
+};
+__device__ __forceinline__ PrefixWork prefix_work(const GroupView& b, int g, int heads_of_group, int tile_rows) {
+    int first, count;
+    b.span(g, first, count);
+    const int rows = count * heads_of_group;
+    return PrefixWork{rows > 0 ? max((b.prefix_len(g) + 127) / 128, 1) : 0, (rows + tile_rows - 1) / tile_rows};
+}
+constexpr int kSms = 148, kPartTries = 128;
+// Key tiles of a part, and the blocks that gives: each of the first kPartTries threads tries one number of parts for the longest prefix.  Times are in
+// microseconds, as measured: a key tile takes 0.95 with row tiles of 128 and 2 with 256, a tile of 64 own keys 1.0 of an SM (0.6 with 64 values
+// a head), and either pass 8 besides.  Called by all `warps` warps; `work` is filled, `best` has two places a warp.
+struct PartChoice {
+    int part, blocks;
+};
+__device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int groups, int tile_rows, int kv_heads, int dim, long long own_tiles, int splits, unsigned* best, int warps) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int longest = 0, row_tiles = 0;
+    for (int g = 0; g < groups; ++g) {
+        longest = max(longest, work[g].tiles);
+        row_tiles += work[g].row_tiles;
+    }
+    const int tries = tid + 1, part = (longest + tries - 1) / tries;
+    int blocks = 0;
+    if (longest > 0)
+        for (int g = 0; g < groups; ++g) blocks += work[g].row_tiles * ((work[g].tiles + part - 1) / part);
+    blocks *= kv_heads;
+    const float prefix_us = 8.f + (float)part * (tile_rows == 128 ? 0.95f : 2.f), own_us = own_tiles > 0 ? (float)own_tiles * (dim <= 64 ? 0.6f : 1.f) : 0.f;
+    const bool beside = own_us > 0.f && blocks < kSms;
+    const float us = beside ? fmaxf(prefix_us, 8.f + own_us / (float)(kSms - blocks)) : prefix_us + own_us / kSms;
+    const bool fits = tid < kPartTries && tries <= splits && blocks <= max(kSms, row_tiles * kv_heads);
+    const unsigned cost = fits ? __float_as_uint(us) : 0x7f800000u;
+    unsigned least = __reduce_min_sync(0xffffffffu, cost);
+    if (lane == 0) best[warp] = least;
+    __syncthreads();
+    least = __reduce_min_sync(0xffffffffu, lane < warps ? best[lane] : 0x7f800000u);
+    const unsigned who = __reduce_min_sync(0xffffffffu, fits && cost == least ? (unsigned)tries : 0xffffu);
+    if (lane == 0) best[warps + warp] = who;
+    __syncthreads();
+    const int parts = (int)__reduce_min_sync(0xffffffffu, lane < warps ? best[warps + lane] : 0xffffu);
+    PartChoice c{max((longest + parts - 1) / parts, 1), 0};
+    for (int g = 0; g < groups; ++g) c.blocks += work[g].row_tiles * ((work[g].tiles + c.part - 1) / c.part) * kv_heads;
+    return c;
+}
+// Whether the pass over the prefixes is cut into parts: where its row tiles leave half of the SMs idle.
+constexpr int kMaxListed = kSms / 2;
+
+enum Keys { kAllKeys, kPrefixKeys, kOwnKeys, kTurnKeys };      // kTurnKeys: a prefix by row tiles of 128 (attn_tc.cu)
 template <int KEYS>
 struct ViewOf {
     using type = Batch;
 };
 template <>
 struct ViewOf<kPrefixKeys> {
+    using type = GroupView;
+};
+template <>
+struct ViewOf<kTurnKeys> {
     using type = GroupView;
 };
 template <>
@@ -323,12 +388,24 @@ int decode(const Call& c, cudaStream_t st);
 // The passes of attention behind a shared prefix; their sums stay in the workspace, undivided, for a join.
 int general_shared(const Call& c, int prefix_splits, int own_splits, cudaStream_t st);
 size_t general_shared_workspace(size_t rows, int parts, int dim);
-int tc_prefix(const Call& c, int splits, cudaStream_t st);
+int tc_prefix(const Call& c, int splits, bool own_rows, cudaStream_t st);      // own_rows: the pass below runs beside it
 int tc_own(const Call& c, int splits, cudaStream_t st);
-size_t tc_parts_bytes(long long slots, int kv_heads, int splits, int dim);
-int decode_own(const Call& c, float* row_o, float2* row_ml, cudaStream_t st);
-// Own keys of each row: as tc_own left them in own.workspace (row_o null), or one sum a row.
-int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const float* row_o, const float2* row_ml, cudaStream_t st);
+size_t tc_parts_bytes(long long slots, int rows, int kv_heads, int splits, int dim);
+// Own keys of few rows a sequence and kv head, where the token steps' kernel left them: rows of sequences that one stretch had to itself are
+// whole; of the others stretch k has [2][rows][D] sums, place 1 of a sequence that begins in it, place 0 of one that goes on.
+struct OwnRows {
+    const float* part_o;
+    const float2* part_ml;
+    const float* row_o;
+    const float2* row_ml;
+    const int2* spans;      // [n_seq][kv_heads]: the first and the last stretch, or -1
+    int rows, blocks;
+};
+bool own_rows_take(const Call& c);
+size_t own_rows_workspace(const KdaPagedShape& s, int max_q);
+int own_rows(const Call& c, int prefix_splits, OwnRows& own, cudaStream_t st);
+// The join: own keys as own_rows left them, or (null) as tc_own did in own.workspace.
+int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const OwnRows* rows, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace kda

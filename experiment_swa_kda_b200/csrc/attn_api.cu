@@ -114,38 +114,36 @@ GroupView groups_of(const KdaPagedShape& s, const KdaPrefixShape& p) {
     v.p.n = p.n_groups;
     return v;
 }
-// Parts of a prefix where its row tiles leave SMs idle, as in split_count; a part has `least` key tiles.
-int prefix_split_count(const KdaPagedShape& s, const KdaPrefixShape& p, int rows, int keys, int resident, int least) {
+// Parts of a prefix at most, where its row tiles leave SMs idle.
+int prefix_split_count(const KdaPagedShape& s, const KdaPrefixShape& p, int rows, int keys, int resident) {
     int per;
     const long long blocks = group_slots(groups_of(s, p), s.q_heads / s.kv_heads, rows, per) * s.kv_heads;
     const long long tiles = ((long long)p.table_width * s.page_size + keys - 1) / keys;
     long long n = resident / (blocks > 0 ? blocks : 1);
-    if (n > tiles / least) n = tiles / least;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+    if (n > tiles) n = tiles;
+    return (int)(n < 1 ? 1 : n > kPartTries ? kPartTries : n);
 }
 int tc_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) {
     int per;
-    const long long slots = group_slots(groups_of(s, p), s.q_heads / s.kv_heads, 256, per);
-    return slots <= 384 && slots * s.kv_heads <= 148 / 2 ? prefix_split_count(s, p, 256, 128, 3 * 148, 1) : 1;
+    const int rows = prefix_rows(s.tokens, p.n_groups, s.q_heads / s.kv_heads);
+    const long long slots = group_slots(groups_of(s, p), s.q_heads / s.kv_heads, rows, per);
+    // a long prefix beside short ones may have more than its share of the blocks
+    return slots * s.kv_heads <= kMaxListed ? prefix_split_count(s, p, rows, 128, p.n_groups > 1 ? 3 * kSms : kSms) : 1;
 }
-int general_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) { return prefix_split_count(s, p, 64, 64, 2 * 148, 1); }
+int general_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) { return prefix_split_count(s, p, 64, 64, 2 * 148); }
 
 // The shares of a workspace on the tensor cores.
 struct SharedSpace {
-    size_t prefix, own, rows_ml, rows_o, all;
+    size_t prefix, own;
 };
 SharedSpace shared_space(const KdaPagedShape& s, const KdaPrefixShape& p, bool packed, bool few) {
     SharedSpace w;
     int per;
     const int group = s.q_heads / s.kv_heads, max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
-    const size_t rows = (size_t)s.tokens * s.q_heads;
-    w.prefix = align_up(tc_parts_bytes(group_slots(groups_of(s, p), group, 256, per), s.kv_heads, tc_prefix_splits(s, p), s.head_dim), 256);
-    w.own = few ? decode_workspace(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, max_q, s.head_dim)
-                : tc_parts_bytes(tile_slots(s.tokens, s.n_seq, max_q, group, 256, packed, per), s.kv_heads, tc_splits(s, packed), s.head_dim);
+    const int rows = prefix_rows(s.tokens, p.n_groups, group);
+    w.prefix = align_up(tc_parts_bytes(group_slots(groups_of(s, p), group, rows, per), rows, s.kv_heads, tc_prefix_splits(s, p), s.head_dim), 256);
+    w.own = few ? own_rows_workspace(s, max_q) : tc_parts_bytes(tile_slots(s.tokens, s.n_seq, max_q, group, 256, packed, per), 256, s.kv_heads, tc_splits(s, packed), s.head_dim);
     w.own = align_up(w.own, 256);
-    w.rows_ml = few ? align_up(rows * sizeof(float2), 256) : 0;
-    w.rows_o = few ? align_up(rows * s.head_dim * sizeof(float), 256) : 0;
-    w.all = w.prefix + w.own + w.rows_ml + w.rows_o;
     return w;
 }
 
@@ -159,8 +157,8 @@ extern "C" size_t kda_shared_prefix_attention_workspace_bytes(const KdaPagedShap
         const size_t g = general_shared_workspace((size_t)s->tokens * s->q_heads, general_prefix_splits(*s, *p) + general_splits(*s, packed), s->head_dim);
         if (g > most) most = g;
         for (int few = 0; few < 2; ++few) {
-            const size_t n = shared_space(*s, *p, packed, few).all;
-            if (n > most) most = n;
+            const SharedSpace w = shared_space(*s, *p, packed, few);
+            if (w.prefix + w.own > most) most = w.prefix + w.own;
         }
     }
     return align_up(most, 256);
@@ -193,15 +191,12 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     c.max_q_len = packed ? s->max_q_len : q_len;
     c.workspace = workspace;
     if (!tc_takes(c)) return general_shared(c, general_prefix_splits(*s, *p), general_splits(*s, packed), st);
-    const bool few = decode_takes(c);
-    const SharedSpace w = shared_space(*s, *p, packed, few);
-    char* ws = static_cast<char*>(workspace);
+    const bool few = own_rows_take(c);
     const int prefix_splits = tc_prefix_splits(*s, *p), own_splits = tc_splits(*s, packed);
-    if (int rc = tc_prefix(c, prefix_splits, st)) return rc;
     Call own = c;
-    own.workspace = ws + w.prefix;
-    float2* row_ml = reinterpret_cast<float2*>(ws + w.prefix + w.own);
-    float* row_o = reinterpret_cast<float*>(ws + w.prefix + w.own + w.rows_ml);
-    if (int rc = few ? decode_own(own, row_o, row_ml, st) : tc_own(own, own_splits, st)) return rc;
-    return tc_shared_join(c, prefix_splits, own, own_splits, few ? row_o : nullptr, row_ml, st);
+    own.workspace = static_cast<char*>(workspace) + shared_space(*s, *p, packed, few).prefix;
+    OwnRows rows;
+    if (int rc = tc_prefix(c, prefix_splits, few, st)) return rc;
+    if (int rc = few ? own_rows(own, prefix_splits, rows, st) : tc_own(own, own_splits, st)) return rc;
+    return tc_shared_join(c, prefix_splits, own, own_splits, few ? &rows : nullptr, st);
 }

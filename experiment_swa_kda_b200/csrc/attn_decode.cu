@@ -34,7 +34,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kMaxRows = 16, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
+constexpr int kMaxRows = 16, kMaxOwnRows = 24, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
 constexpr int kPerSm = 2;             // blocks an SM: 102 KB each, 106 with more than 8 rows
 // Up to so many tiles a sequence and kv head stay together: they take about as long as two of them and the join, which is a launch less (3
 // conversations of 40 tokens 14.5 us in parts, 8.4 whole; 16 of 100 12.5 and 10.4).  Six where there are sequences for every SM (200 of up
@@ -49,9 +49,11 @@ struct Layout {
     static constexpr int kHalf = 16 * 128;                            // 16 keys of 64 values
     static constexpr int kStage = 2 * (DP / 64) * kHalf;              // K and V of 16 keys
     static constexpr int kRowsOf = 8 * NR;
-    static constexpr int kQ = kWarps * kStages * kStage;              // two sequences' queries
-    static constexpr int kBars = kQ + 2 * kRowsOf * DP * 2;
-    static constexpr int kBytes = kBars + 1024 + 1024;      // barriers and what the warps tell each other; slack to align the tiles
+    static constexpr bool kKeepQ = NR <= 2;                           // queries in registers; with more rows they are read with every tile
+    static constexpr int kQ = kWarps * kStages * kStage;              // two sequences' queries, or one's
+    static constexpr int kQBuffers = kKeepQ ? 2 : 1;
+    static constexpr int kBars = kQ + kQBuffers * kRowsOf * DP * 2;
+    static constexpr int kBytes = kBars + 512 + kWarps * kRowsOf * 8 + 1024;      // barriers, what the warps tell each other; slack to align the tiles
 };
 
 struct Args {
@@ -60,8 +62,12 @@ struct Args {
     int whole;            // stretches begin and end with a sequence and kv head: no parts
     float* part_o;        // [blocks][2][rows][D]
     float2* part_ml;      // [blocks][2][rows]
-    float* row_o;         // own keys only: [tokens * q_heads][D], not divided by the sums, and (maximum, sum) of each row
+    // own keys only: [tokens * q_heads][D], not divided by the sums, and (maximum, sum) of each row; and of each sequence and kv head the
+    // stretches that have parts of it, or -1 where the rows are whole
+    float* row_o;
     float2* row_ml;
+    int2* spans;
+    int prefix_splits, prefix_rows;      // of the pass beside this one
 };
 
 // One sequence's tiles and rows.
@@ -265,9 +271,26 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         mbar_fence_init();
     }
     if (tid == 0) flags[0] = flags[1] = flags[2] = 0;
-    const Cut cut = a.whole ? find_start<kThreads, true>(b, Hk, window, a.blocks, blockIdx.x, &start, sums)
-                            : find_start<kThreads, false>(b, Hk, window, a.blocks, blockIdx.x, &start, sums);
-    const int tiles = a.whole ? start.end - start.begin : cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
+    int blocks = a.blocks;
+    if constexpr (KEYS == kOwnKeys) {
+        if (a.prefix_splits > 1) {      // beside the pass over the prefixes: the blocks that leaves room for
+            PrefixWork* work = reinterpret_cast<PrefixWork*>(sm + L::kQ);
+            unsigned* best = reinterpret_cast<unsigned*>(work + kMaxListed);
+            if (tid < b.p.n) work[tid] = prefix_work(a.c.batch, tid, g, a.prefix_rows);
+            int own = 0;
+            for (int n = tid; n < b.n_seq; n += kThreads) own += own_tiles_of(b, n);
+            own = __reduce_add_sync(0xffffffffu, own);
+            if (lane == 0) sums[warp] = own;
+            __syncthreads();
+            own = __reduce_add_sync(0xffffffffu, lane < kWarps ? sums[lane] : 0);
+            const PartChoice c = choose_parts(work, b.p.n, a.prefix_rows, Hk, D, (long long)own * Hk, a.prefix_splits, best, kWarps);
+            blocks = min(blocks, kPerSm * max(kSms - c.blocks, 1));
+            if (c.blocks >= kSms) blocks = a.blocks;
+        }
+    }
+    const Cut cut = a.whole && KEYS == kAllKeys ? find_start<kThreads, true>(b, Hk, window, blocks, blockIdx.x, &start, sums)
+                                                : find_start<kThreads, false>(b, Hk, window, blocks, blockIdx.x, &start, sums);
+    const int tiles = a.whole && KEYS == kAllKeys ? start.end - start.begin : cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
 
     uint8_t* ring = sm + warp * kStages * L::kStage;
     Walk ahead = {}, w = {};
@@ -317,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             }
         }
     };
-    auto q_at = [&](int buffer, int r, int chunk) { return sm + L::kQ + buffer * kRows * DP * 2 + r * DP * 2 + ((chunk ^ (r & 7)) << 4); };
+    auto q_at = [&](int buffer, int r, int chunk) { return sm + L::kQ + buffer % L::kQBuffers * (kRows * DP * 2) + r * DP * 2 + ((chunk ^ (r & 7)) << 4); };
     auto put_q = [&](int buffer) {
 #pragma unroll
         for (int y = 0; y < NR; ++y) {
@@ -345,6 +368,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         const size_t r0 = (size_t)s.first * Hq;
         if constexpr (KEYS == kOwnKeys) {
             for (int e = tid; e < s.count * Hq; e += kThreads) a.row_ml[r0 + e] = make_float2(-INFINITY, 0.f);
+            for (int e = tid; e < Hk; e += kThreads) a.spans[n * Hk + e].x = -1;
         } else {
             for (long long e = tid; e < (long long)s.count * Hq * D; e += kThreads) static_cast<__nv_bfloat16*>(a.c.o)[r0 * D + e] = __float2bfloat16(0.f);
             if (a.c.lse != nullptr)
@@ -359,7 +383,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
     __syncthreads();
 
     const float c = a.c.scale * 1.4426950408889634f, lazy = kLazy / c;
-    uint32_t q[NR][kSteps][2];
+    constexpr bool kKeepQ = L::kKeepQ;
+    uint32_t q[kKeepQ ? NR : 1][kKeepQ ? kSteps : 1][2];
     float acc[NR][kSteps][4], m[NR][2], l[NR][2];      // O^T: values r8, r8 + 8 of each 16, rows 2 c4, 2 c4 + 1 of each 8
     int last[NR][2], first[NR][2], rows = 0, all_lo = 0, all_hi = 0, unit_begin = 0, q_buffer = 0;
     bool fresh = true;
@@ -395,11 +420,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                 for (int t = 0; t < kSteps; ++t)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) acc[y][t][x] = 0.f;
+                if constexpr (kKeepQ) {
 #pragma unroll
-                for (int k = 0; k < kSteps; k += 2) {
-                    uint32_t f[4];
-                    ldm4(f, smem_u32(q_at(q_buffer, 8 * y + mr, 2 * k + mi)));
-                    q[y][k][0] = f[0]; q[y][k][1] = f[1]; q[y][k + 1][0] = f[2]; q[y][k + 1][1] = f[3];
+                    for (int k = 0; k < kSteps; k += 2) {
+                        uint32_t f[4];
+                        ldm4(f, smem_u32(q_at(q_buffer, 8 * y + mr, 2 * k + mi)));
+                        q[y][k][0] = f[0]; q[y][k][1] = f[1]; q[y][k + 1][0] = f[2]; q[y][k + 1][1] = f[3];
+                    }
                 }
             }
         }
@@ -443,12 +470,29 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                 __syncwarp();
             }
             float s2[2][NR][4] = {};      // S^T: keys r8, r8 + 8, rows 2 c4, 2 c4 + 1; two chains
+            if constexpr (kKeepQ) {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                uint32_t kf[4];
-                ldm4(kf, sk + (k >> 2) * L::kHalf + sw128_off((mi & 1) * 8 + mr, 2 * (k & 3) + (mi >> 1)));
+                for (int k = 0; k < kSteps; ++k) {
+                    uint32_t kf[4];
+                    ldm4(kf, sk + (k >> 2) * L::kHalf + sw128_off((mi & 1) * 8 + mr, 2 * (k & 3) + (mi >> 1)));
 #pragma unroll
-                for (int y = 0; y < NR; ++y) mma(s2[k & 1][y], kf, q[y][k][0], q[y][k][1]);
+                    for (int y = 0; y < NR; ++y) mma(s2[k & 1][y], kf, q[y][k][0], q[y][k][1]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSteps; k += 2) {
+                    uint32_t kf[2][4];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        ldm4(kf[x], sk + (k >> 2) * L::kHalf + sw128_off((mi & 1) * 8 + mr, 2 * ((k + x) & 3) + (mi >> 1)));
+#pragma unroll
+                    for (int y = 0; y < NR; ++y) {
+                        uint32_t f[4];
+                        ldm4(f, smem_u32(q_at(q_buffer, 8 * y + mr, 2 * k + mi)));
+                        mma(s2[0][y], kf[0], f[0], f[1]);
+                        mma(s2[1][y], kf[1], f[2], f[3]);
+                    }
+                }
             }
             float sc[NR][4];
             bool grow = false;
@@ -530,80 +574,89 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
             fresh = true;
             // through the ring's places of this tile, which are free until the next but one; [row][value], pieces of eight values
             // exchanged so that the lanes' rows lie in different banks
-            static_assert(L::kStage >= kRows * DP * 4, "a warp's sums fit a place of the ring");
+            constexpr int kAtOnce = NR < 2 ? 8 : 16;      // rows
+            static_assert(L::kStage >= kAtOnce * DP * 4, "a warp's sums fit a place of the ring");
             const int place = i % kStages * L::kStage;
             float* mine = reinterpret_cast<float*>(ring + place);
-#pragma unroll
-            for (int y = 0; y < NR; ++y)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int r = 8 * y + 2 * c4 + x;
-#pragma unroll
-                    for (int o = 4; o < 32; o <<= 1) l[y][x] += __shfl_xor_sync(0xffffffffu, l[y][x], o);
-                    if (r8 == 0) row_ml[warp * kRows + r] = make_float2(m[y][x], l[y][x]);
-#pragma unroll
-                    for (int t = 0; t < kSteps; ++t) {
-                        mine[r * DP + ((16 * t + r8) ^ (c4 << 3))] = acc[y][t][x];
-                        mine[r * DP + ((16 * t + r8 + 8) ^ (c4 << 3))] = acc[y][t][x + 2];
-                    }
-                }
-            __syncthreads();
             const bool begins = unit_begin == w.s.t0, whole = begins && ends;
+            if (KEYS == kOwnKeys && tid == 0) {
+                if (begins) a.spans[w.n * Hk + w.hk].x = whole ? -1 : (int)blockIdx.x;
+                if (ends) a.spans[w.n * Hk + w.hk].y = blockIdx.x;
+            }
             // a stretch's part: place 0 goes on from the block before, place 1 begins here
             const size_t part = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * kRows;
-#pragma unroll 1
-            for (int e = tid; e < rows * (D / 4); e += kThreads) {
-                const int r = e / (D / 4), d = 4 * (e - r * (D / 4));
-                float2 ml[kWarps];
-                float M = -INFINITY, sum = 0.f;
-                f2 o0 = f2_all(0.f), o1 = f2_all(0.f);
 #pragma unroll
-                for (int k = 0; k < kWarps; ++k) {
-                    ml[k] = row_ml[k * kRows + r];
-                    M = max_nan(M, ml[k].x);
-                }
+            for (int r0 = 0; r0 < kRows; r0 += kAtOnce) {
+                if (r0 > 0) __syncthreads();
 #pragma unroll
-                for (int k = 0; k < kWarps; ++k) {
-                    if (ml[k].x == -INFINITY) continue;      // its sums are 0
-                    const float f = ex2((ml[k].x - M) * c);
-                    sum = fmaf(ml[k].y, f, sum);
-                    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm + k * kStages * L::kStage + place) + r * DP + (d ^ (((r >> 1) & 3) << 3)));
-                    o0 = f2_fma(f2_make(x.x, x.y), f2_all(f), o0);
-                    o1 = f2_fma(f2_make(x.z, x.w), f2_all(f), o1);
-                }
-                float2 oa = f2_get(o0), ob = f2_get(o1);
-                float o[4] = {oa.x, oa.y, ob.x, ob.y};
-                if (M == kLowest) sum = 0.f;      // nothing but -inf: 0 / 0
-                if (flags[1 + q_buffer]) {
-                    const int to = w.s.base + r / g, from = KEYS == kOwnKeys ? w.s.lo : first_key(to, window);
-#pragma unroll 1
-                    for (int key = max(from, unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
-                        if (key >= all_lo && key < all_hi) continue;
-                        const int pg = b.page(w.n, key / b.page_size);
-                        if (pg < 0) continue;
-                        const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v) + pg * a.c.strides.v_page + (key % b.page_size) * a.c.strides.v_row +
-                                                 w.hk * a.c.strides.v_head + d;
+                for (int y = r0 / 8; y < (r0 + kAtOnce) / 8 && y < NR; ++y)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const float val = __bfloat162float(v[x]);
-                            if (!isfinite(val)) o[x] += val;
+                    for (int x = 0; x < 2; ++x) {
+                        const int r = 8 * y + 2 * c4 + x;
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) l[y][x] += __shfl_xor_sync(0xffffffffu, l[y][x], o);
+                        if (r8 == 0) row_ml[warp * kRows + r] = make_float2(m[y][x], l[y][x]);
+#pragma unroll
+                        for (int t = 0; t < kSteps; ++t) {
+                            mine[(r - r0) * DP + ((16 * t + r8) ^ (c4 << 3))] = acc[y][t][x];
+                            mine[(r - r0) * DP + ((16 * t + r8 + 8) ^ (c4 << 3))] = acc[y][t][x + 2];
                         }
                     }
+                __syncthreads();
+#pragma unroll 1
+                for (int e = tid; e < min(rows - r0, kAtOnce) * (D / 4); e += kThreads) {
+                    const int in = e / (D / 4), r = r0 + in, d = 4 * (e - in * (D / 4));
+                    float2 ml[kWarps];
+                    float M = -INFINITY, sum = 0.f;
+                    f2 o0 = f2_all(0.f), o1 = f2_all(0.f);
+#pragma unroll
+                    for (int k = 0; k < kWarps; ++k) {
+                        ml[k] = row_ml[k * kRows + r];
+                        M = max_nan(M, ml[k].x);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kWarps; ++k) {
+                        if (ml[k].x == -INFINITY) continue;      // its sums are 0
+                        const float f = ex2((ml[k].x - M) * c);
+                        sum = fmaf(ml[k].y, f, sum);
+                        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm + k * kStages * L::kStage + place) + in * DP + (d ^ (((r >> 1) & 3) << 3)));
+                        o0 = f2_fma(f2_make(x.x, x.y), f2_all(f), o0);
+                        o1 = f2_fma(f2_make(x.z, x.w), f2_all(f), o1);
+                    }
+                    float2 oa = f2_get(o0), ob = f2_get(o1);
+                    float o[4] = {oa.x, oa.y, ob.x, ob.y};
+                    if (M == kLowest) sum = 0.f;      // nothing but -inf: 0 / 0
+                    if (flags[1 + q_buffer]) {
+                        const int to = w.s.base + r / g, from = KEYS == kOwnKeys ? w.s.lo : first_key(to, window);
+#pragma unroll 1
+                        for (int key = max(from, unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
+                            if (key >= all_lo && key < all_hi) continue;
+                            const int pg = b.page(w.n, key / b.page_size);
+                            if (pg < 0) continue;
+                            const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.c.v) + pg * a.c.strides.v_page + (key % b.page_size) * a.c.strides.v_row +
+                                                     w.hk * a.c.strides.v_head + d;
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const float val = __bfloat162float(v[x]);
+                                if (!isfinite(val)) o[x] += val;
+                            }
+                        }
+                    }
+                    if (!whole) {
+                        if (d == 0) a.part_ml[part + r] = make_float2(M == -INFINITY ? M : max_nan(M * c, kLowest), sum);
+                        *reinterpret_cast<float4*>(a.part_o + (part + r) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                        continue;
+                    }
+                    const size_t out = (size_t)(w.s.first + r / g) * Hq + w.hk * g + r % g;
+                    if constexpr (KEYS == kOwnKeys) {
+                        if (d == 0) a.row_ml[out] = make_float2(M == -INFINITY ? M : max_nan(M * c, kLowest), sum);
+                        *reinterpret_cast<float4*>(a.row_o + out * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                        continue;
+                    }
+                    const float inv = M == -INFINITY ? 0.f : 1.f / sum;
+                    if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = M == -INFINITY ? -INFINITY : (M * c + log2f(sum)) * kLn2;
+                    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
                 }
-                if (!whole) {
-                    if (d == 0) a.part_ml[part + r] = make_float2(M == -INFINITY ? M : max_nan(M * c, kLowest), sum);
-                    *reinterpret_cast<float4*>(a.part_o + (part + r) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
-                    continue;
-                }
-                const size_t out = (size_t)(w.s.first + r / g) * Hq + w.hk * g + r % g;
-                if constexpr (KEYS == kOwnKeys) {
-                    if (d == 0) a.row_ml[out] = make_float2(M == -INFINITY ? M : max_nan(M * c, kLowest), sum);
-                    *reinterpret_cast<float4*>(a.row_o + out * D + d) = make_float4(o[0], o[1], o[2], o[3]);
-                    continue;
-                }
-                const float inv = M == -INFINITY ? 0.f : 1.f / sum;
-                if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = M == -INFINITY ? -INFINITY : (M * c + log2f(sum)) * kLn2;
-                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
             }
             q_buffer ^= 1;
             if (tid == 0) flags[1 + q_buffer] = 0;
@@ -622,14 +675,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
 // begins; the first such place inside a sequence takes all its parts.  Four values a thread; with few rows several threads share the
 // parts of one place and add up through shared memory.
 constexpr int kJoinThreads = 512, kMaxBlocks = 148 * kPerSm;
-template <int NR, int KEYS>
+template <int NR>
 __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __grid_constant__ Args a) {
     constexpr int kRows = 8 * NR;
     __shared__ Start start;
     __shared__ int sums[kJoinThreads / 32];
     __shared__ float weight[kMaxBlocks * kRows], row_l[kRows], row_m[kRows];
     __shared__ float4 acc[kJoinThreads];
-    const auto& b = view<KEYS>(a.c);
+    const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Cut cut = find_start<kJoinThreads, false>(b, Hk, window, a.blocks, id, &start, sums);
@@ -692,11 +745,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
             o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
         }
         const size_t out = (size_t)(s.first + r / g) * Hq + start.hk * g + r % g;
-        if constexpr (KEYS == kOwnKeys) {
-            if (d == 0) a.row_ml[out] = make_float2(row_m[r], row_l[r]);
-            *reinterpret_cast<float4*>(a.row_o + out * D + d) = o;
-            return;
-        }
         const float m = row_m[r], l = row_l[r], inv = m == -INFINITY ? 0.f : 1.f / l;
         if (d == 0 && a.c.lse != nullptr) a.c.lse[out] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.c.o) + out * D + d) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
@@ -715,8 +763,8 @@ int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStre
         KDA_LAUNCH("attn_decode_kernel", st, attn_decode_kernel<DP, NR, KEYS><<<a.blocks, kThreads, kBytes, st>>>(mK, mV, a));
     }
     if (int rc = launch_status()) return rc;
-    if (a.blocks == 1 || a.whole) return KDA_OK;
-    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR, KEYS>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
+    if (a.blocks == 1 || a.whole || KEYS == kOwnKeys) return KDA_OK;
+    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
@@ -736,43 +784,77 @@ long long reach_of(int table_width, int page_size, int window, int max_q) {
 
 }  // namespace
 
-bool decode_takes(const Call& c) {
+namespace {
+bool takes(const Call& c, int rows) {
     const long long tiles = (long long)c.batch.n_seq * c.heads.kv_heads * ((long long)c.batch.table_width * c.batch.page_size / kTile + 2);
-    return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= kMaxRows && tiles < 1ll << 31 && tc_takes(c);
+    return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= rows && tiles < 1ll << 31 && tc_takes(c);
+}
+size_t parts_bytes(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim, int rows_each) {
+    const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q)) * 2 * rows_each;
+    return align_up(rows * sizeof(float2), 256) + rows * dim * sizeof(float);
+}
+}  // namespace
+
+bool decode_takes(const Call& c) { return takes(c, kMaxRows); }
+size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim) {
+    return parts_bytes(n_seq, kv_heads, table_width, page_size, window, max_q, dim, kMaxRows);
 }
 
-size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim) {
-    const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q)) * 2 * kMaxRows;
-    return align_up(rows * sizeof(float2), 256) + rows * dim * sizeof(float);
+bool own_rows_take(const Call& c) { return takes(c, kMaxOwnRows); }
+size_t own_rows_workspace(const KdaPagedShape& s, int max_q) {
+    const size_t rows = (size_t)s.tokens * s.q_heads;
+    return align_up(parts_bytes(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, max_q, s.head_dim, kMaxOwnRows), 256) + align_up(rows * sizeof(float2), 256) +
+           align_up(rows * s.head_dim * sizeof(float), 256) + align_up((size_t)s.n_seq * s.kv_heads * sizeof(int2), 256);
 }
 
 namespace {
 
 template <int KEYS>
-int pass(const Call& c, float* row_o, float2* row_ml, cudaStream_t st) {
+int pass(const Call& c, int prefix_splits, OwnRows* own, cudaStream_t st) {
     Args a;
     a.c = c;
-    a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
+    const long long reach = reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len);
+    const int rows = KEYS == kOwnKeys ? kMaxOwnRows : kMaxRows;
+    a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach);
     a.box_rows = c.batch.page_size < 16 ? c.batch.page_size : 16;
-    a.whole = keeps_whole(c.batch.n_seq, c.heads.kv_heads, reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len));
-    a.part_ml = static_cast<float2*>(c.workspace);
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(c.workspace) + align_up((size_t)a.blocks * 2 * kMaxRows * sizeof(float2), 256));
-    a.row_o = row_o;
-    a.row_ml = row_ml;
+    a.whole = keeps_whole(c.batch.n_seq, c.heads.kv_heads, reach);
+    char* ws = static_cast<char*>(c.workspace);
+    a.part_ml = reinterpret_cast<float2*>(ws);
+    ws += align_up((size_t)a.blocks * 2 * rows * sizeof(float2), 256);
+    a.part_o = reinterpret_cast<float*>(ws);
+    a.row_o = nullptr;
+    a.row_ml = nullptr;
+    a.spans = nullptr;
+    a.prefix_splits = prefix_splits;
+    a.prefix_rows = KEYS == kOwnKeys ? prefix_rows(c.batch.tokens, c.batch.p.n, c.heads.group) : 0;
+    const int max_rows = c.max_q_len * c.heads.group;
+    if (KEYS == kOwnKeys) {
+        const size_t all = (size_t)c.batch.tokens * c.heads.q_heads;
+        ws += align_up((size_t)a.blocks * 2 * rows * c.heads.dim * sizeof(float), 256);
+        a.row_ml = reinterpret_cast<float2*>(ws);
+        ws += align_up(all * sizeof(float2), 256);
+        a.row_o = reinterpret_cast<float*>(ws);
+        ws += align_up(all * c.heads.dim * sizeof(float), 256);
+        a.spans = reinterpret_cast<int2*>(ws);
+        *own = OwnRows{a.part_o, a.part_ml, a.row_o, a.row_ml, a.spans, max_rows <= 8 ? 8 : max_rows <= 16 ? 16 : 24, a.blocks};
+    }
     CUtensorMap mK, mV;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
     if (!rc) rc = make_map_paged(&mV, c.v, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.v_row, s.v_head, s.v_page, a.box_rows);
     if (rc) return rc;
-    const bool few = c.max_q_len * c.heads.group <= 8;
+    if constexpr (KEYS == kOwnKeys) {
+        if (max_rows > 16) return c.heads.dim <= 64 ? launch<64, 3, KEYS>(mK, mV, a, st) : launch<128, 3, KEYS>(mK, mV, a, st);
+    }
+    const bool few = max_rows <= 8;
     if (c.heads.dim <= 64) return few ? launch<64, 1, KEYS>(mK, mV, a, st) : launch<64, 2, KEYS>(mK, mV, a, st);
     return few ? launch<128, 1, KEYS>(mK, mV, a, st) : launch<128, 2, KEYS>(mK, mV, a, st);
 }
 
 }  // namespace
 
-int decode(const Call& c, cudaStream_t st) { return pass<kAllKeys>(c, nullptr, nullptr, st); }
-int decode_own(const Call& c, float* row_o, float2* row_ml, cudaStream_t st) { return pass<kOwnKeys>(c, row_o, row_ml, st); }
+int decode(const Call& c, cudaStream_t st) { return pass<kAllKeys>(c, 1, nullptr, st); }
+int own_rows(const Call& c, int prefix_splits, OwnRows& own, cudaStream_t st) { return pass<kOwnKeys>(c, prefix_splits, &own, st); }
 
 }  // namespace attn
 }  // namespace kda

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
     if (!make_unit(b, tiles, blockIdx.x, c.window, u)) {
         int n, tile;
         if (hk == 0 && z == 0 && tid == 0 && tiles.find(b, blockIdx.x, n, tile)) check_batch(b, tiles, n, tile);
+        if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too
         return;
     }
     if (hk == 0 && z == 0 && tid == 0) check_batch(b, tiles, u.n, u.row0 / kRows);
@@ -242,6 +243,7 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
                 if (d < D) st_io(c.o, row * D + d, c.bf16, acc[i][x][j] * inv);
             }
     }
+    if (KEYS == kOwnKeys) dependency_wait();
 }
 
 // Joins the parts of a row: a warp a row.  SHARED: those of the prefix, which come first, only where the row's sequence shares it.
@@ -304,8 +306,9 @@ int launch(const Call& c, const Tiles& t, dim3 grid, int splits, float* part_o, 
     const bool vec = all % unit == 0 && (reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % 16 == 0;
     auto kern = vec ? attn_general_kernel<DP, true, KEYS> : attn_general_kernel<DP, false, KEYS>;
     if (int rc = set_smem_limit(kern, smem)) return rc;
-    KDA_LAUNCH("attn_general_kernel", st, kern<<<grid, kThreads, smem, st>>>(c, t, splits, part_o, part_ml));
-    return launch_status();
+    cudaError_t e = cudaSuccess;      // own keys: beside the pass over the prefix
+    KDA_LAUNCH("attn_general_kernel", st, e = launch_early(kern, grid, kThreads, smem, st, KEYS == kOwnKeys, 1, c, t, splits, part_o, part_ml));
+    return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 template <int KEYS>

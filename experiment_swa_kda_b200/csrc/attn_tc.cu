@@ -63,7 +63,7 @@ struct Layout {
 struct Args {
     Call c;
     Tiles tiles;
-    int slots, splits, box_rows, q_boxes;
+    int slots, splits, box_rows, q_boxes, own_rows;      // own_rows: own keys go to the token steps' kernel, which runs beside
     // Where rows are cut into parts: how many each block's have, [slots][kv heads]; of each part, [splits][slots][kv heads], a row's maximum
     // and sum [256] and its sums [2 row tiles][2 halves of the columns][128][DP / 2], pieces of 16 bytes exchanged within a row as
     // part_off() says.
@@ -114,11 +114,72 @@ struct Range {
     int begin, end;
 };
 
+// The unit and part of this block in a pass over prefixes that is cut into parts, of equal length in key tiles and in one list over the row
+// tiles.  `lists` is shared memory.  False: none is left for this block.
+__device__ __forceinline__ bool prefix_unit(const Args& a, const GroupView& b, int* lists, Unit& u, int& slot, int& hk, int& z, int& parts) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, heads = a.c.heads.kv_heads;
+    int *tiles_of = lists, *own = lists + kThreads;
+    unsigned* best = reinterpret_cast<unsigned*>(own + kThreads / 32);
+    PrefixWork* work = reinterpret_cast<PrefixWork*>(best + 2 * kThreads / 32);
+    Unit* units = reinterpret_cast<Unit*>(work + kMaxListed);
+    Unit v;
+    int tiles = 0, own_of = 0;
+    if (tid < b.p.n) work[tid] = prefix_work(b, tid, a.c.heads.group, a.tiles.rows);
+    if (a.own_rows)
+        for (int n = tid; n < b.n_seq; n += kThreads) own_of += own_tiles_of(b, n);
+    if (tid < a.slots) {
+        if (make_unit(b, a.tiles, tid, 0, v)) {
+            tiles = max((v.hi + kKeys - 1) / kKeys, 1);
+            units[tid] = v;
+        }
+        int n, tile;
+        if (blockIdx.x == 0 && a.tiles.find(b, tid, n, tile)) check_batch(b, a.tiles, n, tile);
+    }
+    tiles_of[tid] = tiles;
+    own_of = __reduce_add_sync(0xffffffffu, own_of);
+    if (lane == 0) own[warp] = own_of;
+    __syncthreads();
+    own_of = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? own[lane] : 0);
+    const int part = choose_parts(work, b.p.n, a.tiles.rows, heads, a.c.heads.dim, (long long)own_of * heads, a.splits, best, kThreads / 32).part;
+    int id = blockIdx.x, i0 = 0, found = -1;
+    for (; i0 < a.slots && found < 0; i0 += 32) {
+        const int n = i0 + lane < a.slots ? (tiles_of[i0 + lane] + part - 1) / part : 0;
+        int upto = n * heads;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, upto > id);
+        if (behind != 0) {
+            const int l = __ffs(behind) - 1;
+            found = i0 + l;
+            parts = __shfl_sync(0xffffffffu, n, l);
+            id -= __shfl_sync(0xffffffffu, upto, l) - parts * heads;
+        } else {
+            id -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    if (found >= 0) {
+        slot = found;
+        hk = id / parts;
+        z = id - hk * parts;
+        u = units[found];
+    }
+    fence_async_smem();      // the lists' place is written by copies next
+    __syncthreads();
+    return found >= 0;
+}
+
 template <int DP, int KEYS>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                               const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mO,
                                                               const __grid_constant__ Args a) {
     using L = Layout<DP>;
+    // Row tiles of 128 alone: their two places take the key tiles in turns, each with sums of its own, so that one's products run while the
+    // other's scores are turned into weights.
+    constexpr bool turns = KEYS == kTurnKeys, in_prefix = turns || KEYS == kPrefixKeys;
+    constexpr int kPartRows = turns ? 128 : kRows;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::kBars);
@@ -130,20 +191,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const auto& b = view<KEYS>(a.c);
-    const int g = a.c.heads.group, D = a.c.heads.dim, hk = blockIdx.y, z = blockIdx.z, window = a.c.window;
-    if (KEYS != kAllKeys) dependents_go();
+    const int g = a.c.heads.group, D = a.c.heads.dim, window = a.c.window;
     // a sequence's last rows see the most keys: they start first
-    const int slot = a.slots - 1 - (int)blockIdx.x;
-    Unit u;
-    const bool some = make_unit(b, a.tiles, slot, window, u);
-    if (hk == 0 && z == 0 && tid == 0) {
-        int n, tile;
-        if (a.tiles.find(b, slot, n, tile)) check_batch(b, a.tiles, n, tile);
+    if (warp == kLoadWarp && elect_one()) {
+        tma_prefetch_desc(&mK);
+        tma_prefetch_desc(&mV);
+        if (a.q_boxes) tma_prefetch_desc(&mQ);
     }
-    if (!some) return;
+    int hk = blockIdx.y, z = blockIdx.z, slot = a.slots - 1 - (int)blockIdx.x, parts = 1;
+    if (KEYS != kAllKeys) dependents_go();
+    Unit u;
+    bool some;
+    if (in_prefix && a.splits > 1) {
+        if (warp == kMmaWarp) tmem_alloc(&tmem_slot, 512);
+        some = prefix_unit(a, a.c.batch, reinterpret_cast<int*>(sm), u, slot, hk, z, parts);
+        if (!some && warp == kMmaWarp) tmem_dealloc(tmem_slot, 512);
+    } else {
+        some = make_unit(b, a.tiles, slot, window, u);
+        if (hk == 0 && z == 0 && tid == 0) {
+            int n, tile;
+            if (a.tiles.find(b, slot, n, tile)) check_batch(b, a.tiles, n, tile);
+        }
+    }
+    if (!some) {
+        if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too
+        return;
+    }
 
     // keys any row of the block sees: [u.lo, u.hi); keys all of them see: [all_lo, all_hi)
-    auto last_of = [&](int prow) { return KEYS == kPrefixKeys ? u.hi - 1 : u.base + prow / g; };      // a row's last key, and its first one
+    auto last_of = [&](int prow) { return in_prefix ? u.hi - 1 : u.base + prow / g; };      // a row's last key, and its first one
     auto first_of = [&](int last) { return KEYS == kAllKeys ? first_key(last, window) : u.from; };
     const int first_pos = last_of(u.row0), last_pos = last_of(u.row0 + u.rows - 1);
     const int all_lo = first_of(last_pos), all_hi = first_pos + 1;
@@ -151,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const int key0 = u.lo / a.box_rows * a.box_rows, nt = max((u.hi - key0 + kKeys - 1) / kKeys, 0);
     int t_begin = 0, t_end = nt;
     bool split = KEYS != kAllKeys;      // the sums of these passes are joined whatever their number of parts
-    if (a.splits > 1) {
+    if (!in_prefix && a.splits > 1) {
         // The shortest parts with which all blocks run side by side, looked for by one length a warp, twice; none where they would be
         // little shorter than the longest row tile's keys (a part costs some 5 tiles of its own, and the join).  The host sees to it
         // that a thread has a slot.
@@ -179,18 +255,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             hi = min(lo + first * step, hi);
             lo = first > 0 ? min(lo + (first - 1) * step + 1, hi) : hi;
         }
-        const int part = 4 * hi > 3 * longest ? longest : hi, parts = min(max((nt + part - 1) / part, 1), a.splits);
-        if (z >= parts) return;
+        const int part = 4 * hi > 3 * longest ? longest : hi;
+        parts = min(max((nt + part - 1) / part, 1), a.splits);
+        if (z >= parts) {
+            if (KEYS == kOwnKeys) dependency_wait();
+            return;
+        }
         fence_async_smem();      // the list's place is written by copies next
         split |= parts > 1;
+    }
+    if (KEYS != kAllKeys || a.splits > 1) {
         t_begin = nt * z / parts;
         t_end = nt * (z + 1) / parts;
         if (z == 0 && tid == 0) a.parts[slot * a.c.heads.kv_heads + hk] = parts;
-    } else if (KEYS != kAllKeys && tid == 0) {
-        a.parts[slot * a.c.heads.kv_heads + hk] = 1;
     }
     auto range_of = [&](int t) {      // key tiles of row tile t
         const int r0 = u.row0 + 128 * t, r1 = min(r0 + 128, u.row0 + u.rows) - 1;
+        if (turns) return Range{t_begin + t, max(t_end, t_begin + t)};
         if (r0 > r1) return Range{0, 0};
         const int hi = last_of(r1) + 1, lo = first_of(last_of(r0));
         Range r{max(t_begin, (lo - key0) / kKeys), min(t_end, (max(hi - key0, 0) + kKeys - 1) / kKeys)};
@@ -198,6 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         return r;
     };
     const Range range[2] = {range_of(0), range_of(1)};
+    constexpr int step = turns ? 2 : 1;      // from one of a row tile's key tiles to the next
     // the tiles some row sees only in part
     auto partial = [&](int j) { return key0 + j * kKeys < all_lo || key0 + (j + 1) * kKeys > all_hi; };
 
@@ -219,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         abort_flag = 0;
         odd_values = 0;
     }
-    if (warp == kMmaWarp) tmem_alloc(&tmem_slot, 512);
+    if (warp == kMmaWarp && !(in_prefix && a.splits > 1)) tmem_alloc(&tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -237,6 +319,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     // stage and phase of the ring's i-th tile
     auto stage = [](int i) { return i % L::kStages; };
     auto turn = [](int i) { return (uint32_t)(i / L::kStages) & 1u; };
+    // K and V of the block's m-th key tile in the order of the ring, that of their use: K 0, V 0, K 1, V 1, ..., or, where two key tiles are under way
+    // at a time, K 0, K 1, V 0, K 2, V 1, ...
+    const int m_end = t_end - t_begin;
+    auto ring_k = [&](int m) { return !turns ? 2 * m : m < 2 ? m : 2 * m - 1; };
+    auto ring_v = [&](int m) { return !turns ? 2 * m + 1 : min(2 * m + 2, 2 * m_end - 1); };
+    auto ring_is_v = [&](int i) { return !turns ? (i & 1) != 0 : i >= min(2, m_end) && ((i & 1) == 0 || i == 2 * m_end - 1); };
+    auto ring_tile = [&](int i) {      // m
+        if (!turns) return i >> 1;
+        if (i < min(2, m_end)) return i;
+        return i == 2 * m_end - 1 ? m_end - 1 : (i & 1) ? (i + 1) >> 1 : (i - 2) >> 1;
+    };
 
     if (warp < kSoftmaxWarps) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 " KDA_SOFTMAX_REGS ";");
@@ -263,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // ------------------------------------------------------------------ softmax of row tile t, a row a thread
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + lanes + cS + 128 * t, tO = tmem + lanes + cO + DP * t;
-        const int row = 128 * t + (tid & 127), prow = u.row0 + row;
+        const int place0 = turns ? 0 : 128 * t, row = place0 + (tid & 127), prow = u.row0 + row;
         const int last = row < u.rows ? last_of(prow) : last_pos;      // rows behind the last one compute along, unseen
         const int first = first_of(last);
         // keys all rows of the warp see
@@ -272,8 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const Range r = t ? range[1] : range[0];
         float m = -INFINITY, l = 0.f;
         bool ok = true;
-        for (int j = r.begin; j < r.end; ++j) {
-            const int i = j - r.begin;
+        for (int j = r.begin, i = 0; j < r.end; j += step, ++i) {
             ok = warp_wait(bar_s + t, i & 1);
             if (!ok) break;
             tc_fence_after();
@@ -353,16 +445,68 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             l += both.x + both.y;
         }
         // ------------------------------------------------------------------ O / l
-        const int n = r.end - r.begin;
+        const int n = (r.end - r.begin + step - 1) / step;
         const bool full = !split && a.q_boxes && 128 * (t + 1) <= u.rows;      // the same for the row tile's warps
         // The output goes through the queries' place.  With a key, what is read there has been read when the last product ends; without one (a
         // row tile of padding, or a part behind its keys) its queries may still be on their way there, if anything fetched them.
-        if (ok && n > 0) {
+        if (ok && turns && t_begin < t_end) {
+            ok = warp_wait(bar_end, 0);      // the queries are the other place's too
+        } else if (ok && n > 0) {
             ok = warp_wait(bar_o + t, (n - 1) & 1);
         } else if (ok && (!a.q_boxes || t_begin < t_end)) {
             ok = warp_wait(bar_q, 0);
         }
-        if (ok && 128 * t + 32 * (warp & 3) < u.rows) {
+        if constexpr (turns) {
+            // The two places' sums become one: each takes half of the columns of both, a row a thread, through the ring, in which nothing is
+            // left.  All of their warps come here whatever their waits said.
+            if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);      // a NaN or +inf among the scores, which ex2_pair does not pass on
+            float2* row_ml = reinterpret_cast<float2*>(sm + L::kRing);
+            if (ok && t_begin < t_end) row_ml[tid] = make_float2(m, l);
+            asm volatile("bar.sync 4, 256;" ::: "memory");
+            if (ok && !abort_flag && 32 * (warp & 3) < u.rows) {
+                tc_fence_after();
+                float2 ml[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+                if (t_begin < t_end) ml[0] = row_ml[tid & 127], ml[1] = row_ml[128 + (tid & 127)];
+                const float top = max_nan(ml[0].x, ml[1].x);
+                float f[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) f[x] = ml[x].x == -INFINITY ? 0.f : ex2((ml[x].x - top) * c);
+                const size_t part = ((size_t)z * a.slots + slot) * a.c.heads.kv_heads + hk;
+                if (t == 0 && row < u.rows)
+                    a.part_ml[part * kPartRows + row] = make_float2(top == -INFINITY ? top : top < INFINITY ? max_nan(top * c, kLowest) : __int_as_float(0x7fffffff),
+                                                                ml[0].y * f[0] + ml[1].y * f[1]);
+                constexpr int kCols = DP / 2;
+                uint8_t* at = sm + L::kRing + 4096 + warp * (32 * kCols * 4);
+#pragma unroll 1
+                for (int q = 0; q < kCols / 32; ++q) {
+                    uint32_t o[2][32];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const bool some = range[x].begin < range[x].end;
+                        if (some) tmem_ld32(tmem + lanes + cO + DP * x + kCols * t + 32 * q, o[x]);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[x][e] = some && ml[x].x != -INFINITY ? __float_as_uint(__uint_as_float(o[x][e]) * f[x]) : 0u;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        float y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = __uint_as_float(o[0][4 * x + e]) + __uint_as_float(o[1][4 * x + e]);
+                        *reinterpret_cast<float4*>(at + part_off<DP>(lane, 8 * q + x)) = make_float4(y[0], y[1], y[2], y[3]);
+                    }
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    const float* dst = a.part_o + (part * 2 + t) * (128 * kCols) + 32 * (warp & 3) * kCols;
+                    const uint32_t bytes = min(32, u.rows - 32 * (warp & 3)) * kCols * 4;      // rows behind the last are nobody's
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(at)), "r"(bytes) : "memory");
+                    tma_store_commit();
+                }
+                tma_store_wait_read();
+            }
+        } else if (ok && place0 + 32 * (warp & 3) < u.rows) {
             tc_fence_after();
             const bool mine = row < u.rows;
             if (!(m < INFINITY)) l = __int_as_float(0x7fffffff);      // a NaN or +inf among the scores, which ex2_pair does not pass on
@@ -477,9 +621,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 const uint32_t s0 = smem_u32(sm);
                 constexpr uint32_t idS = umma_idesc_bf16(128, 128, kMajorK, kMajorK), idO = umma_idesc_bf16(128, DP, kMajorK, kMajorMN);
                 bool ok = wait(bar_q, 0);
-                auto in = [&](int t, int j) { return j >= range[t].begin && j < range[t].end; };
+                auto in = [&](int t, int j) { return j >= range[t].begin && j < range[t].end && (!turns || ((j - range[t].begin) & 1) == 0); };
                 auto scores = [&](int t, int j, int i) {      // S_t = Q_t K_j^T
-                    const UmmaDesc q = umma_smem_desc_sw128(s0 + t * L::kTile, 16, 1024), k = umma_smem_desc_sw128(s0 + L::kRing + stage(i) * L::kTile, 16, 1024);
+                    const UmmaDesc q = umma_smem_desc_sw128(s0 + (turns ? 0 : t) * L::kTile, 16, 1024), k = umma_smem_desc_sw128(s0 + L::kRing + stage(i) * L::kTile, 16, 1024);
 #pragma unroll
                     for (int x = 0; x < DP / 16; ++x) {
                         const uint32_t off = (x >> 2) * 16384 + (x & 3) * 32;
@@ -493,14 +637,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     for (int t = 0; t < 2; ++t)
                         if (in(t, t_begin)) scores(t, t_begin, 0);
                     umma_commit(bar_free + stage(0));
+                    if (turns && t_begin + 1 < t_end) {
+                        ok = wait(bar_full + stage(1), turn(1));
+                        if (ok) {
+                            tc_fence_after();
+                            scores(1, t_begin + 1, 1);
+                            umma_commit(bar_free + stage(1));
+                        }
+                    }
                 }
                 for (int j = t_begin; j < t_end && ok; ++j) {
-                    const int iv = 2 * (j - t_begin) + 1, ik = iv + 1;      // places of V_j and K_j+1 in the ring
+                    const int next = j + step, iv = ring_v(j - t_begin), ik = ring_k(next - t_begin);      // places of V_j and K_next in the ring
                     ok = wait(bar_full + stage(iv), turn(iv));
-                    if (ok && j + 1 < t_end) ok = wait(bar_full + stage(ik), turn(ik));
+                    if (ok && next < t_end) ok = wait(bar_full + stage(ik), turn(ik));
                     for (int t = 0; t < 2 && ok; ++t) {
                         if (in(t, j)) {
-                            const int i = j - range[t].begin;
+                            const int i = (j - range[t].begin) / step;
                             const UmmaDesc v = umma_smem_desc_sw128(s0 + L::kRing + stage(iv) * L::kTile, 16384, 1024);
                             for (int h = 0; h < 2 && ok; ++h) {      // O_t += P_t V_j, half of the keys as soon as their weights are there
                                 ok = wait(bar_p + 2 * t + h, i & 1);
@@ -513,11 +665,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             if (!ok) break;
                             umma_commit(bar_o + t);
                         }
-                        if (j + 1 < t_end && in(t, j + 1)) scores(t, j + 1, ik);
+                        if (next < t_end && in(t, next)) scores(t, next, ik);
                     }
                     if (ok) {
                         umma_commit(bar_free + stage(iv));
-                        if (j + 1 < t_end) umma_commit(bar_free + stage(ik));
+                        if (next < t_end) umma_commit(bar_free + stage(ik));
                     }
                 }
                 // no product may be in flight when the block ends
@@ -540,7 +692,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (page < 0) b.tell(KDA_ERR_BLOCK_TABLE);
                 return page;
             };
-            int row = 0, next_row = 0, page = look(t_begin, row), next_page = -1, i = 0;
+            int row = 0, row1 = 0, page = look(t_begin, row), page1 = -1, i = 0;
+            if constexpr (turns) page1 = look(t_begin + (total > 1 ? ring_tile(1) : 0), row1);      // of the ring's next tile
             if (a.q_boxes && t_begin < t_end) {
                 // 128 rows are whole tokens of g heads.  Rows behind the sequence's last one come along, and stay by themselves.
                 const int tiles = u.rows > 128 ? 2 : 1;
@@ -554,11 +707,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                                  : "memory");
             }
             for (; i < total; ++i) {
-                const int j = t_begin + (i >> 1), s = stage(i);
-                const bool isv = i & 1;
+                const int j = t_begin + ring_tile(i), s = stage(i);
+                const bool isv = ring_is_v(i);
                 if (i >= L::kStages) ok = warp_wait(bar_free + s, turn(i - L::kStages));
                 if (!ok) break;
-                if (!isv) next_page = look(j + 1, next_row);
                 uint64_t* f = isv && partial(j) ? bar_part + s : bar_full + s;
                 const int loads = __popc(__ballot_sync(0xffffffffu, page >= 0));
                 if (lane == 0) mbar_expect_tx(f, loads * box_bytes);
@@ -570,23 +722,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                                  "l"(map), "r"(smem_u32(f)), "r"(half * 64), "r"(row), "r"(hk), "r"(page)
                                  : "memory");
                 }
-                if (isv) {
-                    page = next_page;
-                    row = next_row;
+                if (turns || isv) {
+                    page = page1;
+                    row = row1;
                 }
+                if (turns ? i + 2 < total : !isv) page1 = look(turns ? t_begin + ring_tile(i + 2) : j + 1, row1);
             }
             // no copy may be in flight when the block ends
             if (!ok && a.q_boxes && lane == 0) mbar_poll(bar_q, 0, kSpinLimit / 8);
             if (!ok && lane == 0)
                 for (int x = i > L::kStages ? i - L::kStages : 0; x < i; ++x)
-                    mbar_poll((x & 1) && partial(t_begin + (x >> 1)) ? bar_part + stage(x) : bar_full + stage(x), turn(x), kSpinLimit / 8);
+                    mbar_poll(ring_is_v(x) && partial(t_begin + ring_tile(x)) ? bar_part + stage(x) : bar_full + stage(x), turn(x), kSpinLimit / 8);
         } else {
             // -------------------------------------------------------------- V tiles that some row sees only in part
             uint32_t phase = 0;      // of each stage's barrier
             bool odd = false;
             for (int j = t_begin; j < t_end; ++j) {
                 if (!partial(j)) continue;
-                const int i = 2 * (j - t_begin) + 1, s = stage(i);
+                const int i = ring_v(j - t_begin), s = stage(i);
                 const bool ok = warp_wait(bar_part + s, (phase >> s) & 1u);
                 phase ^= 1u << s;
                 uint8_t* v = sm + L::kRing + s * L::kTile;
@@ -642,6 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
+    if (KEYS == kOwnKeys) dependency_wait();
 }
 
 // Joins the parts of 32 rows: a warp four of them, eight lanes a row.
@@ -704,128 +858,169 @@ __global__ void __launch_bounds__(256) attn_tc_join_kernel(const __grid_constant
 }
 
 struct SharedJoin {
-    Args prefix, own;       // `own` without row_o
-    const float* row_o;     // [tokens * q_heads][D] and (maximum, sum) of each row, or null
-    const float2* row_ml;
+    Args prefix, own;       // `own`: without `rows`
+    OwnRows rows;           // rows.spans null: own keys are in `own`
+    int per_row;            // warps a row
 };
-// Joins the parts of the prefix and of the own keys, 32 rows a block: a warp four of them, eight lanes a row.
+// Joins the parts of the prefix and of the own keys.  DP / 4 lanes read a part's sums of a row, 16 bytes each; a warp takes one part or two at
+// a time, and few rows have several warps each.
+constexpr int kSharedWarps = 8;
 template <int DP>
-__global__ void __launch_bounds__(256) attn_shared_join_kernel(const __grid_constant__ SharedJoin j) {
+__global__ void __launch_bounds__(32 * kSharedWarps, 3) attn_shared_join_kernel(const __grid_constant__ SharedJoin j) {
+    constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes, kAhead = 8;
+    __shared__ float4 sums_o[kSharedWarps][kLanes];
     const GroupView& groups = j.prefix.c.batch;
     const OwnView& b = groups;
     const int g = j.prefix.c.heads.group, D = j.prefix.c.heads.dim, Hk = j.prefix.c.heads.kv_heads, Hq = j.prefix.c.heads.q_heads;
-    const int lane = threadIdx.x & 31, l8 = lane & 7;
-    const long long rows = (long long)b.tokens * Hq, at = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
-    const bool is = at < rows;
-    const size_t row = (size_t)(is ? at : rows - 1);
-    const int tok = (int)(row / Hq), head = (int)(row - (size_t)tok * Hq), hk = head / g;
-    const int n = b.seq_of<8>(tok, l8, 0xffu << (lane & 24));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % j.per_row;      // of the row's warps
+    const long long rows = (long long)b.tokens * Hq, at = ((long long)blockIdx.x * kSharedWarps + warp) / j.per_row;
+    const size_t row = (size_t)(at < rows ? at : rows - 1);
+    const int tok = (int)(row / Hq), head = (int)(row - (size_t)tok * Hq), hk = head / g, hg = head - hk * g;
+    const int n = b.seq_of<32>(tok, lane, 0xffffffffu);
     int first, count;
     b.Batch::span(n, first, count);
     const int base = b.kv_len(n) - count, group = b.group_of(n), prefix = group < 0 ? 0 : b.prefix_len(group);
     const bool inside = tok >= first && tok < first + count, shares = inside && prefix > 0 && base >= prefix;
-    // Where a pass over sequences (or groups) that start at token `from` has this row.
+    // Where a pass over sequences (or groups) whose first token is `from` and whose first slot `start` has this row.  What the device
+    // arrays say is not trusted as an index: parts there are none of outside of the slots.
     struct Place {
         int slot, row;
     };
-    auto place_in = [&](const Args& a, int start, int from) {
-        const long long r = (long long)(tok - from) * g + (head - hk * g);
-        return Place{start + (int)(r / kRows), (int)(r % kRows)};
+    auto place_in = [&](int start, int from, int tile) {
+        const long long r = (long long)(tok - from) * g + hg;
+        return Place{r < 0 ? -1 : start + (int)(r / tile), (int)(r % tile)};
     };
-    Place of_prefix{0, 0}, of_own{0, 0};
-    int n_prefix = 0, n_own = inside ? 1 : 0;
-    if (shares) of_prefix = place_in(j.prefix, j.prefix.tiles.start(groups, group), groups.edge(group));
-    if (inside && j.row_o == nullptr) of_own = place_in(j.own, j.own.tiles.start(b, n), first);
+    Place of_prefix{-1, 0}, of_own{-1, 0};
+    if (shares) of_prefix = place_in(j.prefix.tiles.start(groups, group), groups.edge(group), j.prefix.tiles.rows);
+    if (inside && j.rows.spans == nullptr) of_own = place_in(j.own.tiles.start(b, n), first, kRows);
     dependency_wait();
-    // what the device arrays say is not trusted as an index
     auto parts_of = [&](const Args& a, const Place& p) {
-        if ((unsigned)p.slot >= (unsigned)a.slots || p.row < 0) return 0;
-        const int parts = __float_as_int(ld_after_f32(reinterpret_cast<const float*>(a.parts + p.slot * Hk + hk)));
-        return min(max(parts, 0), a.splits);
+        if ((unsigned)p.slot >= (unsigned)a.slots) return 0;
+        return min(max(__float_as_int(ld_after_f32(reinterpret_cast<const float*>(a.parts + p.slot * Hk + hk))), 0), a.splits);
     };
-    if (shares) n_prefix = parts_of(j.prefix, of_prefix);
-    if (inside && j.row_o == nullptr) n_own = parts_of(j.own, of_own);
-    const int parts = n_prefix + n_own;
-    auto part_at = [&](int k, const Args*& a, const Place*& p, int& z) {
-        const bool of = k < n_prefix;
-        a = of ? &j.prefix : &j.own;
-        p = of ? &of_prefix : &of_own;
-        z = of ? k : k - n_prefix;
+    const int n_prefix = parts_of(j.prefix, of_prefix);
+    int n_own = 0, stretch = -1;
+    if (j.rows.spans == nullptr) {
+        n_own = parts_of(j.own, of_own);
+    } else if (inside) {
+        const uint2 span = ld_after8(j.rows.spans + n * Hk + hk);
+        stretch = (int)span.x;
+        n_own = 1;
+        if (stretch >= 0) {
+            stretch = min(stretch, j.rows.blocks - 1);
+            n_own = min(max((int)span.y, stretch), j.rows.blocks - 1) - stretch + 1;
+        }
+    }
+    const int parts = n_prefix + n_own, in_seq = min((tok - first) * g + hg, j.rows.rows - 1);
+    // (maximum, sum) of part k, and its sums' piece of this lane
+    auto part_in = [&](const Args& a, const Place& p, int z) { return ((size_t)z * a.slots + p.slot) * Hk + hk; };
+    auto stretch_row = [&](int k) { return ((size_t)(stretch + k) * 2 + (k == 0 ? 1 : 0)) * j.rows.rows + in_seq; };
+    auto ml_of = [&](int k) -> const float2* {
+        if (k < n_prefix) return j.prefix.part_ml + part_in(j.prefix, of_prefix, k) * j.prefix.tiles.rows + of_prefix.row;
+        k -= n_prefix;
+        if (j.rows.spans == nullptr) return j.own.part_ml + part_in(j.own, of_own, k) * kRows + of_own.row;
+        return stretch < 0 ? j.rows.row_ml + row : j.rows.part_ml + stretch_row(k);
     };
-    auto ml_at = [&](int k) -> const float2* {
-        if (k >= n_prefix && j.row_o != nullptr) return j.row_ml + row;
-        const Args* a;
-        const Place* p;
-        int z;
-        part_at(k, a, p, z);
-        return a->part_ml + (((size_t)z * a->slots + p->slot) * Hk + hk) * kRows + p->row;
+    const int piece = lane % kLanes, d = 4 * piece;
+    auto o_of = [&](int k) -> const void* {
+        const bool in_prefix = k < n_prefix;
+        if (!in_prefix) k -= n_prefix;
+        if (!in_prefix && j.rows.spans != nullptr) return (stretch < 0 ? j.rows.row_o + row * D : j.rows.part_o + stretch_row(k) * D) + min(d, D - 4);
+        const Args& a = in_prefix ? j.prefix : j.own;
+        const Place& p = in_prefix ? of_prefix : of_own;
+        constexpr int kHalf = DP / 8;
+        return reinterpret_cast<const char*>(a.part_o + (part_in(a, p, k) * (a.tiles.rows >> 7) + (p.row >> 7)) * (128 * DP)) + piece / kHalf * (128 * DP * 2) +
+               part_off<DP>(p.row & 127, piece % kHalf);
     };
+    // Everything that is read depends on the number of parts only, and the first sums are on their way while the maximum is looked for.
+    const int sub = lane / kLanes, step = j.per_row * kAtOnce;
     float m = -INFINITY, l = 0.f;
-    for (int k = l8; k < parts; k += 8) m = max_nan(m, ld_after_f32(&ml_at(k)->x));
+    f2 acc[2] = {f2_all(0.f), f2_all(0.f)};
+    uint4 v[kAhead];
+    auto fetch = [&](int k0) {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffu << (lane & 24), m, o));
-    constexpr int kPieces = DP / 32, kAhead = 4;      // pieces of four values a lane: l8, l8 + 8, ... of the row's; parts on their way
-    f2 acc[kPieces][2];
+        for (int x = 0; x < kAhead; ++x)
+            if (k0 + x * step < parts) v[x] = ld_after16(o_of(min(k0 + x * step + sub, parts - 1)));
+    };
+    uint2 ml = make_uint2(0xff800000u, 0u);      // of part `lane`, then of part 32 + lane, ...
+    if (lane < parts) ml = ld_after8(ml_of(lane));
+    fetch(mine * kAtOnce);
+    m = __uint_as_float(ml.x);
+    for (int k = lane + 32; k < parts; k += 32) m = max_nan(m, ld_after_f32(&ml_of(k)->x));
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) acc[i][0] = acc[i][1] = f2_all(0.f);
-    for (int k0 = 0; k0 < parts; k0 += kAhead) {
-        uint2 ml[kAhead];
-        uint4 v[kAhead][kPieces];
+    for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    int from = 0;      // ml is that of part from + lane
+    float weight = 0.f;
+    auto weigh = [&]() {
+        const float top = __uint_as_float(ml.x);
+        weight = top == -INFINITY ? 0.f : ex2(top - m);      // without a key its sums are 0, or were not written
+        if (mine == 0) l = fmaf(top == -INFINITY ? 0.f : __uint_as_float(ml.y), weight, l);
+    };
+    weigh();
+    for (int k0 = mine * kAtOnce; k0 < parts;) {
+        const int next = k0 + step * kAhead;
 #pragma unroll
         for (int x = 0; x < kAhead; ++x) {
-            const int k = min(k0 + x, parts - 1);
-            ml[x] = ld_after8(ml_at(k));
-            if (k >= n_prefix && j.row_o != nullptr) {
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i) {
-                    const int d = 4 * (l8 + 8 * i);
-                    // a row without a key has no sums there
-                    v[x][i] = d < D && __uint_as_float(ml[x].x) != -INFINITY ? ld_after16(j.row_o + row * D + d) : make_uint4(0, 0, 0, 0);
-                }
-                continue;
+            const int k = k0 + x * step;      // of the warp: part k, or k and k + 1
+            if (k >= parts) break;
+            while (k >= from + 32) {
+                from += 32;
+                ml = make_uint2(0xff800000u, 0u);
+                if (from + lane < parts) ml = ld_after8(ml_of(from + lane));
+                weigh();
             }
-            const Args* a;
-            const Place* p;
-            int z;
-            part_at(k, a, p, z);
-            const size_t part = ((size_t)z * a->slots + p->slot) * Hk + hk;
-            const char* src = reinterpret_cast<const char*>(a->part_o + (part * 2 + (p->row >> 7)) * (128 * DP));
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int piece = l8 + 8 * i, half = piece / (DP / 8), c = piece % (DP / 8);
-                v[x][i] = ld_after16(src + half * (128 * DP * 2) + part_off<DP>(p->row & 127, c));
+            const float f = __shfl_sync(0xffffffffu, weight, k - from + sub);
+            const bool is = k + sub < parts && f != 0.f;      // NaN is
+            if (is) {
+                acc[0] = f2_fma(f2_make(__uint_as_float(v[x].x), __uint_as_float(v[x].y)), f2_all(f), acc[0]);
+                acc[1] = f2_fma(f2_make(__uint_as_float(v[x].z), __uint_as_float(v[x].w)), f2_all(f), acc[1]);
             }
         }
-#pragma unroll
-        for (int x = 0; x < kAhead; ++x) {
-            const float top = __uint_as_float(ml[x].x);
-            if (k0 + x >= parts || top == -INFINITY) continue;      // without a key its sums are 0
-            const float f = ex2(top - m);
-            l = fmaf(__uint_as_float(ml[x].y), f, l);
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                acc[i][0] = f2_fma(f2_make(__uint_as_float(v[x][i].x), __uint_as_float(v[x][i].y)), f2_all(f), acc[i][0]);
-                acc[i][1] = f2_fma(f2_make(__uint_as_float(v[x][i].z), __uint_as_float(v[x][i].w)), f2_all(f), acc[i][1]);
-            }
+        k0 = next;
+        if (k0 < parts) fetch(k0);
+    }
+    if (mine == 0)
+        while (from + 32 < parts) {      // sums of parts that are other warps'
+            from += 32;
+            ml = from + lane < parts ? ld_after8(ml_of(from + lane)) : make_uint2(0xff800000u, 0u);
+            weigh();
+        }
+    l = warp_sum(l);
+    float2 oa = f2_get(acc[0]), ob = f2_get(acc[1]);
+    if (kAtOnce == 2) {
+        oa.x += __shfl_xor_sync(0xffffffffu, oa.x, 16);
+        oa.y += __shfl_xor_sync(0xffffffffu, oa.y, 16);
+        ob.x += __shfl_xor_sync(0xffffffffu, ob.x, 16);
+        ob.y += __shfl_xor_sync(0xffffffffu, ob.y, 16);
+    }
+    if (j.per_row > 1) {
+        if (sub == 0) sums_o[warp][piece] = make_float4(oa.x, oa.y, ob.x, ob.y);
+        __syncthreads();
+        if (mine != 0) return;
+        for (int w = 1; w < j.per_row; ++w) {
+            const float4 x = sums_o[warp + w][piece];
+            oa.x += x.x; oa.y += x.y; ob.x += x.z; ob.y += x.w;
         }
     }
-    if (!is || !inside) return;
+    if (at >= rows || !inside) return;
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
-    if (l8 == 0 && j.prefix.c.lse != nullptr) j.prefix.c.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-        const int d = 4 * (l8 + 8 * i);
-        if (d < D)
-            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(j.prefix.c.o) + row * D + d) =
-                make_uint2(f2_to_bf16(f2_mul(acc[i][0], f2_all(inv))), f2_to_bf16(f2_mul(acc[i][1], f2_all(inv))));
-    }
+    if (lane == 0 && j.prefix.c.lse != nullptr) j.prefix.c.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
+    if (sub == 0 && d < D)
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(j.prefix.c.o) + row * D + d) = make_uint2(pack_bf16(oa.x * inv, oa.y * inv), pack_bf16(ob.x * inv, ob.y * inv));
 }
 
 template <int DP, int KEYS>
 int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CUtensorMap& mQ, const CUtensorMap& mO, const Args& a, cudaStream_t st) {
     if (int rc = set_smem_limit(attn_tc_kernel<DP, KEYS>, Layout<DP>::kBytes)) return rc;
-    const dim3 grid((unsigned)a.slots, (unsigned)c.heads.kv_heads, (unsigned)a.splits);
-    KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP, KEYS><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
+    const bool list = (KEYS == kPrefixKeys || KEYS == kTurnKeys) && a.splits > 1;      // prefix_unit: a block an SM
+    const dim3 grid(list ? 148u : (unsigned)a.slots, list ? 1u : (unsigned)c.heads.kv_heads, list ? 1u : (unsigned)a.splits);
+    if constexpr (KEYS == kOwnKeys) {      // beside the pass over the prefix
+        cudaError_t e = cudaSuccess;
+        KDA_LAUNCH("attn_tc_kernel", st, e = launch_early(attn_tc_kernel<DP, KEYS>, grid, kThreads, Layout<DP>::kBytes, st, true, 1, mK, mV, mQ, mO, a));
+        if (e != cudaSuccess) return KDA_ERR_CUDA;
+    } else {
+        KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP, KEYS><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
+    }
     if (int rc = launch_status()) return rc;
     if (a.splits == 1 || KEYS != kAllKeys) return KDA_OK;
     const dim3 joins((unsigned)a.slots * 8, (unsigned)c.heads.kv_heads);
@@ -858,17 +1053,18 @@ void place_parts(Args& a, const Call& c) {
     char* ws = static_cast<char*>(c.workspace);
     a.parts = reinterpret_cast<int*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + align_up(units * sizeof(int), 256));
-    a.part_o = reinterpret_cast<float*>(a.part_ml + units * a.splits * kRows);
+    a.part_o = reinterpret_cast<float*>(a.part_ml + units * a.splits * a.tiles.rows);
 }
 Args args_of(const Call& c, int keys, int splits) {
     Args a;
     a.c = c;
-    a.tiles = Tiles{kRows, c.heads.group, 0};
-    a.slots = (int)(keys == kPrefixKeys ? group_slots(c.batch, c.heads.group, kRows, a.tiles.per_seq)
-                                        : tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq));
+    const bool prefix = keys == kPrefixKeys || keys == kTurnKeys;
+    a.tiles = Tiles{keys == kTurnKeys ? 128 : kRows, c.heads.group, 0};
+    a.slots = (int)(prefix ? group_slots(c.batch, c.heads.group, a.tiles.rows, a.tiles.per_seq)
+                           : tile_slots(c.batch.tokens, c.batch.n_seq, c.max_q_len, c.heads.group, kRows, c.batch.cu != nullptr, a.tiles.per_seq));
     a.splits = splits;
     a.box_rows = c.batch.page_size < kKeys ? c.batch.page_size : kKeys;
-    a.q_boxes = 0;
+    a.q_boxes = a.own_rows = 0;
     a.parts = nullptr;
     a.part_ml = nullptr;
     a.part_o = nullptr;
@@ -877,8 +1073,9 @@ Args args_of(const Call& c, int keys, int splits) {
 }
 
 template <int KEYS>
-int pass(const Call& c, int splits, cudaStream_t st) {
+int pass(const Call& c, int splits, int own_rows, cudaStream_t st) {
     Args a = args_of(c, KEYS, splits);
+    a.own_rows = own_rows;
     CUtensorMap mK, mV, mQ, mO;
     const Strides& s = c.strides;
     int rc = make_map_paged(&mK, c.k, c.heads.dim, c.batch.page_size, c.heads.kv_heads, c.batch.n_pages, s.k_row, s.k_head, s.k_page, a.box_rows);
@@ -894,31 +1091,35 @@ int pass(const Call& c, int splits, cudaStream_t st) {
 
 }  // namespace
 
-int tc(const Call& c, int splits, cudaStream_t st) { return pass<kAllKeys>(c, splits, st); }
-int tc_prefix(const Call& c, int splits, cudaStream_t st) { return pass<kPrefixKeys>(c, splits, st); }
-int tc_own(const Call& c, int splits, cudaStream_t st) { return pass<kOwnKeys>(c, splits, st); }
+int tc(const Call& c, int splits, cudaStream_t st) { return pass<kAllKeys>(c, splits, 0, st); }
+bool in_turns(const Call& c) { return prefix_rows(c.batch.tokens, c.batch.p.n, c.heads.group) == 128; }
+int tc_prefix(const Call& c, int splits, bool own_rows, cudaStream_t st) {
+    return in_turns(c) ? pass<kTurnKeys>(c, splits, own_rows, st) : pass<kPrefixKeys>(c, splits, own_rows, st);
+}
+int tc_own(const Call& c, int splits, cudaStream_t st) { return pass<kOwnKeys>(c, splits, 0, st); }
 
-int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const float* row_o, const float2* row_ml, cudaStream_t st) {
+int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const OwnRows* rows, cudaStream_t st) {
     SharedJoin j;
-    j.prefix = args_of(prefix, kPrefixKeys, prefix_splits);
-    j.own = row_o == nullptr ? args_of(own, kOwnKeys, own_splits) : j.prefix;
-    j.row_o = row_o;
-    j.row_ml = row_ml;
-    const long long rows = (long long)prefix.batch.tokens * prefix.heads.q_heads;
+    j.prefix = args_of(prefix, in_turns(prefix) ? kTurnKeys : kPrefixKeys, prefix_splits);
+    j.own = rows == nullptr ? args_of(own, kOwnKeys, own_splits) : j.prefix;
+    j.rows = rows == nullptr ? OwnRows{} : *rows;
+    const long long all = (long long)prefix.batch.tokens * prefix.heads.q_heads;
+    for (j.per_row = kSharedWarps; j.per_row > 1 && all * j.per_row > 2 * 148 * kSharedWarps;) j.per_row >>= 1;
+    const long long blocks = (all * j.per_row + kSharedWarps - 1) / kSharedWarps;
     auto kern = prefix.heads.dim <= 64 ? attn_shared_join_kernel<64> : attn_shared_join_kernel<128>;
     cudaError_t e = cudaSuccess;
-    KDA_LAUNCH("attn_shared_join_kernel", st, e = launch_early(kern, dim3((unsigned)((rows + 31) / 32)), 256, 0, st, true, 1, j));
+    KDA_LAUNCH("attn_shared_join_kernel", st, e = launch_early(kern, dim3((unsigned)blocks), 32 * kSharedWarps, 0, st, true, 1, j));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
 // of a call whose rows are cut into `splits` parts at most
 size_t tc_workspace(long long slots, int kv_heads, int splits, int dim) {
     if (splits < 2) return 0;
-    return tc_parts_bytes(slots, kv_heads, splits, dim);
+    return tc_parts_bytes(slots, kRows, kv_heads, splits, dim);
 }
-size_t tc_parts_bytes(long long slots, int kv_heads, int splits, int dim) {
+size_t tc_parts_bytes(long long slots, int rows, int kv_heads, int splits, int dim) {
     const size_t units = (size_t)slots * kv_heads, width = dim <= 64 ? 64 : 128;
-    return align_up(units * sizeof(int), 256) + units * splits * kRows * (sizeof(float2) + width * sizeof(float));
+    return align_up(units * sizeof(int), 256) + units * splits * rows * (sizeof(float2) + width * sizeof(float));
 }
 
 }  // namespace attn

@@ -20,7 +20,7 @@ namespace kda {
 namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32, kBlocks = 8, kColumns = 128;
-constexpr int kMaxRows = 16384;      // two numbers a row in shared memory
+constexpr int kMaxRows = 16384;      // three numbers a row in shared memory
 
 struct PlanArgs {
     int* table;
@@ -66,31 +66,35 @@ __device__ __forceinline__ Ask ask_of(const PlanArgs& a, int n) {
     return r;
 }
 
-// Exclusive sums over the block's threads, and the totals.
-struct Pair {
-    long long need, add;
+// Entries lacking, new tokens and free pages.  The host sees to it that the first and the last fit in 32 bits; new tokens stop at kFull, which is
+// more than any step takes.
+struct Sums {
+    int need, add, free_;
 };
-__device__ __forceinline__ Pair block_scan(Pair mine, Pair* sums, Pair& total) {
+constexpr int kMostTokens = 1 << 30, kFull = kMostTokens + 1;
+__device__ __forceinline__ int add_tokens(int a, int b) { return (int)min((unsigned)a + (unsigned)b, (unsigned)kFull); }
+__device__ __forceinline__ Sums operator+(Sums a, Sums b) { return Sums{a.need + b.need, add_tokens(a.add, b.add), a.free_ + b.free_}; }
+// Sums over the block's threads up to, and without, this one; `total` over all.  `sums` has a place a warp and is written anew by each call.
+__device__ __forceinline__ Sums block_scan(Sums mine, Sums* sums, Sums& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Pair upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, upto.need, o), y = __shfl_up_sync(0xffffffffu, upto.add, o);
-        if (lane >= o) upto.need += x, upto.add += y;
-    }
+    auto scan = [&](Sums x) {
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+            const Sums y{__shfl_up_sync(0xffffffffu, x.need, o), __shfl_up_sync(0xffffffffu, x.add, o), __shfl_up_sync(0xffffffffu, x.free_, o)};
+            if (lane >= o) x = x + y;
+        }
+        return x;
+    };
+    auto from = [&](Sums x, int l) { return Sums{__shfl_sync(0xffffffffu, x.need, l), __shfl_sync(0xffffffffu, x.add, l), __shfl_sync(0xffffffffu, x.free_, l)}; };
+    const Sums upto = scan(mine);
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    const Pair of = sums[lane];      // kWarps == 32
-    Pair before = of;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, before.need, o), y = __shfl_up_sync(0xffffffffu, before.add, o);
-        if (lane >= o) before.need += x, before.add += y;
-    }
-    total = Pair{__shfl_sync(0xffffffffu, before.need, 31), __shfl_sync(0xffffffffu, before.add, 31)};
-    const Pair base = Pair{__shfl_sync(0xffffffffu, before.need - of.need, warp), __shfl_sync(0xffffffffu, before.add - of.add, warp)};
-    __syncthreads();
-    return Pair{base.need + upto.need - mine.need, base.add + upto.add - mine.add};
+    const Sums warps = scan(sums[lane]);      // kWarps == 32
+    total = from(warps, 31);
+    Sums base = from(warps, max(warp - 1, 0)), before{__shfl_up_sync(0xffffffffu, upto.need, 1), __shfl_up_sync(0xffffffffu, upto.add, 1), __shfl_up_sync(0xffffffffu, upto.free_, 1)};
+    if (warp == 0) base = Sums{0, 0, 0};
+    if (lane == 0) before = Sums{0, 0, 0};
+    return base + before;
 }
 static_assert(kWarps == 32, "a warp sums up the warps");
 
@@ -110,45 +114,74 @@ __device__ __forceinline__ unsigned free_bits(const unsigned char* flags, int at
     return bits;
 }
 
+// The items (a row, 128 of its columns) of a table are dealt out to the warps in runs of at most 32; lane l of a warp has what the row of
+// the run's l-th item asks for.
+struct Run {
+    int first, many;      // items
+    int row, col0, col1, col1_without;      // of this lane's item: its row, the columns that shall be held, and their end without the new tokens
+};
+
 __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_constant__ PlanArgs a) {
     extern __shared__ int rows_sm[];
-    int *base_of = rows_sm, *cu = rows_sm + a.rows;      // entries lacking before a row (-1: it is not served); [rows + 1]
-    __shared__ Pair sums[kWarps];
+    // of each row: entries lacking before it (-1: it is not served); new tokens, then the sum before it; its length.   With one block entries missing follow, [items]
+    int *base_of = rows_sm, *cu = base_of + a.rows, *len_of = cu + a.rows + 1;
+    __shared__ Sums sums[2][kWarps];
     __shared__ int counts[kBlocks];                      // free pages of each block's share
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = gridDim.x, rank = blockIdx.x;     // the grid is one cluster
+    int* missing = blocks > 1 ? a.missing : len_of + a.rows;
     auto meet = [&]() {
         if (blocks > 1) cluster_sync();
         else __syncthreads();
     };
+    const int all = a.rows * a.items, warps = blocks * kWarps, run = min((all + warps - 1) / warps, 32);
+    auto run_at = [&](int i0) {
+        Run r{i0, min(run, all - i0), 0, 0, 0, 0};
+        if (lane < r.many) {
+            r.row = (i0 + lane) / a.items;
+            const Ask ask = ask_of(a, r.row);
+            r.col0 = ask.first(a.page);
+            r.col1 = ask.end(a.page);
+            r.col1_without = ask.end_without(a.page);
+        }
+        return r;
+    };
 
     // ------------------------------------------------------------------ 1: what rows hold, and lack
-    const int all = a.rows * a.items;
-    for (int i = rank * kWarps + warp; i < all; i += blocks * kWarps) {
-        const int n = i / a.items, c0 = (i - n * a.items) * kColumns + lane;
-        const Ask r = ask_of(a, n);
-        if (lane == 0 && i == n * a.items) {
-            if (r.bad_len) a.tell(KDA_ERR_BLOCK_TABLE);
-            if (r.bad_new) a.tell(KDA_ERR_CU_SEQLENS);
-        }
-        const int first = r.first(a.page), end = r.end(a.page);
-        int* row = a.table + n * a.table_stride;
-        int entry[kColumns / 32], lacks = 0;
+    constexpr int kAtOnce = 4, kEach = kColumns / 32;
+    for (int i0 = (rank * kWarps + warp) * run; i0 < all; i0 += warps * run) {
+        const Run r = run_at(i0);
+        int lacks = 0;
+        for (int x = 0; x < r.many; x += kAtOnce) {
+            int entry[kAtOnce][kEach];
 #pragma unroll
-        for (int k = 0; k < kColumns / 32; ++k) entry[k] = c0 + 32 * k < a.width ? row[c0 + 32 * k] : -1;
+            for (int y = 0; y < kAtOnce; ++y) {
+                const int n = __shfl_sync(0xffffffffu, r.row, min(x + y, r.many - 1)), c0 = (i0 + x + y - n * a.items) * kColumns + lane;
 #pragma unroll
-        for (int k = 0; k < kColumns / 32; ++k) {
-            const int c = c0 + 32 * k;
-            const bool names = (unsigned)entry[k] < (unsigned)a.n_pages, held = c >= first && c < end;
-            if (entry[k] >= a.n_pages) a.tell(KDA_ERR_BLOCK_TABLE);
-            if (held && !names) ++lacks;
-            if (!held && c < a.width && entry[k] != -1) {
-                if (names) a.free_[entry[k]] = 1;
-                row[c] = -1;
+                for (int k = 0; k < kEach; ++k) entry[y][k] = x + y < r.many && c0 + 32 * k < a.width ? a.table[n * a.table_stride + c0 + 32 * k] : -1;
+            }
+#pragma unroll
+            for (int y = 0; y < kAtOnce; ++y) {
+                const int l = min(x + y, r.many - 1), n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + lane;
+                const int first = __shfl_sync(0xffffffffu, r.col0, l), end = __shfl_sync(0xffffffffu, r.col1, l);
+                if (x + y >= r.many) break;
+                int here = 0;
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    const int c = c0 + 32 * k, e = entry[y][k];
+                    const bool names = (unsigned)e < (unsigned)a.n_pages, held = c >= first && c < end;
+                    if (e >= a.n_pages) a.tell(KDA_ERR_BLOCK_TABLE);
+                    if (held && !names) ++here;
+                    if (!held && e != -1) {
+                        if (names) a.free_[e] = 1;
+                        a.table[n * a.table_stride + c] = -1;
+                    }
+                }
+                here = __reduce_add_sync(0xffffffffu, here);
+                if (lane == l) lacks = here;
             }
         }
-        lacks = __reduce_add_sync(0xffffffffu, lacks);
-        if (lane == 0) a.missing[i] = lacks;
+        if (lane < r.many) missing[i0 + lane] = lacks;
     }
     meet();
 
@@ -159,25 +192,30 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     int my_free = 0;
     for (int p = my_p0; p < my_p1; p += 16) my_free += __popc(free_bits(a.free_, p, my_p1, wide));
     const int each = (a.rows + kThreads - 1) / kThreads, n0 = min(tid * each, a.rows), n1 = min(n0 + each, a.rows);
-    Pair mine{0, 0}, total;
+    Sums mine{0, 0, my_free}, total;
+#pragma unroll 4
     for (int n = n0; n < n1; ++n) {
         int need = 0;
-        for (int i = 0; i < a.items; ++i) need += a.missing[n * a.items + i];
+        for (int i = 0; i < a.items; ++i) need += missing[n * a.items + i];
+        const Ask r = ask_of(a, n);
+        if (n % blocks == rank) {
+            if (r.bad_len) a.tell(KDA_ERR_BLOCK_TABLE);
+            if (r.bad_new) a.tell(KDA_ERR_CU_SEQLENS);
+        }
         base_of[n] = need;
-        mine.need += need;
-        mine.add += ask_of(a, n).add;
+        cu[n] = r.add;
+        len_of[n] = r.len;
+        mine = mine + Sums{need, r.add, 0};
     }
-    Pair before = block_scan(mine, sums, total);
-    Pair shares;
-    const int free_before = (int)block_scan(Pair{my_free, 0}, sums, shares).need;
+    const Sums before = block_scan(mine, sums[0], total);
     if (blocks > 1) {
         if (tid < blocks) {
             uint32_t at;
             asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(counts + rank)), "r"(tid));
-            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"((int)shares.need) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(total.free_) : "memory");
         }
     } else if (tid == 0) {
-        counts[0] = (int)shares.need;
+        counts[0] = total.free_;
     }
     meet();
 
@@ -187,19 +225,28 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
         if (b < rank) free_base += counts[b];
         free_all += counts[b];
     }
-    mine = Pair{0, 0};
+    Sums upto = before;
+    bool all_served = true;
+    mine = Sums{0, 0, 0};
     for (int n = n0; n < n1; ++n) {
-        const int need = base_of[n], add = ask_of(a, n).add;
-        const long long upto = before.need + need, tokens = before.add + add;
-        const bool served = (upto <= free_all && tokens <= a.max_tokens) || (need == 0 && add == 0);
-        base_of[n] = served ? (int)before.need : -1;
-        cu[n] = served ? add : 0;
-        if (served) mine.need += need, mine.add += add;
-        before = Pair{upto, tokens};
+        const Sums row{base_of[n], cu[n], 0};
+        upto = upto + row;
+        const bool served = (upto.need <= free_all && upto.add <= a.max_tokens) || (row.need == 0 && row.add == 0);
+        if (served) {
+            base_of[n] = upto.need - row.need;
+            mine = mine + row;
+        } else {
+            base_of[n] = -1;
+            cu[n] = 0;
+            len_of[n] -= row.add;
+            all_served = false;
+        }
     }
-    Pair given = block_scan(mine, sums, total);
-    const int dealt = (int)total.need;
-    int at = (int)given.add;
+    // Rows that lack pages and are served are the first of those that lack any, so the sums of all rows hold for what they lack, and for
+    // the tokens too if nobody waits.
+    int at = before.add;
+    if (!__syncthreads_and(all_served)) at = block_scan(mine, sums[1], total).add;
+    const int dealt = total.need;
     for (int n = n0; n < n1; ++n) {
         const int add = cu[n];
         cu[n] = at;
@@ -207,11 +254,11 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
         at += add;
     }
     if (tid == 0) {
-        cu[a.rows] = (int)total.add;
-        if (rank == 0) a.cu[a.rows] = (int)total.add;
+        cu[a.rows] = total.add;
+        if (rank == 0) a.cu[a.rows] = total.add;
     }
     if (dealt > 0) {
-        int k = free_base + free_before;
+        int k = free_base + before.free_;
         for (int p = my_p0; p < my_p1 && k < dealt; p += 16) {
             unsigned bits = free_bits(a.free_, p, my_p1, wide);
             while (bits != 0 && k < dealt) {
@@ -225,60 +272,69 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     meet();
 
     // ------------------------------------------------------------------ 4: entries that were missing
-    for (int i = rank * kWarps + warp; i < all; i += blocks * kWarps) {
-        const int n = i / a.items, item = i - n * a.items, c0 = item * kColumns + lane, base = base_of[n];
-        if (base >= 0 && a.missing[i] == 0) continue;
-        const Ask r = ask_of(a, n);
-        int* row = a.table + n * a.table_stride;
-        if (base < 0) {      // it waits: its columns end where they did
-            const int end = r.end_without(a.page);
-            for (int k = 0; k < kColumns / 32; ++k) {
-                const int c = c0 + 32 * k;
-                if (c >= a.width || c < end) continue;
-                const int entry = row[c];
-                if (entry == -1) continue;
-                if ((unsigned)entry < (unsigned)a.n_pages) a.free_[entry] = 1;
-                row[c] = -1;
-            }
-            continue;
+    for (int i0 = (rank * kWarps + warp) * run; i0 < all; i0 += warps * run) {
+        const Run r = run_at(i0);
+        int lacks = 0, base = 0, from = 0;
+        if (lane < r.many) {
+            lacks = missing[i0 + lane];
+            base = from = base_of[r.row];
+            if (base >= 0 && lacks > 0)
+                for (int i = r.row * a.items; i < i0 + lane; ++i) from += missing[i];
         }
-        const int first = r.first(a.page), end = r.end(a.page);
-        int k0 = base;
-        for (int j = 0; j < item; ++j) k0 += a.missing[n * a.items + j];
-#pragma unroll 1
-        for (int k = 0; k < kColumns / 32; ++k) {
-            const int c = c0 + 32 * k;
-            const bool lacks = c >= first && c < end && (unsigned)row[c] >= (unsigned)a.n_pages;
-            const unsigned who = __ballot_sync(0xffffffffu, lacks);
-            if (lacks) row[c] = a.dealt[k0 + __popc(who & ((1u << lane) - 1))];
-            k0 += __popc(who);
+        for (unsigned todo = __ballot_sync(0xffffffffu, base < 0 || lacks > 0); todo != 0; todo &= todo - 1) {
+            const int l = __ffs(todo) - 1, n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + lane;
+            const bool waits = __shfl_sync(0xffffffffu, base, l) < 0;
+            const int first = __shfl_sync(0xffffffffu, r.col0, l), end = __shfl_sync(0xffffffffu, waits ? r.col1_without : r.col1, l);
+            int k0 = __shfl_sync(0xffffffffu, from, l), entry[kEach];
+            int* row = a.table + n * a.table_stride;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) entry[k] = c0 + 32 * k < a.width ? row[c0 + 32 * k] : -1;
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) {
+                const int c = c0 + 32 * k;
+                if (waits) {      // its columns end where they did
+                    if (c < end || entry[k] == -1) continue;
+                    if ((unsigned)entry[k] < (unsigned)a.n_pages) a.free_[entry[k]] = 1;
+                    row[c] = -1;
+                } else {
+                    const bool is = c >= first && c < end && (unsigned)entry[k] >= (unsigned)a.n_pages;
+                    const unsigned who = __ballot_sync(0xffffffffu, is);
+                    if (is) row[c] = a.dealt[k0 + __popc(who & ((1u << lane) - 1))];
+                    k0 += __popc(who);
+                }
+            }
         }
     }
     meet();
 
     // ------------------------------------------------------------------ 5: where the new tokens go
-    for (int n = rank * kThreads + tid; n < a.rows; n += blocks * kThreads) {
-        const Ask r = ask_of(a, n);
-        const int len = base_of[n] < 0 ? r.len - r.add : r.len;
-        if (base_of[n] < 0 || r.bad_len) a.kv_lens[n] = len;      // rows without tokens below
-    }
-    const int tokens = cu[a.rows];
-    for (int t = rank * kThreads + tid; t < a.max_tokens; t += blocks * kThreads) {
-        int pos = -1;
-        long long slot = -1;
-        if (t < tokens) {
+    for (int n = rank * kThreads + tid; n < a.rows; n += blocks * kThreads)
+        if (a.kv_lens[n] != len_of[n]) a.kv_lens[n] = len_of[n];
+    const int tokens = cu[a.rows], stride = blocks * kThreads;
+    for (int t0 = rank * kThreads + tid; t0 < a.max_tokens; t0 += kAtOnce * stride) {
+        int pos[kAtOnce], col[kAtOnce], entry[kAtOnce];
+#pragma unroll
+        for (int y = 0; y < kAtOnce; ++y) {
+            const int t = t0 + y * stride;
+            pos[y] = -1;
+            if (t >= tokens) continue;
             int lo = 0, hi = a.rows;      // cu[lo] <= t < cu[hi]
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (cu[mid] <= t) lo = mid;
                 else hi = mid;
             }
-            pos = a.kv_lens[lo] - (cu[lo + 1] - cu[lo]) + (t - cu[lo]);
-            const int col = pos / a.page;
-            slot = (long long)a.table[lo * a.table_stride + col] * a.page + (pos - col * a.page);
+            pos[y] = len_of[lo] - (cu[lo + 1] - t);
+            col[y] = pos[y] / a.page;
+            entry[y] = a.table[lo * a.table_stride + col[y]];
         }
-        a.positions[t] = pos;
-        a.slots[t] = slot;
+#pragma unroll
+        for (int y = 0; y < kAtOnce; ++y) {
+            const int t = t0 + y * stride;
+            if (t >= a.max_tokens) break;
+            a.positions[t] = pos[y];
+            a.slots[t] = pos[y] < 0 ? -1ll : (long long)entry[y] * a.page + (pos[y] - col[y] * a.page);
+        }
     }
 }
 
@@ -286,7 +342,7 @@ int check(const KdaPlanShape* s) {
     if (!s) return KDA_ERR_NULL;
     if (s->rows <= 0 || s->width <= 0 || s->page_size <= 0 || s->n_pages < 0 || s->max_tokens < 0) return KDA_ERR_BAD_SHAPE;
     if (s->rows > kMaxRows) return KDA_ERR_UNSUPPORTED;
-    if ((long long)s->width * s->page_size >= 1ll << 31 || (long long)s->rows * s->width >= 1ll << 31 || s->n_pages > (1 << 30) || s->max_tokens > (1 << 30))
+    if ((long long)s->width * s->page_size >= 1ll << 31 || (long long)s->rows * s->width >= 1ll << 31 || s->n_pages > (1 << 30) || s->max_tokens > kMostTokens)
         return KDA_ERR_BAD_SHAPE;
     return KDA_OK;
 }
@@ -316,11 +372,11 @@ extern "C" int kda_plan_pages(const KdaPlanShape* s, int32_t* block_table, int32
     a.dealt = reinterpret_cast<int*>(static_cast<char*>(workspace) + align_up((size_t)a.rows * a.items * sizeof(int), 256));
     a.mirror = status_mirror();
     a.table_stride = s->table_stride;
-    const size_t smem = (2 * (size_t)a.rows + 1) * sizeof(int);
-    if (int rc = set_smem_limit(plan_pages_kernel, smem)) return rc;
     // what one block reads in a few loads a thread
     const bool small = a.rows * a.items <= 2 * kWarps && a.n_pages <= 16 * kThreads && a.max_tokens <= 2 * kThreads;
     const int blocks = small ? 1 : kBlocks;
+    const size_t smem = (3 * (size_t)a.rows + 1 + (small ? a.rows * a.items : 0)) * sizeof(int);
+    if (int rc = set_smem_limit(plan_pages_kernel, smem)) return rc;
     cudaError_t e = cudaSuccess;
     KDA_LAUNCH("plan_pages_kernel", (cudaStream_t)stream,
                e = launch_early(plan_pages_kernel, dim3(blocks), kThreads, smem, (cudaStream_t)stream, false, blocks, a));

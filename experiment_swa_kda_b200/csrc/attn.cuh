@@ -128,6 +128,11 @@ struct OwnView : Batch {
         }
         return true;
     }
+    // the page of column `col` of group g's prefix, or -1
+    __device__ __forceinline__ int prefix_page(int g, int col) const {
+        const int at = __ldg(p.table + g * p.table_stride + col);
+        return (unsigned)at < (unsigned)n_pages ? at : -1;
+    }
     __device__ __forceinline__ bool prefix_ok(int g) const {
         const int len = __ldg(p.lens + g);
         return len >= 0 && (long long)len <= (long long)p.width * page_size;
@@ -145,10 +150,7 @@ struct GroupView : OwnView {
         first = edge(g);
         count = max(edge(g + 1) - first, 0);
     }
-    __device__ __forceinline__ int page(int g, int col) const {
-        const int at = __ldg(p.table + g * p.table_stride + col);
-        return (unsigned)at < (unsigned)n_pages ? at : -1;
-    }
+    __device__ __forceinline__ int page(int g, int col) const { return prefix_page(g, col); }
 };
 
 // Tiles of `rows` packed rows (token-major, the query heads of one kv head beside each other) of all sequences.  With a bound
@@ -246,10 +248,12 @@ __device__ __forceinline__ bool make_unit(const B& b, const Tiles& t, int slot, 
     return true;
 }
 // What a batch got wrong is reported by the blocks of the first tile of each sequence.
-__device__ __forceinline__ void check_batch(const GroupView& b, const Tiles&, int g, int tile) {
-    if (tile != 0) return;
+__device__ __forceinline__ void check_group(const OwnView& b, int g) {
     if (!b.groups_ok(g)) b.tell(KDA_ERR_CU_SEQLENS);
     if (!b.prefix_ok(g)) b.tell(KDA_ERR_BLOCK_TABLE);
+}
+__device__ __forceinline__ void check_batch(const GroupView& b, const Tiles&, int g, int tile) {
+    if (tile == 0) check_group(b, g);
 }
 __device__ __forceinline__ void check_batch(const Batch& b, const Tiles& t, int n, int tile) {
     if (tile != 0) return;
@@ -334,7 +338,7 @@ __device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int g
 // Whether the pass over the prefixes is cut into parts: where its row tiles leave half of the SMs idle.
 constexpr int kMaxListed = kSms / 2;
 
-enum Keys { kAllKeys, kPrefixKeys, kOwnKeys, kTurnKeys };      // kTurnKeys: a prefix by row tiles of 128 (attn_tc.cu)
+enum Keys { kAllKeys, kPrefixKeys, kOwnKeys, kTurnKeys, kBothKeys };      // kTurnKeys: a prefix by row tiles of 128 (attn_tc.cu); kBothKeys: prefix, then own
 template <int KEYS>
 struct ViewOf {
     using type = Batch;
@@ -346,6 +350,10 @@ struct ViewOf<kPrefixKeys> {
 template <>
 struct ViewOf<kTurnKeys> {
     using type = GroupView;
+};
+template <>
+struct ViewOf<kBothKeys> {
+    using type = OwnView;
 };
 template <>
 struct ViewOf<kOwnKeys> {
@@ -390,6 +398,7 @@ int general_shared(const Call& c, int prefix_splits, int own_splits, cudaStream_
 size_t general_shared_workspace(size_t rows, int parts, int dim);
 int tc_prefix(const Call& c, int splits, bool own_rows, cudaStream_t st);      // own_rows: the pass below runs beside it
 int tc_own(const Call& c, int splits, cudaStream_t st);
+int tc_both(const Call& c, int splits, cudaStream_t st);      // prefix and own keys one after the other, a finished result
 size_t tc_parts_bytes(long long slots, int rows, int kv_heads, int splits, int dim);
 // Own keys of few rows a sequence and kv head, where the token steps' kernel left them: rows of sequences that one stretch had to itself are
 // whole; of the others stretch k has [2][rows][D] sums, place 1 of a sequence that begins in it, place 0 of one that goes on.

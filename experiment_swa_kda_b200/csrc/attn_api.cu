@@ -132,6 +132,9 @@ int tc_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) {
 }
 int general_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) { return prefix_split_count(s, p, 64, 64, 2 * 148); }
 
+// Sequences whose rows fill row tiles by themselves go through the prefix and their own keys one after the other: nothing is left to join.
+bool takes_both(const KdaPagedShape& s) { return (long long)s.tokens * (s.q_heads / s.kv_heads) >= 192ll * s.n_seq; }
+
 // The shares of a workspace on the tensor cores.
 struct SharedSpace {
     size_t prefix, own;
@@ -156,6 +159,10 @@ extern "C" size_t kda_shared_prefix_attention_workspace_bytes(const KdaPagedShap
         if (!packed && s->tokens % s->n_seq != 0) continue;
         const size_t g = general_shared_workspace((size_t)s->tokens * s->q_heads, general_prefix_splits(*s, *p) + general_splits(*s, packed), s->head_dim);
         if (g > most) most = g;
+        int per;
+        const size_t both = tc_workspace(tile_slots(s->tokens, s->n_seq, packed ? s->max_q_len : s->tokens / s->n_seq, s->q_heads / s->kv_heads, 256, packed, per),
+                                         s->kv_heads, tc_splits(*s, packed), s->head_dim);
+        if (both > most) most = both;
         for (int few = 0; few < 2; ++few) {
             const SharedSpace w = shared_space(*s, *p, packed, few);
             if (w.prefix + w.own > most) most = w.prefix + w.own;
@@ -191,6 +198,7 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     c.max_q_len = packed ? s->max_q_len : q_len;
     c.workspace = workspace;
     if (!tc_takes(c)) return general_shared(c, general_prefix_splits(*s, *p), general_splits(*s, packed), st);
+    if (takes_both(*s)) return tc_both(c, tc_splits(*s, packed), st);
     const bool few = own_rows_take(c);
     const int prefix_splits = tc_prefix_splits(*s, *p), own_splits = tc_splits(*s, packed);
     Call own = c;

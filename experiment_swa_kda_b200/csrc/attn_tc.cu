@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     using L = Layout<DP>;
     // Row tiles of 128 alone: their two places take the key tiles in turns, each with sums of its own, so that one's products run while the
     // other's scores are turned into weights.
-    constexpr bool turns = KEYS == kTurnKeys, in_prefix = turns || KEYS == kPrefixKeys;
+    constexpr bool turns = KEYS == kTurnKeys, in_prefix = turns || KEYS == kPrefixKeys, both = KEYS == kBothKeys;
+    constexpr bool sums_only = in_prefix || KEYS == kOwnKeys;      // for a join
     constexpr int kPartRows = turns ? 128 : kRows;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (a.q_boxes) tma_prefetch_desc(&mQ);
     }
     int hk = blockIdx.y, z = blockIdx.z, slot = a.slots - 1 - (int)blockIdx.x, parts = 1;
-    if (KEYS != kAllKeys) dependents_go();
+    if (sums_only) dependents_go();
     Unit u;
     bool some;
     if (in_prefix && a.splits > 1) {
@@ -212,6 +213,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             int n, tile;
             if (a.tiles.find(b, slot, n, tile)) check_batch(b, a.tiles, n, tile);
         }
+        if constexpr (both)
+            if (hk == 0 && z == 0)
+                for (int i = blockIdx.x * kThreads + tid; i < b.p.n; i += gridDim.x * kThreads) check_group(b, i);
     }
     if (!some) {
         if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too
@@ -220,13 +224,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
     // keys any row of the block sees: [u.lo, u.hi); keys all of them see: [all_lo, all_hi)
     auto last_of = [&](int prow) { return in_prefix ? u.hi - 1 : u.base + prow / g; };      // a row's last key, and its first one
-    auto first_of = [&](int last) { return KEYS == kAllKeys ? first_key(last, window) : u.from; };
+    auto first_of = [&](int last) { return KEYS == kAllKeys ? first_key(last, window) : u.from; };      // both: of its own keys
     const int first_pos = last_of(u.row0), last_pos = last_of(u.row0 + u.rows - 1);
     const int all_lo = first_of(last_pos), all_hi = first_pos + 1;
     // Key tiles start at the first box in reach, not at multiples of their size: a window of 1,024 keys and 64 rows is 9 tiles, not 10.
-    const int key0 = u.lo / a.box_rows * a.box_rows, nt = max((u.hi - key0 + kKeys - 1) / kKeys, 0);
+    const int key0 = u.lo / a.box_rows * a.box_rows, np = both ? (u.from + kKeys - 1) / kKeys : 0;      // np of them are the prefix's
+    const int nt = np + max((u.hi - key0 + kKeys - 1) / kKeys, 0);
+    auto tile_key = [&](int j) { return both && j < np ? j * kKeys : key0 + (j - np) * kKeys; };
+    // of a key tile: keys any row sees, and keys all rows see
+    auto reach_lo = [&](int j) { return both && j < np ? 0 : u.lo; };
+    auto reach_hi = [&](int j) { return both && j < np ? u.from : u.hi; };
+    auto all_from = [&](int j) { return both && j < np ? 0 : all_lo; };
+    auto all_to = [&](int j) { return both && j < np ? u.from : all_hi; };
     int t_begin = 0, t_end = nt;
-    bool split = KEYS != kAllKeys;      // the sums of these passes are joined whatever their number of parts
+    bool split = sums_only;      // the sums of these passes are joined whatever their number of parts
     if (!in_prefix && a.splits > 1) {
         // The shortest parts with which all blocks run side by side, looked for by one length a warp, twice; none where they would be
         // little shorter than the longest row tile's keys (a part costs some 5 tiles of its own, and the join).  The host sees to it
@@ -235,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         int *tiles_of = reinterpret_cast<int*>(sm), *blocks_of = tiles_of + kThreads;      // nothing else is there yet
         int tiles = 0;
         Unit v;
-        if (tid < a.slots && make_unit(b, a.tiles, tid, window, v)) tiles = max((v.hi - v.lo / a.box_rows * a.box_rows + kKeys - 1) / kKeys, 1);
+        if (tid < a.slots && make_unit(b, a.tiles, tid, window, v)) tiles = (both ? (v.from + kKeys - 1) / kKeys : 0) + max((v.hi - v.lo / a.box_rows * a.box_rows + kKeys - 1) / kKeys, 1);
         tiles_of[tid] = tiles;
         __syncthreads();
         int longest = 0;
@@ -264,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         fence_async_smem();      // the list's place is written by copies next
         split |= parts > 1;
     }
-    if (KEYS != kAllKeys || a.splits > 1) {
+    if (sums_only || a.splits > 1) {
         t_begin = nt * z / parts;
         t_end = nt * (z + 1) / parts;
         if (z == 0 && tid == 0) a.parts[slot * a.c.heads.kv_heads + hk] = parts;
@@ -274,14 +285,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (turns) return Range{t_begin + t, max(t_end, t_begin + t)};
         if (r0 > r1) return Range{0, 0};
         const int hi = last_of(r1) + 1, lo = first_of(last_of(r0));
-        Range r{max(t_begin, (lo - key0) / kKeys), min(t_end, (max(hi - key0, 0) + kKeys - 1) / kKeys)};
+        Range r{max(t_begin, both ? 0 : (lo - key0) / kKeys), min(t_end, np + (max(hi - key0, 0) + kKeys - 1) / kKeys)};
         if (r.end < r.begin) r.end = r.begin;
         return r;
     };
     const Range range[2] = {range_of(0), range_of(1)};
     constexpr int step = turns ? 2 : 1;      // from one of a row tile's key tiles to the next
     // the tiles some row sees only in part
-    auto partial = [&](int j) { return key0 + j * kKeys < all_lo || key0 + (j + 1) * kKeys > all_hi; };
+    auto partial = [&](int j) { return tile_key(j) < all_from(j) || tile_key(j) + kKeys > all_to(j); };
 
     if (warp == 0 && elect_one()) {
         mbar_init(bar_q, a.q_boxes ? 1 : kSoftmaxWarps);
@@ -374,9 +385,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, s[q]);
             tmem_ld_wait();
             float top = kLowest;
-            const int k0 = key0 + j * kKeys;
-            if (k0 < w_lo || k0 + kKeys > w_hi) {
-                const int from = first - k0, to = last - k0;      // of the tile's keys the row sees [from, to]
+            const int k0 = tile_key(j);
+            const bool of_prefix = both && j < np;
+            if (of_prefix ? k0 + kKeys > u.from : k0 < w_lo || k0 + kKeys > w_hi) {
+                const int from = (of_prefix ? 0 : first) - k0, to = (of_prefix ? u.from - 1 : last) - k0;      // of the tile's keys the row sees [from, to]
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int lo = min(max(from - 32 * q, 0), 32), hi = min(max(to - 32 * q + 1, 0), 32);
@@ -532,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (odd_values && n > 0) {
                     // keys that only some rows of the block see: [u.lo, all_lo) and [all_hi, u.hi)
 #pragma unroll 1
-                    for (int key = max(first, key0 + r.begin * kKeys); key <= min(last, key0 + r.end * kKeys - 1); ++key) {
+                    for (int key = max(first, tile_key(max(r.begin, np))); key <= min(last, tile_key(max(r.end, np)) - 1); ++key) {
                         if (key >= all_lo && key < all_hi) {
                             key = all_hi - 1;
                             continue;
@@ -683,12 +695,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const uint32_t box_bytes = (uint32_t)a.box_rows * 128;
             bool ok = true;
             const int total = 2 * (t_end - t_begin);
+            int group = 0;
+            if constexpr (both) group = max(b.group_of(u.n), 0);      // one that has a prefix
             auto look = [&](int j, int& row) {      // page of this lane's box, -1: nothing to load
-                const int key = key0 + j * kKeys + box * a.box_rows;
-                if (box >= boxes || j >= t_end || key >= u.hi || key + a.box_rows <= u.lo) return -1;
+                const int key = tile_key(j) + box * a.box_rows;
+                if (box >= boxes || j >= t_end || key >= reach_hi(j) || key + a.box_rows <= reach_lo(j)) return -1;
                 const int col = key / b.page_size;
                 row = key - col * b.page_size;
-                const int page = b.page(u.n, col);
+                int page;
+                if constexpr (both) page = j < np ? b.prefix_page(group, col) : b.page(u.n, col);
+                else page = b.page(u.n, col);
                 if (page < 0) b.tell(KDA_ERR_BLOCK_TABLE);
                 return page;
             };
@@ -746,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 // Keys [0, head) and [tail, 128) of the tile, a piece of eight values a thread, DP / 8 threads a row: those outside of
                 // [u.lo, u.hi) are blanked, the others looked through.  The product of the tile waits for this.
                 constexpr int kChunks = DP / 8, kStep = 64 / kChunks;
-                const int k0 = key0 + j * kKeys, head = min(max(all_lo - k0, 0), kKeys), tail = max(min(max(all_hi - k0, 0), kKeys), head);
+                const int k0 = tile_key(j), head = min(max(all_from(j) - k0, 0), kKeys), tail = max(min(max(all_to(j) - k0, 0), kKeys), head);
                 const int x = tid - kFixWarp * 32, ch = x % kChunks, y0 = x / kChunks;
                 auto place = [&](int r) { return reinterpret_cast<uint4*>(v + (ch >> 3) * 16384 + sw128_off(r, ch & 7)); };
                 auto through = [&](int from, int to) {
@@ -774,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 auto blank = [&](int from, int to) {
                     for (int r = from + y0; r < to; r += kStep) *place(r) = make_uint4(0, 0, 0, 0);
                 };
-                const int lo = min(max(u.lo - k0, 0), kKeys), hi = min(max(u.hi - k0, 0), kKeys);      // keys in reach
+                const int lo = min(max(reach_lo(j) - k0, 0), kKeys), hi = min(max(reach_hi(j) - k0, 0), kKeys);      // keys in reach
                 if (ok) {
                     blank(0, min(lo, head));
                     through(min(lo, head), min(head, hi));
@@ -1022,7 +1038,7 @@ int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CU
         KDA_LAUNCH("attn_tc_kernel", st, attn_tc_kernel<DP, KEYS><<<grid, kThreads, Layout<DP>::kBytes, st>>>(mK, mV, mQ, mO, a));
     }
     if (int rc = launch_status()) return rc;
-    if (a.splits == 1 || KEYS != kAllKeys) return KDA_OK;
+    if (a.splits == 1 || (KEYS != kAllKeys && KEYS != kBothKeys)) return KDA_OK;
     const dim3 joins((unsigned)a.slots * 8, (unsigned)c.heads.kv_heads);
     KDA_LAUNCH("attn_tc_join_kernel", st, attn_tc_join_kernel<DP><<<joins, 256, 0, st>>>(a));
     return launch_status();
@@ -1068,7 +1084,7 @@ Args args_of(const Call& c, int keys, int splits) {
     a.parts = nullptr;
     a.part_ml = nullptr;
     a.part_o = nullptr;
-    if (splits > 1 || keys != kAllKeys) place_parts(a, c);
+    if (splits > 1 || (keys != kAllKeys && keys != kBothKeys)) place_parts(a, c);
     return a;
 }
 
@@ -1083,7 +1099,7 @@ int pass(const Call& c, int splits, int own_rows, cudaStream_t st) {
     mQ = mO = mK;
     a.q_boxes = 128 % c.heads.group == 0 && s.q_head > 0 && s.q_token > 0 && s.q_head < 1ll << 39 && s.q_token < 1ll << 39;
     if (!rc && a.q_boxes) rc = make_map_packed(&mQ, c.q, c.heads.dim, c.heads.q_heads, c.batch.tokens, s.q_head, s.q_token, c.heads.group, 128 / c.heads.group);
-    if (!rc && a.q_boxes && KEYS == kAllKeys)
+    if (!rc && a.q_boxes && (KEYS == kAllKeys || KEYS == kBothKeys))
         rc = make_map_packed(&mO, c.o, c.heads.dim, c.heads.q_heads, c.batch.tokens, c.heads.dim, (int64_t)c.heads.q_heads * c.heads.dim, c.heads.group, 128 / c.heads.group);
     if (!rc) rc = c.heads.dim <= 64 ? launch<64, KEYS>(c, mK, mV, mQ, mO, a, st) : launch<128, KEYS>(c, mK, mV, mQ, mO, a, st);
     return rc;
@@ -1096,6 +1112,7 @@ bool in_turns(const Call& c) { return prefix_rows(c.batch.tokens, c.batch.p.n, c
 int tc_prefix(const Call& c, int splits, bool own_rows, cudaStream_t st) {
     return in_turns(c) ? pass<kTurnKeys>(c, splits, own_rows, st) : pass<kPrefixKeys>(c, splits, own_rows, st);
 }
+int tc_both(const Call& c, int splits, cudaStream_t st) { return pass<kBothKeys>(c, splits, 0, st); }
 int tc_own(const Call& c, int splits, cudaStream_t st) { return pass<kOwnKeys>(c, splits, 0, st); }
 
 int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const OwnRows* rows, cudaStream_t st) {

@@ -105,6 +105,11 @@ CASES = [  # heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups
     (12, 4, 64, 16, BF16, [1] * 23, [(7 * i) % 40 + 1 for i in range(23)], [64, 1, 200, 15], [0, 10, 11, 20, 23]),
     (16, 4, 128, 64, BF16, [100, 33, 260], [130, 33, 261], [515], [0, 3]),
     (5, 1, 128, 64, BF16, [90, 1, 17], [100, 1, 20], [130], [0, 3]),
+    (8, 2, 64, 16, BF16, [300], [301], [2100], [0, 1]),
+    (4, 2, 128, 128, BF16, [200, 130], [260, 131], [1000, 127], [0, 1, 2]),
+    (6, 1, 128, 16, BF16, [4] * 30, [4 + i for i in range(30)], [400], [0, 30]),
+    (16, 4, 128, 16, BF16, [1] * 70, [1 + (i * 5) % 70 for i in range(70)], [900, 33], [0, 60, 70]),
+    (16, 8, 64, 64, BF16, [1] * 150, [1 + (i * 3) % 50 for i in range(150)], [200], [0, 150]),
     (4, 2, 8, 16, BF16, [1, 3], [4, 3], [31], [0, 2]),
     (4, 4, 128, 48, BF16, [1, 9, 2], [50, 9, 3], [97], [0, 3]),
     (2, 1, 200, 16, BF16, [1, 20], [10, 20], [70], [0, 2]),
@@ -125,7 +130,7 @@ def test_against_the_restatement(heads, kv_heads, dim, page, dtype, q_lens, own,
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("q", [1, 3, 40])
+@pytest.mark.parametrize("q", [1, 3, 40, 110])
 def test_sequences_that_do_not_share(dtype, q):
     """Places without a request, texts shorter than the prefix, sequences of no group, a group without sequences, a prefix of nothing."""
     import experiment_swa_kda_b200 as m
@@ -144,8 +149,8 @@ def test_sequences_that_do_not_share(dtype, q):
 
 def test_equal_groups_and_lengths_without_their_tables():
     import experiment_swa_kda_b200 as m
-    for q in (1, 6):
-        b = Batch(8, 2, 128, 16, BF16, [q] * 6, [q, q + 1, 40, 9, 8, 100], [77, 128, 200], [0, 2, 4, 6])
+    for q in (1, 6, 70):
+        b = Batch(8, 2, 128, 16, BF16, [q] * 6, [q, q + 1, 70, 79, 78, 100], [77, 128, 200], [0, 2, 4, 6])
         args = b.device()
         args[7] = args[8] = None
         o, lse = m.shared_prefix_attention(*args, return_lse=True, scale=0.2)
@@ -153,7 +158,7 @@ def test_equal_groups_and_lengths_without_their_tables():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("q", [1, 24])
+@pytest.mark.parametrize("q", [1, 10, 24, 130])
 def test_values_that_are_not_finite(dtype, q):
     """Infinite and undefined values at keys that are seen, in the prefix and behind it; scores of -inf throughout."""
     import experiment_swa_kda_b200 as m
@@ -213,15 +218,15 @@ def test_inconsistent_arrays_are_bounded_and_told():
     fine.check(o)
 
 
-def test_captured_on_another_stream_and_two_graphs_at_once():
+def test_captured_on_another_stream_and_graphs_at_once():
     import experiment_swa_kda_b200 as m
-    batches = [Batch(16, 4, 128, 16, BF16, [q] * 12, [(13 * i) % 90 + q for i in range(12)], [600], [0, 12], seed=q) for q in (1, 6)]
+    batches = [Batch(16, 4, 128, 16, BF16, [q] * 12, [(13 * i) % 90 + q for i in range(12)], [600], [0, 12], seed=q) for q in (1, 6, 100)]
     args = [b.device() for b in batches]
-    wants = [m.shared_prefix_attention(*a, max_q_len=q) for a, q in zip(args, (1, 6))]
+    wants = [m.shared_prefix_attention(*a, max_q_len=q) for a, q in zip(args, (1, 6, 100))]
     for b, w in zip(batches, wants):
         b.check(w)
     graphs, outs = [], []
-    for a, q in zip(args, (1, 6)):
+    for a, q in zip(args, (1, 6, 100)):
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             outs.append(m.shared_prefix_attention(*a, max_q_len=q))

@@ -118,6 +118,10 @@ struct OwnView : Batch {
     }
     // the prefix of sequence n's group, whether or not the sequence shares it
     __device__ __forceinline__ int prefix_of(int n) const {
+        if (p.n == 1) {      // nothing here waits for anything else
+            const int a = group_edge(0), b = group_edge(1), len = prefix_len(0);
+            return n >= a && n < b ? len : 0;
+        }
         const int g = group_of(n);
         return g < 0 ? 0 : prefix_len(g);
     }
@@ -300,9 +304,14 @@ __device__ __forceinline__ PrefixWork prefix_work(const GroupView& b, int g, int
     return PrefixWork{rows > 0 ? max((b.prefix_len(g) + 127) / 128, 1) : 0, (rows + tile_rows - 1) / tile_rows};
 }
 constexpr int kSms = 148, kPartTries = 128;
-// Key tiles of a part, and the blocks that gives: each of the first kPartTries threads tries one number of parts for the longest prefix.  Times are in
-// microseconds, as measured: a key tile takes 0.95 with row tiles of 128 and 2 with 256, a tile of 64 own keys 1.0 of an SM (0.6 with 64 values
-// a head), and either pass 8 besides.  Called by all `warps` warps; `work` is filled, `best` has two places a warp.
+// Microseconds that both passes take, as measured, where the one over prefixes has `blocks` SMs and parts of `part` key tiles: a key tile takes 0.95 with
+// row tiles of 128 and 2 with 256, a tile of 64 own keys 1.0 of an SM (0.6 with 64 values a head), and either pass 8 besides.
+__host__ __device__ __forceinline__ float passes_us(int part, int blocks, int tile_rows, int dim, long long own_tiles) {
+    const float prefix_us = 8.f + (float)part * (tile_rows == 128 ? 0.95f : 2.f), own_us = own_tiles > 0 ? (float)own_tiles * (dim <= 64 ? 0.6f : 1.f) : 0.f;
+    return own_us > 0.f && blocks < kSms ? fmaxf(prefix_us, 8.f + own_us / (float)(kSms - blocks)) : prefix_us + own_us / kSms;
+}
+// Key tiles of a part, and the blocks that gives: each of the first kPartTries threads tries one number of parts for the longest prefix.  Called by all
+// `warps` warps; `work` is filled, `best` has two places a warp.
 struct PartChoice {
     int part, blocks;
 };
@@ -318,9 +327,7 @@ __device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int g
     if (longest > 0)
         for (int g = 0; g < groups; ++g) blocks += work[g].row_tiles * ((work[g].tiles + part - 1) / part);
     blocks *= kv_heads;
-    const float prefix_us = 8.f + (float)part * (tile_rows == 128 ? 0.95f : 2.f), own_us = own_tiles > 0 ? (float)own_tiles * (dim <= 64 ? 0.6f : 1.f) : 0.f;
-    const bool beside = own_us > 0.f && blocks < kSms;
-    const float us = beside ? fmaxf(prefix_us, 8.f + own_us / (float)(kSms - blocks)) : prefix_us + own_us / kSms;
+    const float us = passes_us(part, blocks, tile_rows, dim, own_tiles);
     const bool fits = tid < kPartTries && tries <= splits && blocks <= max(kSms, row_tiles * kv_heads);
     const unsigned cost = fits ? __float_as_uint(us) : 0x7f800000u;
     unsigned least = __reduce_min_sync(0xffffffffu, cost);
@@ -411,8 +418,9 @@ struct OwnRows {
     int rows, blocks;
 };
 bool own_rows_take(const Call& c);
+int own_rows_per_sm(int dim, int rows);      // blocks an SM
 size_t own_rows_workspace(const KdaPagedShape& s, int max_q);
-int own_rows(const Call& c, int prefix_splits, OwnRows& own, cudaStream_t st);
+int own_rows(const Call& c, int prefix_splits, int most_blocks, OwnRows& own, cudaStream_t st);
 // The join: own keys as own_rows left them, or (null) as tc_own did in own.workspace.
 int tc_shared_join(const Call& prefix, int prefix_splits, const Call& own, int own_splits, const OwnRows* rows, cudaStream_t st);
 

@@ -1,5 +1,7 @@
 // C entries of the attention over a paged cache: argument checks, and which kernel takes a call.
 
+#include <math.h>
+
 #include "attn.cuh"
 
 using namespace kda;
@@ -135,6 +137,28 @@ int general_prefix_splits(const KdaPagedShape& s, const KdaPrefixShape& p) { ret
 // Sequences whose rows fill row tiles by themselves go through the prefix and their own keys one after the other: nothing is left to join.
 bool takes_both(const KdaPagedShape& s) { return (long long)s.tokens * (s.q_heads / s.kv_heads) >= 192ll * s.n_seq; }
 
+// Blocks of the pass over own keys.  A block that finds no work costs 6 us where it starts late, once others have ended, so there are as many as
+// find a place beside the prefixes, by what the tables' widths say: prefixes fill theirs, and sequences go on for 0.6 of what theirs have
+// besides.  How the work is cut is decided on the device, by the lengths.
+int own_blocks(const KdaPagedShape& s, const KdaPrefixShape& p, bool packed, int splits) {
+    const int group = s.q_heads / s.kv_heads, rows = prefix_rows(s.tokens, p.n_groups, group);
+    const long long behind = (long long)(s.table_width > p.table_width ? s.table_width - p.table_width : 0) * s.page_size;
+    const long long most = ((behind + 63) / 64 + 1) * s.n_seq * s.kv_heads / 2, own_tiles = (behind * 3 / 5 + 32) * s.n_seq * s.kv_heads / 64;
+    int best = 0;
+    if (splits > 1) {
+        const long long tiles = ((long long)p.table_width * s.page_size + 127) / 128;
+        const long long row_tiles = (((long long)s.tokens * group + p.n_groups - 1) / p.n_groups + rows - 1) / rows * p.n_groups * s.kv_heads;
+        float least = INFINITY;
+        for (int tries = 1; tries <= splits && row_tiles * tries <= kSms; ++tries) {
+            const int part = (int)((tiles + tries - 1) / tries), blocks = (int)(row_tiles * ((tiles + part - 1) / (part > 0 ? part : 1)));
+            const float us = passes_us(part, blocks, rows, s.head_dim, own_tiles);
+            if (us < least) least = us, best = blocks;
+        }
+    }
+    const long long n = (long long)own_rows_per_sm(s.head_dim, (packed ? s.max_q_len : s.tokens / s.n_seq) * group) * (best < kSms ? kSms - best : kSms);
+    return (int)(most < 2 ? 2 : most < n ? most : n);
+}
+
 // The shares of a workspace on the tensor cores.
 struct SharedSpace {
     size_t prefix, own;
@@ -205,6 +229,6 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     own.workspace = static_cast<char*>(workspace) + shared_space(*s, *p, packed, few).prefix;
     OwnRows rows;
     if (int rc = tc_prefix(c, prefix_splits, few, st)) return rc;
-    if (int rc = few ? own_rows(own, prefix_splits, rows, st) : tc_own(own, own_splits, st)) return rc;
+    if (int rc = few ? own_rows(own, prefix_splits, own_blocks(*s, *p, packed, prefix_splits), rows, st) : tc_own(own, own_splits, st)) return rc;
     return tc_shared_join(c, prefix_splits, own, own_splits, few ? &rows : nullptr, st);
 }

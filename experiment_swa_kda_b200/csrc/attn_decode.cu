@@ -36,6 +36,9 @@ using namespace tc;
 
 constexpr int kMaxRows = 16, kMaxOwnRows = 24, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
 constexpr int kPerSm = 2;             // blocks an SM: 102 KB each, 106 with more than 8 rows
+// ... of own keys: a tile of heads 64 wide is bound by the latency of what is done to it, and four blocks fit
+template <int DP, int NR, int KEYS>
+constexpr int kPerSmOf = KEYS == kOwnKeys && DP == 64 && NR == 1 ? 4 : kPerSm;
 // Up to so many tiles a sequence and kv head stay together: they take about as long as two of them and the join, which is a launch less (3
 // conversations of 40 tokens 14.5 us in parts, 8.4 whole; 16 of 100 12.5 and 10.4).  Six where there are sequences for every SM (200 of up
 // to 380 36 and 33), four where parts would have some to themselves (one of 300 12.4 and 13.2 with six).
@@ -49,6 +52,7 @@ struct Layout {
     static constexpr int kHalf = 16 * 128;                            // 16 keys of 64 values
     static constexpr int kStage = 2 * (DP / 64) * kHalf;              // K and V of 16 keys
     static constexpr int kRowsOf = 8 * NR;
+    static constexpr bool kTwoTerms = NR <= 2;                        // of a weight; with more rows the products count, and one rounded term is as good as the tensor cores'
     static constexpr bool kKeepQ = NR <= 2;                           // queries in registers; with more rows they are read with every tile
     static constexpr int kQ = kWarps * kStages * kStage;              // two sequences' queries, or one's
     static constexpr int kQBuffers = kKeepQ ? 2 : 1;
@@ -118,11 +122,13 @@ struct Start {
 };
 // The cut, and where stretch `id` begins.  Called by all THREADS of a block; `sums` has a place for each warp.  The host takes
 // care that the list has less than 2^31 tiles.
-template <int THREADS, bool whole, class B>
-__device__ __forceinline__ Cut find_start(const B& b, int kv_heads, int window, int blocks, int id, Start* start, int* sums) {
+// `blocks_of` says how many stretches there may be for a list of so many tiles.
+template <int THREADS, bool whole, class B, class F>
+__device__ __forceinline__ Cut find_start(const B& b, int kv_heads, int window, F blocks_of, int id, Start* start, int* sums) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int each = (b.n_seq + THREADS - 1) / THREADS, n0 = min(tid * each, b.n_seq), n1 = min(n0 + each, b.n_seq);
     int mine = 0;
+#pragma unroll 2
     for (int n = n0; n < n1; ++n) {
         const Seq s = seq_at(b, n, window);
         mine += (s.t1 - s.t0) * kv_heads;
@@ -142,9 +148,10 @@ __device__ __forceinline__ Cut find_start(const B& b, int kv_heads, int window, 
         if (w < warp) upto += sums[w];
         cut.total += sums[w];
     }
-    cut.used = min(blocks, max(whole ? cut.total : cut.total / kMinTiles, 1));
+    cut.used = min(blocks_of(cut.total), max(whole ? cut.total : cut.total / kMinTiles, 1));
     cut.each = cut.total / cut.used;
     cut.longer = cut.total - cut.each * cut.used;
+    if (!whole && id >= cut.used) return cut;
     if (whole) {
         if (tid == 0) {
             start->begin = cut.begin(id);
@@ -249,7 +256,7 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {      // an 8 x 8 tile o
 }
 
 template <int DP, int NR, int KEYS>
-__global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
+__global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                                        const __grid_constant__ Args a) {
     using L = Layout<DP, NR>;
     constexpr int kHalves = DP / 64, kSteps = DP / 16, kRows = 8 * NR;
@@ -271,25 +278,20 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
         mbar_fence_init();
     }
     if (tid == 0) flags[0] = flags[1] = flags[2] = 0;
-    int blocks = a.blocks;
-    if constexpr (KEYS == kOwnKeys) {
-        if (a.prefix_splits > 1) {      // beside the pass over the prefixes: the blocks that leaves room for
-            PrefixWork* work = reinterpret_cast<PrefixWork*>(sm + L::kQ);
-            unsigned* best = reinterpret_cast<unsigned*>(work + kMaxListed);
-            if (tid < b.p.n) work[tid] = prefix_work(a.c.batch, tid, g, a.prefix_rows);
-            int own = 0;
-            for (int n = tid; n < b.n_seq; n += kThreads) own += own_tiles_of(b, n);
-            own = __reduce_add_sync(0xffffffffu, own);
-            if (lane == 0) sums[warp] = own;
-            __syncthreads();
-            own = __reduce_add_sync(0xffffffffu, lane < kWarps ? sums[lane] : 0);
-            const PartChoice c = choose_parts(work, b.p.n, a.prefix_rows, Hk, D, (long long)own * Hk, a.prefix_splits, best, kWarps);
-            blocks = min(blocks, kPerSm * max(kSms - c.blocks, 1));
-            if (c.blocks >= kSms) blocks = a.blocks;
-        }
-    }
-    const Cut cut = a.whole && KEYS == kAllKeys ? find_start<kThreads, true>(b, Hk, window, blocks, blockIdx.x, &start, sums)
-                                                : find_start<kThreads, false>(b, Hk, window, blocks, blockIdx.x, &start, sums);
+    // own keys: the blocks that the pass over the prefixes beside this one leaves room for
+    PrefixWork* work = reinterpret_cast<PrefixWork*>(sm + L::kQ);
+    if constexpr (KEYS == kOwnKeys)
+        if (a.prefix_splits > 1 && tid < b.p.n) work[tid] = prefix_work(a.c.batch, tid, g, a.prefix_rows);
+    auto blocks_of = [&](int total) {
+        if constexpr (KEYS == kOwnKeys)
+            if (a.prefix_splits > 1 && total > kMinTiles * kPerSmOf<DP, NR, KEYS>) {
+                const int sms = kSms - choose_parts(work, b.p.n, a.prefix_rows, Hk, D, total, a.prefix_splits, reinterpret_cast<unsigned*>(work + kMaxListed), kWarps).blocks;
+                if (sms > 0) return min(a.blocks, kPerSmOf<DP, NR, KEYS> * sms);
+            }
+        return a.blocks;
+    };
+    const Cut cut = a.whole && KEYS == kAllKeys ? find_start<kThreads, true>(b, Hk, window, blocks_of, blockIdx.x, &start, sums)
+                                                : find_start<kThreads, false>(b, Hk, window, blocks_of, blockIdx.x, &start, sums);
     const int tiles = a.whole && KEYS == kAllKeys ? start.end - start.begin : cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
 
     uint8_t* ring = sm + warp * kStages * L::kStage;
@@ -549,6 +551,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
                     const float p0 = ex2(fmaf(sc[y][2 * t], c, -mc[0])), p1 = ex2(fmaf(sc[y][2 * t + 1], c, -mc[1]));
                     l[y][0] += p0;
                     l[y][1] += p1;
+                    if constexpr (!L::kTwoTerms) {
+                        hi[y][t] = turned(pack_bf16(p0, p1));
+                        continue;
+                    }
                     // hi cut, not rounded, and lo at least 2^-20 of the weight: both of one sign, neither 0, or their sum with an infinite value were NaN
                     const uint32_t h = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
                     hi[y][t] = turned(h);
@@ -562,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) attn_decode_kernel(const __g
 #pragma unroll
                 for (int y = 0; y < NR; ++y) {
                     mma(acc[y][t], vf, hi[y][0], hi[y][1]);
-                    mma(acc[y][t], vf, lo[y][0], lo[y][1]);
+                    if constexpr (L::kTwoTerms) mma(acc[y][t], vf, lo[y][0], lo[y][1]);
                 }
             }
         }
@@ -685,7 +691,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
     const Batch& b = a.c.batch;
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const Cut cut = find_start<kJoinThreads, false>(b, Hk, window, a.blocks, id, &start, sums);
+    const Cut cut = find_start<kJoinThreads, false>(b, Hk, window, [&](int) { return a.blocks; }, id, &start, sums);
     // No block ends before the stretches have: whoever is launched behind this kernel takes that for the end of both.
     if (id >= cut.used) {
         dependency_wait();
@@ -772,9 +778,9 @@ bool keeps_whole(int n_seq, int kv_heads, long long reach) {
     return reach <= ((long long)n_seq * kv_heads >= 148 ? kWholeTilesOfMany : kWholeTiles) * kTile;
 }
 // Stretches: as many as the machine holds, or as the longest batch that fits the table could use.
-int stretches(int n_seq, int kv_heads, long long reach) {
+int stretches(int n_seq, int kv_heads, long long reach, int most = kMaxBlocks) {
     const long long tiles = ((reach + kTile - 1) / kTile + 1) * n_seq * kv_heads, n = keeps_whole(n_seq, kv_heads, reach) ? tiles : tiles / kMinTiles;
-    return (int)(n < 1 ? 1 : n < kMaxBlocks ? n : kMaxBlocks);
+    return (int)(n < 1 ? 1 : n < most ? n : most);
 }
 long long reach_of(int table_width, int page_size, int window, int max_q) {
     long long reach = (long long)table_width * page_size;
@@ -789,33 +795,35 @@ bool takes(const Call& c, int rows) {
     const long long tiles = (long long)c.batch.n_seq * c.heads.kv_heads * ((long long)c.batch.table_width * c.batch.page_size / kTile + 2);
     return c.max_q_len > 0 && (long long)c.max_q_len * c.heads.group <= rows && tiles < 1ll << 31 && tc_takes(c);
 }
-size_t parts_bytes(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim, int rows_each) {
-    const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q)) * 2 * rows_each;
+size_t parts_bytes(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim, int rows_each, int most) {
+    const size_t rows = (size_t)stretches(n_seq, kv_heads, reach_of(table_width, page_size, window, max_q), most) * 2 * rows_each;
     return align_up(rows * sizeof(float2), 256) + rows * dim * sizeof(float);
 }
 }  // namespace
 
 bool decode_takes(const Call& c) { return takes(c, kMaxRows); }
 size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim) {
-    return parts_bytes(n_seq, kv_heads, table_width, page_size, window, max_q, dim, kMaxRows);
+    return parts_bytes(n_seq, kv_heads, table_width, page_size, window, max_q, dim, kMaxRows, kMaxBlocks);
 }
 
+constexpr int kMaxOwnBlocks = 148 * 4;
 bool own_rows_take(const Call& c) { return takes(c, kMaxOwnRows); }
+int own_rows_per_sm(int dim, int rows) { return dim <= 64 && rows <= 8 ? kPerSmOf<64, 1, kOwnKeys> : kPerSm; }
 size_t own_rows_workspace(const KdaPagedShape& s, int max_q) {
     const size_t rows = (size_t)s.tokens * s.q_heads;
-    return align_up(parts_bytes(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, max_q, s.head_dim, kMaxOwnRows), 256) + align_up(rows * sizeof(float2), 256) +
+    return align_up(parts_bytes(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, max_q, s.head_dim, kMaxOwnRows, kMaxOwnBlocks), 256) + align_up(rows * sizeof(float2), 256) +
            align_up(rows * s.head_dim * sizeof(float), 256) + align_up((size_t)s.n_seq * s.kv_heads * sizeof(int2), 256);
 }
 
 namespace {
 
 template <int KEYS>
-int pass(const Call& c, int prefix_splits, OwnRows* own, cudaStream_t st) {
+int pass(const Call& c, int prefix_splits, int most_blocks, OwnRows* own, cudaStream_t st) {
     Args a;
     a.c = c;
     const long long reach = reach_of(c.batch.table_width, c.batch.page_size, c.window, c.max_q_len);
     const int rows = KEYS == kOwnKeys ? kMaxOwnRows : kMaxRows;
-    a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach);
+    a.blocks = stretches(c.batch.n_seq, c.heads.kv_heads, reach, most_blocks);
     a.box_rows = c.batch.page_size < 16 ? c.batch.page_size : 16;
     a.whole = keeps_whole(c.batch.n_seq, c.heads.kv_heads, reach);
     char* ws = static_cast<char*>(c.workspace);
@@ -853,8 +861,10 @@ int pass(const Call& c, int prefix_splits, OwnRows* own, cudaStream_t st) {
 
 }  // namespace
 
-int decode(const Call& c, cudaStream_t st) { return pass<kAllKeys>(c, 1, nullptr, st); }
-int own_rows(const Call& c, int prefix_splits, OwnRows& own, cudaStream_t st) { return pass<kOwnKeys>(c, prefix_splits, &own, st); }
+int decode(const Call& c, cudaStream_t st) { return pass<kAllKeys>(c, 1, kMaxBlocks, nullptr, st); }
+int own_rows(const Call& c, int prefix_splits, int most_blocks, OwnRows& own, cudaStream_t st) {
+    return pass<kOwnKeys>(c, prefix_splits, most_blocks, &own, st);
+}
 
 }  // namespace attn
 }  // namespace kda

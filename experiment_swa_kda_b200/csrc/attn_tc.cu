@@ -882,8 +882,8 @@ struct SharedJoin {
 // a time, and few rows have several warps each.
 constexpr int kSharedWarps = 8;
 template <int DP>
-__global__ void __launch_bounds__(32 * kSharedWarps, 3) attn_shared_join_kernel(const __grid_constant__ SharedJoin j) {
-    constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes, kAhead = 8;
+__global__ void __launch_bounds__(32 * kSharedWarps, 4) attn_shared_join_kernel(const __grid_constant__ SharedJoin j) {
+    constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes, kAhead = 4;
     __shared__ float4 sums_o[kSharedWarps][kLanes];
     const GroupView& groups = j.prefix.c.batch;
     const OwnView& b = groups;
@@ -1029,7 +1029,8 @@ template <int DP, int KEYS>
 int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CUtensorMap& mQ, const CUtensorMap& mO, const Args& a, cudaStream_t st) {
     if (int rc = set_smem_limit(attn_tc_kernel<DP, KEYS>, Layout<DP>::kBytes)) return rc;
     const bool list = (KEYS == kPrefixKeys || KEYS == kTurnKeys) && a.splits > 1;      // prefix_unit: a block an SM
-    const dim3 grid(list ? 148u : (unsigned)a.slots, list ? 1u : (unsigned)c.heads.kv_heads, list ? 1u : (unsigned)a.splits);
+    const long long most = (long long)a.slots * c.heads.kv_heads * a.splits;
+    const dim3 grid(list ? (unsigned)(most < kSms ? most : kSms) : (unsigned)a.slots, list ? 1u : (unsigned)c.heads.kv_heads, list ? 1u : (unsigned)a.splits);
     if constexpr (KEYS == kOwnKeys) {      // beside the pass over the prefix
         cudaError_t e = cudaSuccess;
         KDA_LAUNCH("attn_tc_kernel", st, e = launch_early(attn_tc_kernel<DP, KEYS>, grid, kThreads, Layout<DP>::kBytes, st, true, 1, mK, mV, mQ, mO, a));

@@ -6,13 +6,13 @@
 // are at most the free pages, and the new tokens up to and with it at most max_tokens; one that is not goes without its new tokens.
 //
 // All of it is a handful of sums over rows and over pages, each of which the next step waits for: bound by latency, not by bytes
-// (256 rows of 256 columns and 32,768 pages are 300 KB).  So it is one launch, a cluster of blocks that meet at its barriers:
+// (256 rows of 256 columns and 32,768 pages are 300 KB).  So it is one launch, a cluster of blocks that meet at its barriers (0.5 us each):
 //   1  entries outside of their row's columns go back; missing ones are counted, 128 columns a warp
-//   2  free pages of each block's share are counted; every block sums up all rows for itself
+//   2  every block sums up all rows and all free pages for itself, which costs less than meeting once more
 //   3  who is served; the first free pages are listed in order
 //   4  missing entries take theirs; rows that have to wait give back what their new tokens would have needed
 //   5  position and slot of each new token
-// A batch that one block can read at once takes a single block, whose barriers cost less.
+// A block has a range of the rows from 1 to 5.  A batch that one block can read at once takes a single block, which keeps its lists to itself.
 
 #include "common.cuh"
 
@@ -35,6 +35,8 @@ struct PlanArgs {
     int* mirror;
     long long table_stride;
     int rows, width, page, n_pages, max_tokens, items;
+    int split, slice;       // blocks count free pages by shares of `slice`, a multiple of 512
+    int thread_pages;       // pages whose flags a thread counts: a power of two, 16 at least
 
     __device__ __forceinline__ void tell(int code) const {
         if (mirror != nullptr) *reinterpret_cast<volatile int*>(mirror) = code;
@@ -114,29 +116,29 @@ __device__ __forceinline__ unsigned free_bits(const unsigned char* flags, int at
     return bits;
 }
 
-// The items (a row, 128 of its columns) of a table are dealt out to the warps in runs of at most 32; lane l of a warp has what the row of
-// the run's l-th item asks for.
-struct Run {
-    int first, many;      // items
-    int row, col0, col1, col1_without;      // of this lane's item: its row, the columns that shall be held, and their end without the new tokens
-};
-
 __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_constant__ PlanArgs a) {
     extern __shared__ int rows_sm[];
-    // of each row: entries lacking before it (-1: it is not served); new tokens, then the sum before it; its length.   With one block entries missing follow, [items]
+    // of each row: entries lacking before it (-1: it is not served); new tokens, then the sum before it; its length.  One block alone also has
+    // the entries lacking of each item and the pages dealt out here.
     int *base_of = rows_sm, *cu = base_of + a.rows, *len_of = cu + a.rows + 1;
     __shared__ Sums sums[2][kWarps];
-    __shared__ int counts[kBlocks];                      // free pages of each block's share
+    __shared__ int free_before[kThreads], counts[kBlocks];      // free pages before each thread's; of each block's share
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = gridDim.x, rank = blockIdx.x;     // the grid is one cluster
-    int* missing = blocks > 1 ? a.missing : len_of + a.rows;
+    const bool alone = blocks == 1;
+    int *missing = alone ? len_of + a.rows : a.missing, *dealt = alone ? missing + a.rows * a.items : a.dealt;
     auto meet = [&]() {
-        if (blocks > 1) cluster_sync();
-        else __syncthreads();
+        if (alone) __syncthreads();
+        else cluster_sync();
     };
-    const int all = a.rows * a.items, warps = blocks * kWarps, run = min((all + warps - 1) / warps, 32);
+    // this block's rows, in items of 128 columns; a warp takes a run of at most 32 of them, lane l the l-th one's row
+    const int r0 = (int)((long long)a.rows * rank / blocks), r1 = (int)((long long)a.rows * (rank + 1) / blocks);
+    const int item0 = r0 * a.items, item1 = r1 * a.items, run = min((item1 - item0 + kWarps - 1) / kWarps, 32);
+    struct Run {
+        int many, row, col0, col1, col1_without;      // the columns that the row shall hold, and their end without its new tokens
+    };
     auto run_at = [&](int i0) {
-        Run r{i0, min(run, all - i0), 0, 0, 0, 0};
+        Run r{min(run, item1 - i0), 0, 0, 0, 0};
         if (lane < r.many) {
             r.row = (i0 + lane) / a.items;
             const Ask ask = ask_of(a, r.row);
@@ -147,34 +149,59 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
         return r;
     };
 
+    // all rows, for the sums: a thread has a few beside each other
+    const int each = (a.rows + kThreads - 1) / kThreads, n0 = min(tid * each, a.rows), n1 = min(n0 + each, a.rows);
+    for (int n = n0; n < n1; ++n) {
+        const Ask r = ask_of(a, n);
+        if (n >= r0 && n < r1) {
+            if (r.bad_len) a.tell(KDA_ERR_BLOCK_TABLE);
+            if (r.bad_new) a.tell(KDA_ERR_CU_SEQLENS);
+        }
+        cu[n] = r.add;
+        len_of[n] = r.len;
+    }
+
     // ------------------------------------------------------------------ 1: what rows hold, and lack
     constexpr int kAtOnce = 4, kEach = kColumns / 32;
-    for (int i0 = (rank * kWarps + warp) * run; i0 < all; i0 += warps * run) {
+    const bool wide_rows = (reinterpret_cast<uintptr_t>(a.table) | (uintptr_t)a.table_stride * 4) % 16 == 0;
+    for (int i0 = item0 + warp * run; i0 < item1; i0 += kWarps * run) {
         const Run r = run_at(i0);
         int lacks = 0;
         for (int x = 0; x < r.many; x += kAtOnce) {
-            int entry[kAtOnce][kEach];
+            int entry[kAtOnce][kEach];      // of columns 4 lane .. 4 lane + 3 of an item
 #pragma unroll
             for (int y = 0; y < kAtOnce; ++y) {
-                const int n = __shfl_sync(0xffffffffu, r.row, min(x + y, r.many - 1)), c0 = (i0 + x + y - n * a.items) * kColumns + lane;
+                const int l = min(x + y, r.many - 1), n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + kEach * lane;
+                const int* at = a.table + n * a.table_stride + c0;
+                if (wide_rows && c0 + kEach <= a.width) {
+                    const int4 v = *reinterpret_cast<const int4*>(at);
+                    entry[y][0] = v.x, entry[y][1] = v.y, entry[y][2] = v.z, entry[y][3] = v.w;
+                } else {
 #pragma unroll
-                for (int k = 0; k < kEach; ++k) entry[y][k] = x + y < r.many && c0 + 32 * k < a.width ? a.table[n * a.table_stride + c0 + 32 * k] : -1;
+                    for (int k = 0; k < kEach; ++k) entry[y][k] = c0 + k < a.width ? at[k] : -1;
+                }
             }
 #pragma unroll
             for (int y = 0; y < kAtOnce; ++y) {
-                const int l = min(x + y, r.many - 1), n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + lane;
-                const int first = __shfl_sync(0xffffffffu, r.col0, l), end = __shfl_sync(0xffffffffu, r.col1, l);
-                if (x + y >= r.many) break;
+                const int l = min(x + y, r.many - 1), n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + kEach * lane;
+                const int first = __shfl_sync(0xffffffffu, r.col0, l), held = max(__shfl_sync(0xffffffffu, r.col1, l) - first, 0);
                 int here = 0;
+                bool other = false;      // an entry to give back
 #pragma unroll
                 for (int k = 0; k < kEach; ++k) {
-                    const int c = c0 + 32 * k, e = entry[y][k];
-                    const bool names = (unsigned)e < (unsigned)a.n_pages, held = c >= first && c < end;
-                    if (e >= a.n_pages) a.tell(KDA_ERR_BLOCK_TABLE);
-                    if (held && !names) ++here;
-                    if (!held && e != -1) {
-                        if (names) a.free_[e] = 1;
-                        a.table[n * a.table_stride + c] = -1;
+                    const bool hold = (unsigned)(c0 + k - first) < (unsigned)held;
+                    here += hold && (unsigned)entry[y][k] >= (unsigned)a.n_pages;
+                    other |= hold ? entry[y][k] >= a.n_pages : entry[y][k] != -1;
+                }
+                if (x + y >= r.many) break;
+                if (other) {
+#pragma unroll
+                    for (int k = 0; k < kEach; ++k) {
+                        const int e = entry[y][k];
+                        if (e >= a.n_pages) a.tell(KDA_ERR_BLOCK_TABLE);
+                        if ((unsigned)(c0 + k - first) < (unsigned)held || e == -1) continue;
+                        if ((unsigned)e < (unsigned)a.n_pages) a.free_[e] = 1;
+                        a.table[n * a.table_stride + c0 + k] = -1;
                     }
                 }
                 here = __reduce_add_sync(0xffffffffu, here);
@@ -185,46 +212,38 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     }
     meet();
 
-    // ------------------------------------------------------------------ 2: free pages of this block's share; sums over all rows
-    const int share = ((a.n_pages + blocks - 1) / blocks + 15) / 16 * 16, p0 = min(rank * share, a.n_pages), p1 = min(p0 + share, a.n_pages);
-    const int each_page = ((share + kThreads - 1) / kThreads + 15) / 16 * 16, my_p0 = min(p0 + tid * each_page, p1), my_p1 = min(my_p0 + each_page, p1);
+    // ------------------------------------------------------------------ 2: sums over all rows, and over free pages
+    // of a large pool each block counts its share, and they tell each other
+    const int s0 = a.split ? rank * a.slice : 0, s1 = a.split ? min(s0 + a.slice, a.n_pages) : a.n_pages;
+    const int each_page = a.thread_pages, p0 = (int)min((long long)s0 + (long long)tid * each_page, (long long)s1), p1 = min(p0 + each_page, s1);
     const bool wide = reinterpret_cast<uintptr_t>(a.free_) % 16 == 0;
-    int my_free = 0;
-    for (int p = my_p0; p < my_p1; p += 16) my_free += __popc(free_bits(a.free_, p, my_p1, wide));
-    const int each = (a.rows + kThreads - 1) / kThreads, n0 = min(tid * each, a.rows), n1 = min(n0 + each, a.rows);
-    Sums mine{0, 0, my_free}, total;
+    Sums mine{0, 0, 0}, total;
 #pragma unroll 4
+    for (int p = p0; p < p1; p += 16) mine.free_ += __popc(free_bits(a.free_, p, p1, wide));
     for (int n = n0; n < n1; ++n) {
         int need = 0;
         for (int i = 0; i < a.items; ++i) need += missing[n * a.items + i];
-        const Ask r = ask_of(a, n);
-        if (n % blocks == rank) {
-            if (r.bad_len) a.tell(KDA_ERR_BLOCK_TABLE);
-            if (r.bad_new) a.tell(KDA_ERR_CU_SEQLENS);
-        }
         base_of[n] = need;
-        cu[n] = r.add;
-        len_of[n] = r.len;
-        mine = mine + Sums{need, r.add, 0};
+        mine = mine + Sums{need, cu[n], 0};
     }
     const Sums before = block_scan(mine, sums[0], total);
-    if (blocks > 1) {
+    free_before[tid] = before.free_;
+    int free_all = total.free_, free_base = 0;
+    if (a.split) {
         if (tid < blocks) {
             uint32_t at;
             asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(counts + rank)), "r"(tid));
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(total.free_) : "memory");
         }
-    } else if (tid == 0) {
-        counts[0] = total.free_;
+        cluster_sync();
+        free_all = 0;
+        for (int b = 0; b < blocks; ++b) {
+            if (b < rank) free_base += counts[b];
+            free_all += counts[b];
+        }
     }
-    meet();
 
     // ------------------------------------------------------------------ 3: who is served; the free pages they take, in order
-    int free_all = 0, free_base = 0;
-    for (int b = 0; b < blocks; ++b) {
-        if (b < rank) free_base += counts[b];
-        free_all += counts[b];
-    }
     Sums upto = before;
     bool all_served = true;
     mine = Sums{0, 0, 0};
@@ -246,33 +265,38 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     // the tokens too if nobody waits.
     int at = before.add;
     if (!__syncthreads_and(all_served)) at = block_scan(mine, sums[1], total).add;
-    const int dealt = total.need;
+    const int taken = total.need;
     for (int n = n0; n < n1; ++n) {
         const int add = cu[n];
         cu[n] = at;
-        if (n % blocks == rank) a.cu[n] = at;
+        if (n >= r0 && n < r1) a.cu[n] = at;
         at += add;
     }
     if (tid == 0) {
         cu[a.rows] = total.add;
         if (rank == 0) a.cu[a.rows] = total.add;
     }
-    if (dealt > 0) {
-        int k = free_base + before.free_;
-        for (int p = my_p0; p < my_p1 && k < dealt; p += 16) {
-            unsigned bits = free_bits(a.free_, p, my_p1, wide);
-            while (bits != 0 && k < dealt) {
-                const int page = p + __ffs(bits) - 1;
-                bits &= bits - 1;
-                a.dealt[k++] = page;
-                a.free_[page] = 0;
+    // A warp lists those of 512 pages at a time, 16 a lane.  The flags change once nobody counts any more.
+    const int unit = max(512, each_page), u_warp = a.split ? warp : rank * kWarps + warp, u_warps = a.split ? kWarps : blocks * kWarps;
+    for (int u0 = u_warp * unit; s0 + u0 < s1; u0 += u_warps * unit) {
+        int k = free_base + free_before[u0 / each_page];
+        for (int q = s0 + u0; q < min(s0 + u0 + unit, s1) && k < taken; q += 512) {
+            unsigned bits = q + 16 * lane < s1 ? free_bits(a.free_, q + 16 * lane, s1, wide) : 0;
+            int upto_lane = __popc(bits);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto_lane, o);
+                if (lane >= o) upto_lane += x;
             }
+            for (int i = k + upto_lane - __popc(bits); bits != 0 && i < taken; bits &= bits - 1) dealt[i++] = q + 16 * lane + __ffs(bits) - 1;
+            k += __shfl_sync(0xffffffffu, upto_lane, 31);
         }
     }
     meet();
 
     // ------------------------------------------------------------------ 4: entries that were missing
-    for (int i0 = (rank * kWarps + warp) * run; i0 < all; i0 += warps * run) {
+    for (int k = rank * kThreads + tid; k < taken; k += blocks * kThreads) a.free_[dealt[k]] = 0;
+    for (int i0 = item0 + warp * run; i0 < item1; i0 += kWarps * run) {
         const Run r = run_at(i0);
         int lacks = 0, base = 0, from = 0;
         if (lane < r.many) {
@@ -281,44 +305,59 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
             if (base >= 0 && lacks > 0)
                 for (int i = r.row * a.items; i < i0 + lane; ++i) from += missing[i];
         }
-        for (unsigned todo = __ballot_sync(0xffffffffu, base < 0 || lacks > 0); todo != 0; todo &= todo - 1) {
-            const int l = __ffs(todo) - 1, n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + lane;
-            const bool waits = __shfl_sync(0xffffffffu, base, l) < 0;
-            const int first = __shfl_sync(0xffffffffu, r.col0, l), end = __shfl_sync(0xffffffffu, waits ? r.col1_without : r.col1, l);
-            int k0 = __shfl_sync(0xffffffffu, from, l), entry[kEach];
-            int* row = a.table + n * a.table_stride;
+        for (unsigned todo = __ballot_sync(0xffffffffu, base < 0 || lacks > 0); todo != 0;) {
+            int of[kAtOnce], entry[kAtOnce][kEach];      // the next items, of columns lane, 32 + lane, ...
 #pragma unroll
-            for (int k = 0; k < kEach; ++k) entry[k] = c0 + 32 * k < a.width ? row[c0 + 32 * k] : -1;
+            for (int y = 0; y < kAtOnce; ++y) {
+                of[y] = __ffs(todo) - 1;
+                todo &= todo - 1;
+                const int l = max(of[y], 0), n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + lane;
 #pragma unroll
-            for (int k = 0; k < kEach; ++k) {
-                const int c = c0 + 32 * k;
-                if (waits) {      // its columns end where they did
-                    if (c < end || entry[k] == -1) continue;
-                    if ((unsigned)entry[k] < (unsigned)a.n_pages) a.free_[entry[k]] = 1;
-                    row[c] = -1;
-                } else {
-                    const bool is = c >= first && c < end && (unsigned)entry[k] >= (unsigned)a.n_pages;
-                    const unsigned who = __ballot_sync(0xffffffffu, is);
-                    if (is) row[c] = a.dealt[k0 + __popc(who & ((1u << lane) - 1))];
-                    k0 += __popc(who);
+                for (int k = 0; k < kEach; ++k) entry[y][k] = of[y] >= 0 && c0 + 32 * k < a.width ? a.table[n * a.table_stride + c0 + 32 * k] : -1;
+            }
+#pragma unroll
+            for (int y = 0; y < kAtOnce; ++y) {
+                if (of[y] < 0) break;
+                const int l = of[y], n = __shfl_sync(0xffffffffu, r.row, l), c0 = (i0 + l - n * a.items) * kColumns + lane;
+                const bool waits = __shfl_sync(0xffffffffu, base, l) < 0;
+                const int first = __shfl_sync(0xffffffffu, r.col0, l), end = __shfl_sync(0xffffffffu, waits ? r.col1_without : r.col1, l);
+                int k0 = __shfl_sync(0xffffffffu, from, l);
+                int* row = a.table + n * a.table_stride;
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) {
+                    const int c = c0 + 32 * k, e = entry[y][k];
+                    if (waits) {      // its columns end where they did
+                        if (c < end || e == -1) continue;
+                        if ((unsigned)e < (unsigned)a.n_pages) a.free_[e] = 1;
+                        row[c] = -1;
+                    } else {
+                        const bool is = c >= first && c < end && (unsigned)e >= (unsigned)a.n_pages;
+                        const unsigned who = __ballot_sync(0xffffffffu, is);
+                        if (is) row[c] = dealt[k0 + __popc(who & ((1u << lane) - 1))];
+                        k0 += __popc(who);
+                    }
                 }
             }
         }
     }
-    meet();
+    // A block's rows are its own, and so are their tokens, unless there are so many that all blocks share them.
+    const int tokens = cu[a.rows];
+    const bool share = !alone && tokens > 8 * kThreads;
+    if (share) cluster_sync();
+    else __syncthreads();
 
     // ------------------------------------------------------------------ 5: where the new tokens go
-    for (int n = rank * kThreads + tid; n < a.rows; n += blocks * kThreads)
+    for (int n = r0 + tid; n < r1; n += kThreads)
         if (a.kv_lens[n] != len_of[n]) a.kv_lens[n] = len_of[n];
-    const int tokens = cu[a.rows], stride = blocks * kThreads;
-    for (int t0 = rank * kThreads + tid; t0 < a.max_tokens; t0 += kAtOnce * stride) {
+    const int stride = share ? blocks * kThreads : kThreads, t_begin = share ? rank * kThreads : cu[r0], t_end = share ? tokens : cu[r1];
+    const int n_begin = share ? 0 : r0, n_end = share ? a.rows : r1;
+    for (int t0 = t_begin + tid; t0 < t_end; t0 += kAtOnce * stride) {
         int pos[kAtOnce], col[kAtOnce], entry[kAtOnce];
 #pragma unroll
         for (int y = 0; y < kAtOnce; ++y) {
             const int t = t0 + y * stride;
-            pos[y] = -1;
-            if (t >= tokens) continue;
-            int lo = 0, hi = a.rows;      // cu[lo] <= t < cu[hi]
+            if (t >= t_end) continue;
+            int lo = n_begin, hi = n_end;      // cu[lo] <= t < cu[hi]
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
                 if (cu[mid] <= t) lo = mid;
@@ -331,10 +370,14 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
 #pragma unroll
         for (int y = 0; y < kAtOnce; ++y) {
             const int t = t0 + y * stride;
-            if (t >= a.max_tokens) break;
+            if (t >= t_end) break;
             a.positions[t] = pos[y];
-            a.slots[t] = pos[y] < 0 ? -1ll : (long long)entry[y] * a.page + (pos[y] - col[y] * a.page);
+            a.slots[t] = (long long)entry[y] * a.page + (pos[y] - col[y] * a.page);
         }
+    }
+    for (int t = tokens + rank * kThreads + tid; t < a.max_tokens; t += blocks * kThreads) {
+        a.positions[t] = -1;
+        a.slots[t] = -1;
     }
 }
 
@@ -347,6 +390,8 @@ int check(const KdaPlanShape* s) {
     return KDA_OK;
 }
 int items_of(const KdaPlanShape& s) { return ceil_div(s.width, kColumns); }
+// What one block reads in a few loads a thread, and keeps in shared memory.
+bool alone(const KdaPlanShape& s) { return (long long)s.rows * items_of(s) <= 2 * kWarps && s.n_pages <= 16 * kThreads && s.max_tokens <= 2 * kThreads; }
 
 }  // namespace
 }  // namespace kda
@@ -354,7 +399,7 @@ int items_of(const KdaPlanShape& s) { return ceil_div(s.width, kColumns); }
 using namespace kda;
 
 extern "C" size_t kda_plan_pages_workspace_bytes(const KdaPlanShape* s) {
-    if (check(s)) return 0;
+    if (check(s) || alone(*s)) return 0;
     return align_up((size_t)s->rows * items_of(*s) * sizeof(int), 256) + align_up((size_t)(s->n_pages + 1) * sizeof(int), 256);
 }
 
@@ -362,20 +407,26 @@ extern "C" int kda_plan_pages(const KdaPlanShape* s, int32_t* block_table, int32
                               int32_t* cu_seqlens, int32_t* positions, int64_t* slots, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = check(s)) return rc;
     if (!block_table || !kv_lens || !new_lens || !cu_seqlens || (s->n_pages > 0 && !page_free) || (s->max_tokens > 0 && (!positions || !slots))) return KDA_ERR_NULL;
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < kda_plan_pages_workspace_bytes(s)) return KDA_ERR_WORKSPACE;
+    const size_t need = kda_plan_pages_workspace_bytes(s);
+    if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need)) return KDA_ERR_WORKSPACE;
     PlanArgs a;
     a.table = block_table; a.kv_lens = kv_lens; a.free_ = page_free; a.new_lens = new_lens; a.starts = starts;
     a.cu = cu_seqlens; a.positions = positions; a.slots = reinterpret_cast<long long*>(slots);
     a.rows = s->rows; a.width = s->width; a.page = s->page_size; a.n_pages = s->n_pages; a.max_tokens = s->max_tokens;
     a.items = items_of(*s);
-    a.missing = static_cast<int*>(workspace);
-    a.dealt = reinterpret_cast<int*>(static_cast<char*>(workspace) + align_up((size_t)a.rows * a.items * sizeof(int), 256));
+    // every block for itself: 2 us for 262,144 pages, where meeting once more costs 0.6
+    a.split = a.n_pages > 64 * kThreads;
+    a.slice = ceil_div(ceil_div(a.n_pages, kBlocks), 512) * 512;
+    for (a.thread_pages = 16; (long long)a.thread_pages * kThreads < (a.split ? a.slice : a.n_pages);) a.thread_pages *= 2;
+    a.missing = a.dealt = nullptr;
+    if (need > 0) {
+        a.missing = static_cast<int*>(workspace);
+        a.dealt = reinterpret_cast<int*>(static_cast<char*>(workspace) + align_up((size_t)a.rows * a.items * sizeof(int), 256));
+    }
     a.mirror = status_mirror();
     a.table_stride = s->table_stride;
-    // what one block reads in a few loads a thread
-    const bool small = a.rows * a.items <= 2 * kWarps && a.n_pages <= 16 * kThreads && a.max_tokens <= 2 * kThreads;
-    const int blocks = small ? 1 : kBlocks;
-    const size_t smem = (3 * (size_t)a.rows + 1 + (small ? a.rows * a.items : 0)) * sizeof(int);
+    const int blocks = need > 0 ? kBlocks : 1;
+    const size_t smem = (3 * (size_t)a.rows + 1 + (need > 0 ? 0 : a.rows * a.items + a.n_pages)) * sizeof(int);
     if (int rc = set_smem_limit(plan_pages_kernel, smem)) return rc;
     cudaError_t e = cudaSuccess;
     KDA_LAUNCH("plan_pages_kernel", (cudaStream_t)stream,

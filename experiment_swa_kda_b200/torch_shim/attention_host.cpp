@@ -311,10 +311,11 @@ PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const 
     s.table_stride = table.stride(0);
     Tensor cu = empty({N + 1}, at::kInt, table), positions = empty({max_tokens}, at::kInt, table), slots = empty({max_tokens}, at::kLong, table);
     const size_t need = kda_plan_pages_workspace_bytes(&s);
-    Tensor ws = bytes(need, table);
+    Tensor ws;
+    if (need > 0) ws = bytes(need, table);
     must(kda_plan_pages(&s, table.mutable_data_ptr<int32_t>(), lens.mutable_data_ptr<int32_t>(), static_cast<uint8_t*>(free.mutable_data_ptr()),
                         news.const_data_ptr<int32_t>(), iptr(starts), cu.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
-                        ws.data_ptr(), need, stream_of(table)),
+                        need > 0 ? ws.data_ptr() : nullptr, need, stream_of(table)),
          "kda_plan_pages");
     for (const Tensor* t : {&table, &lens, &free}) t->unsafeGetTensorImpl()->bump_version();
     return std::make_tuple(cu, positions, slots);

@@ -143,8 +143,11 @@ struct OwnView : Batch {
     }
 };
 
+// A batch of which every sequence sees the prefix it shares, and then its own keys.
+struct BothView : OwnView {};
+
 // The same batch with each group as one sequence: all new tokens of the group see the whole prefix, and nothing else.
-struct GroupView : OwnView {
+struct GroupView : BothView {
     __device__ __forceinline__ int many() const { return p.n; }
     __device__ __forceinline__ int edge(int g) const {
         const int s = group_edge(g);
@@ -360,7 +363,7 @@ struct ViewOf<kTurnKeys> {
 };
 template <>
 struct ViewOf<kBothKeys> {
-    using type = OwnView;
+    using type = BothView;
 };
 template <>
 struct ViewOf<kOwnKeys> {
@@ -400,6 +403,7 @@ size_t tc_workspace(long long slots, int kv_heads, int splits, int dim);
 bool decode_takes(const Call& c);      // ... and at most 16 rows a sequence and kv head
 size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size, int window, int max_q, int dim);
 int decode(const Call& c, cudaStream_t st);
+int decode_both(const Call& c, cudaStream_t st);      // prefix and own keys one after the other, a finished result
 // The passes of attention behind a shared prefix; their sums stay in the workspace, undivided, for a join.
 int general_shared(const Call& c, int prefix_splits, int own_splits, cudaStream_t st);
 size_t general_shared_workspace(size_t rows, int parts, int dim);

@@ -77,6 +77,7 @@ struct Args {
 // One sequence's tiles and rows.
 struct Seq {
     int first, count, base, lo, hi, t0, t1;
+    int np;      // both: so many of the tiles are the prefix's, keys [0, lo); the others go on from lo's
 };
 // what a sequence is read from: the ends of its new tokens and its length, as they stand in memory, and its group's prefix
 struct Raw {
@@ -92,6 +93,12 @@ __device__ __forceinline__ Raw raw_at(const B& b, int n) {
     const int p = prefix_at(b, n);
     return b.cu != nullptr ? Raw{__ldg(b.cu + n), __ldg(b.cu + n + 1), __ldg(b.kv_lens + n), p} : Raw{n * b.q_len, (n + 1) * b.q_len, __ldg(b.kv_lens + n), p};
 }
+__device__ __forceinline__ void number_tiles(const Batch&, Seq&) {}
+__device__ __forceinline__ void number_tiles(const BothView&, Seq& s) {
+    s.np = (s.lo + kTile - 1) / kTile;
+    s.t1 = s.hi > 0 ? s.np + s.t1 - s.t0 : 0;
+    s.t0 = 0;
+}
 template <class B>
 __device__ __forceinline__ Seq seq_of_raw(const B& b, const Raw& r, int window) {
     Seq s;
@@ -104,6 +111,8 @@ __device__ __forceinline__ Seq seq_of_raw(const B& b, const Raw& r, int window) 
     s.lo = min(max(first_key(s.base, window), own_key(b, r, s.base)), s.hi);
     s.t0 = s.lo / kTile;
     s.t1 = (s.hi + kTile - 1) / kTile;
+    s.np = 0;
+    number_tiles(b, s);
     return s;
 }
 template <class B>
@@ -290,26 +299,32 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             }
         return a.blocks;
     };
-    const Cut cut = a.whole && KEYS == kAllKeys ? find_start<kThreads, true>(b, Hk, window, blocks_of, blockIdx.x, &start, sums)
+    const Cut cut = a.whole && KEYS != kOwnKeys ? find_start<kThreads, true>(b, Hk, window, blocks_of, blockIdx.x, &start, sums)
                                                 : find_start<kThreads, false>(b, Hk, window, blocks_of, blockIdx.x, &start, sums);
-    const int tiles = a.whole && KEYS == kAllKeys ? start.end - start.begin : cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
+    const int tiles = a.whole && KEYS != kOwnKeys ? start.end - start.begin : cut.begin(blockIdx.x + 1) - cut.begin(blockIdx.x);
 
     uint8_t* ring = sm + warp * kStages * L::kStage;
     Walk ahead = {}, w = {};
+    constexpr bool both = KEYS == kBothKeys;
+    // of a tile: its first key, and the keys of it that any row sees
+    auto tile_key = [&](const Walk& x, int tile) { return !both ? tile * kTile : (tile < x.s.np ? tile : tile - x.s.np + x.s.lo / kTile) * kTile; };
+    auto reach_lo = [&](const Walk& x) { return both && x.tile < x.s.np ? 0 : x.s.lo; };
+    auto reach_hi = [&](const Walk& x) { return both && x.tile < x.s.np ? x.s.lo : x.s.hi; };
     auto in_reach = [&](const Walk& x) {
-        const int k0 = x.tile * kTile + 16 * warp;
-        return k0 < x.s.hi && k0 + 16 > x.s.lo;
+        const int k0 = tile_key(x, x.tile) + 16 * warp;
+        return k0 < reach_hi(x) && k0 + 16 > reach_lo(x);
     };
     // a box a lane: K or V, half of the head, rows of one page
     const int boxes = 16 / a.box_rows, l_kv = lane / (kHalves * boxes), l_half = lane / boxes % kHalves, l_box = lane % boxes;
     int row = 0, page = -1;
     auto look = [&]() {
-        const int key = ahead.tile * kTile + 16 * warp + l_box * a.box_rows;
+        const int key = tile_key(ahead, ahead.tile) + 16 * warp + l_box * a.box_rows;
         page = -1;
-        if (l_kv < 2 && ahead.n < b.n_seq && key < ahead.s.hi && key + a.box_rows > ahead.s.lo) {
+        if (l_kv < 2 && ahead.n < b.n_seq && key < reach_hi(ahead) && key + a.box_rows > reach_lo(ahead)) {
             const int col = key / b.page_size;
             row = key - col * b.page_size;
-            page = b.page(ahead.n, col);
+            if constexpr (both) page = ahead.tile < ahead.s.np ? b.prefix_page(max(b.group_of(ahead.n), 0), col) : b.page(ahead.n, col);
+            else page = b.page(ahead.n, col);
             if (page < 0) b.tell(KDA_ERR_BLOCK_TABLE);
         }
     };
@@ -359,6 +374,8 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
         fetch_q(w);
         for (; issued < kStages - 1 && issued < tiles; ++issued) load(issued);
     }
+    if constexpr (both)
+        for (int i = blockIdx.x * kThreads + tid; i < b.p.n; i += gridDim.x * kThreads) check_group(b, i);
     // sequences without a key in reach have no tile: their rows are nothing
     for (int n = blockIdx.x; n < b.n_seq; n += gridDim.x) {
         const Seq s = seq_at(b, n, window);
@@ -406,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             if (tiles - i > w.s.t1 - w.tile) fetch_q(then);
             rows = min(w.s.count * g, kRows);
             unit_begin = w.tile;
-            all_lo = KEYS == kOwnKeys ? w.s.lo : first_key(w.s.base + (rows - 1) / g, window);
+            all_lo = KEYS != kAllKeys ? w.s.lo : first_key(w.s.base + (rows - 1) / g, window);
             all_hi = w.s.base + 1;
 #pragma unroll
             for (int y = 0; y < NR; ++y) {
@@ -414,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
                 for (int x = 0; x < 2; ++x) {
                     const int r = 8 * y + 2 * c4 + x;
                     last[y][x] = r < rows ? w.s.base + r / g : -1;
-                    first[y][x] = KEYS == kOwnKeys ? w.s.lo : first_key(last[y][x], window);
+                    first[y][x] = KEYS != kAllKeys ? w.s.lo : first_key(last[y][x], window);
                     m[y][x] = -INFINITY;
                     l[y][x] = 0.f;
                 }
@@ -433,7 +450,8 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             }
         }
         if (in_reach(w)) {
-            const int s = i % kStages, k0 = w.tile * kTile + 16 * warp;
+            const int s = i % kStages, k0 = tile_key(w, w.tile) + 16 * warp;
+            const bool of_prefix = both && w.tile < w.s.np;      // whose keys all rows see
             if (!flags[0] && !mbar_poll(bar + s, (phases >> s) & 1u, kSpinLimit)) {      // carries on: the warps meet further down
                 flags[0] = 1;
                 b.tell(kStatusWait);
@@ -442,16 +460,16 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             phases ^= 1u << s;
             uint8_t* kv = ring + s * L::kStage;
             const uint32_t sk = smem_u32(kv), sv = sk + kHalves * L::kHalf;
-            const bool partial = k0 < all_lo || k0 + 16 > all_hi;
+            const bool partial = of_prefix ? k0 + 16 > w.s.lo : k0 < all_lo || k0 + 16 > all_hi;
             if (partial) {
                 // keys that no row sees hold anything: their values are blanked, and so are values that are not finite at keys
                 // only some rows see (added at the end by those that do)
 #pragma unroll 1
                 for (int e = lane; e < 16 * kHalves * 8; e += 32) {
                     const int r = e & 15, ch = e >> 4, key = k0 + r;
-                    if (key >= all_lo && key < all_hi) continue;
+                    if (of_prefix ? key < w.s.lo : key >= all_lo && key < all_hi) continue;
                     uint4* at = reinterpret_cast<uint4*>(kv + (kHalves + (ch >> 3)) * L::kHalf + sw128_off(r, ch & 7));
-                    if (key < w.s.lo || key >= w.s.hi) {
+                    if (of_prefix || key < w.s.lo || key >= w.s.hi) {
                         *at = make_uint4(0, 0, 0, 0);
                         continue;
                     }
@@ -509,11 +527,11 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const int key = k0 + r8 + 8 * (x >> 1);
-                        if (key < first[y][x & 1] || key > last[y][x & 1]) sc[y][x] = -INFINITY;
+                        if (of_prefix ? key >= w.s.lo : key < first[y][x & 1] || key > last[y][x & 1]) sc[y][x] = -INFINITY;
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        if (last[y][x] < k0 || first[y][x] >= k0 + 16) top[y][x] = -INFINITY;
+                        if (!of_prefix && (last[y][x] < k0 || first[y][x] >= k0 + 16)) top[y][x] = -INFINITY;
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -633,9 +651,9 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
                     float o[4] = {oa.x, oa.y, ob.x, ob.y};
                     if (M == kLowest) sum = 0.f;      // nothing but -inf: 0 / 0
                     if (flags[1 + q_buffer]) {
-                        const int to = w.s.base + r / g, from = KEYS == kOwnKeys ? w.s.lo : first_key(to, window);
+                        const int to = w.s.base + r / g, from = KEYS != kAllKeys ? w.s.lo : first_key(to, window);
 #pragma unroll 1
-                        for (int key = max(from, unit_begin * kTile); key <= min(to, (w.tile + 1) * kTile - 1); ++key) {
+                        for (int key = max(from, tile_key(w, max(unit_begin, w.s.np))); key <= min(to, tile_key(w, max(w.tile + 1, w.s.np)) - 1); ++key) {
                             if (key >= all_lo && key < all_hi) continue;
                             const int pg = b.page(w.n, key / b.page_size);
                             if (pg < 0) continue;
@@ -681,14 +699,14 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
 // begins; the first such place inside a sequence takes all its parts.  Four values a thread; with few rows several threads share the
 // parts of one place and add up through shared memory.
 constexpr int kJoinThreads = 512, kMaxBlocks = 148 * kPerSm;
-template <int NR>
+template <int NR, int KEYS>
 __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __grid_constant__ Args a) {
     constexpr int kRows = 8 * NR;
     __shared__ Start start;
     __shared__ int sums[kJoinThreads / 32];
     __shared__ float weight[kMaxBlocks * kRows], row_l[kRows], row_m[kRows];
     __shared__ float4 acc[kJoinThreads];
-    const Batch& b = a.c.batch;
+    const auto& b = view<KEYS>(a.c);
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window, id = blockIdx.x + 1;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Cut cut = find_start<kJoinThreads, false>(b, Hk, window, [&](int) { return a.blocks; }, id, &start, sums);
@@ -770,7 +788,8 @@ int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStre
     }
     if (int rc = launch_status()) return rc;
     if (a.blocks == 1 || a.whole || KEYS == kOwnKeys) return KDA_OK;
-    KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
+    if constexpr (KEYS != kOwnKeys)
+        KDA_LAUNCH("attn_decode_join_kernel", st, e = launch_early(attn_decode_join_kernel<NR, KEYS>, dim3(a.blocks - 1), kJoinThreads, 0, st, true, 1, a));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 
@@ -862,6 +881,7 @@ int pass(const Call& c, int prefix_splits, int most_blocks, OwnRows* own, cudaSt
 }  // namespace
 
 int decode(const Call& c, cudaStream_t st) { return pass<kAllKeys>(c, 1, kMaxBlocks, nullptr, st); }
+int decode_both(const Call& c, cudaStream_t st) { return pass<kBothKeys>(c, 1, kMaxBlocks, nullptr, st); }
 int own_rows(const Call& c, int prefix_splits, int most_blocks, OwnRows& own, cudaStream_t st) {
     return pass<kOwnKeys>(c, prefix_splits, most_blocks, &own, st);
 }

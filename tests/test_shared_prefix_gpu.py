@@ -34,8 +34,9 @@ def close(got, want, size, dtype):
 class Batch:
     """Sequences of groups, with garbage wherever nothing may be read."""
 
-    def __init__(self, heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, seed=0, garbage=float("nan"), layout="dense", shares=None):
-        """own[n]: tokens behind the prefix (the new ones among them); shares[n] false: own[n] tokens in all, none of them shared."""
+    def __init__(self, heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, seed=0, garbage=float("nan"), layout="dense", shares=None, room=0):
+        """own[n]: tokens behind the prefix (the new ones among them); shares[n] false: own[n] tokens in all, none of them shared.  room:
+        tokens that the sequences' tables have besides; which kernels take a call goes by the tables' widths."""
         gen = torch.Generator().manual_seed(seed)
         n = len(q_lens)
         group = [next((g for g in range(len(prefix)) if cu_groups[g] <= i < cu_groups[g + 1]), None) for i in range(n)]
@@ -43,7 +44,7 @@ class Batch:
         base = [prefix[g] if g is not None and s else 0 for g, s in zip(group, shares)]
         self.kv_lens = [b + o for b, o in zip(base, own)]
         self.q_lens, self.prefix, self.cu_groups, self.dtype = list(q_lens), list(prefix), list(cu_groups), dtype
-        width = max(1, max(-(-x // page) for x in self.kv_lens)) + 1
+        width = max(1, max(-(-x // page) for x in self.kv_lens)) + 1 + room // page
         pw = max(1, max(-(-x // page) for x in prefix))
         need = sum(max(0, -(-x // page) - b // page) for x, b in zip(self.kv_lens, base)) + sum(-(-x // page) for x in prefix)
         pages = need + 3
@@ -122,16 +123,18 @@ CASES = [  # heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups
 
 @pytest.mark.parametrize("heads,kv_heads,dim,page,dtype,q_lens,own,prefix,cu_groups", CASES)
 @pytest.mark.parametrize("bound", [True, False])
-def test_against_the_restatement(heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, bound):
+@pytest.mark.parametrize("room", [0, 60000])
+def test_against_the_restatement(heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, bound, room):
     import experiment_swa_kda_b200 as m
-    b = Batch(heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, layout="strided" if bound else "dense")
+    b = Batch(heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups, layout="strided" if bound else "dense", room=room)
     o, lse = m.shared_prefix_attention(*b.device(), max_q_len=max(q_lens) if bound else 0, return_lse=True)
     b.check(o, lse)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("q", [1, 3, 40, 110])
-def test_sequences_that_do_not_share(dtype, q):
+@pytest.mark.parametrize("q", [1, 3, 10, 40, 110])
+@pytest.mark.parametrize("room", [0, 60000])
+def test_sequences_that_do_not_share(dtype, q, room):
     """Places without a request, texts shorter than the prefix, sequences of no group, a group without sequences, a prefix of nothing."""
     import experiment_swa_kda_b200 as m
     n = 13
@@ -141,16 +144,17 @@ def test_sequences_that_do_not_share(dtype, q):
     own[4], shares[4] = max(q - 1, 0), False      # padding first, then tokens (q = 1: padding only)
     own[6], shares[6] = 20 + q, False       # shorter than its group's prefix
     own[9], shares[9] = 49 + q, False       # the prefix would begin behind its first new token
-    b = Batch(4, 2, 64, 16, dtype, [q] * n, own, [50, 50, 0], [2, 8, 8, 12], shares=shares)
+    b = Batch(4, 2, 64, 16, dtype, [q] * n, own, [50, 50, 0], [2, 8, 8, 12], shares=shares, room=room)
     for max_q in (q, 0):
         o, lse = m.shared_prefix_attention(*b.device(), max_q_len=max_q, return_lse=True)
         b.check(o, lse)
 
 
-def test_equal_groups_and_lengths_without_their_tables():
+@pytest.mark.parametrize("room", [0, 60000])
+def test_equal_groups_and_lengths_without_their_tables(room):
     import experiment_swa_kda_b200 as m
     for q in (1, 6, 70):
-        b = Batch(8, 2, 128, 16, BF16, [q] * 6, [q, q + 1, 70, 79, 78, 100], [77, 128, 200], [0, 2, 4, 6])
+        b = Batch(8, 2, 128, 16, BF16, [q] * 6, [q, q + 1, 70, 79, 78, 100], [77, 128, 200], [0, 2, 4, 6], room=room)
         args = b.device()
         args[7] = args[8] = None
         o, lse = m.shared_prefix_attention(*args, return_lse=True, scale=0.2)
@@ -159,11 +163,12 @@ def test_equal_groups_and_lengths_without_their_tables():
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("q", [1, 10, 24, 130])
-def test_values_that_are_not_finite(dtype, q):
+@pytest.mark.parametrize("room", [0, 60000])
+def test_values_that_are_not_finite(dtype, q, room):
     """Infinite and undefined values at keys that are seen, in the prefix and behind it; scores of -inf throughout."""
     import experiment_swa_kda_b200 as m
     for where in ("prefix_v", "prefix_k", "own_v", "last_v", "minus"):
-        b = Batch(4, 2, 64, 16, dtype, [q] * 5, [q + 3, q, 30 + q, 2 + q, q], [150], [0, 5], seed=3)
+        b = Batch(4, 2, 64, 16, dtype, [q] * 5, [q + 3, q, 30 + q, 2 + q, q], [150], [0, 5], seed=3, room=room)
         page = 16
         at = {"prefix_v": (int(b.prefix_table[0, 3]), 5), "prefix_k": (int(b.prefix_table[0, 9]), 2), "own_v": (int(b.table[2, (160) // page]), 160 % page),
               "last_v": (int(b.table[0, (b.kv_lens[0] - 1) // page]), (b.kv_lens[0] - 1) % page)}.get(where)
@@ -200,14 +205,15 @@ def test_equals_paged_attention_where_rows_hold_the_prefix():
     assert (one.double() - two.double()).norm() <= 3 * U * two.double().norm()
 
 
-def test_inconsistent_arrays_are_bounded_and_told():
+@pytest.mark.parametrize("room", [0, 60000])
+def test_inconsistent_arrays_are_bounded_and_told(room):
     import experiment_swa_kda_b200 as m
     fine = Batch(4, 2, 64, 16, BF16, [1] * 4, [3, 4, 5, 6], [40], [0, 4])
     for dtype in (BF16, F32):
         for at, bad, match in ((7, [0, 9], "cu_seqlens"), (7, [3, 1], "cu_seqlens|block table"), (7, [-2, 4], "cu_seqlens"), (6, [-1], "block table"), (6, [10 ** 6], "block table"),
                                (8, [0, 1, 2, 9, 4], "cu_seqlens"), (8, [0, 1, 2, 3, 3], "cu_seqlens"), (4, [43, 10 ** 6, 45, 46], "block table"),
                                (5, [[-1, 99, -7]], "block table")):
-            args = Batch(4, 2, 64, 16, dtype, [1] * 4, [3, 4, 5, 6], [40], [0, 4], garbage=0.0).device()
+            args = Batch(4, 2, 64, 16, dtype, [1] * 4, [3, 4, 5, 6], [40], [0, 4], garbage=0.0, room=room).device()
             args[at] = torch.tensor(bad, dtype=torch.int32, device=DEV)
             for max_q in (1, 0):
                 m.shared_prefix_attention(*args, max_q_len=max_q)
@@ -218,9 +224,10 @@ def test_inconsistent_arrays_are_bounded_and_told():
     fine.check(o)
 
 
-def test_captured_on_another_stream_and_graphs_at_once():
+@pytest.mark.parametrize("room", [0, 60000])
+def test_captured_on_another_stream_and_graphs_at_once(room):
     import experiment_swa_kda_b200 as m
-    batches = [Batch(16, 4, 128, 16, BF16, [q] * 12, [(13 * i) % 90 + q for i in range(12)], [600], [0, 12], seed=q) for q in (1, 6, 100)]
+    batches = [Batch(16, 4, 128, 16, BF16, [q] * 12, [(13 * i) % 90 + q for i in range(12)], [600], [0, 12], seed=q, room=room) for q in (1, 6, 100)]
     args = [b.device() for b in batches]
     wants = [m.shared_prefix_attention(*a, max_q_len=q) for a, q in zip(args, (1, 6, 100))]
     for b, w in zip(batches, wants):

@@ -308,17 +308,21 @@ __device__ __forceinline__ PrefixWork prefix_work(const GroupView& b, int g, int
 }
 constexpr int kSms = 148, kPartTries = 128;
 // Microseconds that both passes take, as measured, where the one over prefixes has `blocks` SMs and parts of `part` key tiles: a key tile takes 0.95 with
-// row tiles of 128 and 2 with 256, a tile of 64 own keys 1.0 of an SM (0.6 with 64 values a head), and either pass 8 besides.
-__host__ __device__ __forceinline__ float passes_us(int part, int blocks, int tile_rows, int dim, long long own_tiles) {
-    const float prefix_us = 8.f + (float)part * (tile_rows == 128 ? 0.95f : 2.f), own_us = own_tiles > 0 ? (float)own_tiles * (dim <= 64 ? 0.6f : 1.f) : 0.f;
-    return own_us > 0.f && blocks < kSms ? fmaxf(prefix_us, 8.f + own_us / (float)(kSms - blocks)) : prefix_us + own_us / kSms;
+// row tiles of 128 and 2 with 256, all own keys `own_us` of an SM (own_tiles_us), and either pass 10 besides.
+__host__ __device__ __forceinline__ float passes_us(int part, int blocks, int tile_rows, float own_us) {
+    const float prefix_us = 10.f + (float)part * (tile_rows == 128 ? 0.95f : 2.f);
+    return own_us > 0.f && blocks < kSms ? fmaxf(prefix_us, 10.f + own_us / (float)(kSms - blocks)) : prefix_us + own_us / kSms;
+}
+// ... by tiles of 64, with so many rows a sequence and kv head
+__host__ __device__ __forceinline__ float own_tiles_us(long long tiles, int dim, int rows) {
+    return (float)tiles * (rows > 16 ? 1.5f : rows > 8 ? 1.2f : 0.8f) * (dim <= 64 ? 0.75f : 1.f);
 }
 // Key tiles of a part, and the blocks that gives: each of the first kPartTries threads tries one number of parts for the longest prefix.  Called by all
 // `warps` warps; `work` is filled, `best` has two places a warp.
 struct PartChoice {
     int part, blocks;
 };
-__device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int groups, int tile_rows, int kv_heads, int dim, long long own_tiles, int splits, unsigned* best, int warps) {
+__device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int groups, int tile_rows, int kv_heads, float own_us, int splits, unsigned* best, int warps) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int longest = 0, row_tiles = 0;
     for (int g = 0; g < groups; ++g) {
@@ -330,7 +334,7 @@ __device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int g
     if (longest > 0)
         for (int g = 0; g < groups; ++g) blocks += work[g].row_tiles * ((work[g].tiles + part - 1) / part);
     blocks *= kv_heads;
-    const float us = passes_us(part, blocks, tile_rows, dim, own_tiles);
+    const float us = passes_us(part, blocks, tile_rows, own_us);
     const bool fits = tid < kPartTries && tries <= splits && blocks <= max(kSms, row_tiles * kv_heads);
     const unsigned cost = fits ? __float_as_uint(us) : 0x7f800000u;
     unsigned least = __reduce_min_sync(0xffffffffu, cost);

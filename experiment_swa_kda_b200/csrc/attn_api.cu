@@ -140,16 +140,17 @@ long long behind_of(const KdaPagedShape& s, const KdaPrefixShape& p) {
 }
 
 // The best that the passes over prefixes and over own keys of few rows can do side by side, and the blocks of the first with which they do.
-float side_by_side_us(const KdaPagedShape& s, const KdaPrefixShape& p, int splits, long long own_tiles, int& blocks) {
+float side_by_side_us(const KdaPagedShape& s, const KdaPrefixShape& p, int splits, int max_q, long long own_tiles, int& blocks) {
     const int group = s.q_heads / s.kv_heads, rows = prefix_rows(s.tokens, p.n_groups, group);
     const long long tiles = ((long long)p.table_width * s.page_size + 127) / 128;
     const long long row_tiles = (((long long)s.tokens * group + p.n_groups - 1) / p.n_groups + rows - 1) / rows * p.n_groups * s.kv_heads;
+    const float own_us = own_tiles_us(own_tiles, s.head_dim, max_q * group);
     blocks = 0;
-    if (splits < 2 || tiles == 0) return (float)(8.0 + (double)row_tiles * tiles * 2 / kSms + own_tiles * 1.0 / kSms);
+    if (splits < 2 || tiles == 0) return (float)(10.0 + (double)row_tiles * tiles * 2 / kSms + own_us / kSms);
     float least = INFINITY;
     for (int tries = 1; tries <= splits && (tries == 1 || row_tiles * tries <= kSms); ++tries) {
         const int part = (int)((tiles + tries - 1) / tries), n = (int)(row_tiles * ((tiles + part - 1) / part));
-        const float us = passes_us(part, n, rows, s.head_dim, own_tiles);
+        const float us = passes_us(part, n, rows, own_us);
         if (us < least) least = us, blocks = n;
     }
     return least;
@@ -164,17 +165,17 @@ bool few_keys(const KdaPagedShape& s) {
 // So do sequences of more rows where that is quicker, by estimates in microseconds.  One pass: blocks of a row tile of a sequence, 1.3 a key tile of 128
 // (2 with more than 128 rows) and 8 besides.  Two: the prefix in whole row tiles, own keys in blocks as these or by the token steps' kernel, and the join.
 // 16 sequences of 40 rows behind 2,000 tokens 31 and 44 us with 3 heads, 78 and 70 with 16; 30 of 400 behind 1,000 61 and 132; 64 of 20 behind 4,097 150 and 68.
-bool takes_both(const KdaPagedShape& s, const KdaPrefixShape& p) {
+bool takes_both(const KdaPagedShape& s, const KdaPrefixShape& p, long long max_q) {      // max_q: a bound on a sequence's new tokens, 0: unknown
     const int group = s.q_heads / s.kv_heads;
     const double rows = (double)s.tokens * group / s.n_seq;      // of a sequence and kv head
-    const bool few = s.max_q_len > 0 ? (long long)s.max_q_len * group <= 24 : rows <= 24;
-    if (rows <= 16) return false;
+    const bool few = max_q > 0 && max_q * group <= 24;
+    if (max_q > 0 && max_q * group <= 16) return false;
     const double each = rows <= 128 ? 1.3 : 2.0, tiles = (double)s.table_width * s.page_size / 128 + 1, own = behind_of(s, p) * 0.6 / 128 + 1;
     const double units = (double)s.n_seq * s.kv_heads * ceil(rows / 256);
     const double one = units <= kSms / 2 ? 12 + each * fmax(fmin(tiles, 8), tiles * units / kSms) : ceil(units / kSms) * (8 + each * tiles);
     const double join = 4 + (double)s.tokens * s.q_heads / 800;
     int blocks;
-    if (few) return one < side_by_side_us(s, p, tc_prefix_splits(s, p), (long long)(2 * own * s.n_seq * s.kv_heads), blocks) + 8 + join;
+    if (few) return one < side_by_side_us(s, p, tc_prefix_splits(s, p), (int)max_q, (long long)(2 * own * s.n_seq * s.kv_heads), blocks) + 6 + join;
     const double row_tiles = ceil((double)s.tokens * group / 256) * s.kv_heads, prefix = (double)p.table_width * s.page_size / 128;
     const double two = 10 + fmax(row_tiles * prefix * 2 / kSms, row_tiles > kSms / 2 ? ceil(row_tiles / kSms) * prefix * 2 : 0) + ceil(units / kSms) * (10 + each * own) + join;
     return one < two;
@@ -188,8 +189,9 @@ int own_blocks(const KdaPagedShape& s, const KdaPrefixShape& p, bool packed, int
     const long long behind = behind_of(s, p);
     const long long most = ((behind + 63) / 64 + 1) * s.n_seq * s.kv_heads / 2, own_tiles = (behind * 3 / 5 + 32) * s.n_seq * s.kv_heads / 64;
     int best = 0;
-    side_by_side_us(s, p, splits, own_tiles, best);
-    const long long n = (long long)own_rows_per_sm(s.head_dim, (packed ? s.max_q_len : s.tokens / s.n_seq) * group) * (best < kSms ? kSms - best : kSms);
+    const int max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
+    side_by_side_us(s, p, splits, max_q, own_tiles, best);
+    const long long n = (long long)own_rows_per_sm(s.head_dim, max_q * group) * (best < kSms ? kSms - best : kSms);
     return (int)(most < 2 ? 2 : most < n ? most : n);
 }
 
@@ -258,7 +260,7 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     c.max_q_len = packed ? s->max_q_len : q_len;
     c.workspace = workspace;
     if (!tc_takes(c)) return general_shared(c, general_prefix_splits(*s, *p), general_splits(*s, packed), st);
-    if (takes_both(*s, *p)) return tc_both(c, tc_splits(*s, packed), st);
+    if (takes_both(*s, *p, c.max_q_len)) return tc_both(c, tc_splits(*s, packed), st);
     if (few_keys(*s) && decode_takes(c)) return decode_both(c, st);
     const bool few = own_rows_take(c);
     const int prefix_splits = tc_prefix_splits(*s, *p), own_splits = tc_splits(*s, packed);

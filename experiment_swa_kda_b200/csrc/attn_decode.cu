@@ -34,11 +34,12 @@ namespace {
 
 using namespace tc;
 
-constexpr int kMaxRows = 16, kMaxOwnRows = 24, kTile = 64, kWarps = 4, kThreads = 128, kStages = 3;
+constexpr int kMaxRows = 16, kMaxOwnRows = 24, kTile = 64, kWarps = 4, kThreads = 128;
 constexpr int kPerSm = 2;             // blocks an SM: 102 KB each, 106 with more than 8 rows
-// ... of own keys: a tile of heads 64 wide is bound by the latency of what is done to it, and four blocks fit
+// ... of own keys, beside another pass, where what is done to a tile takes as long as its bytes and more warps hide it: three with rings of two stages
+// instead of three, four of heads 64 wide
 template <int DP, int NR, int KEYS>
-constexpr int kPerSmOf = KEYS == kOwnKeys && DP == 64 && NR == 1 ? 4 : kPerSm;
+constexpr int kPerSmOf = KEYS == kOwnKeys && NR == 1 ? (DP == 64 ? 4 : 3) : kPerSm;
 // Up to so many tiles a sequence and kv head stay together: they take about as long as two of them and the join, which is a launch less (3
 // conversations of 40 tokens 14.5 us in parts, 8.4 whole; 16 of 100 12.5 and 10.4).  Six where there are sequences for every SM (200 of up
 // to 380 36 and 33), four where parts would have some to themselves (one of 300 12.4 and 13.2 with six).
@@ -47,8 +48,9 @@ constexpr int kMinTiles = 2;          // a stretch has at least these many tiles
 constexpr float kLazy = 8.f;          // as in the kernel for long chunks: sums are rescaled when a maximum grew by 2^8
 constexpr int kStatusWait = 121;
 
-template <int DP, int NR>
+template <int DP, int NR, int KEYS>
 struct Layout {
+    static constexpr int kStages = DP == 128 && kPerSmOf<DP, NR, KEYS> > 2 ? 2 : 3;
     static constexpr int kHalf = 16 * 128;                            // 16 keys of 64 values
     static constexpr int kStage = 2 * (DP / 64) * kHalf;              // K and V of 16 keys
     static constexpr int kRowsOf = 8 * NR;
@@ -267,7 +269,8 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {      // an 8 x 8 tile o
 template <int DP, int NR, int KEYS>
 __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                                        const __grid_constant__ Args a) {
-    using L = Layout<DP, NR>;
+    using L = Layout<DP, NR, KEYS>;
+    constexpr int kStages = L::kStages;
     constexpr int kHalves = DP / 64, kSteps = DP / 16, kRows = 8 * NR;
     extern __shared__ uint8_t raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
     auto blocks_of = [&](int total) {
         if constexpr (KEYS == kOwnKeys)
             if (a.prefix_splits > 1 && total > kMinTiles * kPerSmOf<DP, NR, KEYS>) {
-                const int sms = kSms - choose_parts(work, b.p.n, a.prefix_rows, Hk, D, total, a.prefix_splits, reinterpret_cast<unsigned*>(work + kMaxListed), kWarps).blocks;
+                const int sms = kSms - choose_parts(work, b.p.n, a.prefix_rows, Hk, own_tiles_us(total, D, a.c.max_q_len * g), a.prefix_splits, reinterpret_cast<unsigned*>(work + kMaxListed), kWarps).blocks;
                 if (sms > 0) return min(a.blocks, kPerSmOf<DP, NR, KEYS> * sms);
             }
         return a.blocks;
@@ -777,7 +780,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const __
 
 template <int DP, int NR, int KEYS>
 int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStream_t st) {
-    constexpr int kBytes = Layout<DP, NR>::kBytes;
+    constexpr int kBytes = Layout<DP, NR, KEYS>::kBytes;
     if (int rc = set_smem_limit(attn_decode_kernel<DP, NR, KEYS>, kBytes)) return rc;
     cudaError_t e = cudaSuccess;
     if constexpr (KEYS == kOwnKeys) {      // beside the pass over the prefix
@@ -827,7 +830,7 @@ size_t decode_workspace(int n_seq, int kv_heads, int table_width, int page_size,
 
 constexpr int kMaxOwnBlocks = 148 * 4;
 bool own_rows_take(const Call& c) { return takes(c, kMaxOwnRows); }
-int own_rows_per_sm(int dim, int rows) { return dim <= 64 && rows <= 8 ? kPerSmOf<64, 1, kOwnKeys> : kPerSm; }
+int own_rows_per_sm(int dim, int rows) { return rows > 8 ? kPerSm : dim <= 64 ? kPerSmOf<64, 1, kOwnKeys> : kPerSmOf<128, 1, kOwnKeys>; }
 size_t own_rows_workspace(const KdaPagedShape& s, int max_q) {
     const size_t rows = (size_t)s.tokens * s.q_heads;
     return align_up(parts_bytes(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, max_q, s.head_dim, kMaxOwnRows, kMaxOwnBlocks), 256) + align_up(rows * sizeof(float2), 256) +

@@ -140,7 +140,7 @@ __device__ __forceinline__ bool prefix_unit(const Args& a, const GroupView& b, i
     if (lane == 0) own[warp] = own_of;
     __syncthreads();
     own_of = __reduce_add_sync(0xffffffffu, lane < kThreads / 32 ? own[lane] : 0);
-    const int part = choose_parts(work, b.p.n, a.tiles.rows, heads, a.c.heads.dim, (long long)own_of * heads, a.splits, best, kThreads / 32).part;
+    const int part = choose_parts(work, b.p.n, a.tiles.rows, heads, own_tiles_us((long long)own_of * heads, a.c.heads.dim, a.c.max_q_len * a.c.heads.group), a.splits, best, kThreads / 32).part;
     int id = blockIdx.x, i0 = 0, found = -1;
     for (; i0 < a.slots && found < 0; i0 += 32) {
         const int n = i0 + lane < a.slots ? (tiles_of[i0 + lane] + part - 1) / part : 0;

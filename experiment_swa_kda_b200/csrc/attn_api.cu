@@ -204,7 +204,8 @@ SharedSpace shared_space(const KdaPagedShape& s, const KdaPrefixShape& p, bool p
     int per;
     const int group = s.q_heads / s.kv_heads, max_q = packed ? s.max_q_len : s.tokens / s.n_seq;
     const int rows = prefix_rows(s.tokens, p.n_groups, group);
-    w.prefix = align_up(tc_parts_bytes(group_slots(groups_of(s, p), group, rows, per), rows, s.kv_heads, tc_prefix_splits(s, p), s.head_dim), 256);
+    w.prefix = align_up(tc_parts_bytes(group_slots(groups_of(s, p), group, rows, per), rows, s.kv_heads, tc_prefix_splits(s, p), s.head_dim), 256) +
+               align_up((size_t)s.tokens * sizeof(int4), 256);
     w.own = few ? own_rows_workspace(s, max_q) : tc_parts_bytes(tile_slots(s.tokens, s.n_seq, max_q, group, 256, packed, per), 256, s.kv_heads, tc_splits(s, packed), s.head_dim);
     w.own = align_up(w.own, 256);
     return w;

@@ -70,6 +70,9 @@ struct Args {
     int* parts;
     float2* part_ml;
     float* part_o;
+    // a pass over prefixes: of each token its group's first slot (-1: it shares no prefix), the place of its first row behind it, its sequence (-1: none)
+    // and its place there
+    int4* places;
 };
 // byte offset of 16-byte piece c of row r in half a row tile's sums
 template <int DP>
@@ -171,6 +174,24 @@ __device__ __forceinline__ bool prefix_unit(const Args& a, const GroupView& b, i
     return found >= 0;
 }
 
+// What the join has to know of this block's share of the tokens; thread t of `threads`.
+__device__ __forceinline__ void write_places(const Args& a, const GroupView& b, int t, int threads) {
+    const int block = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), blocks = gridDim.x * gridDim.y * gridDim.z;
+    for (int tok = block * threads + t; tok < b.tokens; tok += blocks * threads) {
+        const int n = b.seq_of(tok);
+        int first, count;
+        b.Batch::span(n, first, count);
+        const bool inside = tok >= first && tok < first + count;
+        const int group = b.group_of(n), prefix = group < 0 ? 0 : b.prefix_len(group);
+        int4 p = make_int4(-1, 0, inside ? n : -1, tok - first);
+        if (inside && prefix > 0 && b.kv_len(n) - count >= prefix) {
+            const int from = b.edge(group);
+            if (tok >= from) p.x = a.tiles.start(b, group), p.y = (tok - from) * a.c.heads.group;
+        }
+        a.places[tok] = p;
+    }
+}
+
 template <int DP, int KEYS>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                               const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mO,
@@ -218,6 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 for (int i = blockIdx.x * kThreads + tid; i < b.p.n; i += gridDim.x * kThreads) check_group(b, i);
     }
     if (!some) {
+        if constexpr (in_prefix)
+            if (tid < 64) write_places(a, a.c.batch, tid, 64);
         if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too
         return;
     }
@@ -751,6 +774,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     mbar_poll(ring_is_v(x) && partial(t_begin + ring_tile(x)) ? bar_part + stage(x) : bar_full + stage(x), turn(x), kSpinLimit / 8);
         } else {
             // -------------------------------------------------------------- V tiles that some row sees only in part
+            if constexpr (in_prefix) write_places(a, a.c.batch, tid - kFixWarp * 32, 64);
             uint32_t phase = 0;      // of each stage's barrier
             bool odd = false;
             for (int j = t_begin; j < t_end; ++j) {
@@ -885,31 +909,27 @@ template <int DP>
 __global__ void __launch_bounds__(32 * kSharedWarps, 4) attn_shared_join_kernel(const __grid_constant__ SharedJoin j) {
     constexpr int kLanes = DP / 4, kAtOnce = 32 / kLanes, kAhead = 4;
     __shared__ float4 sums_o[kSharedWarps][kLanes];
-    const GroupView& groups = j.prefix.c.batch;
-    const OwnView& b = groups;
     const int g = j.prefix.c.heads.group, D = j.prefix.c.heads.dim, Hk = j.prefix.c.heads.kv_heads, Hq = j.prefix.c.heads.q_heads;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % j.per_row;      // of the row's warps
-    const long long rows = (long long)b.tokens * Hq, at = ((long long)blockIdx.x * kSharedWarps + warp) / j.per_row;
+    const long long rows = (long long)j.prefix.c.batch.tokens * Hq, at = ((long long)blockIdx.x * kSharedWarps + warp) / j.per_row;
     const size_t row = (size_t)(at < rows ? at : rows - 1);
     const int tok = (int)(row / Hq), head = (int)(row - (size_t)tok * Hq), hk = head / g, hg = head - hk * g;
-    const int n = b.seq_of<32>(tok, lane, 0xffffffffu);
-    int first, count;
-    b.Batch::span(n, first, count);
-    const int base = b.kv_len(n) - count, group = b.group_of(n), prefix = group < 0 ? 0 : b.prefix_len(group);
-    const bool inside = tok >= first && tok < first + count, shares = inside && prefix > 0 && base >= prefix;
-    // Where a pass over sequences (or groups) whose first token is `from` and whose first slot `start` has this row.  What the device
-    // arrays say is not trusted as an index: parts there are none of outside of the slots.
+    dependency_wait();
+    const uint4 known = ld_after16(j.prefix.places + tok);
+    const int n = (int)known.z, in_seq = (int)known.w * g + hg;
+    const bool inside = n >= 0;
+    // Where a pass whose tiles of `tile` rows begin at slot `start` has this row.  What the device arrays say is not trusted as an index: there
+    // are no parts outside of the slots.
     struct Place {
         int slot, row;
     };
-    auto place_in = [&](int start, int from, int tile) {
-        const long long r = (long long)(tok - from) * g + hg;
-        return Place{r < 0 ? -1 : start + (int)(r / tile), (int)(r % tile)};
-    };
+    auto place_in = [&](int start, int r, int tile) { return Place{start + r / tile, r % tile}; };
     Place of_prefix{-1, 0}, of_own{-1, 0};
-    if (shares) of_prefix = place_in(j.prefix.tiles.start(groups, group), groups.edge(group), j.prefix.tiles.rows);
-    if (inside && j.rows.spans == nullptr) of_own = place_in(j.own.tiles.start(b, n), first, kRows);
-    dependency_wait();
+    if ((int)known.x >= 0) of_prefix = place_in((int)known.x, (int)known.y + hg, j.prefix.tiles.rows);
+    if (inside && j.rows.spans == nullptr) {      // Tiles::start, of a sequence whose first token is known
+        const Tiles& t = j.own.tiles;
+        of_own = place_in(t.per_seq > 0 ? n * t.per_seq : (int)((long long)(tok - (int)known.w) * t.group / t.rows) + n, in_seq, kRows);
+    }
     auto parts_of = [&](const Args& a, const Place& p) {
         if ((unsigned)p.slot >= (unsigned)a.slots) return 0;
         return min(max(__float_as_int(ld_after_f32(reinterpret_cast<const float*>(a.parts + p.slot * Hk + hk))), 0), a.splits);
@@ -927,10 +947,10 @@ __global__ void __launch_bounds__(32 * kSharedWarps, 4) attn_shared_join_kernel(
             n_own = min(max((int)span.y, stretch), j.rows.blocks - 1) - stretch + 1;
         }
     }
-    const int parts = n_prefix + n_own, in_seq = min((tok - first) * g + hg, j.rows.rows - 1);
+    const int parts = n_prefix + n_own;
     // (maximum, sum) of part k, and its sums' piece of this lane
     auto part_in = [&](const Args& a, const Place& p, int z) { return ((size_t)z * a.slots + p.slot) * Hk + hk; };
-    auto stretch_row = [&](int k) { return ((size_t)(stretch + k) * 2 + (k == 0 ? 1 : 0)) * j.rows.rows + in_seq; };
+    auto stretch_row = [&](int k) { return ((size_t)(stretch + k) * 2 + (k == 0 ? 1 : 0)) * j.rows.rows + min(in_seq, j.rows.rows - 1); };
     auto ml_of = [&](int k) -> const float2* {
         if (k < n_prefix) return j.prefix.part_ml + part_in(j.prefix, of_prefix, k) * j.prefix.tiles.rows + of_prefix.row;
         k -= n_prefix;
@@ -1071,6 +1091,7 @@ void place_parts(Args& a, const Call& c) {
     a.parts = reinterpret_cast<int*>(ws);
     a.part_ml = reinterpret_cast<float2*>(ws + align_up(units * sizeof(int), 256));
     a.part_o = reinterpret_cast<float*>(a.part_ml + units * a.splits * a.tiles.rows);
+    a.places = reinterpret_cast<int4*>(ws + align_up(tc_parts_bytes(a.slots, a.tiles.rows, c.heads.kv_heads, a.splits, c.heads.dim), 256));
 }
 Args args_of(const Call& c, int keys, int splits) {
     Args a;
@@ -1082,6 +1103,7 @@ Args args_of(const Call& c, int keys, int splits) {
     a.splits = splits;
     a.box_rows = c.batch.page_size < kKeys ? c.batch.page_size : kKeys;
     a.q_boxes = a.own_rows = 0;
+    a.places = nullptr;
     a.parts = nullptr;
     a.part_ml = nullptr;
     a.part_o = nullptr;

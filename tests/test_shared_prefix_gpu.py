@@ -309,3 +309,63 @@ def test_serving_with_a_pool_and_a_prefix():
         # two attention outputs of one rounding and one set of rounded weights each, through one projection
         assert (got.double() - want.double()).norm() <= 1e-2 * want.double().norm()
     assert int((~pool.page_free).sum()) == -(-prefix // page) + sum(-(-n // page) - prefix // page for n in lens)
+
+
+def test_a_captured_step_of_a_scheduler():
+    """Lengths, pages, cache and attention of a token step in one graph, replayed across page borders."""
+    import experiment_swa_kda_b200 as m
+    torch.manual_seed(6)
+    layer = m.PagedAttention(256, 4, 2, 64, max_positions=512).to(DEV)
+    page, prefix, rows = 8, 45, 3
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    text = torch.randn(1, prefix, 256, device=DEV).bfloat16()
+    pool = m.PagedCache.pool(rows + 1, 200, 60, page, 2, 64, DEV)      # the last row holds the prefix
+    pool.kv_lens.copy_(i32([0] * rows + [prefix]))
+    layer(text, pool, pool.plan(i32([0] * rows + [prefix]), prefix)[0], max_q_len=prefix)
+    whole = m.PagedCache.zeros(rows, 200, page, 2, 64, DEV)
+    whole.kv_lens.fill_(prefix)
+    layer(text.expand(rows, -1, -1), whole)
+    serve = m.PagedCache(pool.k, pool.v, pool.block_table[:rows], pool.kv_lens[:rows], prefix_table=pool.block_table[rows:], prefix_lens=pool.kv_lens[rows:])
+    pool.kv_lens[:rows] = prefix
+    new, starts, x = i32([1] * rows + [0]), i32([prefix] * rows + [0]), torch.zeros(1, rows, 256, device=DEV, dtype=BF16)
+
+    def step():
+        pool.kv_lens[:rows] += 1
+        cu, _, slots = pool.plan(new, rows, starts=starts)
+        return layer(x, serve, cu[:rows + 1], max_q_len=1), slots
+
+    kept = pool.block_table.clone(), pool.page_free.clone()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):      # a first call outside of the graph
+        step()
+    torch.cuda.synchronize()
+    pool.block_table.copy_(kept[0]), pool.page_free.copy_(kept[1]), pool.kv_lens[:rows].fill_(prefix)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, slots = step()
+    for i in range(20):
+        x.copy_(torch.randn(1, rows, 256, device=DEV))
+        graph.replay()
+        whole.kv_lens += 1
+        want = layer(x[0][:, None], whole)
+        assert (y[0].double() - want[:, 0].double()).norm() <= 1e-2 * want.double().norm()
+        assert torch.equal(slots // page, pool.block_table[:rows, (prefix + i) // page].long()) and bool((slots % page == (prefix + i) % page).all())
+    assert pool.kv_lens.tolist() == [prefix + 20] * rows + [prefix]
+
+
+def test_calls_on_two_streams_at_once():
+    """Two calls on two streams at once, each with a workspace of its own."""
+    import experiment_swa_kda_b200 as m
+    batches = [Batch(16, 4, 128, 64, BF16, [1] * 40, [(17 * i) % 300 + 1 for i in range(40)], [1500], [0, 40], seed=s, room=60000) for s in (1, 2)]
+    args = [b.device() for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(8):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(m.shared_prefix_attention(*args[i], max_q_len=1))
+    torch.cuda.synchronize()
+    for b, of in zip(batches, outs):
+        b.check(of[0])
+        assert all(torch.equal(of[0], o) for o in of)

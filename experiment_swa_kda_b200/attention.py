@@ -239,7 +239,7 @@ def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens
     request has ended has length 0, one that takes back rejected tokens a smaller length.  IN PLACE the rows of `block_table` [N,P]
     then hold exactly the columns from starts[n] / page_size (None: 0) up to their length: what they held besides goes back to the
     pool `page_free` [pages] bool, and what they lack takes the lowest free pages, rows in order.  `starts` is where a row's own pages
-    begin: behind a prefix it shares, or where a sliding window has left off.
+    begin: behind a prefix it shares, or where a sliding window has left off; a new token before it has no page and a negative slot.
 
     A row is served if the pages lacking up to and with it are there and the new tokens up to and with it are at most `max_tokens`.  One
     that is not waits: IN PLACE its length is less by its new tokens, none of which cu_seqlens counts.

@@ -20,6 +20,11 @@
 //   go as two bf16 terms, p = hi + lo to 2^-16, which leaves the output with the error of its own rounding.
 // - What runs once a sequence (its queries, the join of the warps' sums) is kept short in code: unrolled it was fetched anew every time
 //   and took 5 us.
+//
+// Behind a shared prefix (KEYS): kOwnKeys, the keys of each sequence from its prefix's end on, up to 24 rows; sums stay in the workspace with a note of the stretches
+// that have them.  This pass runs beside the one over prefixes, on the SMs that one leaves.  There a tile's 500 instructions a warp count, not its bytes, so three or
+// four blocks share an SM (256 sequences of up to 1,024 own tokens 102 -> 93 us in all), and more than 16 rows go with one rounded term a weight.  kBothKeys, for few
+// keys in all: a sequence's list is its prefix's tiles and then its own, so that the tile in which the prefix ends is gone through twice.
 
 #include "attn.cuh"
 #include "tc_common.cuh"

@@ -26,6 +26,15 @@
 // in registers, to weights of exactly 0; in its V tile the keys that no row sees are blanked, since 0 times what lies in an unused slot may be NaN, and
 // so are values that are not finite at keys only some rows see: these are added by the rows that see them at the end.
 
+// Behind a shared prefix (KEYS) the kernel does four more things.  kPrefixKeys: the new tokens of all sequences of a group are the rows, the group's prefix the
+// keys, every row sees all of them, and the sums are left for a join; kTurnKeys: the same for groups of at most 128 rows, whose row tile goes through the key tiles
+// in two streams that take turns (1.25 us a key tile; one stream alone takes 1.7).  kOwnKeys: each sequence's rows over its own keys, sums left for the join.
+// kBothKeys: a sequence's rows go through the prefix's pages and then through its own, a finished result.  Prefix passes are cut into one list of equal
+// parts, a block an SM, of which there are as many as the pass over own keys beside them leaves: 32 sequences behind 16,384 tokens, 16 heads on 4, take 23 us in both
+// (64 blocks of 8 key tiles: 7 until the first scores are there, 2.5 for the first weights, whose code is fetched then, 2.5 to leave the sums) and 6 in the join.
+// Measured and left out: a part as long as 8 key tiles at least (49 us for the above), two sums a row tile for the join (47), tiles brought into L2 ahead
+// of the ring (30 for the prefix pass, not 24), the streams of kTurnKeys chosen by a block at run time (all prefix passes 15 to 30 percent slower, by registers).
+
 #include "attn.cuh"
 #include "tc_common.cuh"
 

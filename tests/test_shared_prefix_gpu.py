@@ -110,6 +110,8 @@ CASES = [  # heads, kv_heads, dim, page, dtype, q_lens, own, prefix, cu_groups
     (4, 2, 128, 128, BF16, [200, 130], [260, 131], [1000, 127], [0, 1, 2]),
     (6, 1, 128, 16, BF16, [4] * 30, [4 + i for i in range(30)], [400], [0, 30]),
     (16, 4, 128, 16, BF16, [1] * 70, [1 + (i * 5) % 70 for i in range(70)], [900, 33], [0, 60, 70]),
+    (8, 4, 64, 16, BF16, [1] * 50, [1 + i % 37 for i in range(50)], [20 + 3 * i for i in range(40)], list(range(40)) + [50]),
+    (160, 1, 64, 16, BF16, [1, 2, 1], [40, 3, 1], [200], [0, 3]),
     (16, 8, 64, 64, BF16, [1] * 150, [1 + (i * 3) % 50 for i in range(150)], [200], [0, 150]),
     (4, 2, 8, 16, BF16, [1, 3], [4, 3], [31], [0, 2]),
     (4, 4, 128, 48, BF16, [1, 9, 2], [50, 9, 3], [97], [0, 3]),

@@ -136,7 +136,8 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
         else cluster_sync();
     };
     // this block's rows, in items of 128 columns; a warp takes a run of at most 32 of them, lane l the l-th one's row
-    const int r0 = (int)((long long)a.rows * rank / blocks), r1 = (int)((long long)a.rows * (rank + 1) / blocks);
+    auto first_row = [&](int b) { return alone ? b * a.rows : a.rows * b / kBlocks; };
+    const int r0 = first_row(rank), r1 = first_row(rank + 1);
     const int item0 = r0 * a.items, item1 = r1 * a.items, run = min((item1 - item0 + kWarps - 1) / kWarps, 32);
     struct Run {
         int many, row, col0, col1, col1_without;      // the columns that the row shall hold, and their end without its new tokens
@@ -344,9 +345,11 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
             }
         }
     }
-    // A block's rows are its own, and so are their tokens, unless there are so many that all blocks share them.
+    // A block's rows are its own, and so are their tokens, unless one block has so many that all of them share.
     const int tokens = cu[a.rows];
-    const bool share = !alone && tokens > 8 * kThreads;
+    bool share = false;
+    if (!alone && tokens > 8 * kThreads)
+        for (int b = 0; b < blocks; ++b) share |= cu[first_row(b + 1)] - cu[first_row(b)] > 8 * kThreads;
     if (share) cluster_sync();
     else __syncthreads();
 

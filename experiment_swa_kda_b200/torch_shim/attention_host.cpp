@@ -309,7 +309,16 @@ PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const 
     KdaPlanShape s = {};
     s.rows = (int32_t)N, s.width = (int32_t)width, s.page_size = (int32_t)page, s.n_pages = (int32_t)pages, s.max_tokens = (int32_t)max_tokens;
     s.table_stride = table.stride(0);
-    Tensor cu = empty({N + 1}, at::kInt, table), positions = empty({max_tokens}, at::kInt, table), slots = empty({max_tokens}, at::kLong, table);
+    // the three results out of one allocation: a trip to the allocator is a tenth of a small call
+    const size_t at_positions = up256(max_tokens * sizeof(int64_t)), at_cu = at_positions + up256(max_tokens * sizeof(int32_t));
+    const Tensor all = bytes(at_cu + (N + 1) * sizeof(int32_t), table);
+    auto part = [&](size_t offset, int64_t n, at::ScalarType type) {
+        Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_storage_offset((int64_t)(offset / c10::elementSize(type)));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(at::IntArrayRef(&n, 1));
+        return t;
+    };
+    Tensor slots = part(0, max_tokens, at::kLong), positions = part(at_positions, max_tokens, at::kInt), cu = part(at_cu, N + 1, at::kInt);
     const size_t need = kda_plan_pages_workspace_bytes(&s);
     Tensor ws;
     if (need > 0) ws = bytes(need, table);

@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = gridDim.x, rank = blockIdx.x;     // the grid is one cluster
     const bool alone = blocks == 1;
+    dependency_wait();
     int *missing = alone ? len_of + a.rows : a.missing, *dealt = alone ? missing + a.rows * a.items : a.dealt;
     auto meet = [&]() {
         if (alone) __syncthreads();
@@ -437,6 +438,6 @@ extern "C" int kda_plan_pages(const KdaPlanShape* s, int32_t* block_table, int32
     if (int rc = set_smem_limit(plan_pages_kernel, smem)) return rc;
     cudaError_t e = cudaSuccess;
     KDA_LAUNCH("plan_pages_kernel", (cudaStream_t)stream,
-               e = launch_early(plan_pages_kernel, dim3(blocks), kThreads, smem, (cudaStream_t)stream, false, blocks, a));
+               e = launch_early(plan_pages_kernel, dim3(blocks), kThreads, smem, (cudaStream_t)stream, true, blocks, a));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }

@@ -6,6 +6,13 @@
 namespace kda {
 namespace attn {
 
+// A load of what the caller's arrays hold: not one of constant memory, which the compiler may move ahead of a wait for the launch before.  The kernels behind a
+// shared prefix start early: the first of a call waits for everything before it and lets the second start only then, which reads the batch without a wait.
+template <class T>
+__device__ __forceinline__ T ld_input(const T* p) {
+    return *p;
+}
+
 // A batch of new tokens over a paged cache.  Every array is the caller's and read on the device, so nothing that is read
 // there is trusted as an index before it has been clamped.
 struct Batch {
@@ -23,7 +30,7 @@ struct Batch {
     }
     __device__ __forceinline__ int many() const { return n_seq; }
     // first new token of sequence n of a packed batch
-    __device__ __forceinline__ int edge(int n) const { return min(max(__ldg(cu + n), 0), tokens); }
+    __device__ __forceinline__ int edge(int n) const { return min(max(ld_input(cu + n), 0), tokens); }
     // new tokens [first, first + count) of sequence n
     __device__ __forceinline__ void span(int n, int& first, int& count) const {
         if (cu == nullptr) {
@@ -31,29 +38,29 @@ struct Batch {
             count = q_len;
             return;
         }
-        const int a = __ldg(cu + n), b = __ldg(cu + n + 1);
+        const int a = ld_input(cu + n), b = ld_input(cu + n + 1);
         first = min(max(a, 0), tokens);
         count = min(max(b, first), tokens) - first;
     }
     // whether the table of new tokens is consistent at sequence n
     __device__ __forceinline__ bool span_ok(int n) const {
         if (cu == nullptr) return true;
-        const int a = __ldg(cu + n), b = __ldg(cu + n + 1);
+        const int a = ld_input(cu + n), b = ld_input(cu + n + 1);
         return a >= 0 && a <= b && b <= tokens && (n > 0 || a == 0) && (n + 1 < n_seq || b == tokens);
     }
     // tokens of sequence n that the table has room for
     __device__ __forceinline__ int kv_len(int n) const {
         const long long room = (long long)table_width * page_size;
-        const int len = max(__ldg(kv_lens + n), 0);
+        const int len = max(ld_input(kv_lens + n), 0);
         return (long long)len > room ? (int)room : len;
     }
     __device__ __forceinline__ bool kv_len_ok(int n) const {
-        const int len = __ldg(kv_lens + n);
+        const int len = ld_input(kv_lens + n);
         return len >= 0 && (long long)len <= (long long)table_width * page_size;
     }
     // the page of column `col`, or -1 where the table names none
     __device__ __forceinline__ int page(int n, int col) const {
-        const int p = __ldg(table + n * table_stride + col);
+        const int p = ld_input(table + n * table_stride + col);
         return (unsigned)p < (unsigned)n_pages ? p : -1;
     }
     // sequence of token t: the last one that starts at or before it
@@ -62,7 +69,7 @@ struct Batch {
         int lo = 0, hi = n_seq;      // cu[lo] <= t < cu[hi]
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (__ldg(cu + mid) <= t) lo = mid;
+            if (ld_input(cu + mid) <= t) lo = mid;
             else hi = mid;
         }
         return lo;
@@ -73,11 +80,11 @@ struct Batch {
     __device__ __forceinline__ int seq_of(int t, int l, unsigned mask) const {
         if (cu == nullptr) return t / q_len;
         const int guess = (int)((long long)t * n_seq / tokens);
-        if (__ldg(cu + guess) <= t && t < __ldg(cu + guess + 1)) return guess;
+        if (ld_input(cu + guess) <= t && t < ld_input(cu + guess + 1)) return guess;
         int lo = 0, hi = n_seq;
         while (hi - lo > 1) {
             const int step = (hi - lo + LANES - 1) / LANES, at = lo + step * l;
-            const unsigned below = __ballot_sync(mask, at < hi && __ldg(cu + at) <= t) & mask;
+            const unsigned below = __ballot_sync(mask, at < hi && ld_input(cu + at) <= t) & mask;
             lo += step * max(__popc(below) - 1, 0);
             hi = min(hi, lo + step);
         }
@@ -99,7 +106,7 @@ struct Prefix {
 // A batch of which every sequence sees its own keys only: those behind its prefix.
 struct OwnView : Batch {
     Prefix p;
-    __device__ __forceinline__ int group_edge(int g) const { return p.groups == nullptr ? g * p.each : min(max(__ldg(p.groups + g), 0), n_seq); }
+    __device__ __forceinline__ int group_edge(int g) const { return p.groups == nullptr ? g * p.each : min(max(ld_input(p.groups + g), 0), n_seq); }
     // the group of sequence n, or -1
     __device__ __forceinline__ int group_of(int n) const {
         if (p.groups == nullptr) return n / p.each;
@@ -113,7 +120,7 @@ struct OwnView : Batch {
     }
     __device__ __forceinline__ int prefix_len(int g) const {
         const long long room = (long long)p.width * page_size;
-        const int len = max(__ldg(p.lens + g), 0);
+        const int len = max(ld_input(p.lens + g), 0);
         return (long long)len > room ? (int)room : len;
     }
     // the prefix of sequence n's group, whether or not the sequence shares it
@@ -127,18 +134,18 @@ struct OwnView : Batch {
     }
     __device__ __forceinline__ bool groups_ok(int g) const {
         if (p.groups != nullptr) {
-            const int a = __ldg(p.groups + g), b = __ldg(p.groups + g + 1);
+            const int a = ld_input(p.groups + g), b = ld_input(p.groups + g + 1);
             if (a < 0 || a > b || b > n_seq) return false;
         }
         return true;
     }
     // the page of column `col` of group g's prefix, or -1
     __device__ __forceinline__ int prefix_page(int g, int col) const {
-        const int at = __ldg(p.table + g * p.table_stride + col);
+        const int at = ld_input(p.table + g * p.table_stride + col);
         return (unsigned)at < (unsigned)n_pages ? at : -1;
     }
     __device__ __forceinline__ bool prefix_ok(int g) const {
-        const int len = __ldg(p.lens + g);
+        const int len = ld_input(p.lens + g);
         return len >= 0 && (long long)len <= (long long)p.width * page_size;
     }
 };
@@ -151,7 +158,7 @@ struct GroupView : BothView {
     __device__ __forceinline__ int many() const { return p.n; }
     __device__ __forceinline__ int edge(int g) const {
         const int s = group_edge(g);
-        return cu == nullptr ? s * q_len : min(max(__ldg(cu + s), 0), tokens);
+        return cu == nullptr ? s * q_len : min(max(ld_input(cu + s), 0), tokens);
     }
     __device__ __forceinline__ void span(int g, int& first, int& count) const {
         first = edge(g);

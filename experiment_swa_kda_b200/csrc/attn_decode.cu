@@ -23,7 +23,7 @@
 //
 // Behind a shared prefix (KEYS): kOwnKeys, the keys of each sequence from its prefix's end on, up to 24 rows; sums stay in the workspace with a note of the stretches
 // that have them.  This pass runs beside the one over prefixes, on the SMs that one leaves.  There a tile's 500 instructions a warp count, not its bytes, so three or
-// four blocks share an SM (256 sequences of up to 1,024 own tokens 102 -> 93 us in all), and more than 16 rows go with one rounded term a weight.  kBothKeys, for few
+// four blocks share an SM (256 sequences of up to 1,024 own tokens 102 -> 93 us in all, now 89), and more than 16 rows go with one rounded term a weight.  kBothKeys, for few
 // keys in all: a sequence's list is its prefix's tiles and then its own, so that the tile in which the prefix ends is gone through twice.
 
 #include "attn.cuh"
@@ -98,7 +98,7 @@ template <class B>
 __device__ __forceinline__ Raw raw_at(const B& b, int n) {
     if (n >= b.n_seq) return Raw{0, 0, 0, 0};
     const int p = prefix_at(b, n);
-    return b.cu != nullptr ? Raw{__ldg(b.cu + n), __ldg(b.cu + n + 1), __ldg(b.kv_lens + n), p} : Raw{n * b.q_len, (n + 1) * b.q_len, __ldg(b.kv_lens + n), p};
+    return b.cu != nullptr ? Raw{ld_input(b.cu + n), ld_input(b.cu + n + 1), ld_input(b.kv_lens + n), p} : Raw{n * b.q_len, (n + 1) * b.q_len, ld_input(b.kv_lens + n), p};
 }
 __device__ __forceinline__ void number_tiles(const Batch&, Seq&) {}
 __device__ __forceinline__ void number_tiles(const BothView&, Seq& s) {
@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
     const int g = a.c.heads.group, D = a.c.heads.dim, Hk = a.c.heads.kv_heads, Hq = a.c.heads.q_heads, window = a.c.window;
 
     uint64_t* bar = bars + warp * kStages;
+    if (KEYS == kBothKeys) dependency_wait();      // launched early; so is its join, which takes all before this kernel for done
     dependents_go();
     if (lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(bar + s, 1);
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             piece[y] = make_uint4(0, 0, 0, 0);
             if (r < rows && d < D) {
                 const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(a.c.q) + (x.s.first + r / g) * a.c.strides.q_token + (x.hk * g + r % g) * a.c.strides.q_head + d;
-                piece[y] = __ldg(reinterpret_cast<const uint4*>(src));
+                piece[y] = ld_input(reinterpret_cast<const uint4*>(src));
             }
         }
     };
@@ -788,7 +789,7 @@ int launch(const CUtensorMap& mK, const CUtensorMap& mV, const Args& a, cudaStre
     constexpr int kBytes = Layout<DP, NR, KEYS>::kBytes;
     if (int rc = set_smem_limit(attn_decode_kernel<DP, NR, KEYS>, kBytes)) return rc;
     cudaError_t e = cudaSuccess;
-    if constexpr (KEYS == kOwnKeys) {      // beside the pass over the prefix
+    if constexpr (KEYS != kAllKeys) {      // own keys: beside the pass over the prefix
         KDA_LAUNCH("attn_decode_kernel", st, e = launch_early(attn_decode_kernel<DP, NR, KEYS>, dim3(a.blocks), kThreads, kBytes, st, true, 1, mK, mV, a));
         if (e != cudaSuccess) return KDA_ERR_CUDA;
     } else {

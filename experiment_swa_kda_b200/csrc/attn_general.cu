@@ -44,7 +44,7 @@ __device__ __forceinline__ bool fetch(float* dst, const void* src, long long at,
         for (int i = 0; i < DP / 32; ++i) {
             const int d = 8 * part + 32 * i;
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (d < width) x = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(src) + at + d));
+            if (d < width) x = ld_input(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(src) + at + d));
             const float2 f0 = f2_get(f2_from_bf16(x.x)), f1 = f2_get(f2_from_bf16(x.y)), f2_ = f2_get(f2_from_bf16(x.z)), f3 = f2_get(f2_from_bf16(x.w));
             fine &= isfinite(f0.x) && isfinite(f0.y) && isfinite(f1.x) && isfinite(f1.y) && isfinite(f2_.x) && isfinite(f2_.y) && isfinite(f3.x) && isfinite(f3.y);
             *reinterpret_cast<float4*>(dst + d) = make_float4(f0.x, f0.y, f1.x, f1.y);
@@ -55,7 +55,7 @@ __device__ __forceinline__ bool fetch(float* dst, const void* src, long long at,
         for (int i = 0; i < DP / 16; ++i) {
             const int d = 4 * part + 16 * i;
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (d < width) x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(src) + at + d));
+            if (d < width) x = ld_input(reinterpret_cast<const float4*>(static_cast<const float*>(src) + at + d));
             fine &= isfinite(x.x) && isfinite(x.y) && isfinite(x.z) && isfinite(x.w);
             *reinterpret_cast<float4*>(dst + d) = x;
         }
@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int hk = blockIdx.y, z = blockIdx.z, g = c.heads.group, D = c.heads.dim;
     const auto& b = view<KEYS>(c);
+    if (KEYS == kPrefixKeys) dependency_wait();      // launched early; what is launched early behind it may take all before it for done
     dependents_go();
     Unit u;
     if (!make_unit(b, tiles, blockIdx.x, c.window, u)) {
@@ -306,8 +307,8 @@ int launch(const Call& c, const Tiles& t, dim3 grid, int splits, float* part_o, 
     const bool vec = all % unit == 0 && (reinterpret_cast<uintptr_t>(c.q) | reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % 16 == 0;
     auto kern = vec ? attn_general_kernel<DP, true, KEYS> : attn_general_kernel<DP, false, KEYS>;
     if (int rc = set_smem_limit(kern, smem)) return rc;
-    cudaError_t e = cudaSuccess;      // own keys: beside the pass over the prefix
-    KDA_LAUNCH("attn_general_kernel", st, e = launch_early(kern, grid, kThreads, smem, st, KEYS == kOwnKeys, 1, c, t, splits, part_o, part_ml));
+    cudaError_t e = cudaSuccess;      // of own keys: beside the pass over the prefix
+    KDA_LAUNCH("attn_general_kernel", st, e = launch_early(kern, grid, kThreads, smem, st, KEYS != kAllKeys, 1, c, t, splits, part_o, part_ml));
     return e == cudaSuccess ? launch_status() : KDA_ERR_CUDA;
 }
 

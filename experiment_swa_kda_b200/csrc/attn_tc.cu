@@ -32,7 +32,7 @@
 // kBothKeys: a sequence's rows go through the prefix's pages and then through its own, a finished result.  Prefix passes are cut into one list of equal
 // parts, a block an SM, of which there are as many as the pass over own keys beside them leaves: 32 sequences behind 16,384 tokens, 16 heads on 4, take 23 us in both
 // (64 blocks of 8 key tiles: 7 until the first scores are there, 2.5 for the first weights, whose code is fetched then, 2.5 to leave the sums) and 6 in the join.
-// Measured and left out: a part as long as 8 key tiles at least (49 us for the above), two sums a row tile for the join (47), tiles brought into L2 ahead
+// Measured and left out: a part as long as 8 key tiles at least (49 us for the above, in all, now 31), two sums a row tile for the join (47), tiles brought into L2 ahead
 // of the ring (30 for the prefix pass, not 24), the streams of kTurnKeys chosen by a block at run time (all prefix passes 15 to 30 percent slower, by registers).
 
 #include "attn.cuh"
@@ -230,6 +230,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (a.q_boxes) tma_prefetch_desc(&mQ);
     }
     int hk = blockIdx.y, z = blockIdx.z, slot = a.slots - 1 - (int)blockIdx.x, parts = 1;
+    if (in_prefix || both) dependency_wait();      // launched early; what is launched early behind it may take all before it for done
     if (sums_only) dependents_go();
     Unit u;
     bool some;
@@ -1060,7 +1061,7 @@ int launch(const Call& c, const CUtensorMap& mK, const CUtensorMap& mV, const CU
     const bool list = (KEYS == kPrefixKeys || KEYS == kTurnKeys) && a.splits > 1;      // prefix_unit: a block an SM
     const long long most = (long long)a.slots * c.heads.kv_heads * a.splits;
     const dim3 grid(list ? (unsigned)(most < kSms ? most : kSms) : (unsigned)a.slots, list ? 1u : (unsigned)c.heads.kv_heads, list ? 1u : (unsigned)a.splits);
-    if constexpr (KEYS == kOwnKeys) {      // beside the pass over the prefix
+    if constexpr (KEYS != kAllKeys) {      // own keys: beside the pass over the prefix
         cudaError_t e = cudaSuccess;
         KDA_LAUNCH("attn_tc_kernel", st, e = launch_early(attn_tc_kernel<DP, KEYS>, grid, kThreads, Layout<DP>::kBytes, st, true, 1, mK, mV, mQ, mO, a));
         if (e != cudaSuccess) return KDA_ERR_CUDA;

@@ -14,7 +14,7 @@
 //   5  position and slot of each new token
 // A block has a range of the rows from 1 to 5.  A batch that one block can read at once takes a single block, which keeps its lists to itself.
 //
-// One conversation 5.6 us from first to last instruction (8 a call, which is the host's), 256 rows 9 to 15, 4,096 rows of 128 columns with 262,144 pages 34, of
+// One conversation 5.6 us from first to last instruction (6 a call), 256 rows 9 to 14, 4,096 rows of 128 columns with 262,144 pages 33, of
 // which 10 are phase 1 (16 rows a warp, four on their way) and 13 are 4 and 5.  Measured and left out: one barrier more to count free pages by shares also in small
 // pools (0.6 us), pages listed by the threads that counted them (4,096 rows 37 -> 50), scans of 64-bit sums (0.5 each).
 
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int blocks = gridDim.x, rank = blockIdx.x;     // the grid is one cluster
     const bool alone = blocks == 1;
-    dependency_wait();
+    dependency_wait();      // launched early: two calls one behind the other 17 us, not 13, without
     int *missing = alone ? len_of + a.rows : a.missing, *dealt = alone ? missing + a.rows * a.items : a.dealt;
     auto meet = [&]() {
         if (alone) __syncthreads();

@@ -371,3 +371,30 @@ def test_calls_on_two_streams_at_once():
     for b, of in zip(batches, outs):
         b.check(of[0])
         assert all(torch.equal(of[0], o) for o in of)
+
+
+@pytest.mark.parametrize("q,room,dtype", [(1, 0, BF16), (1, 60000, BF16), (6, 60000, BF16), (100, 0, BF16), (100, 60000, BF16), (3, 0, F32)])
+def test_inputs_written_just_before_the_call(q, room, dtype):
+    """Kernels that start while the launch before them ends read what that one wrote."""
+    import experiment_swa_kda_b200 as m
+    two = [Batch(8, 2, 64, 16, dtype, [q] * 24, [(s + 11 * i) % 60 + q for i in range(24)], [300 + 16 * s], [0, 24], seed=s, room=room) for s in (1, 4)]
+    width = max(b.table.shape[1] for b in two), max(b.prefix_table.shape[1] for b in two)
+    pages = max(b.k.shape[0] for b in two)
+    fit = lambda t, n, d: torch.cat((t, t.new_zeros((n - t.shape[d],) + t.shape[1:]) if d == 0 else t.new_full((t.shape[0], n - t.shape[1]), -1)), d)
+    sets = []
+    for b in two:
+        a = b.device()
+        a[1], a[2], a[3], a[5] = fit(a[1], pages, 0), fit(a[2], pages, 0), fit(a[3], width[0], 1), fit(a[5], width[1], 1)
+        sets.append([t.contiguous() for t in a])
+    live = [t.clone() for t in sets[0]]
+    wants = [m.shared_prefix_attention(*a, max_q_len=q) for a in sets]
+    for b, w in zip(two, wants):
+        b.check(w)
+    torch.cuda.synchronize()
+    order = [0, 1, 1, 0] * 8
+    outs = []
+    for i in order:
+        for t, src in zip(live, sets[i]):
+            t.copy_(src)
+        outs.append(m.shared_prefix_attention(*live, max_q_len=q))
+    assert all(torch.equal(o, wants[i]) for o, i in zip(outs, order))

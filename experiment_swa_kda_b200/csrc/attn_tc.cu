@@ -996,11 +996,13 @@ __global__ void __launch_bounds__(32 * kSharedWarps, 4) attn_shared_join_kernel(
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     int from = 0;      // ml is that of part from + lane
-    float weight = 0.f;
+    // A part without a key is left out: its sums are 0, or were not written.  One whose weight vanishes is not: a NaN or an infinite value that the row sees stays.
+    constexpr float kNoKey = -1.f;
+    float weight = kNoKey;
     auto weigh = [&]() {
         const float top = __uint_as_float(ml.x);
-        weight = top == -INFINITY ? 0.f : ex2(top - m);      // without a key its sums are 0, or were not written
-        if (mine == 0) l = fmaf(top == -INFINITY ? 0.f : __uint_as_float(ml.y), weight, l);
+        weight = top == -INFINITY ? kNoKey : ex2(top - m);
+        if (mine == 0 && top != -INFINITY) l = fmaf(__uint_as_float(ml.y), weight, l);
     };
     weigh();
     for (int k0 = mine * kAtOnce; k0 < parts;) {
@@ -1016,8 +1018,7 @@ __global__ void __launch_bounds__(32 * kSharedWarps, 4) attn_shared_join_kernel(
                 weigh();
             }
             const float f = __shfl_sync(0xffffffffu, weight, k - from + sub);
-            const bool is = k + sub < parts && f != 0.f;      // NaN is
-            if (is) {
+            if (k + sub < parts && f != kNoKey) {
                 acc[0] = f2_fma(f2_make(__uint_as_float(v[x].x), __uint_as_float(v[x].y)), f2_all(f), acc[0]);
                 acc[1] = f2_fma(f2_make(__uint_as_float(v[x].z), __uint_as_float(v[x].w)), f2_all(f), acc[1]);
             }

@@ -31,7 +31,7 @@ class RotaryShape(C.Structure):
 
 class PagedShape(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("tokens", "n_seq", "max_q_len", "q_heads", "kv_heads", "head_dim", "io_dtype", "n_pages", "page_size",
-                                         "table_width", "window")] + [("scale", C.c_float)] + [
+                                         "table_width", "window")] + [("scale", C.c_float), ("padded", C.c_int32)] + [
         (n, C.c_int64) for n in ("table_stride", "q_token_stride", "q_head_stride", "k_page_stride", "k_row_stride", "k_head_stride", "v_page_stride",
                                  "v_row_stride", "v_head_stride")]
 

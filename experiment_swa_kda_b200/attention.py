@@ -14,6 +14,8 @@ kernels of this package:
 A batch of new tokens is packed, [tokens, heads, D], with `cu_seqlens` [N+1] as in `chunk_kda`, or without it when every
 sequence has as many.  `kv_lens` [N] counts a sequence's tokens, the new ones among them; `block_table` [N, P] names their
 pages.  These three are read on the device: a decode loop captures the calls in a CUDA graph and updates the arrays in place.
+Tokens behind cu_seqlens[N] belong to no sequence.  A step of fixed size, as a captured one is, has such tokens wherever a request waits or
+ends (`plan_pages`) and says so with `padded`: they are padding then.  Without it they are reported as an inconsistent `cu_seqlens`.
 """
 
 from __future__ import annotations
@@ -130,15 +132,16 @@ def _no_grad(what: str, *tensors: Optional[Tensor]) -> None:
 
 def qk_norm_rope_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
                         kv_lens: Tensor, cu_seqlens: Optional[Tensor] = None, *, q_weight: Optional[Tensor] = None,
-                        k_weight: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> Tensor:
+                        k_weight: Optional[Tensor] = None, eps: float = 1e-6, interleaved: bool = False, padded: bool = False) -> Tensor:
     """`qk_norm_rope` of a serving batch with its keys and values going to their pages: returns q' [tokens,Hq,D], dense, and
     writes k' and v IN PLACE into k_cache, v_cache [pages, page_size, Hk, D].
 
     The i-th of a sequence's n new tokens has position kv_len - n + i; a token whose position is negative is padding (q' = 0,
-    nothing is written).  Inference only."""
+    nothing is written), and so is one behind the last sequence (`padded`: there may be some).  Inference only."""
     out = None
     if q.is_cuda:
-        out = _native.load().append(q, k, v, cos, sin, k_cache, v_cache, block_table, kv_lens, cu_seqlens, q_weight, k_weight, eps, bool(interleaved))
+        out = _native.load().append(q, k, v, cos, sin, k_cache, v_cache, block_table, kv_lens, cu_seqlens, q_weight, k_weight, eps, bool(interleaved),
+                                     bool(padded))
     if out is not None:
         return out
     _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
@@ -156,7 +159,7 @@ def qk_norm_rope_append(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tenso
 
 
 def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kv_lens: Tensor, cu_seqlens: Optional[Tensor] = None, *,
-                    max_q_len: int = 0, window: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+                    max_q_len: int = 0, window: int = 0, scale: Optional[float] = None, return_lse: bool = False, padded: bool = False):
     """Causal attention of new tokens q [tokens,Hq,D] over a paged cache that holds their own keys and values already.
 
     The token at position p sees positions p - window + 1 .. p (window 0: all up to p); Hq / Hk query heads share a kv head.
@@ -169,11 +172,11 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
     cores, 14 times slower and more: take such page sizes where there is a choice.
 
     Returns o [tokens,Hq,D], or (o, lse [tokens,Hq]) with the natural log of each row's sum of exponentials.  A padding token
-    (negative position) gets o = 0 and lse = -inf.  Pages that no new token reaches are not touched, and their entries in
+    (negative position, or behind the last sequence; `padded`: there may be some of these) gets o = 0 and lse = -inf.  Pages that no new token reaches are not touched, and their entries in
     the table may be anything.  Inference only."""
     out = None
     if q.is_cuda:
-        out = _native.load().attention(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, max_q_len, window, scale, bool(return_lse))
+        out = _native.load().attention(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, max_q_len, window, scale, bool(return_lse), bool(padded))
     if out is not None:
         return out if return_lse else out[0]
     _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
@@ -187,7 +190,7 @@ def paged_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Te
 
 def shared_prefix_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor, kv_lens: Tensor, prefix_table: Tensor, prefix_lens: Tensor,
                             cu_groups: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None, *, max_q_len: int = 0,
-                            scale: Optional[float] = None, return_lse: bool = False):
+                            scale: Optional[float] = None, return_lse: bool = False, padded: bool = False):
     """`paged_attention` of sequences that start with a common text: its keys and values are in the cache once, and read once for all of
     the sequences.
 
@@ -204,7 +207,7 @@ def shared_prefix_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_t
     out = None
     if q.is_cuda:
         out = _native.load().shared_attention(q, k_cache, v_cache, block_table, kv_lens, prefix_table, prefix_lens, cu_groups, cu_seqlens, max_q_len, scale,
-                                              bool(return_lse))
+                                              bool(return_lse), bool(padded))
     if out is not None:
         return out if return_lse else out[0]
     _check_paged(q, k_cache, v_cache, block_table, kv_lens, cu_seqlens)
@@ -245,7 +248,8 @@ def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens
     that is not waits: IN PLACE its length is less by its new tokens, none of which cu_seqlens counts.
 
     positions [max_tokens] int32 are the new tokens' places in their sequences, slots [max_tokens] int64 those in a cache of
-    [pages * page_size] rows; -1 behind the last.  Nothing synchronises; a captured graph follows the arrays.  A pool starts out with all
+    [pages * page_size] rows; -1 behind the last.  Nothing synchronises; a captured graph follows the arrays.  What goes on from here with
+    max_tokens tokens - `qk_norm_rope_append`, the attention, `PagedAttention` - takes this cu_seqlens with `padded`, since a step need not be full.  A pool starts out with all
     pages free and a table of -1."""
     out = None
     if block_table.is_cuda:
@@ -345,8 +349,9 @@ class PagedAttention(nn.Module):
         return self
 
     @torch.no_grad()
-    def forward(self, hidden_states: Tensor, cache: PagedCache, cu_seqlens: Optional[Tensor] = None, max_q_len: int = 0) -> Tensor:
-        """hidden_states [B,T,hidden], T new tokens of each of the cache's B sequences, or [1,tokens,hidden], packed, with `cu_seqlens`."""
+    def forward(self, hidden_states: Tensor, cache: PagedCache, cu_seqlens: Optional[Tensor] = None, max_q_len: int = 0, padded: bool = False) -> Tensor:
+        """hidden_states [B,T,hidden], T new tokens of each of the cache's B sequences, or [1,tokens,hidden], packed, with `cu_seqlens`
+        (`padded`: which may end before the last token)."""
         lead = hidden_states.shape[:-1]
         if self.window and cache.prefix_table is not None:
             raise ValueError("a sliding-window layer does not share a prefix: its cache must not have one")
@@ -358,11 +363,12 @@ class PagedAttention(nn.Module):
         qkv = self.qkv_proj(hidden_states).reshape(-1, self.num_heads + 2 * self.num_kv_heads, self.head_dim)
         q, k, v = qkv.split((self.num_heads, self.num_kv_heads, self.num_kv_heads), 1)
         place = (cache.k, cache.v, cache.block_table, cache.kv_lens, cu_seqlens)
-        q = qk_norm_rope_append(q, k, v, self.cos, self.sin, *place, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.norm_eps)
+        q = qk_norm_rope_append(q, k, v, self.cos, self.sin, *place, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.norm_eps, padded=padded)
         if cache.prefix_table is None:
-            o = paged_attention(q, *place, max_q_len=max_q_len, window=self.window)
+            o = paged_attention(q, *place, max_q_len=max_q_len, window=self.window, padded=padded)
         else:
-            o = shared_prefix_attention(q, *place[:4], cache.prefix_table, cache.prefix_lens, cache.cu_groups, cu_seqlens, max_q_len=max_q_len)
+            o = shared_prefix_attention(q, *place[:4], cache.prefix_table, cache.prefix_lens, cache.cu_groups, cu_seqlens, max_q_len=max_q_len,
+                                        padded=padded)
         return self.o_proj(o.reshape(*lead, -1))
 
 

@@ -22,6 +22,7 @@ struct Batch {
     int* mirror;            // page-locked host word for errors found here, or null
     long long table_stride;
     int n_seq, tokens, q_len, n_pages, page_size, table_width;
+    int padded;             // tokens behind the last sequence are expected
 
     // Said by every thread that finds it, as long as the call runs: these calls have no status word of their own in which a first teller could be
     // known (a captured call has nothing that tells one replay from the next).  The host therefore clears the word behind the stream's work.
@@ -46,8 +47,10 @@ struct Batch {
     __device__ __forceinline__ bool span_ok(int n) const {
         if (cu == nullptr) return true;
         const int a = ld_input(cu + n), b = ld_input(cu + n + 1);
-        return a >= 0 && a <= b && b <= tokens && (n > 0 || a == 0) && (n + 1 < n_seq || b == tokens);
+        return a >= 0 && a <= b && b <= tokens && (n > 0 || a == 0) && (n + 1 < n_seq || b == tokens || padded);
     }
+    // tokens that are some sequence's; those from here on are padding
+    __device__ __forceinline__ int end() const { return cu == nullptr ? tokens : edge(n_seq); }
     // tokens of sequence n that the table has room for
     __device__ __forceinline__ int kv_len(int n) const {
         const long long room = (long long)table_width * page_size;

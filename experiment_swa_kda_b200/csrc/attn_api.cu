@@ -83,7 +83,7 @@ extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const 
     Call c;
     c.batch = GroupView{};
     static_cast<Batch&>(c.batch) =
-        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width};
+        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width, s->padded};
     c.heads = Heads{s->q_heads, s->kv_heads, s->q_heads / s->kv_heads, s->head_dim};
     c.strides = Strides{s->q_token_stride, s->q_head_stride, s->k_page_stride, s->k_row_stride, s->k_head_stride, s->v_page_stride, s->v_row_stride, s->v_head_stride};
     c.q = q; c.k = k_cache; c.v = v_cache; c.o = o; c.lse = lse;
@@ -250,7 +250,7 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     Call c;
     c.batch = GroupView{};
     static_cast<Batch&>(c.batch) =
-        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width};
+        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width, s->padded};
     c.batch.p = Prefix{prefix_table, prefix_lens, cu_groups, p->table_stride, p->n_groups, p->table_width, s->n_seq / p->n_groups};
     c.heads = Heads{s->q_heads, s->kv_heads, s->q_heads / s->kv_heads, s->head_dim};
     c.strides = Strides{s->q_token_stride, s->q_head_stride, s->k_page_stride, s->k_row_stride, s->k_head_stride, s->v_page_stride, s->v_row_stride, s->v_head_stride};

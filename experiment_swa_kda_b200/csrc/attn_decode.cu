@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
     PrefixWork* work = reinterpret_cast<PrefixWork*>(sm + L::kQ);
     if constexpr (KEYS == kOwnKeys)
         if (a.prefix_splits > 1 && tid < b.p.n) work[tid] = prefix_work(a.c.batch, tid, g, a.prefix_rows);
+    const int batch_end = KEYS == kOwnKeys ? 0 : b.end();      // read here, where nothing waits for it
     auto blocks_of = [&](int total) {
         if constexpr (KEYS == kOwnKeys)
             if (a.prefix_splits > 1 && total > kMinTiles * kPerSmOf<DP, NR, KEYS>) {
@@ -402,6 +403,13 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             if (a.c.lse != nullptr)
                 for (int e = tid; e < s.count * Hq; e += kThreads) a.c.lse[r0 + e] = -INFINITY;
         }
+    }
+    if constexpr (KEYS != kOwnKeys) {      // padding behind the last sequence; of own keys the join does this
+        const long long rest = (long long)(b.tokens - batch_end) * Hq, at = (long long)batch_end * Hq;
+        for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest * D / 8; e += gridDim.x * kThreads)
+            reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.o) + at * D)[e] = make_uint4(0, 0, 0, 0);
+        if (a.c.lse != nullptr)
+            for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest; e += gridDim.x * kThreads) a.c.lse[at + e] = -INFINITY;
     }
     if (tiles <= 0) {
         if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too

@@ -72,6 +72,12 @@ __global__ void __launch_bounds__(kThreads) attn_general_kernel(Call c, Tiles ti
     const auto& b = view<KEYS>(c);
     if (KEYS == kPrefixKeys) dependency_wait();      // launched early; what is launched early behind it may take all before it for done
     dependents_go();
+    if (KEYS == kAllKeys && splits == 1 && hk == 0) {      // padding behind the last sequence; elsewhere the join does this
+        const long long from = (long long)b.end() * c.heads.q_heads, to = (long long)b.tokens * c.heads.q_heads, step = (long long)gridDim.x * kThreads;
+        for (long long e = from * D + (long long)blockIdx.x * kThreads + tid; e < to * D; e += step) st_io(c.o, e, c.bf16, 0.f);
+        if (c.lse != nullptr)
+            for (long long e = from + (long long)blockIdx.x * kThreads + tid; e < to; e += step) c.lse[e] = -INFINITY;
+    }
     Unit u;
     if (!make_unit(b, tiles, blockIdx.x, c.window, u)) {
         int n, tile;
@@ -255,8 +261,10 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
     const int lane = threadIdx.x & 31;
     dependency_wait();      // in every block: the end of this kernel stands for that of the one before too
     if (row >= rows) return;
-    int z_first = 0;
-    if (SHARED) {
+    int z_first = 0, z_end = c.splits;
+    if (row / c.q_heads >= c.batch.Batch::end()) {      // padding behind the last sequence has no parts
+        z_end = 0;
+    } else if (SHARED) {
         const int n = c.batch.seq_of<32>((int)(row / c.q_heads), lane, 0xffffffffu);
         int first, count;
         c.batch.OwnView::span(n, first, count);
@@ -264,12 +272,12 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(Combine c) {
         if (prefix == 0 || c.batch.kv_len(n) - count < prefix) z_first = c.prefix_splits;
     }
     float m = -INFINITY;
-    for (int z = z_first + lane; z < c.splits; z += 32) m = fmaxf(m, ld_after_f32(&c.part_ml[z * rows + row].x));
+    for (int z = z_first + lane; z < z_end; z += 32) m = fmaxf(m, ld_after_f32(&c.part_ml[z * rows + row].x));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float acc[8] = {}, l = 0.f;
     constexpr int kAhead = 4;
-    for (int z0 = z_first; z0 < c.splits; z0 += kAhead) {
+    for (int z0 = z_first; z0 < z_end; z0 += kAhead) {
         uint2 ml[kAhead];
         float v[kAhead][8];
 #pragma unroll

@@ -792,7 +792,7 @@ extern "C" int kda_norm_rope_append(const KdaRotaryShape* s, const KdaPagedShape
     Rope p = fill(*s, q, k, cos, sin, nullptr, q_weight, k_weight);
     p.v = v; p.q_out = q_out; p.k_out = k_cache; p.v_out = v_cache;
     p.batch = Batch{block_table, kv_lens, cu_seqlens, p.mirror, g->table_stride, g->n_seq, g->tokens, cu_seqlens ? 0 : g->tokens / g->n_seq,
-                    g->n_pages, g->page_size, g->table_width};
+                    g->n_pages, g->page_size, g->table_width, g->padded};
     p.cache = Strides{0, 0, g->k_page_stride, g->k_row_stride, g->k_head_stride, g->v_page_stride, g->v_row_stride, g->v_head_stride};
     cudaStream_t st = (cudaStream_t)stream;
     if (rows8(p, {s->q_token_stride, s->q_head_stride, s->k_token_stride, s->k_head_stride, s->v_token_stride, s->v_head_stride, g->k_page_stride, g->k_row_stride,

@@ -240,6 +240,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (!some && warp == kMmaWarp) tmem_dealloc(tmem_slot, 512);
     } else {
         some = make_unit(b, a.tiles, slot, window, u);
+        if (!sums_only && hk == 0 && z == 0) {      // padding behind the last sequence; where sums are joined the join does this
+            const long long from = (long long)b.end() * a.c.heads.q_heads, rest = (long long)b.tokens * a.c.heads.q_heads - from;
+            const int step = gridDim.x * kThreads;
+            for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest * D / 8; e += step)
+                reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.o) + from * D)[e] = make_uint4(0, 0, 0, 0);
+            if (a.c.lse != nullptr)
+                for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest; e += step) a.c.lse[from + e] = -INFINITY;
+        }
         if (hk == 0 && z == 0 && tid == 0) {
             int n, tile;
             if (a.tiles.find(b, slot, n, tile)) check_batch(b, a.tiles, n, tile);
@@ -1049,7 +1057,7 @@ __global__ void __launch_bounds__(32 * kSharedWarps, 4) attn_shared_join_kernel(
             oa.x += x.x; oa.y += x.y; ob.x += x.z; ob.y += x.w;
         }
     }
-    if (at >= rows || !inside) return;
+    if (at >= rows) return;      // a token of no sequence has no parts: 0, as padding
     const float inv = m == -INFINITY ? 0.f : 1.f / l;
     if (lane == 0 && j.prefix.c.lse != nullptr) j.prefix.c.lse[row] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * kLn2;
     if (sub == 0 && d < D)

@@ -153,7 +153,7 @@ TensorPair norm_rope(const Tensor& q_, const Tensor& k_, const Tensor& cos_, con
 
 // q [tokens, heads, D] with adjacent values beside a cache [pages, page, kv heads, D] and the batch's device arrays
 bool paged_shape(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const OptTensor& cu, int64_t max_q, int64_t window,
-                 KdaPagedShape& s) {
+                 bool padded, KdaPagedShape& s) {
     if (q.dim() != 3 || kc.dim() != 4 || vc.sizes() != kc.sizes() || !q.is_cuda() || !is_io(q)) return false;
     if (kc.scalar_type() != q.scalar_type() || vc.scalar_type() != q.scalar_type() || !on(kc, q) || !on(vc, q)) return false;
     const int64_t T = q.size(0), H = q.size(1), D = q.size(2), pages = kc.size(0), page = kc.size(1), hk = kc.size(2);
@@ -177,6 +177,7 @@ bool paged_shape(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
     s.n_pages = (int32_t)pages, s.page_size = (int32_t)page, s.table_width = (int32_t)width;
     s.window = (int32_t)std::min(window, kInt);      // no sequence is longer
     s.scale = 1.f;
+    s.padded = padded;
     s.table_stride = table.stride(0);
     s.q_token_stride = q.stride(0), s.q_head_stride = q.stride(1);
     s.k_page_stride = kc.stride(0), s.k_row_stride = kc.stride(1), s.k_head_stride = kc.stride(2);
@@ -186,9 +187,9 @@ bool paged_shape(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
 const int32_t* iptr(const OptTensor& t) { return has(t) ? t->const_data_ptr<int32_t>() : nullptr; }
 
 OptTensor append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos_, const Tensor& sin_, const Tensor& kc, const Tensor& vc, const Tensor& table,
-                 const Tensor& lens, const OptTensor& cu, const OptTensor& qw_, const OptTensor& kw_, double eps, bool interleaved) {
+                 const Tensor& lens, const OptTensor& cu, const OptTensor& qw_, const OptTensor& kw_, double eps, bool interleaved, bool padded) {
     KdaPagedShape pg;
-    if (tracing() || !paged_shape(q, kc, vc, table, lens, cu, 0, 0, pg)) return c10::nullopt;
+    if (tracing() || !paged_shape(q, kc, vc, table, lens, cu, 0, 0, padded, pg)) return c10::nullopt;
     const int64_t T = q.size(0), D = q.size(2), hk = kc.size(2);
     const int64_t want[3] = {T, hk, D};
     if (k.sizes() != at::IntArrayRef(want, 3) || v.sizes() != k.sizes() || !on(k, q) || !on(v, q) || k.scalar_type() != q.scalar_type() ||
@@ -228,9 +229,9 @@ Tensor wide(const Tensor& q) {
 }
 
 AttentionOut attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const OptTensor& cu, int64_t max_q,
-                       int64_t window, c10::optional<double> scale, bool want_lse) {
+                       int64_t window, c10::optional<double> scale, bool want_lse, bool padded) {
     KdaPagedShape pg;
-    if (tracing() || !paged_shape(q_, kc, vc, table, lens, cu, max_q, window, pg)) return c10::nullopt;
+    if (tracing() || !paged_shape(q_, kc, vc, table, lens, cu, max_q, window, padded, pg)) return c10::nullopt;
     if (at::GradMode::is_enabled() && (q_.requires_grad() || kc.requires_grad() || vc.requires_grad())) return c10::nullopt;
     pg.scale = scale.has_value() ? (float)*scale : (float)(1.0 / std::sqrt((double)pg.head_dim));
     if (!(pg.scale > 0.f) || !std::isfinite(pg.scale)) return c10::nullopt;
@@ -252,9 +253,10 @@ AttentionOut attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
 }
 
 AttentionOut shared_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, const Tensor& prefix_table,
-                              const Tensor& prefix_lens, const OptTensor& groups, const OptTensor& cu, int64_t max_q, c10::optional<double> scale, bool want_lse) {
+                              const Tensor& prefix_lens, const OptTensor& groups, const OptTensor& cu, int64_t max_q, c10::optional<double> scale, bool want_lse,
+                              bool padded) {
     KdaPagedShape pg;
-    if (tracing() || !paged_shape(q_, kc, vc, table, lens, cu, max_q, 0, pg)) return c10::nullopt;
+    if (tracing() || !paged_shape(q_, kc, vc, table, lens, cu, max_q, 0, padded, pg)) return c10::nullopt;
     if (prefix_table.dim() != 2 || prefix_table.scalar_type() != at::kInt || !on(prefix_table, q_)) return c10::nullopt;
     const int64_t G = prefix_table.size(0), width = prefix_table.size(1);
     if (G < 1 || G > pg.n_seq || width > kInt / pg.page_size || (width > 1 && prefix_table.stride(1) != 1)) return c10::nullopt;

@@ -396,6 +396,8 @@ int kda_norm_rope_bwd(const KdaRotaryShape* shape, const void* q, const void* k,
  * them.  cu_seqlens [n_seq+1] int32: new tokens of the packed batch, or NULL: tokens / n_seq each.  The i-th of a
  * sequence's n new tokens is at position kv_len - n + i; a negative one is padding.  max_q_len: a bound on the new tokens of
  * any sequence, or 0.  All three are read on the device, and pages that no new token reaches are never touched.
+ * Tokens behind cu_seqlens[n_seq] are padding too.  Where `padded` is 0 there should be none, and the status word reports
+ * KDA_ERR_CU_SEQLENS; a step of fixed size whose tokens are known on the device alone sets it.
  */
 typedef struct KdaPagedShape {
     int32_t tokens, n_seq, max_q_len;
@@ -404,6 +406,7 @@ typedef struct KdaPagedShape {
     int32_t n_pages, page_size, table_width;
     int32_t window;                 /* a token sees itself and window - 1 before it; 0: all */
     float scale;                    /* > 0 */
+    int32_t padded;                 /* cu_seqlens may end before `tokens` */
     int64_t table_stride;
     int64_t q_token_stride, q_head_stride;
     int64_t k_page_stride, k_row_stride, k_head_stride, v_page_stride, v_row_stride, v_head_stride;

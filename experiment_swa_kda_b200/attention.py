@@ -369,7 +369,7 @@ class PagedAttention(nn.Module):
         else:
             o = shared_prefix_attention(q, *place[:4], cache.prefix_table, cache.prefix_lens, cache.cu_groups, cu_seqlens, max_q_len=max_q_len,
                                         padded=padded)
-        return self.o_proj(o.reshape(*lead, -1))
+        return self.o_proj(o.reshape(*lead, self.num_heads * self.head_dim))
 
 
 __all__ = ["PagedAttention", "PagedCache", "paged_attention", "plan_pages", "qk_norm_rope", "qk_norm_rope_append", "shared_prefix_attention"]

@@ -249,7 +249,8 @@ def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens
 
     positions [max_tokens] int32 are the new tokens' places in their sequences, slots [max_tokens] int64 those in a cache of
     [pages * page_size] rows; -1 behind the last.  Nothing synchronises; a captured graph follows the arrays.  What goes on from here with
-    max_tokens tokens - `qk_norm_rope_append`, the attention, `PagedAttention` - takes this cu_seqlens with `padded`, since a step need not be full.  A pool starts out with all
+    max_tokens tokens - `qk_norm_rope_append`, the attention, `PagedAttention` - takes this cu_seqlens with `padded`, since a step need not be full.
+    A call without cu_seqlens counts new tokens in every row, and would write one that waits over the last of what it has.  A pool starts out with all
     pages free and a table of -1."""
     out = None
     if block_table.is_cuda:

@@ -41,7 +41,7 @@ class PrefixShape(C.Structure):
 
 
 class PlanShape(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("rows", "width", "page_size", "n_pages", "max_tokens")] + [("table_stride", C.c_int64)]
+    _fields_ = [(n, C.c_int32) for n in ("rows", "width", "page_size", "n_pages", "max_tokens", "overtake")] + [("table_stride", C.c_int64)]
 
 
 _P = C.c_void_p

@@ -235,7 +235,7 @@ def shared_prefix_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_t
 
 
 def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens: Tensor, *, page_size: int, max_tokens: int,
-               starts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+               starts: Optional[Tensor] = None, overtake: bool = False) -> Tuple[Tensor, Tensor, Tensor]:
     """Deals out the pages of a step and maps its new tokens to them; returns (cu_seqlens [N+1], positions [max_tokens], slots [max_tokens]).
 
     The caller sets `kv_lens` [N] to what its requests shall have after the step, `new_lens` [N] of these being new; a row whose
@@ -245,7 +245,10 @@ def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens
     begin: behind a prefix it shares, or where a sliding window has left off; a new token before it has no page and a negative slot.
 
     A row is served if the pages lacking up to and with it are there and the new tokens up to and with it are at most `max_tokens`.  One
-    that is not waits: IN PLACE its length is less by its new tokens, none of which cu_seqlens counts.
+    that is not waits: IN PLACE its length is less by its new tokens, none of which cu_seqlens counts.  The sums run over the rows that wait as
+    well, so rows are served in their order, and one that asks for more than there is holds up every row behind it that asks for anything, running
+    requests among them: keep prompts behind these, or pass `overtake`.  Then a row that waits counts for nothing, and all are served that still
+    find their pages and tokens.
 
     positions [max_tokens] int32 are the new tokens' places in their sequences, slots [max_tokens] int64 those in a cache of
     [pages * page_size] rows; -1 behind the last.  Nothing synchronises; a captured graph follows the arrays.  What goes on from here with
@@ -254,7 +257,7 @@ def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens
     pages free and a table of -1."""
     out = None
     if block_table.is_cuda:
-        out = _native.load().plan(block_table, kv_lens, page_free, new_lens, starts, page_size, max_tokens)
+        out = _native.load().plan(block_table, kv_lens, page_free, new_lens, starts, page_size, max_tokens, bool(overtake))
     if out is not None:
         return out
     if block_table.ndim != 2 or block_table.dtype != torch.int32 or 0 in block_table.shape:
@@ -309,11 +312,12 @@ class PagedCache:
         return PagedCache(store(), store(), table, torch.zeros(sequences, device=device, dtype=torch.int32),
                           torch.ones(pages, device=device, dtype=torch.bool))
 
-    def plan(self, new_lens: Tensor, max_tokens: int, starts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    def plan(self, new_lens: Tensor, max_tokens: int, starts: Optional[Tensor] = None, overtake: bool = False) -> Tuple[Tensor, Tensor, Tensor]:
         """`plan_pages` of this cache, whose `kv_lens` the caller has set for the step."""
         if self.page_free is None:
             raise RuntimeError("this cache's pages are dealt out already; PagedCache.pool makes one whose pages are planned")
-        return plan_pages(self.block_table, self.kv_lens, self.page_free, new_lens, page_size=self.k.shape[1], max_tokens=max_tokens, starts=starts)
+        return plan_pages(self.block_table, self.kv_lens, self.page_free, new_lens, page_size=self.k.shape[1], max_tokens=max_tokens, starts=starts,
+                          overtake=overtake)
 
 
 class PagedAttention(nn.Module):

@@ -9,7 +9,7 @@
 // (256 rows of 256 columns and 32,768 pages are 300 KB).  So it is one launch, a cluster of blocks that meet at its barriers (0.5 us each):
 //   1  entries outside of their row's columns go back; missing ones are counted, 128 columns a warp
 //   2  every block sums up all rows and all free pages for itself, which costs less than meeting once more
-//   3  who is served; the first free pages are listed in order
+//   3  who is served: the first rows that fit, or (overtake) all that still fit; the first free pages are listed in order
 //   4  missing entries take theirs; rows that have to wait give back what their new tokens would have needed
 //   5  position and slot of each new token
 // A block has a range of the rows from 1 to 5.  A batch that one block can read at once takes a single block, which keeps its lists to itself.
@@ -38,7 +38,7 @@ struct PlanArgs {
     int* dealt;             // [n_pages]: the free pages in order
     int* mirror;
     long long table_stride;
-    int rows, width, page, n_pages, max_tokens, items;
+    int rows, width, page, n_pages, max_tokens, items, overtake;
     int split, slice;       // blocks count free pages by shares of `slice`, a multiple of 512
     int thread_pages;       // pages whose flags a thread counts: a power of two, 16 at least
 
@@ -250,33 +250,61 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     }
 
     // ------------------------------------------------------------------ 3: who is served; the free pages they take, in order
-    Sums upto = before;
-    bool all_served = true;
+    const bool enough = total.need <= free_all && total.add <= a.max_tokens;      // for everybody
+    if (!enough && a.overtake) {
+        // Who is served depends on all before, so a warp goes through the rows, 32 of them at once where all of these are served: 32 rows one by one take
+        // some 500 cycles.
+        if (warp == 0) {
+            int left = free_all, tokens = 0;
+            for (int m0 = 0; m0 < a.rows; m0 += 32) {
+                const int n = min(m0 + lane, a.rows - 1), need = m0 + lane < a.rows ? base_of[n] : 0, add = m0 + lane < a.rows ? cu[n] : 0;
+                int all_add = min(add, kFull);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) all_add = add_tokens(all_add, __shfl_xor_sync(0xffffffffu, all_add, o));
+                const int all_need = __reduce_add_sync(0xffffffffu, need);      // fits, as the sum of all rows does
+                if (all_need <= left && add_tokens(tokens, all_add) <= a.max_tokens) {
+                    left -= all_need;
+                    tokens += all_add;
+                    continue;
+                }
+                bool served = true;
+#pragma unroll
+                for (int l = 0; l < 32; ++l) {
+                    const int x = __shfl_sync(0xffffffffu, need, l), y = __shfl_sync(0xffffffffu, add, l);
+                    const bool fits = (x <= left && add_tokens(tokens, y) <= a.max_tokens) || (x == 0 && y == 0);
+                    if (fits) left -= x, tokens += y;
+                    if (lane == l) served = fits;
+                }
+                if (!served) base_of[n] = -1;
+            }
+        }
+        __syncthreads();
+    }
+    Sums upto = before, at = before;
     mine = Sums{0, 0, 0};
     for (int n = n0; n < n1; ++n) {
         const Sums row{base_of[n], cu[n], 0};
         upto = upto + row;
-        const bool served = (upto.need <= free_all && upto.add <= a.max_tokens) || (row.need == 0 && row.add == 0);
-        if (served) {
-            base_of[n] = upto.need - row.need;
+        if (enough || (a.overtake ? row.need >= 0 : (upto.need <= free_all && upto.add <= a.max_tokens) || (row.need == 0 && row.add == 0))) {
             mine = mine + row;
         } else {
             base_of[n] = -1;
             cu[n] = 0;
             len_of[n] -= row.add;
-            all_served = false;
         }
     }
-    // Rows that lack pages and are served are the first of those that lack any, so the sums of all rows hold for what they lack, and for
-    // the tokens too if nobody waits.
-    int at = before.add;
-    if (!__syncthreads_and(all_served)) at = block_scan(mine, sums[1], total).add;
+    __syncthreads();
+    if (!enough) at = block_scan(mine, sums[1], total);      // of the rows served
     const int taken = total.need;
     for (int n = n0; n < n1; ++n) {
-        const int add = cu[n];
-        cu[n] = at;
-        if (n >= r0 && n < r1) a.cu[n] = at;
-        at += add;
+        const int need = base_of[n], add = cu[n];
+        if (need >= 0) {
+            base_of[n] = at.need;
+            at.need += need;
+        }
+        cu[n] = at.add;
+        if (n >= r0 && n < r1) a.cu[n] = at.add;
+        at.add += add;
     }
     if (tid == 0) {
         cu[a.rows] = total.add;
@@ -420,7 +448,7 @@ extern "C" int kda_plan_pages(const KdaPlanShape* s, int32_t* block_table, int32
     PlanArgs a;
     a.table = block_table; a.kv_lens = kv_lens; a.free_ = page_free; a.new_lens = new_lens; a.starts = starts;
     a.cu = cu_seqlens; a.positions = positions; a.slots = reinterpret_cast<long long*>(slots);
-    a.rows = s->rows; a.width = s->width; a.page = s->page_size; a.n_pages = s->n_pages; a.max_tokens = s->max_tokens;
+    a.rows = s->rows; a.width = s->width; a.page = s->page_size; a.n_pages = s->n_pages; a.max_tokens = s->max_tokens; a.overtake = s->overtake;
     a.items = items_of(*s);
     // every block for itself: 2 us for 262,144 pages, where meeting once more costs 0.6
     a.split = a.n_pages > 64 * kThreads;

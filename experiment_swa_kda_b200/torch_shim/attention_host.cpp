@@ -294,7 +294,7 @@ AttentionOut shared_attention(const Tensor& q_, const Tensor& kc, const Tensor& 
 
 using PlanOut = c10::optional<std::tuple<Tensor, Tensor, Tensor>>;
 
-PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const Tensor& news, const OptTensor& starts, int64_t page, int64_t max_tokens) {
+PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const Tensor& news, const OptTensor& starts, int64_t page, int64_t max_tokens, bool overtake) {
     constexpr int64_t kRows = 16384, kMost = 1 << 30;
     if (tracing() || !table.is_cuda() || table.dim() != 2 || table.scalar_type() != at::kInt) return c10::nullopt;
     const int64_t N = table.size(0), width = table.size(1), pages = free.numel();
@@ -311,6 +311,7 @@ PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const 
     KdaPlanShape s = {};
     s.rows = (int32_t)N, s.width = (int32_t)width, s.page_size = (int32_t)page, s.n_pages = (int32_t)pages, s.max_tokens = (int32_t)max_tokens;
     s.table_stride = table.stride(0);
+    s.overtake = overtake;
     // the three results out of one allocation: a trip to the allocator is a tenth of a small call
     const size_t at_positions = up256(max_tokens * sizeof(int64_t)), at_cu = at_positions + up256(max_tokens * sizeof(int32_t));
     const Tensor all = bytes(at_cu + (N + 1) * sizeof(int32_t), table);

@@ -446,7 +446,8 @@ int kda_shared_prefix_attention(const KdaPagedShape* shape, const KdaPrefixShape
  * ceil(kv_lens[n] / page_size)), starts clamped to the length (NULL: 0).  Entries outside go back to the pool (entry -1, page_free[page] = 1);
  * entries that name no page in [0, n_pages) are missing, and in the order of rows and columns take the pages with page_free != 0 in
  * ascending order.  A row is served if the entries missing up to and with it are at most the free pages and the new tokens up to and
- * with it at most max_tokens, or if it lacks nothing and asks for nothing; of one that is not, kv_lens[n] -= new_lens[n], and columns that
+ * with it at most max_tokens, or if it lacks nothing and asks for nothing - with `overtake` the sums leave out rows that are not served, so that these hold up
+ * nobody behind them -; of one that is not, kv_lens[n] -= new_lens[n], and columns that
  * this leaves unneeded go back, too late for this call.  cu_seqlens [rows + 1]: new tokens of the rows served.  positions, slots
  * [max_tokens]: of each of them its place in its sequence, kv_len - new + i, and in the cache, page * page_size + place in the page;
  * -1 behind the last.  kv_lens count the new tokens, as in kda_paged_attention.  A negative length or one the table has no room for, and an
@@ -454,6 +455,7 @@ int kda_shared_prefix_attention(const KdaPagedShape* shape, const KdaPrefixShape
  * left out or cut.  At most 16,384 rows. */
 typedef struct KdaPlanShape {
     int32_t rows, width, page_size, n_pages, max_tokens;
+    int32_t overtake;
     int64_t table_stride;
 } KdaPlanShape;
 size_t kda_plan_pages_workspace_bytes(const KdaPlanShape* shape);

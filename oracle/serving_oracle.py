@@ -5,8 +5,9 @@ import math
 import torch
 
 
-def plan_pages(table, kv_lens, page_free, new_lens, page_size, max_tokens, starts=None):
-    """Lists in, (table, kv_lens, page_free, cu_seqlens, positions, slots) out; the lists given are left as they are."""
+def plan_pages(table, kv_lens, page_free, new_lens, page_size, max_tokens, starts=None, overtake=False):
+    """Lists in, (table, kv_lens, page_free, cu_seqlens, positions, slots) out; the lists given are left as they are.  overtake: rows that wait
+    do not count against those behind them."""
     table, kv_lens, page_free, new_lens = [list(r) for r in table], list(kv_lens), list(page_free), list(new_lens)
     rows, width, pages = len(table), len(table[0]), len(page_free)
     starts = [0] * rows if starts is None else list(starts)
@@ -44,6 +45,8 @@ def plan_pages(table, kv_lens, page_free, new_lens, page_size, max_tokens, start
         else:
             kv_lens[n] -= new_lens[n]
             waits.append(n)
+            if overtake:
+                need, tokens = need - len(lacks[n]), tokens - new_lens[n]
         cu.append(len(positions))
     for n in waits:      # what its new tokens would have needed, and only that
         end = -(-kv_lens[n] // page_size)

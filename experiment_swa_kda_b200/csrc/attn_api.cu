@@ -74,8 +74,7 @@ extern "C" int kda_paged_attention(const KdaPagedShape* s, const void* q, const 
     if (int rc = check(s, cu_seqlens != nullptr)) return rc;
     if (s->tokens == 0) return KDA_OK;
     if (!q || !kv_lens || !o) return KDA_ERR_NULL;
-    const bool cached = s->n_pages > 0 && s->table_width > 0;
-    if (cached && (!k_cache || !v_cache || !block_table)) return KDA_ERR_NULL;
+    if (s->table_width > 0 && (!block_table || (s->n_pages > 0 && (!k_cache || !v_cache)))) return KDA_ERR_NULL;      // a table is read whether or not there are pages
     const size_t need = kda_paged_attention_workspace_bytes(s);
     if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need)) return KDA_ERR_WORKSPACE;
     const bool packed = cu_seqlens != nullptr;
@@ -241,7 +240,7 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     if (int rc = check_prefix(s, p, cu_seqlens != nullptr, cu_groups != nullptr)) return rc;
     if (s->tokens == 0) return KDA_OK;
     if (!q || !kv_lens || !o || !prefix_lens) return KDA_ERR_NULL;
-    if (s->n_pages > 0 && ((s->table_width > 0 && !block_table) || (p->table_width > 0 && !prefix_table) || !k_cache || !v_cache)) return KDA_ERR_NULL;
+    if ((s->table_width > 0 && !block_table) || (p->table_width > 0 && !prefix_table) || (s->n_pages > 0 && (!k_cache || !v_cache))) return KDA_ERR_NULL;
     const size_t need = kda_shared_prefix_attention_workspace_bytes(s, p);
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need) return KDA_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;

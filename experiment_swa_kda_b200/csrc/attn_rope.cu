@@ -788,7 +788,7 @@ extern "C" int kda_norm_rope_append(const KdaRotaryShape* s, const KdaPagedShape
     if (!cu_seqlens && g->tokens % g->n_seq != 0) return KDA_ERR_BAD_SHAPE;
     if (s->tokens == 0) return KDA_OK;
     if (!q || !k || !v || !kv_lens || !q_out || (s->rotary_dim > 0 && (!cos || !sin))) return KDA_ERR_NULL;
-    if (g->n_pages > 0 && g->table_width > 0 && (!block_table || !k_cache || !v_cache)) return KDA_ERR_NULL;
+    if (g->table_width > 0 && (!block_table || (g->n_pages > 0 && (!k_cache || !v_cache)))) return KDA_ERR_NULL;
     Rope p = fill(*s, q, k, cos, sin, nullptr, q_weight, k_weight);
     p.v = v; p.q_out = q_out; p.k_out = k_cache; p.v_out = v_cache;
     p.batch = Batch{block_table, kv_lens, cu_seqlens, p.mirror, g->table_stride, g->n_seq, g->tokens, cu_seqlens ? 0 : g->tokens / g->n_seq,

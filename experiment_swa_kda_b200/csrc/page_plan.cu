@@ -18,6 +18,8 @@
 // which 10 are phase 1 (16 rows a warp, four on their way) and 13 are 4 and 5.  Measured and left out: one barrier more to count free pages by shares also in small
 // pools (0.6 us), pages listed by the threads that counted them (4,096 rows 37 -> 50), scans of 64-bit sums (0.5 each).
 
+#include <limits.h>
+
 #include "common.cuh"
 
 namespace kda {
@@ -423,6 +425,8 @@ int check(const KdaPlanShape* s) {
     if (s->rows > kMaxRows) return KDA_ERR_UNSUPPORTED;
     if ((long long)s->width * s->page_size >= 1ll << 31 || (long long)s->rows * s->width >= 1ll << 31 || s->n_pages > (1 << 30) || s->max_tokens > kMostTokens)
         return KDA_ERR_BAD_SHAPE;
+    // columns are counted in whole items, in 32 bits; rows are written, each by its own block
+    if (s->width > INT_MAX - kColumns || (s->rows > 1 && s->table_stride < s->width)) return KDA_ERR_BAD_SHAPE;
     return KDA_OK;
 }
 int items_of(const KdaPlanShape& s) { return ceil_div(s.width, kColumns); }

@@ -298,7 +298,7 @@ PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const 
     constexpr int64_t kRows = 16384, kMost = 1 << 30;
     if (tracing() || !table.is_cuda() || table.dim() != 2 || table.scalar_type() != at::kInt) return c10::nullopt;
     const int64_t N = table.size(0), width = table.size(1), pages = free.numel();
-    if (N < 1 || N > kRows || width < 1 || width > kInt || (width > 1 && table.stride(1) != 1) || (N > 1 && table.stride(0) < width)) return c10::nullopt;
+    if (N < 1 || N > kRows || width < 1 || width > kInt - 128 || (width > 1 && table.stride(1) != 1) || (N > 1 && table.stride(0) < width)) return c10::nullopt;
     for (const Tensor* t : {&lens, &news})
         if (t->dim() != 1 || t->numel() != N || t->scalar_type() != at::kInt || !on(*t, table) || !t->is_contiguous()) return c10::nullopt;
     if (has(starts) && (starts->dim() != 1 || starts->numel() != N || starts->scalar_type() != at::kInt || !on(*starts, table) || !starts->is_contiguous()))

@@ -95,6 +95,7 @@ _SIGNATURES = {
     "kda_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedShape)]),
     "kda_paged_attention": (C.c_int, [C.POINTER(PagedShape)] + [_P] * 9 + [C.c_size_t, _P]),
     "kda_shared_prefix_attention_workspace_bytes": (C.c_size_t, [C.POINTER(PagedShape), C.POINTER(PrefixShape)]),
+    "kda_shared_prefix_attention_call_bytes": (C.c_size_t, [C.POINTER(PagedShape), C.POINTER(PrefixShape)] + [_P] * 5),
     "kda_shared_prefix_attention": (C.c_int, [C.POINTER(PagedShape), C.POINTER(PrefixShape)] + [_P] * 12 + [C.c_size_t, _P]),
     "kda_plan_pages_workspace_bytes": (C.c_size_t, [C.POINTER(PlanShape)]),
     "kda_plan_pages": (C.c_int, [C.POINTER(PlanShape)] + [_P] * 9 + [C.c_size_t, _P]),

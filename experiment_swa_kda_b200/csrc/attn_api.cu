@@ -2,6 +2,8 @@
 
 #include <math.h>
 
+#include <initializer_list>
+
 #include "attn.cuh"
 
 using namespace kda;
@@ -210,27 +212,72 @@ SharedSpace shared_space(const KdaPagedShape& s, const KdaPrefixShape& p, bool p
     return w;
 }
 
+// The ways a call can go, and the workspace of each.  Nothing is asked for but what the way taken needs: prompts in one pass need next to nothing, where the sums
+// of two passes over 65,536 tokens of 16 heads are a gigabyte.
+enum class Way { general, one_pass, one_list, two_passes };
+Way way_of(const Call& c, const KdaPagedShape& s, const KdaPrefixShape& p) {
+    if (!tc_takes(c)) return Way::general;
+    if (takes_both(s, p, c.max_q_len)) return Way::one_pass;
+    return few_keys(s) && decode_takes(c) ? Way::one_list : Way::two_passes;
+}
+size_t workspace_of(const Call& c, const KdaPagedShape& s, const KdaPrefixShape& p) {
+    const bool packed = c.batch.cu != nullptr;
+    int per_seq;
+    switch (way_of(c, s, p)) {
+        case Way::general:
+            return general_shared_workspace((size_t)s.tokens * s.q_heads, general_prefix_splits(s, p) + general_splits(s, packed), s.head_dim);
+        case Way::one_pass:
+            return tc_workspace(tile_slots(s.tokens, s.n_seq, c.max_q_len, c.heads.group, 256, packed, per_seq), s.kv_heads, tc_splits(s, packed), s.head_dim);
+        case Way::one_list:
+            return decode_workspace(s.n_seq, s.kv_heads, s.table_width, s.page_size, 0, c.max_q_len, s.head_dim);
+        case Way::two_passes: {
+            const SharedSpace w = shared_space(s, p, packed, own_rows_take(c));
+            return w.prefix + w.own;
+        }
+    }
+    return 0;
+}
+
+Call call_of(const KdaPagedShape* s, const KdaPrefixShape* p, const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* kv_lens,
+             const int32_t* cu_seqlens, const int32_t* prefix_table, const int32_t* prefix_lens, const int32_t* cu_groups, void* o, float* lse, void* workspace) {
+    const int q_len = cu_seqlens ? 0 : s->tokens / s->n_seq;
+    Call c;
+    c.batch = GroupView{};
+    static_cast<Batch&>(c.batch) =
+        Batch{block_table, kv_lens, cu_seqlens, nullptr, s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width, s->padded};
+    c.batch.p = Prefix{prefix_table, prefix_lens, cu_groups, p->table_stride, p->n_groups, p->table_width, s->n_seq / p->n_groups};
+    c.heads = Heads{s->q_heads, s->kv_heads, s->q_heads / s->kv_heads, s->head_dim};
+    c.strides = Strides{s->q_token_stride, s->q_head_stride, s->k_page_stride, s->k_row_stride, s->k_head_stride, s->v_page_stride, s->v_row_stride, s->v_head_stride};
+    c.q = q; c.k = k_cache; c.v = v_cache; c.o = o; c.lse = lse;
+    c.scale = s->scale;
+    c.window = 0;
+    c.bf16 = s->io_dtype == KDA_DTYPE_BF16;
+    c.max_q_len = cu_seqlens ? s->max_q_len : q_len;
+    c.workspace = workspace;
+    return c;
+}
+
 }  // namespace
+
+extern "C" size_t kda_shared_prefix_attention_call_bytes(const KdaPagedShape* s, const KdaPrefixShape* p, const void* q, const void* k_cache, const void* v_cache,
+                                                         const int32_t* cu_seqlens, const void* o) {
+    if (check_prefix(s, p, cu_seqlens != nullptr, true) || s->tokens == 0) return 0;
+    return align_up(workspace_of(call_of(s, p, q, k_cache, v_cache, nullptr, nullptr, cu_seqlens, nullptr, nullptr, nullptr, const_cast<void*>(o), nullptr, nullptr), *s, *p), 256);
+}
 
 extern "C" size_t kda_shared_prefix_attention_workspace_bytes(const KdaPagedShape* s, const KdaPrefixShape* p) {
     if (check_prefix(s, p, true, true)) return 0;
-    size_t most = general_shared_workspace((size_t)s->tokens * s->q_heads, general_prefix_splits(*s, *p) + general_splits(*s, true), s->head_dim);
-    for (int packed = 0; packed < 2; ++packed) {      // whether the batch has cu_seqlens is not known here
-        if (!packed && s->tokens % s->n_seq != 0) continue;
-        const size_t g = general_shared_workspace((size_t)s->tokens * s->q_heads, general_prefix_splits(*s, *p) + general_splits(*s, packed), s->head_dim);
-        if (g > most) most = g;
-        int per;
-        const size_t both = tc_workspace(tile_slots(s->tokens, s->n_seq, packed ? s->max_q_len : s->tokens / s->n_seq, s->q_heads / s->kv_heads, 256, packed, per),
-                                         s->kv_heads, tc_splits(*s, packed), s->head_dim);
-        if (both > most) most = both;
-        const size_t step = decode_workspace(s->n_seq, s->kv_heads, s->table_width, s->page_size, 0, packed ? s->max_q_len : s->tokens / s->n_seq, s->head_dim);
-        if (step > most) most = step;
-        for (int few = 0; few < 2; ++few) {
-            const SharedSpace w = shared_space(*s, *p, packed, few);
-            if (w.prefix + w.own > most) most = w.prefix + w.own;
+    size_t most = 256;
+    const int32_t any = 0;
+    // whether the batch has cu_seqlens is not known here, nor where the arrays lie: on 16 bytes, or not
+    for (const int32_t* cu : {&any, static_cast<const int32_t*>(nullptr)})
+        for (uintptr_t at : {uintptr_t(256), uintptr_t(1)}) {
+            const void* x = reinterpret_cast<const void*>(at);
+            if (cu == nullptr && s->tokens % s->n_seq != 0) continue;
+            const size_t need = kda_shared_prefix_attention_call_bytes(s, p, x, x, x, cu, x);
+            if (need > most) most = need;
         }
-    }
-    return align_up(most, 256);
+    return most;
 }
 
 extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPrefixShape* p, const void* q, const void* k_cache, const void* v_cache,
@@ -241,27 +288,18 @@ extern "C" int kda_shared_prefix_attention(const KdaPagedShape* s, const KdaPref
     if (s->tokens == 0) return KDA_OK;
     if (!q || !kv_lens || !o || !prefix_lens) return KDA_ERR_NULL;
     if ((s->table_width > 0 && !block_table) || (p->table_width > 0 && !prefix_table) || (s->n_pages > 0 && (!k_cache || !v_cache))) return KDA_ERR_NULL;
-    const size_t need = kda_shared_prefix_attention_workspace_bytes(s, p);
-    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need) return KDA_ERR_WORKSPACE;
+    Call c = call_of(s, p, q, k_cache, v_cache, block_table, kv_lens, cu_seqlens, prefix_table, prefix_lens, cu_groups, o, lse, workspace);
+    const size_t need = workspace_of(c, *s, *p);
+    if (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 || workspace_bytes < need)) return KDA_ERR_WORKSPACE;
+    c.batch.mirror = status_mirror();
     const cudaStream_t st = (cudaStream_t)stream;
     const bool packed = cu_seqlens != nullptr;
-    const int q_len = packed ? 0 : s->tokens / s->n_seq;
-    Call c;
-    c.batch = GroupView{};
-    static_cast<Batch&>(c.batch) =
-        Batch{block_table, kv_lens, cu_seqlens, status_mirror(), s->table_stride, s->n_seq, s->tokens, q_len, s->n_pages, s->page_size, s->table_width, s->padded};
-    c.batch.p = Prefix{prefix_table, prefix_lens, cu_groups, p->table_stride, p->n_groups, p->table_width, s->n_seq / p->n_groups};
-    c.heads = Heads{s->q_heads, s->kv_heads, s->q_heads / s->kv_heads, s->head_dim};
-    c.strides = Strides{s->q_token_stride, s->q_head_stride, s->k_page_stride, s->k_row_stride, s->k_head_stride, s->v_page_stride, s->v_row_stride, s->v_head_stride};
-    c.q = q; c.k = k_cache; c.v = v_cache; c.o = o; c.lse = lse;
-    c.scale = s->scale;
-    c.window = 0;
-    c.bf16 = s->io_dtype == KDA_DTYPE_BF16;
-    c.max_q_len = packed ? s->max_q_len : q_len;
-    c.workspace = workspace;
-    if (!tc_takes(c)) return general_shared(c, general_prefix_splits(*s, *p), general_splits(*s, packed), st);
-    if (takes_both(*s, *p, c.max_q_len)) return tc_both(c, tc_splits(*s, packed), st);
-    if (few_keys(*s) && decode_takes(c)) return decode_both(c, st);
+    switch (way_of(c, *s, *p)) {
+        case Way::general: return general_shared(c, general_prefix_splits(*s, *p), general_splits(*s, packed), st);
+        case Way::one_pass: return tc_both(c, tc_splits(*s, packed), st);
+        case Way::one_list: return decode_both(c, st);
+        case Way::two_passes: break;
+    }
     const bool few = own_rows_take(c);
     const int prefix_splits = tc_prefix_splits(*s, *p), own_splits = tc_splits(*s, packed);
     Call own = c;

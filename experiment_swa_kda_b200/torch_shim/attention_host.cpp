@@ -281,11 +281,12 @@ AttentionOut shared_attention(const Tensor& q_, const Tensor& kc, const Tensor& 
     Tensor o = empty(q.sizes(), q.scalar_type(), q), ws;
     OptTensor lse;
     if (want_lse) lse = empty({q.size(0), q.size(1)}, at::kFloat, q);
-    const size_t need = kda_shared_prefix_attention_workspace_bytes(&pg, &px);
-    ws = bytes(need, q);
+    const size_t need = kda_shared_prefix_attention_call_bytes(&pg, &px, q.const_data_ptr(), kc.const_data_ptr(), vc.const_data_ptr(), iptr(cu), o.const_data_ptr());
+    if (need > 0) ws = bytes(need, q);
     must(kda_shared_prefix_attention(&pg, &px, q.const_data_ptr(), kc.const_data_ptr(), vc.const_data_ptr(), table.const_data_ptr<int32_t>(),
                                      lens.const_data_ptr<int32_t>(), iptr(cu), prefix_table.const_data_ptr<int32_t>(), prefix_lens.const_data_ptr<int32_t>(),
-                                     iptr(groups), o.data_ptr(), want_lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr(), need, stream_of(q)),
+                                     iptr(groups), o.data_ptr(), want_lse ? lse->data_ptr<float>() : nullptr, need > 0 ? ws.data_ptr() : nullptr, need,
+                                     stream_of(q)),
          "kda_shared_prefix_attention");
     return std::make_tuple(o, lse);
 }

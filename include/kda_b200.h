@@ -435,6 +435,10 @@ typedef struct KdaPrefixShape {
     int32_t n_groups, table_width;
     int64_t table_stride;
 } KdaPrefixShape;
+/* What one call needs: q, k_cache, v_cache and o are looked at for how they are aligned, cu_seqlens for whether there is one.  The other is the
+ * most that any call of these shapes needs, aligned or not, packed or not. */
+size_t kda_shared_prefix_attention_call_bytes(const KdaPagedShape* shape, const KdaPrefixShape* prefix, const void* q, const void* k_cache, const void* v_cache,
+                                              const int32_t* cu_seqlens, const void* o);
 size_t kda_shared_prefix_attention_workspace_bytes(const KdaPagedShape* shape, const KdaPrefixShape* prefix);
 int kda_shared_prefix_attention(const KdaPagedShape* shape, const KdaPrefixShape* prefix, const void* q, const void* k_cache, const void* v_cache,
                                 const int32_t* block_table, const int32_t* kv_lens, const int32_t* cu_seqlens, const int32_t* prefix_table,

@@ -254,28 +254,30 @@ __global__ void __launch_bounds__(kThreads, 1) plan_pages_kernel(const __grid_co
     // ------------------------------------------------------------------ 3: who is served; the free pages they take, in order
     const bool enough = total.need <= free_all && total.add <= a.max_tokens;      // for everybody
     if (!enough && a.overtake) {
-        // Who is served depends on all before, so a warp goes through the rows, 32 of them at once where all of these are served: 32 rows one by one take
-        // some 500 cycles.
+        // Who is served depends on all before, so a warp goes through the rows, 32 at a time.  What is more than is left never fits again and drops out at once;
+        // of the others those up to the first that fits no more are served.  Needs are at most what is left, and all of them fit in 32 bits.
+        // 16,384 rows none of which fits take 52 us more than without (144), 4,096 13, 256 1; one row after the other took 1,020, 255 and 16.
         if (warp == 0) {
             int left = free_all, tokens = 0;
             for (int m0 = 0; m0 < a.rows; m0 += 32) {
                 const int n = min(m0 + lane, a.rows - 1), need = m0 + lane < a.rows ? base_of[n] : 0, add = m0 + lane < a.rows ? cu[n] : 0;
-                int all_add = min(add, kFull);
+                bool open = need > 0 || add > 0, served = !open;      // open: not known yet
+                for (;;) {
+                    open = open && need <= left && add <= a.max_tokens - tokens;
+                    if (!__any_sync(0xffffffffu, open)) break;
+                    Sums upto{open ? need : 0, open ? add : 0, 0};
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) all_add = add_tokens(all_add, __shfl_xor_sync(0xffffffffu, all_add, o));
-                const int all_need = __reduce_add_sync(0xffffffffu, need);      // fits, as the sum of all rows does
-                if (all_need <= left && add_tokens(tokens, all_add) <= a.max_tokens) {
-                    left -= all_need;
-                    tokens += all_add;
-                    continue;
-                }
-                bool served = true;
-#pragma unroll
-                for (int l = 0; l < 32; ++l) {
-                    const int x = __shfl_sync(0xffffffffu, need, l), y = __shfl_sync(0xffffffffu, add, l);
-                    const bool fits = (x <= left && add_tokens(tokens, y) <= a.max_tokens) || (x == 0 && y == 0);
-                    if (fits) left -= x, tokens += y;
-                    if (lane == l) served = fits;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const Sums x{__shfl_up_sync(0xffffffffu, upto.need, o), __shfl_up_sync(0xffffffffu, upto.add, o), 0};
+                        if (lane >= o) upto = upto + x;
+                    }
+                    const unsigned over = __ballot_sync(0xffffffffu, open && (upto.need > left || upto.add > a.max_tokens - tokens));
+                    const int first = over != 0 ? __ffs(over) - 1 : 32;      // not lane 0's: an open row fits by itself
+                    served |= open && lane < first;
+                    open = open && lane > first;
+                    left -= __shfl_sync(0xffffffffu, upto.need, first - 1);
+                    tokens += __shfl_sync(0xffffffffu, upto.add, first - 1);
+                    if (over == 0) break;
                 }
                 if (!served) base_of[n] = -1;
             }

@@ -70,6 +70,19 @@ def test_steps_of_a_scheduler(rows, width, pages, page, wide, offset):
     assert waited or rows < 3
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_rows_that_just_fit_between_rows_that_do_not(seed):
+    """Rows of one to seven pages and tokens against a pool and a step that run out little by little."""
+    rng = random.Random(seed)
+    rows = 200
+    pool = Overtaking(rows, 8, 300, 2)
+    asks = [rng.choice((0, 1, 2, 3, 9, 14)) for _ in range(rows)]
+    pool.step(asks, asks, 500 if seed % 2 else 10 ** 6)
+    lens = pool.lens
+    asks = [min(16, a + rng.choice((0, 1, 2, 5))) for a in lens]
+    pool.step(asks, [b - a for a, b in zip(lens, asks)], 150 if seed % 2 else 10 ** 6)
+
+
 def test_numbers_at_the_edge_of_32_bits():
     """Rows that ask for as many tokens as fit in 32 bits, next to ones that ask for few."""
     big = 2 ** 31 - 2 ** 20

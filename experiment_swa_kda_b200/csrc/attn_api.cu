@@ -184,10 +184,12 @@ bool takes_both(const KdaPagedShape& s, const KdaPrefixShape& p, long long max_q
 
 // Blocks of the pass over own keys.  A block that finds no work costs 6 us where it starts late, once others have ended, so there are as many as
 // find a place beside the prefixes, by what the tables' widths say: prefixes fill theirs, and sequences go on for 0.6 of what theirs have
-// besides.  How the work is cut is decided on the device, by the lengths.
+// besides.  Where both are as wide, as rows of one pool's table are, that says nothing, and own keys may fill theirs as well: too many blocks cost
+// 3 to 6 us, too few as often the pass as they are too few (256 sequences in a pool's table 90 us, 290 to 1,340 with blocks for own keys of half a page).
+// How the work is cut is decided on the device, by the lengths.
 int own_blocks(const KdaPagedShape& s, const KdaPrefixShape& p, bool packed, int splits) {
     const int group = s.q_heads / s.kv_heads;
-    const long long behind = behind_of(s, p);
+    const long long behind = p.table_width < s.table_width ? behind_of(s, p) : (long long)s.table_width * s.page_size;
     const long long most = ((behind + 63) / 64 + 1) * s.n_seq * s.kv_heads / 2, own_tiles = (behind * 3 / 5 + 32) * s.n_seq * s.kv_heads / 64;
     int best = 0;
     const int max_q = packed ? s.max_q_len : s.tokens / s.n_seq;

@@ -300,7 +300,6 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
     PrefixWork* work = reinterpret_cast<PrefixWork*>(sm + L::kQ);
     if constexpr (KEYS == kOwnKeys)
         if (a.prefix_splits > 1 && tid < b.p.n) work[tid] = prefix_work(a.c.batch, tid, g, a.prefix_rows);
-    const int batch_end = KEYS == kOwnKeys ? 0 : b.end();      // read here, where nothing waits for it
     auto blocks_of = [&](int total) {
         if constexpr (KEYS == kOwnKeys)
             if (a.prefix_splits > 1 && total > kMinTiles * kPerSmOf<DP, NR, KEYS>) {
@@ -388,10 +387,19 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
         for (int i = blockIdx.x * kThreads + tid; i < b.p.n; i += gridDim.x * kThreads) check_group(b, i);
     // sequences without a key in reach have no tile: their rows are nothing
     for (int n = blockIdx.x; n < b.n_seq; n += gridDim.x) {
+        const int end = KEYS == kOwnKeys ? b.tokens : b.end();      // read beside the sequence's lengths: 0.4 us of every call where all blocks read it by itself
         const Seq s = seq_at(b, n, window);
         if (tid == 0) {
             if (!b.span_ok(n) || s.count * g > kRows) b.tell(KDA_ERR_CU_SEQLENS);
             if (!b.kv_len_ok(n)) b.tell(KDA_ERR_BLOCK_TABLE);
+        }
+        // padding behind the last sequence, a token of so many each; of own keys the join does this
+#pragma unroll 1
+        for (int t = end + n; t < b.tokens; t += b.n_seq) {
+            uint4* o = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.o) + (size_t)t * Hq * D);
+            for (int e = tid; e < Hq * D / 8; e += kThreads) o[e] = make_uint4(0, 0, 0, 0);
+            if (a.c.lse != nullptr)
+                for (int e = tid; e < Hq; e += kThreads) a.c.lse[(size_t)t * Hq + e] = -INFINITY;
         }
         if (s.t1 > s.t0) continue;
         const size_t r0 = (size_t)s.first * Hq;
@@ -403,13 +411,6 @@ __global__ void __launch_bounds__(kThreads, kPerSmOf<DP, NR, KEYS>) attn_decode_
             if (a.c.lse != nullptr)
                 for (int e = tid; e < s.count * Hq; e += kThreads) a.c.lse[r0 + e] = -INFINITY;
         }
-    }
-    if constexpr (KEYS != kOwnKeys) {      // padding behind the last sequence; of own keys the join does this
-        const long long rest = (long long)(b.tokens - batch_end) * Hq, at = (long long)batch_end * Hq;
-        for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest * D / 8; e += gridDim.x * kThreads)
-            reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.o) + at * D)[e] = make_uint4(0, 0, 0, 0);
-        if (a.c.lse != nullptr)
-            for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest; e += gridDim.x * kThreads) a.c.lse[at + e] = -INFINITY;
     }
     if (tiles <= 0) {
         if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too

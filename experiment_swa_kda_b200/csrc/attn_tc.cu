@@ -201,6 +201,16 @@ __device__ __forceinline__ void write_places(const Args& a, const GroupView& b, 
     }
 }
 
+// This block's share of the padding behind the last sequence; thread t of `threads`, in the blocks of one kv head and part.  Where sums are left for a join the
+// join does this.
+__device__ __forceinline__ void blank_rest(const Args& a, const Batch& b, int t, int threads) {
+    const long long from = (long long)b.end() * a.c.heads.q_heads, rest = (long long)b.tokens * a.c.heads.q_heads - from;
+    const int begin = blockIdx.x * threads + t, step = gridDim.x * threads, D = a.c.heads.dim;
+    for (long long e = begin; e < rest * D / 8; e += step) reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.o) + from * D)[e] = make_uint4(0, 0, 0, 0);
+    if (a.c.lse != nullptr)
+        for (long long e = begin; e < rest; e += step) a.c.lse[from + e] = -INFINITY;
+}
+
 template <int DP, int KEYS>
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ CUtensorMap mK, const __grid_constant__ CUtensorMap mV,
                                                               const __grid_constant__ CUtensorMap mQ, const __grid_constant__ CUtensorMap mO,
@@ -240,14 +250,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         if (!some && warp == kMmaWarp) tmem_dealloc(tmem_slot, 512);
     } else {
         some = make_unit(b, a.tiles, slot, window, u);
-        if (!sums_only && hk == 0 && z == 0) {      // padding behind the last sequence; where sums are joined the join does this
-            const long long from = (long long)b.end() * a.c.heads.q_heads, rest = (long long)b.tokens * a.c.heads.q_heads - from;
-            const int step = gridDim.x * kThreads;
-            for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest * D / 8; e += step)
-                reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.c.o) + from * D)[e] = make_uint4(0, 0, 0, 0);
-            if (a.c.lse != nullptr)
-                for (long long e = (long long)blockIdx.x * kThreads + tid; e < rest; e += step) a.c.lse[from + e] = -INFINITY;
-        }
         if (hk == 0 && z == 0 && tid == 0) {
             int n, tile;
             if (a.tiles.find(b, slot, n, tile)) check_batch(b, a.tiles, n, tile);
@@ -259,6 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (!some) {
         if constexpr (in_prefix)
             if (tid < 64) write_places(a, a.c.batch, tid, 64);
+        if constexpr (!sums_only)
+            if (hk == 0 && z == 0 && tid < 64) blank_rest(a, b, tid, 64);
         if (KEYS == kOwnKeys) dependency_wait();      // the end of this kernel stands for that of the one before too
         return;
     }
@@ -793,6 +797,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         } else {
             // -------------------------------------------------------------- V tiles that some row sees only in part
             if constexpr (in_prefix) write_places(a, a.c.batch, tid - kFixWarp * 32, 64);
+            if constexpr (!sums_only)
+                if (hk == 0 && z == 0) blank_rest(a, b, tid - kFixWarp * 32, 64);
             uint32_t phase = 0;      // of each stage's barrier
             bool odd = false;
             for (int j = t_begin; j < t_end; ++j) {

@@ -184,6 +184,11 @@ bool paged_shape(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
     s.v_page_stride = vc.stride(0), s.v_row_stride = vc.stride(1), s.v_head_stride = vc.stride(2);
     return true;
 }
+// What a call is about to write in place.  Refused by torch are tensors made in inference mode, outside of it: before anything is written.
+template <class... T>
+void written(const T&... t) {
+    (t.unsafeGetTensorImpl()->bump_version(), ...);
+}
 const int32_t* iptr(const OptTensor& t) { return has(t) ? t->const_data_ptr<int32_t>() : nullptr; }
 
 OptTensor append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cos_, const Tensor& sin_, const Tensor& kc, const Tensor& vc, const Tensor& table,
@@ -211,12 +216,11 @@ OptTensor append(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
     sh.q_token_stride = q.stride(0), sh.q_head_stride = q.stride(1);
     sh.k_token_stride = k.stride(0), sh.k_head_stride = k.stride(1);
     sh.v_token_stride = v.stride(0), sh.v_head_stride = v.stride(1);
+    written(kc, vc);
     must(kda_norm_rope_append(&sh, &pg, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), fptr(cos), fptr(sin), fptr(qw), fptr(kw),
                               table.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), iptr(cu), out.data_ptr(), kc.mutable_data_ptr(),
                               vc.mutable_data_ptr(), stream_of(q)),
          "kda_norm_rope_append");
-    kc.unsafeGetTensorImpl()->bump_version();
-    vc.unsafeGetTensorImpl()->bump_version();
     return out;
 }
 
@@ -326,11 +330,11 @@ PlanOut plan(const Tensor& table, const Tensor& lens, const Tensor& free, const 
     const size_t need = kda_plan_pages_workspace_bytes(&s);
     Tensor ws;
     if (need > 0) ws = bytes(need, table);
+    written(table, lens, free);
     must(kda_plan_pages(&s, table.mutable_data_ptr<int32_t>(), lens.mutable_data_ptr<int32_t>(), static_cast<uint8_t*>(free.mutable_data_ptr()),
                         news.const_data_ptr<int32_t>(), iptr(starts), cu.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), slots.data_ptr<int64_t>(),
                         need > 0 ? ws.data_ptr() : nullptr, need, stream_of(table)),
          "kda_plan_pages");
-    for (const Tensor* t : {&table, &lens, &free}) t->unsafeGetTensorImpl()->bump_version();
     return std::make_tuple(cu, positions, slots);
 }
 

@@ -16,6 +16,7 @@ sequence has as many.  `kv_lens` [N] counts a sequence's tokens, the new ones am
 pages.  These three are read on the device: a decode loop captures the calls in a CUDA graph and updates the arrays in place.
 Tokens behind cu_seqlens[N] belong to no sequence.  A step of fixed size, as a captured one is, has such tokens wherever a request waits or
 ends (`plan_pages`) and says so with `padded`: they are padding then.  Without it they are reported as an inconsistent `cu_seqlens`.
+(The KDA layers beside these take packed batches that are full.)
 """
 
 from __future__ import annotations
@@ -202,8 +203,15 @@ def shared_prefix_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_t
     has all of its keys in its own pages.
 
     bfloat16 under the conditions of `paged_attention` runs on the tensor cores, where the new tokens of all sequences of a group share each
-    key tile of the prefix.  Returns o, or (o, lse), as `paged_attention` does.  There is no window: a sliding-window layer sees little of
-    a prefix.  Inference only."""
+    key tile of the prefix.  Weights are rounded to bfloat16 there, as `paged_attention` does with chunks, but for those of own keys where
+    max_q_len * Hq / Hk <= 16: an error of up to 2^-8 of the sum of weights times |v|, measured 1.35 times that of rounding the result alone.
+    `paged_attention` of token steps holds all weights to 2^-16; where that is wanted, rows that name the prefix's pages in their own tables have it,
+    at the price of reading them each.
+
+    Which kernels take a call goes by the widths of the two tables, since lengths are not known on the host: they may be as wide as one another, as rows of one
+    pool's table are, or end where the texts do.
+
+    Returns o, or (o, lse), as `paged_attention` does.  There is no window: a sliding-window layer sees little of a prefix.  Inference only."""
     out = None
     if q.is_cuda:
         out = _native.load().shared_attention(q, k_cache, v_cache, block_table, kv_lens, prefix_table, prefix_lens, cu_groups, cu_seqlens, max_q_len, scale,
@@ -251,7 +259,8 @@ def plan_pages(block_table: Tensor, kv_lens: Tensor, page_free: Tensor, new_lens
     find their pages and tokens.
 
     positions [max_tokens] int32 are the new tokens' places in their sequences, slots [max_tokens] int64 those in a cache of
-    [pages * page_size] rows; -1 behind the last.  Nothing synchronises; a captured graph follows the arrays.  What goes on from here with
+    [pages * page_size] rows; -1 behind the last.  They are for layers of the caller's own: append and attention go by lengths and tables, and
+    `qk_norm_rope` takes no position of -1.  Nothing synchronises; a captured graph follows the arrays.  What goes on from here with
     max_tokens tokens - `qk_norm_rope_append`, the attention, `PagedAttention` - takes this cu_seqlens with `padded`, since a step need not be full.
     A call without cu_seqlens counts new tokens in every row, and would write one that waits over the last of what it has.  A pool starts out with all
     pages free and a table of -1."""

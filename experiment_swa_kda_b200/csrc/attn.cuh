@@ -295,7 +295,6 @@ struct Strides {
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Which keys a pass goes through.
 // Own keys of sequence n in tiles of 64.
 __device__ __forceinline__ int own_tiles_of(const OwnView& b, int n) {
     int first, count;
@@ -317,8 +316,9 @@ __device__ __forceinline__ PrefixWork prefix_work(const GroupView& b, int g, int
     return PrefixWork{rows > 0 ? max((b.prefix_len(g) + 127) / 128, 1) : 0, (rows + tile_rows - 1) / tile_rows};
 }
 constexpr int kSms = 148, kPartTries = 128;
-// Microseconds that both passes take, as measured, where the one over prefixes has `blocks` SMs and parts of `part` key tiles: a key tile takes 0.95 with
-// row tiles of 128 and 2 with 256, all own keys `own_us` of an SM (own_tiles_us), and either pass 10 besides.
+// Microseconds that both passes take where the one over prefixes has `blocks` SMs and parts of `part` key tiles: 0.95 a key tile with row tiles of 128 and 2
+// with 256, all own keys `own_us` of an SM (own_tiles_us), and either pass 10 besides.  A model of whole calls, fitted to them: the loop itself takes 1.25 (64
+// blocks) to 1.45 (120) a key tile of 128 rows and 1.7 to 1.9 of 256, but with 1.3 here 32 sequences behind 16,384 tokens take 28.8, not 27.5, and no case less.
 __host__ __device__ __forceinline__ float passes_us(int part, int blocks, int tile_rows, float own_us) {
     const float prefix_us = 10.f + (float)part * (tile_rows == 128 ? 0.95f : 2.f);
     return own_us > 0.f && blocks < kSms ? fmaxf(prefix_us, 10.f + own_us / (float)(kSms - blocks)) : prefix_us + own_us / kSms;
@@ -362,6 +362,7 @@ __device__ __forceinline__ PartChoice choose_parts(const PrefixWork* work, int g
 // Whether the pass over the prefixes is cut into parts: where its row tiles leave half of the SMs idle.
 constexpr int kMaxListed = kSms / 2;
 
+// Which keys a pass goes through.
 enum Keys { kAllKeys, kPrefixKeys, kOwnKeys, kTurnKeys, kBothKeys };      // kTurnKeys: a prefix by row tiles of 128 (attn_tc.cu); kBothKeys: prefix, then own
 template <int KEYS>
 struct ViewOf {

@@ -158,7 +158,8 @@ float side_by_side_us(const KdaPagedShape& s, const KdaPrefixShape& p, int split
 }
 
 // Token steps whose sequences have few keys all in all go through the prefix and their own keys one after the other: reading a short prefix again for
-// each costs less than two passes and their join.  In tiles of 64 keys, us: 288 17 and 22, 768 19 and 21, 1,200 22 and 21, 1,600 25 and 22, 3,200 33 and 25.
+// each costs less than two passes and their join.  In tiles of 64 keys, us: 288 13 and 21, 768 15 and 19, 1,188 19 and 20; beyond, one pass goes on to grow with them
+// and two hardly (1,536 21, 3,200 21).  The tiles are the table's, as nothing else is known here: a batch of 768 in a table of 4,096 tokens takes two, 21 us.
 bool few_keys(const KdaPagedShape& s) {
     return ((long long)s.table_width * s.page_size + 63) / 64 * s.n_seq * s.kv_heads <= 1200;
 }
@@ -184,7 +185,7 @@ bool takes_both(const KdaPagedShape& s, const KdaPrefixShape& p, long long max_q
 
 // Blocks of the pass over own keys.  A block that finds no work costs 6 us where it starts late, once others have ended, so there are as many as
 // find a place beside the prefixes, by what the tables' widths say: prefixes fill theirs, and sequences go on for 0.6 of what theirs have
-// besides.  Where both are as wide, as rows of one pool's table are, that says nothing, and own keys may fill theirs as well: too many blocks cost
+// besides (an assumption, of lengths spread from little to all).  Where both are as wide, as rows of one pool's table are, that says nothing, and own keys may fill theirs as well: too many blocks cost
 // 3 to 6 us, too few as often the pass as they are too few (256 sequences in a pool's table 90 us, 290 to 1,340 with blocks for own keys of half a page).
 // How the work is cut is decided on the device, by the lengths.
 int own_blocks(const KdaPagedShape& s, const KdaPrefixShape& p, bool packed, int splits) {

@@ -28,7 +28,7 @@
 
 // Behind a shared prefix (KEYS) the kernel does four more things.  kPrefixKeys: the new tokens of all sequences of a group are the rows, the group's prefix the
 // keys, every row sees all of them, and the sums are left for a join; kTurnKeys: the same for groups of at most 128 rows, whose row tile goes through the key tiles
-// in two streams that take turns (1.25 us a key tile; one stream alone takes 1.7).  kOwnKeys: each sequence's rows over its own keys, sums left for the join.
+// in two streams that take turns (1.25 us a key tile with 64 blocks, 1.45 with 120; one stream alone takes 1.7).  kOwnKeys: each sequence's rows over its own keys, sums left for the join.
 // kBothKeys: a sequence's rows go through the prefix's pages and then through its own, a finished result.  Prefix passes are cut into one list of equal
 // parts, a block an SM, of which there are as many as the pass over own keys beside them leaves: 32 sequences behind 16,384 tokens, 16 heads on 4, take 23 us in both
 // (64 blocks of 8 key tiles: 7 until the first scores are there, 2.5 for the first weights, whose code is fetched then, 2.5 to leave the sums) and 6 in the join.

@@ -5,8 +5,9 @@
 // and on nothing else (a call repeated on its own result changes nothing).  A row is served if the entries lacking up to and with it
 // are at most the free pages, and the new tokens up to and with it at most max_tokens; one that is not goes without its new tokens.
 //
-// All of it is a handful of sums over rows and over pages, each of which the next step waits for: bound by latency, not by bytes
-// (256 rows of 256 columns and 32,768 pages are 300 KB).  So it is one launch, a cluster of blocks that meet at its barriers (0.5 us each):
+// All of it is a handful of sums over rows and over pages, each of which the next step waits for: up to some hundred rows bound by latency, not by bytes
+// (256 rows of 256 columns and 32,768 pages are 300 KB).  So it is one launch, a cluster of blocks that meet at its barriers (0.5 us each); thousands of rows
+// are bound by what its eight SMs get through:
 //   1  entries outside of their row's columns go back; missing ones are counted, 128 columns a warp
 //   2  every block sums up all rows and all free pages for itself, which costs less than meeting once more
 //   3  who is served: the first rows that fit, or (overtake) all that still fit; the first free pages are listed in order

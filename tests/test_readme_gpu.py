@@ -1,4 +1,4 @@
-"""The serving lines of README.md, run as they stand there."""
+"""The serving lines of the package's introduction, run as they stand there."""
 
 import os
 
